@@ -27,7 +27,8 @@ from .ops import (
     uniform_initialize,
 )
 from .layers import ColumnParallelLinear, MoEMLP, RowParallelLinear, TensorParallelMLP
-from .moe import GemmGroupedV3AGScatter, GemmGroupedV3GatherRS, calc_gather_index, calc_scatter_index
+from .moe import (GemmGroupedV3AGScatter, GemmGroupedV3GatherRS, calc_gather_index, calc_scatter_index, moe_permute,
+                  moe_route, moe_unpermute)
 from .shm import GroupBarrier, default_comm, flux_create_tensor_list, get_comm, init_flux_shm
 from .util import bench_func, get_arch, group_profile, torch_allclose, with_torch_deterministic
 
@@ -39,5 +40,5 @@ __all__ = [
     "GroupBarrier", "flux_create_tensor_list", "create_tensor_list", "get_comm", "init_flux_shm", "bench_func",
     "get_arch", "group_profile", "GemmGroupedV3AGScatter", "GemmGroupedV3GatherRS", "calc_scatter_index",
     "calc_gather_index", "default_comm", "torch_allclose", "with_torch_deterministic", "FluxbError", "Tuning", "util", "TuningRecord", "load_tuning_record",
-    "layers", "tune", "ColumnParallelLinear", "RowParallelLinear", "TensorParallelMLP", "MoEMLP",
+    "moe_route", "moe_permute", "moe_unpermute", "layers", "tune", "ColumnParallelLinear", "RowParallelLinear", "TensorParallelMLP", "MoEMLP",
 ]

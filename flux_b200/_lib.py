@@ -64,6 +64,7 @@ _vp = C.c_void_p
 _i = C.c_int
 _f = C.c_float
 _sz = C.c_size_t
+_ll = C.c_longlong
 _pp = C.POINTER(C.c_void_p)
 _tun = C.POINTER(Tuning)
 
@@ -102,6 +103,11 @@ SIGNATURES = {
     "fluxb_gemm_rs_forward": (_i, [_vp, _vp, _vp, _i, _i, _i, _vp, _vp, _i, _vp, _vp, _f, _i, _tun, _vp]),
     "fluxb_moe_scatter_index": (_i, [_vp, _i, _i, _i, _vp, _vp, _vp]),
     "fluxb_moe_gather_index": (_i, [_vp, _i, _i, _vp, _vp, _vp]),
+    "fluxb_moe_route": (_i, [_vp, _i, _i, _i, _i, _vp, _vp, _vp]),
+    "fluxb_moe_route_backward": (_i, [_vp, _vp, _vp, _i, _i, _i, _i, _vp, _vp]),
+    "fluxb_moe_permute": (_i, [_vp, _i, _i, _ll, _vp, _i, _vp, _vp, _vp]),
+    "fluxb_moe_unpermute": (_i, [_vp, _i, _i, _i, _i, _vp, _vp, _i, _vp, _vp]),
+    "fluxb_moe_unpermute_backward": (_i, [_vp, _vp, _i, _i, _i, _i, _vp, _i, _vp, _vp, _i, _vp, _vp, _vp]),
     "fluxb_moe_ag_scatter_workspace_bytes": (_sz, [_i, _i, _i, _i, _i]),
     "fluxb_moe_ag_scatter_create": (_i, [_vp, _i, _i, _i, _i, _i, _i, _i, _pp, _pp, _vp, _pp]),
     "fluxb_moe_ag_scatter_destroy": (_i, [_vp]),

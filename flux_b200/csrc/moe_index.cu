@@ -113,6 +113,8 @@ scatter_index_kernel(const int* __restrict__ chosen, int total, int nexperts, in
     if (valid) {
       scatter_index[i] = base[e] + first + rank;
       if (rank == 0) wc[e] = first + __popc(peers);
+    } else if (i < hi) {
+      scatter_index[i] = -1;  // no expert, no row
     }
     __syncwarp();
   }

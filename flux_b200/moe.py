@@ -5,6 +5,8 @@
   GemmGroupedV3GatherRS  - src/pybind/gemm_grouped_v3_gather_rs.cc:35-126
                            (src/moe_gather_rs/ths_op/gemm_grouped_v3_gather_rs.cc)
   calc_scatter_index     - src/pybind/ths_op.cc:59-76 (stable order here)
+  moe_route, moe_permute, moe_unpermute - the token side of a layer as operators with gradients (the reference has
+                           them as torch code around its ops, python/flux/testing/moe_utils.py:60-144)
 Tensor parallelism over the ffn dimension; with an `ep_group` the experts are additionally split over
 `ep_size` groups of `world / ep_size` ranks (DistEnvTPWithEP, src/ths_op/ths_op.cc:334-346).
 """
@@ -17,7 +19,7 @@ import torch
 
 from . import _lib
 from . import tune as _tune
-from .ops import (DistEnvTPWithEP, MoeArguments, _check, _cur_stream, _out_dtype, _profile, _ptr, _tuning,
+from .ops import (DistEnvTPWithEP, MoeArguments, _check, _cur_device, _cur_stream, _out_dtype, _profile, _ptr, _tuning,
                   is_fp8_dtype)
 from .shm import SymmBuffer, default_comm, fluxb_dtype, get_comm
 
@@ -27,7 +29,7 @@ def calc_scatter_index(choosed_experts: torch.Tensor, splits: Optional[torch.Ten
     """`flux.calc_scatter_index(choosed_experts, splits)`: row of every (token, k) pair in the
     expert-sorted order. Stable (ties keep token order), i.e. the reference's
     `calc_scatter_index_stable` (python/flux/testing/moe_utils.py:141-144); the number of experts is
-    taken from `splits`."""
+    taken from `splits`. A pair whose expert is outside [0, nexperts) takes no row: its entry is -1."""
     _check(choosed_experts.is_cuda and choosed_experts.dtype == torch.int32 and choosed_experts.dim() == 2,
            "calc_scatter_index: choosed_experts must be a CUDA int32 [ntokens, topk] tensor")
     ntokens, topk = choosed_experts.shape
@@ -54,6 +56,168 @@ def calc_gather_index(scatter_index: torch.Tensor):
     _lib.check(_lib.load().fluxb_moe_gather_index(si.data_ptr(), ntokens, topk, gi.data_ptr(), ti.data_ptr(),
                                                   _cur_stream()))
     return gi, ti
+
+
+_FLOATS = (torch.float32, torch.bfloat16, torch.float16)
+
+
+def _on_device(t: torch.Tensor) -> bool:
+    """The library launches on the current device: tensors of another one are refused."""
+    return t.is_cuda and t.device.index == _cur_device()
+
+
+def _check_index(name: str, splits: torch.Tensor, scatter_index: torch.Tensor, ntokens: Optional[int] = None) -> None:
+    if not (_on_device(splits) and splits.dtype == torch.int32 and splits.dim() == 1 and splits.numel() >= 1 and splits.is_contiguous()):
+        raise RuntimeError(f"{name}: splits must be a contiguous int32 [nexperts] tensor on the current CUDA device")
+    if not (_on_device(scatter_index) and scatter_index.dtype == torch.int32 and scatter_index.dim() == 2 and scatter_index.shape[1] >= 1
+            and scatter_index.is_contiguous()):
+        raise RuntimeError(f"{name}: scatter_index must be a contiguous int32 [ntokens, topk] tensor on the current CUDA device")
+    if ntokens is not None and scatter_index.shape[0] != ntokens:
+        raise RuntimeError(f"{name}: scatter_index has {scatter_index.shape[0]} tokens, not {ntokens}")
+
+
+def _route_forward(logits: torch.Tensor, topk: int):
+    ntokens, nexperts = logits.shape
+    chosen = torch.empty((ntokens, topk), dtype=torch.int32, device=logits.device)
+    weights = torch.empty((ntokens, topk), dtype=torch.float32, device=logits.device)
+    _lib.check(_lib.load().fluxb_moe_route(logits.data_ptr(), fluxb_dtype(logits.dtype), ntokens, nexperts, topk, chosen.data_ptr(),
+                                           weights.data_ptr(), _cur_stream()))
+    return chosen, weights
+
+
+class _RouteFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, topk):
+        chosen, weights = _route_forward(logits, topk)
+        ctx.save_for_backward(chosen, weights)
+        ctx.mark_non_differentiable(chosen)
+        ctx.like = (logits.dtype, logits.shape[1])
+        return chosen, weights
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, _, dweights):
+        chosen, weights = ctx.saved_tensors
+        dtype, nexperts = ctx.like
+        ntokens, topk = chosen.shape
+        dlogits = torch.empty((ntokens, nexperts), dtype=dtype, device=chosen.device)
+        _lib.check(_lib.load().fluxb_moe_route_backward(
+            dweights.contiguous().data_ptr(), chosen.data_ptr(), weights.data_ptr(), fluxb_dtype(dtype), ntokens, nexperts, topk,
+            dlogits.data_ptr(), _cur_stream()))
+        return dlogits, None
+
+
+def moe_route(logits: torch.Tensor, topk: int):
+    """(chosen experts int32 [ntokens, topk], their weights fp32 [ntokens, topk]) from router logits [ntokens, nexperts]
+    (fp32, bf16 or fp16): the topk largest of every token in descending order, ties to the lower expert, and the softmax
+    over them. A logit of minus infinity is never chosen; where fewer than topk are left the entries are expert -1 with
+    weight 0, which `calc_scatter_index` gives no row. Differentiable in the logits."""
+    if not (_on_device(logits) and logits.dim() == 2 and logits.dtype in _FLOATS):
+        raise RuntimeError("moe_route: logits must be a fp32, bf16 or fp16 [ntokens, nexperts] tensor on the current CUDA device")
+    topk = int(topk)
+    if not 1 <= topk <= logits.shape[1]:
+        raise RuntimeError(f"moe_route: topk={topk} for {logits.shape[1]} experts")
+    if not logits.is_contiguous():
+        logits = logits.contiguous()
+    if logits.requires_grad and torch.is_grad_enabled():
+        return _RouteFn.apply(logits, topk)
+    return _route_forward(logits, topk)
+
+
+def _permute(tokens: torch.Tensor, splits: torch.Tensor, scatter_index: torch.Tensor) -> torch.Tensor:
+    ntokens, topk = scatter_index.shape
+    if not tokens.is_contiguous():
+        tokens = tokens.contiguous()
+    rows = torch.empty((ntokens * topk, tokens.shape[1]), dtype=tokens.dtype, device=tokens.device)
+    _lib.check(_lib.load().fluxb_moe_permute(tokens.data_ptr(), ntokens, topk, tokens.shape[1] * tokens.element_size(), splits.data_ptr(),
+                                             splits.numel(), scatter_index.data_ptr(), rows.data_ptr(), _cur_stream()))
+    return rows
+
+
+def _unpermute(rows: torch.Tensor, scatter_index: torch.Tensor, weights: Optional[torch.Tensor]) -> torch.Tensor:
+    ntokens, topk = scatter_index.shape
+    if not rows.is_contiguous():
+        rows = rows.contiguous()
+    out = torch.empty((ntokens, rows.shape[1]), dtype=rows.dtype, device=rows.device)
+    _lib.check(_lib.load().fluxb_moe_unpermute(rows.data_ptr(), fluxb_dtype(rows.dtype), ntokens, topk, rows.shape[1], scatter_index.data_ptr(),
+                                               _ptr(weights), 0 if weights is None else fluxb_dtype(weights.dtype), out.data_ptr(), _cur_stream()))
+    return out
+
+
+class _PermuteFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, tokens, splits, scatter_index):
+        ctx.save_for_backward(scatter_index)
+        return _permute(tokens, splits, scatter_index)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, drows):
+        return _unpermute(drows, ctx.saved_tensors[0], None), None, None
+
+
+class _UnpermuteFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, rows, splits, scatter_index, weights):
+        ctx.like = (rows.dtype, rows.shape[1])
+        need_rows = weights is not None and weights.requires_grad
+        ctx.save_for_backward(rows if need_rows else None, splits, scatter_index, weights)
+        return _unpermute(rows, scatter_index, weights)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dout):
+        rows, splits, scatter_index, weights = ctx.saved_tensors
+        if weights is None:
+            return _permute(dout, splits, scatter_index), None, None, None
+        ntokens, topk = scatter_index.shape
+        dtype, hidden = ctx.like
+        dout = dout.contiguous()
+        drows = dweights = None
+        if ctx.needs_input_grad[0]:
+            drows = torch.empty((ntokens * topk, hidden), dtype=dtype, device=dout.device)
+        if ctx.needs_input_grad[3]:
+            # pairs without an expert get a gradient of zero like the others get theirs: the kernel writes every entry
+            dweights = torch.empty((ntokens, topk), dtype=weights.dtype, device=dout.device)
+            rows = rows.contiguous()
+        else:
+            rows = None
+        _lib.check(_lib.load().fluxb_moe_unpermute_backward(
+            dout.data_ptr(), _ptr(rows), fluxb_dtype(dtype), ntokens, topk, hidden, splits.data_ptr(), splits.numel(), scatter_index.data_ptr(),
+            weights.data_ptr(), fluxb_dtype(weights.dtype), _ptr(drows), _ptr(dweights), _cur_stream()))
+        return drows, None, None, dweights
+
+
+def moe_permute(tokens: torch.Tensor, splits: torch.Tensor, scatter_index: torch.Tensor) -> torch.Tensor:
+    """Tokens in the order of their experts: rows [ntokens * topk, hidden] with rows[scatter_index[t, j]] = tokens[t], for
+    `splits` and `scatter_index` as `calc_scatter_index` makes them. Pairs without an expert (entry -1) have no row; the
+    rows past sum(splits) are zero. Any element type; differentiable in floating-point tokens."""
+    _check(_on_device(tokens) and tokens.dim() == 2 and tokens.shape[1] >= 1, "moe_permute: tokens must be a [ntokens, hidden] tensor on the current CUDA device")
+    _check_index("moe_permute", splits, scatter_index, tokens.shape[0])
+    if tokens.requires_grad and torch.is_grad_enabled():
+        _check(tokens.dtype in _FLOATS, "moe_permute: only fp32, bf16 and fp16 tokens have gradients")
+        return _PermuteFn.apply(tokens, splits, scatter_index)
+    return _permute(tokens, splits, scatter_index)
+
+
+def moe_unpermute(rows: torch.Tensor, splits: torch.Tensor, scatter_index: torch.Tensor,
+                  weights: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """The way back: out[t] = sum over j of weights[t, j] * rows[scatter_index[t, j]], summed in fp32 in the order of j and
+    rounded once. `rows` [ntokens * topk, hidden] and `weights` [ntokens, topk] (None: all 1) are fp32, bf16 or fp16 each.
+    A token none of whose choices has a row gets zeros. Differentiable in the rows and in the weights."""
+    if not (_on_device(rows) and rows.dim() == 2 and rows.shape[1] >= 1 and rows.dtype in _FLOATS):
+        raise RuntimeError("moe_unpermute: rows must be a fp32, bf16 or fp16 [ntokens * topk, hidden] tensor on the current CUDA device")
+    _check_index("moe_unpermute", splits, scatter_index)
+    if rows.shape[0] != scatter_index.numel():
+        raise RuntimeError(f"moe_unpermute: {rows.shape[0]} rows for {scatter_index.numel()} entries of scatter_index")
+    if weights is not None:
+        _check(_on_device(weights) and weights.dtype in _FLOATS and weights.shape == scatter_index.shape,
+               "moe_unpermute: weights must be a fp32, bf16 or fp16 [ntokens, topk] tensor on the current CUDA device")
+        if not weights.is_contiguous():
+            weights = weights.contiguous()
+    if torch.is_grad_enabled() and (rows.requires_grad or (weights is not None and weights.requires_grad)):
+        return _UnpermuteFn.apply(rows, splits, scatter_index, weights)
+    return _unpermute(rows, scatter_index, weights)
 
 
 class GemmGroupedV3AGScatter:

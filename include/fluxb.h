@@ -201,12 +201,42 @@ int fluxb_gemm_rs_forward(fluxb_gemm_rs_t op, const void* a, const void* b, int 
  * fluxb_moe_scatter_index: stable scatter index + splits from the chosen
  * experts (python/flux/testing/moe_utils.py:141-144 calc_scatter_index_stable;
  * device counterpart src/cuda/moe_utils.cu:23-75 calc_scatter_index, whose
- * order inside an expert is not deterministic).
+ * order inside an expert is not deterministic). A pair whose expert is outside [0, nexperts) takes no row: its entry is -1
+ * (the rows of the others are 0 .. sum(splits) - 1).
  * fluxb_moe_gather_index: inverse permutation (src/moe_ag_scatter/sort_util.cu:39-92). */
 int fluxb_moe_scatter_index(const int* chosen_experts, int ntokens, int topk, int nexperts,
                             int* splits_out, int* scatter_index_out, fluxb_stream_t stream);
 int fluxb_moe_gather_index(const int* scatter_index, int ntokens, int topk, int* gather_index_out,
                            int* topk_index_out, fluxb_stream_t stream);
+
+/* ------------------------------------------- MoE routing and token order
+ * The token side of a MoE layer on one GPU as operators of their own, each with its gradient (the reference has them
+ * inside its grouped GEMMs, or as torch code around them: python/flux/testing/moe_utils.py:60-144, examples/moe.py:141-211).
+ * Sums are in fp32, in a fixed order.
+ *
+ * fluxb_moe_route: of `logits` [ntokens, nexperts] (fp32, bf16 or fp16) the topk largest of every token (ties: the lower
+ * expert; NaN counts as the largest) and the softmax over them. A logit of minus infinity is never chosen: where fewer
+ * than topk are left, the other entries are expert -1 with weight 0. nexperts <= 1024, topk <= 32.
+ * fluxb_moe_route_backward: dlogits (type `dtype`), zero for experts that were not chosen.
+ *
+ * fluxb_moe_permute: rows_out[scatter_index[t, j]] = tokens[t], rows of any type, row_bytes each.
+ * fluxb_moe_unpermute: out[t] = sum over j of weights[t, j] * rows[scatter_index[t, j]] (weights NULL: the plain sum, which
+ * is the gradient of fluxb_moe_permute).
+ * fluxb_moe_unpermute_backward: drows[scatter_index[t, j]] = weights[t, j] * dout[t] and
+ * dweights[t, j] = <dout[t], rows[scatter_index[t, j]]>; drows may be NULL, and `rows` with `dweights`.
+ * The row matrices have ntokens * topk rows. `splits` and `scatter_index` belong together as fluxb_moe_scatter_index makes
+ * them: entries outside [0, ntokens * topk) are skipped, rows from sum(splits) on are written as zero. */
+int fluxb_moe_route(const void* logits, int dtype, int ntokens, int nexperts, int topk, int* chosen_out,
+                    float* weights_out, fluxb_stream_t stream);
+int fluxb_moe_route_backward(const float* dweights, const int* chosen, const float* weights, int dtype, int ntokens,
+                             int nexperts, int topk, void* dlogits, fluxb_stream_t stream);
+int fluxb_moe_permute(const void* tokens, int ntokens, int topk, long long row_bytes, const int* splits, int nexperts,
+                      const int* scatter_index, void* rows_out, fluxb_stream_t stream);
+int fluxb_moe_unpermute(const void* rows, int dtype, int ntokens, int topk, int hidden, const int* scatter_index,
+                        const void* weights, int weights_dtype, void* out, fluxb_stream_t stream);
+int fluxb_moe_unpermute_backward(const void* dout, const void* rows, int dtype, int ntokens, int topk, int hidden,
+                                 const int* splits, int nexperts, const int* scatter_index, const void* weights,
+                                 int weights_dtype, void* drows, void* dweights, fluxb_stream_t stream);
 
 /* ------------------------------------------------------ MoE AG + scatter
  * Replaces GemmGroupedV3AGScatterOp

@@ -1,0 +1,61 @@
+"""Refusals of the routing and sort operators: they need no GPU."""
+import ctypes as C
+
+import pytest
+import torch
+
+import flux_b200 as flux
+from flux_b200 import _lib
+
+
+def test_tensors_off_the_gpu_are_refused():
+    x, si, splits = torch.zeros(4, 8), torch.zeros(4, 2, dtype=torch.int32), torch.zeros(4, dtype=torch.int32)
+    with pytest.raises(RuntimeError, match="moe_route: logits"):
+        flux.moe_route(x, 2)
+    with pytest.raises(RuntimeError, match="moe_permute: tokens"):
+        flux.moe_permute(x, splits, si)
+    with pytest.raises(RuntimeError, match="moe_unpermute: rows"):
+        flux.moe_unpermute(torch.zeros(8, 8), splits, si)
+
+
+@pytest.mark.parametrize("dtype,ntokens,nexperts,topk", [(_lib.E4M3, 4, 8, 2), (_lib.S8, 4, 8, 2), (_lib.F32, -1, 8, 2), (_lib.F32, 4, 0, 1),
+                                                         (_lib.F32, 4, 1025, 2), (_lib.F32, 4, 8, 0), (_lib.F32, 4, 8, 9), (_lib.F32, 4, 64, 33),
+                                                         (_lib.F32, 1 << 30, 8, 2), (_lib.F32, 4, 8, 2)])
+def test_route_arguments(dtype, ntokens, nexperts, topk):
+    lib = _lib.load()  # (the last case has NULL pointers only)
+    assert lib.fluxb_moe_route(None, dtype, ntokens, nexperts, topk, None, None, None) == _lib.FLUXB_ERR_INVALID
+    assert "moe_route" in _lib.last_error()
+    assert lib.fluxb_moe_route_backward(None, None, None, dtype, ntokens, nexperts, topk, None, None) == _lib.FLUXB_ERR_INVALID
+    assert "moe_route_backward" in _lib.last_error()
+
+
+@pytest.mark.parametrize("ntokens,topk,size,nexperts", [(-1, 2, 64, 8), (4, 0, 64, 8), (4, 2, 0, 8), (1 << 29, 2, 64, 8), (4, 2, 1 << 30, 8),
+                                                        (4, 2, 64, 0), (4, 2, 64, 8)])
+def test_sort_arguments(ntokens, topk, size, nexperts):
+    lib = _lib.load()
+    assert lib.fluxb_moe_permute(None, ntokens, topk, size, None, nexperts, None, None, None) == _lib.FLUXB_ERR_INVALID
+    assert "moe_permute" in _lib.last_error()
+    if nexperts:
+        assert lib.fluxb_moe_unpermute(None, _lib.BF16, ntokens, topk, size, None, None, 0, None, None) == _lib.FLUXB_ERR_INVALID
+        assert "moe_unpermute" in _lib.last_error()
+    assert lib.fluxb_moe_unpermute_backward(None, None, _lib.BF16, ntokens, topk, size, None, nexperts, None, None, _lib.F32, None, None,
+                                            None) == _lib.FLUXB_ERR_INVALID
+    assert "moe_unpermute_backward" in _lib.last_error()
+
+
+def test_sort_types_and_null_pairs():
+    lib = _lib.load()
+    p = C.c_void_p(256)  # never read: the call is refused first
+    assert lib.fluxb_moe_unpermute(p, _lib.E4M3, 4, 2, 64, p, None, 0, p, None) == _lib.FLUXB_ERR_INVALID
+    assert lib.fluxb_moe_unpermute(p, _lib.BF16, 4, 2, 64, p, p, _lib.S8, p, None) == _lib.FLUXB_ERR_INVALID
+    # the rows without the weights' gradient, and the other way round
+    for rows, dw in ((p, None), (None, p)):
+        assert lib.fluxb_moe_unpermute_backward(p, rows, _lib.BF16, 4, 2, 64, p, 8, p, p, _lib.F32, p, dw, None) == _lib.FLUXB_ERR_INVALID
+        assert "gradient" in _lib.last_error()
+
+
+def test_no_tokens_is_no_work():
+    lib = _lib.load()
+    assert lib.fluxb_moe_route(None, _lib.F32, 0, 8, 2, None, None, None) == _lib.FLUXB_OK
+    assert lib.fluxb_moe_permute(None, 0, 2, 64, None, 8, None, None, None) == _lib.FLUXB_OK
+    assert lib.fluxb_moe_unpermute(None, _lib.F32, 0, 2, 64, None, None, 0, None, None) == _lib.FLUXB_OK
