@@ -1,0 +1,318 @@
+// Microscaled 4-bit floating point (the OCP MX format MXFP4): blocks of 32 values along K share one power of two.
+//   s = floor(log2(max |x|)) - 2 (2: the exponent of e2m1's largest binade), at least -127, stored as s + 127;
+//   q = x / 2^s rounded to the nearest of 0, 0.5, 1, 1.5, 2, 3, 4, 6 (ties to the even code), 6 at most.
+// Dividing by the power of two is exact, so every q is the correctly rounded value. A block that holds an infinity or a
+// NaN has the scale 255, which makes all of it NaN.
+//
+// Bound by memory: 4 lanes share a block, 8 values each, so that a warp's loads are 512 contiguous bytes (16-bit types)
+// and its stores 128. Four such pieces of a thread are in flight together.
+#include "internal.h"
+#include "mx_gemm.cuh"
+#include "plain_gemm.cuh"
+
+namespace fluxb {
+
+constexpr int kQuantThreads = 256;
+constexpr int kQuantUnroll = 4;
+constexpr int kQuantTailCtas = 148;
+
+struct QuantParams {
+  const void* x;
+  long long ldx;      // elements between rows
+  int rows, units;    // units of 8 values in a row
+  FastDiv div;        // by units
+  long long total;    // rows * units
+  uint8_t* data;
+  uint8_t* scales;
+  long long pitch;
+  // quantised into the order of the experts: row t goes to the rows index[t, j]; else null
+  const int* index;
+  const int* splits;
+  int topk, nexperts, main_ctas;
+};
+
+// 8 values of one of the input types, 16 or 32 bytes
+template <class T>
+struct Eight {
+  uint4 v[sizeof(T) / 2];
+};
+template <class T>
+__device__ __forceinline__ void eight_load(Eight<T>& e, const T* p, bool aligned) {
+  if (aligned) {
+#pragma unroll
+    for (int i = 0; i < static_cast<int>(sizeof(T) / 2); ++i) e.v[i] = __ldg(reinterpret_cast<const uint4*>(p) + i);
+  } else {
+    T* t = reinterpret_cast<T*>(e.v);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) t[i] = p[i];
+  }
+}
+__device__ __forceinline__ void eight_floats(const Eight<float>& e, float (&f)[8]) {
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    f[4 * i] = __uint_as_float(e.v[i].x);
+    f[4 * i + 1] = __uint_as_float(e.v[i].y);
+    f[4 * i + 2] = __uint_as_float(e.v[i].z);
+    f[4 * i + 3] = __uint_as_float(e.v[i].w);
+  }
+}
+__device__ __forceinline__ void eight_floats(const Eight<__nv_bfloat16>& e, float (&f)[8]) {
+  const uint32_t w[4] = {e.v[0].x, e.v[0].y, e.v[0].z, e.v[0].w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    f[2 * i] = __uint_as_float(w[i] << 16);
+    f[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+  }
+}
+__device__ __forceinline__ void eight_floats(const Eight<__half>& e, float (&f)[8]) {
+  const uint32_t w[4] = {e.v[0].x, e.v[0].y, e.v[0].z, e.v[0].w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+    f[2 * i] = v.x;
+    f[2 * i + 1] = v.y;
+  }
+}
+
+// eight e2m1 codes, the first in the low bits
+__device__ __forceinline__ uint32_t pack_e2m1(const float (&f)[8]) {
+  uint32_t r;
+  asm("{\n\t.reg .b8 a, b, c, d;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 a, %2, %1;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b, %4, %3;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 c, %6, %5;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 d, %8, %7;\n\t"
+      "mov.b32 %0, {a, b, c, d};\n\t}"
+      : "=r"(r)
+      : "f"(f[0]), "f"(f[1]), "f"(f[2]), "f"(f[3]), "f"(f[4]), "f"(f[5]), "f"(f[6]), "f"(f[7]));
+  return r;
+}
+
+template <class T>
+__global__ void __launch_bounds__(kQuantThreads)
+mx_quantize_kernel(const __grid_constant__ QuantParams p, const int aligned) {
+  pdl_wait();
+  if (threadIdx.x == 0) pdl_trigger();
+  if (static_cast<int>(blockIdx.x) >= p.main_ctas) {
+    // the rows that belong to no expert: zeros
+    __shared__ long long part[kQuantThreads / 32];
+    long long s = 0;
+    for (int e = threadIdx.x; e < p.nexperts; e += kQuantThreads) s += p.splits[e];
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
+    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = s;
+    __syncthreads();
+    s = 0;
+#pragma unroll
+    for (int w = 0; w < kQuantThreads / 32; ++w) s += part[w];
+    if (s < 0) s = 0;
+    const long long rows = static_cast<long long>(p.rows) * p.topk;
+    for (long long r = s + static_cast<int>(blockIdx.x) - p.main_ctas; r < rows; r += static_cast<int>(gridDim.x) - p.main_ctas)
+      for (int u = threadIdx.x; u < p.units; u += kQuantThreads) {
+        reinterpret_cast<uint32_t*>(p.data)[r * p.units + u] = 0u;
+        if ((u & 3) == 0) p.scales[r * p.pitch + (u >> 2)] = 0;
+      }
+    return;
+  }
+  const int lane = threadIdx.x & 31;
+  const long long u0 = static_cast<long long>(blockIdx.x) * (kQuantThreads * kQuantUnroll) + threadIdx.x;
+  Eight<T> in[kQuantUnroll];
+  int row[kQuantUnroll], unit[kQuantUnroll];
+#pragma unroll
+  for (int i = 0; i < kQuantUnroll; ++i) {
+    const long long u = u0 + i * kQuantThreads;
+    row[i] = -1;
+    if (u < p.total) {
+      row[i] = p.div.quot(static_cast<int>(u));
+      unit[i] = static_cast<int>(u) - row[i] * p.units;
+      eight_load(in[i], static_cast<const T*>(p.x) + row[i] * p.ldx + unit[i] * 8, aligned != 0);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < kQuantUnroll; ++i) {
+    float f[8];
+    if (row[i] >= 0) {
+      eight_floats(in[i], f);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) f[j] = 0.0f;
+    }
+    uint32_t most = 0;  // |x| as integers: infinities and NaN come out on top
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const uint32_t b = __float_as_uint(f[j]) & 0x7FFFFFFFu;
+      most = b > most ? b : most;
+    }
+#pragma unroll
+    for (int off = 1; off < 4; off <<= 1) {
+      const uint32_t o = __shfl_xor_sync(0xffffffffu, most, off);
+      most = o > most ? o : most;
+    }
+    const uint32_t field = most >> 23;
+    uint32_t code = 0u, scale = 255u;
+    if (field != 255u) {
+      scale = field < 2u ? 0u : field - 2u;
+      const float inv = __uint_as_float((254u - scale) << 23);  // 2^(127 - scale): between 2^2 and 2^127, or 2^-125 and up
+#pragma unroll
+      for (int j = 0; j < 8; ++j) f[j] *= inv;
+      code = pack_e2m1(f);
+    }
+    if (row[i] < 0) continue;
+    if (p.index == nullptr) {
+      reinterpret_cast<uint32_t*>(p.data)[static_cast<long long>(row[i]) * p.units + unit[i]] = code;
+      if ((lane & 3) == 0) p.scales[row[i] * p.pitch + (unit[i] >> 2)] = static_cast<uint8_t>(scale);
+    } else {
+      const int* idx = p.index + static_cast<long long>(row[i]) * p.topk;
+      const long long rows = static_cast<long long>(p.rows) * p.topk;
+      for (int j = 0; j < p.topk; ++j) {
+        const long long r = __ldg(idx + j);
+        if (r < 0 || r >= rows) continue;
+        reinterpret_cast<uint32_t*>(p.data)[r * p.units + unit[i]] = code;
+        if ((lane & 3) == 0) p.scales[r * p.pitch + (unit[i] >> 2)] = static_cast<uint8_t>(scale);
+      }
+    }
+  }
+}
+
+// Eight codes times their block's scale. Exact in fp32 (below 2^128), then one rounding to the output's type.
+template <class T>
+__device__ __forceinline__ T mx_out(float v);
+template <>
+__device__ __forceinline__ float mx_out(float v) { return v; }
+template <>
+__device__ __forceinline__ __nv_bfloat16 mx_out(float v) { return __float2bfloat16_rn(v); }
+template <>
+__device__ __forceinline__ __half mx_out(float v) { return __float2half_rn(v); }
+
+template <class T>
+__global__ void __launch_bounds__(kQuantThreads)
+mx_dequantize_kernel(const uint32_t* __restrict__ data, const uint8_t* __restrict__ scales, long long pitch, int units, FastDiv div,
+                     long long total, T* __restrict__ out) {
+  pdl_wait();
+  if (threadIdx.x == 0) pdl_trigger();
+  const long long u0 = static_cast<long long>(blockIdx.x) * (kQuantThreads * kQuantUnroll) + threadIdx.x;
+  uint32_t code[kQuantUnroll], scale[kQuantUnroll];
+#pragma unroll
+  for (int i = 0; i < kQuantUnroll; ++i) {
+    const long long u = u0 + i * kQuantThreads;
+    if (u < total) {
+      const int row = div.quot(static_cast<int>(u));
+      code[i] = __ldg(data + u);
+      scale[i] = __ldg(scales + row * pitch + ((static_cast<int>(u) - row * units) >> 2));
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < kQuantUnroll; ++i) {
+    const long long u = u0 + i * kQuantThreads;
+    if (u >= total) break;
+    const float s = scale[i] == 255u ? __uint_as_float(0x7FC00000u) : scale[i] == 0u ? __uint_as_float(0x00400000u) : __uint_as_float(scale[i] << 23);
+    union {
+      uint4 v[sizeof(T) / 2];
+      T e[8];
+    } o;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const uint32_t c = (code[i] >> (4 * j)) & 15u;
+      // e2m1: 2^(e - 1) (1 + m / 2), or m / 2 where e = 0
+      const uint32_t e = (c >> 1) & 3u, m = c & 1u;
+      const float mag = e == 0u ? 0.5f * static_cast<float>(m) : __uint_as_float(((126u + e) << 23) | (m << 22));
+      o.e[j] = mx_out<T>((c & 8u) ? -mag * s : mag * s);
+    }
+#pragma unroll
+    for (int j = 0; j < static_cast<int>(sizeof(T) / 2); ++j) reinterpret_cast<uint4*>(out + u * 8)[j] = o.v[j];
+  }
+}
+
+static int mx_elt_bytes(int dt) { return dt == FLUXB_F32 ? 4 : dt == FLUXB_BF16 || dt == FLUXB_F16 ? 2 : 0; }
+
+// Rows per launch: a unit's number is a 31-bit integer.
+static int mx_rows_per_launch(int units) { return static_cast<int>(((1ll << 31) - kQuantThreads * kQuantUnroll - 1) / units); }
+
+}  // namespace fluxb
+
+using namespace fluxb;
+
+extern "C" {
+
+int fluxb_mx_quantize(const void* x, int dtype, int rows, int k, long long ldx, void* data, void* scales, long long scales_pitch,
+                      const int* splits_dev, int nexperts, const int* scatter_index_dev, int topk, fluxb_stream_t stream) {
+  const int eb = mx_elt_bytes(dtype);
+  FLUXB_REQUIRE(eb != 0, "mx_quantize: the input must be fp32, bf16 or fp16");
+  FLUXB_REQUIRE(rows >= 0 && k >= kMxBlock && k % kMxBlock == 0, "mx_quantize: rows=%d k=%d invalid (k must be a multiple of %d)", rows, k, kMxBlock);
+  FLUXB_REQUIRE(scales_pitch >= k / kMxBlock, "mx_quantize: rows of scales are %lld bytes apart, fewer than they hold", scales_pitch);
+  const bool scatter = scatter_index_dev != nullptr;
+  FLUXB_REQUIRE(scatter == (splits_dev != nullptr), "mx_quantize: splits and scatter_index belong together");
+  FLUXB_REQUIRE(!scatter || (topk >= 1 && nexperts >= 1), "mx_quantize: topk=%d nexperts=%d invalid", topk, nexperts);
+  FLUXB_REQUIRE(!scatter || static_cast<long long>(rows) * topk < (1ll << 30), "mx_quantize: too many routed rows");
+  if (rows == 0) return FLUXB_OK;
+  FLUXB_REQUIRE(x != nullptr && data != nullptr && scales != nullptr, "mx_quantize: NULL argument");
+  FLUXB_REQUIRE((reinterpret_cast<uintptr_t>(x) & (eb - 1)) == 0 && (reinterpret_cast<uintptr_t>(data) & 3) == 0,
+                "mx_quantize: the input must be aligned to its type, the packed values to 4 bytes");
+  const int units = k / 8;
+  const int most = mx_rows_per_launch(units);
+  FLUXB_REQUIRE(!scatter || rows <= most, "mx_quantize: too many values");
+  const int aligned = ((reinterpret_cast<uintptr_t>(x) | static_cast<uintptr_t>(ldx * eb)) & 15) == 0 ? 1 : 0;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  for (int r0 = 0; r0 < rows; r0 += most) {
+    QuantParams p;
+    memset(&p, 0, sizeof(p));
+    p.x = static_cast<const uint8_t*>(x) + static_cast<long long>(r0) * ldx * eb;
+    p.ldx = ldx;
+    p.rows = rows - r0 < most ? rows - r0 : most;
+    p.units = units;
+    p.div.set(static_cast<uint32_t>(units));
+    p.total = static_cast<long long>(p.rows) * units;
+    p.data = static_cast<uint8_t*>(data) + static_cast<long long>(r0) * (k / 2);
+    p.scales = static_cast<uint8_t*>(scales) + r0 * scales_pitch;
+    p.pitch = scales_pitch;
+    p.index = scatter_index_dev;
+    p.splits = splits_dev;
+    p.topk = topk;
+    p.nexperts = nexperts;
+    p.main_ctas = static_cast<int>((p.total + kQuantThreads * kQuantUnroll - 1) / (kQuantThreads * kQuantUnroll));
+    const long long out_rows = static_cast<long long>(rows) * topk;
+    const int grid = p.main_ctas + (!scatter ? 0 : out_rows < kQuantTailCtas ? static_cast<int>(out_rows) : kQuantTailCtas);
+    const int rc = dtype == FLUXB_F32    ? launch_pdl(mx_quantize_kernel<float>, grid, kQuantThreads, s, p, aligned)
+                   : dtype == FLUXB_BF16 ? launch_pdl(mx_quantize_kernel<__nv_bfloat16>, grid, kQuantThreads, s, p, aligned)
+                                         : launch_pdl(mx_quantize_kernel<__half>, grid, kQuantThreads, s, p, aligned);
+    if (rc != FLUXB_OK) return rc;
+    if (rows - r0 <= most) break;
+  }
+  return FLUXB_OK;
+}
+
+int fluxb_mx_dequantize(const void* data, const void* scales, long long scales_pitch, int rows, int k, int out_dtype, void* out,
+                        fluxb_stream_t stream) {
+  const int eb = mx_elt_bytes(out_dtype);
+  FLUXB_REQUIRE(eb != 0, "mx_dequantize: the output must be fp32, bf16 or fp16");
+  FLUXB_REQUIRE(rows >= 0 && k >= kMxBlock && k % kMxBlock == 0, "mx_dequantize: rows=%d k=%d invalid (k must be a multiple of %d)", rows, k, kMxBlock);
+  FLUXB_REQUIRE(scales_pitch >= k / kMxBlock, "mx_dequantize: rows of scales are %lld bytes apart, fewer than they hold", scales_pitch);
+  if (rows == 0) return FLUXB_OK;
+  FLUXB_REQUIRE(data != nullptr && scales != nullptr && out != nullptr, "mx_dequantize: NULL argument");
+  FLUXB_REQUIRE((reinterpret_cast<uintptr_t>(data) & 3) == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0,
+                "mx_dequantize: the packed values must be 4-byte aligned, the output 16-byte");
+  const int units = k / 8;
+  const int most = mx_rows_per_launch(units);
+  FastDiv div;
+  div.set(static_cast<uint32_t>(units));
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  for (int r0 = 0; r0 < rows; r0 += most) {
+    const int n = rows - r0 < most ? rows - r0 : most;
+    const long long total = static_cast<long long>(n) * units;
+    const uint32_t* d = reinterpret_cast<const uint32_t*>(data) + static_cast<long long>(r0) * units;
+    const uint8_t* sc = static_cast<const uint8_t*>(scales) + r0 * scales_pitch;
+    uint8_t* o = static_cast<uint8_t*>(out) + static_cast<long long>(r0) * k * eb;
+    const int grid = static_cast<int>((total + kQuantThreads * kQuantUnroll - 1) / (kQuantThreads * kQuantUnroll));
+    const int rc =
+        out_dtype == FLUXB_F32    ? launch_pdl(mx_dequantize_kernel<float>, grid, kQuantThreads, s, d, sc, scales_pitch, units, div, total, reinterpret_cast<float*>(o))
+        : out_dtype == FLUXB_BF16 ? launch_pdl(mx_dequantize_kernel<__nv_bfloat16>, grid, kQuantThreads, s, d, sc, scales_pitch, units, div, total,
+                                               reinterpret_cast<__nv_bfloat16*>(o))
+                                  : launch_pdl(mx_dequantize_kernel<__half>, grid, kQuantThreads, s, d, sc, scales_pitch, units, div, total,
+                                               reinterpret_cast<__half*>(o));
+    if (rc != FLUXB_OK) return rc;
+    if (rows - r0 <= most) break;
+  }
+  return FLUXB_OK;
+}
+
+}  // extern "C"

@@ -1,0 +1,185 @@
+"""Microscaled 4-bit floating point (MXFP4): quantisation and products on the tensor cores. No counterpart in the
+reference, whose narrowest type is fp8; here it stands beside `GemmOnly` and the grouped ops for serving with weights of
+4.25 bits a value.
+
+Format: 32 consecutive values along K share a power of two (e8m0: the exponent + 127 in a byte, 255 = NaN), the values
+are e2m1 (0, 0.5, 1, 1.5, 2, 3, 4, 6 and their negatives), two to a byte, the first in the low half.
+
+    w = flux.mx_quantize(weight)                        # once, when the weights are loaded
+    y = flux.mx_gemm(flux.mx_quantize(x), w)            # y[M, N] = x[M, K] . weight[N, K]^T
+"""
+from __future__ import annotations
+
+from typing import Dict, Optional
+
+import torch
+
+from . import _lib
+from .moe import _FLOATS, _check_index, _on_device
+from .ops import _check, _cur_device, _cur_stream, _ptr, _tuning
+from .shm import _LAST, Comm, fluxb_dtype, get_comm
+
+BLOCK = 32
+_COMMS: Dict[int, Comm] = {}
+
+
+def _comm() -> Comm:
+    """A communicator of the current device (its status word and time-out): the process's own, or one of one rank."""
+    dev = _cur_device()
+    if _LAST and _LAST[0].device.index == dev:
+        return _LAST[0]
+    c = _COMMS.get(dev)
+    if c is None:
+        c = get_comm(None)
+        if c.device.index != dev:
+            c = Comm(None)
+        _COMMS[dev] = c
+    return c
+
+
+def _scale_pitch(k: int) -> int:
+    """Bytes between rows of scales: 16 for every 512 values, so that every stage of a product reads aligned pieces."""
+    return (k + 511) // 512 * 16
+
+
+class MXTensor:
+    """Values [..., K] as packed e2m1 and scales: `data` uint8 [..., K / 2], `scales` uint8 [..., K / 32]. The
+    constructor takes them as a checkpoint holds them and brings the scales into the layout that the products read (rows
+    a multiple of 16 bytes apart); `mx_quantize` makes them that way."""
+
+    __slots__ = ("data", "_scales", "k", "pitch")
+
+    def __init__(self, data: torch.Tensor, scales: torch.Tensor):
+        _check(_on_device(data) and _on_device(scales), "MXTensor: data and scales must be on the current CUDA device")
+        _check(data.dtype == torch.uint8 and scales.dtype == torch.uint8, "MXTensor: data and scales must be uint8")
+        _check(data.dim() >= 2 and data.shape[-1] >= BLOCK // 2 and data.shape[-1] % (BLOCK // 2) == 0,
+               "MXTensor: data must be [..., K / 2] with K a multiple of 32")
+        k = data.shape[-1] * 2
+        if tuple(scales.shape) != (*data.shape[:-1], k // BLOCK):
+            raise RuntimeError(f"MXTensor: scales shape {tuple(scales.shape)} != {(*data.shape[:-1], k // BLOCK)}")
+        data = data.contiguous()
+        if data.data_ptr() % 16:
+            data = data.clone()
+        self.data, self.k, self.pitch = data, k, _scale_pitch(k)
+        self._scales = torch.zeros((*data.shape[:-1], self.pitch), dtype=torch.uint8, device=data.device)
+        self._scales[..., :k // BLOCK] = scales
+
+    @classmethod
+    def _of(cls, data: torch.Tensor, padded_scales: torch.Tensor, k: int) -> "MXTensor":
+        t = cls.__new__(cls)
+        t.data, t._scales, t.k, t.pitch = data, padded_scales, k, padded_scales.shape[-1]
+        return t
+
+    @property
+    def scales(self) -> torch.Tensor:
+        return self._scales[..., :self.k // BLOCK]
+
+    @property
+    def shape(self) -> torch.Size:
+        return torch.Size((*self.data.shape[:-1], self.k))
+
+    @property
+    def device(self) -> torch.device:
+        return self.data.device
+
+    def dequantize(self, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+        return mx_dequantize(self, dtype)
+
+    def __repr__(self) -> str:
+        return f"MXTensor(shape={tuple(self.shape)}, device={self.device})"
+
+
+def mx_quantize(x: torch.Tensor, splits: Optional[torch.Tensor] = None, scatter_index: Optional[torch.Tensor] = None) -> MXTensor:
+    """Quantise x [..., K] (fp32, bf16 or fp16; K a multiple of 32): scale 2^(floor(log2 max|x|) - 2) for every 32 values,
+    values rounded to nearest, ties to even, at most 6 in magnitude. A block with an infinity or a NaN becomes NaN.
+    With `splits` and `scatter_index` (as `calc_scatter_index` makes them) the tokens x [ntokens, K] go into the order of
+    their experts on the way, as in `moe_permute`: the result has ntokens * topk rows, and the rows past sum(splits) are
+    zero. Has no gradient."""
+    if not (_on_device(x) and x.dim() >= 2 and x.dtype in _FLOATS and x.shape[-1] >= BLOCK and x.shape[-1] % BLOCK == 0):
+        raise RuntimeError("mx_quantize: x must be a fp32, bf16 or fp16 [..., K] tensor on the current CUDA device, K a multiple of 32")
+    _check(not (x.requires_grad and torch.is_grad_enabled()), "mx_quantize has no gradient: detach x, or call it under torch.no_grad()")
+    k = x.shape[-1]
+    if x.dim() > 2 or x.stride(1) != 1:
+        x2 = x.contiguous().view(-1, k)
+    else:
+        x2 = x
+    rows = x2.shape[0]
+    topk = nexperts = 0
+    if scatter_index is None:
+        _check(splits is None, "mx_quantize: splits and scatter_index belong together")
+        shape = x.shape[:-1]
+    else:
+        _check(splits is not None and x.dim() == 2, "mx_quantize: into the order of experts go [ntokens, K] tokens, with splits and scatter_index")
+        _check_index("mx_quantize", splits, scatter_index, rows)
+        topk, nexperts = scatter_index.shape[1], splits.numel()
+        shape = (rows * topk,)
+    pitch = _scale_pitch(k)
+    data = torch.empty((*shape, k // 2), dtype=torch.uint8, device=x.device)
+    scales = torch.empty((*shape, pitch), dtype=torch.uint8, device=x.device)
+    _lib.check(_lib.load().fluxb_mx_quantize(x2.data_ptr(), fluxb_dtype(x.dtype), rows, k, x2.stride(0), data.data_ptr(), scales.data_ptr(), pitch,
+                                             _ptr(splits), nexperts, _ptr(scatter_index), topk, _cur_stream()))
+    return MXTensor._of(data, scales, k)
+
+
+def mx_dequantize(q: MXTensor, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """The values that `q` stands for, as fp32, bf16 or fp16 (exact in bf16 but beyond its range)."""
+    _check(isinstance(q, MXTensor) and _on_device(q.data), "mx_dequantize: q must be an MXTensor on the current CUDA device")
+    _check(dtype in _FLOATS, "mx_dequantize: the output must be fp32, bf16 or fp16")
+    out = torch.empty((*q.data.shape[:-1], q.k), dtype=dtype, device=q.data.device)
+    rows = q.data.numel() // (q.k // 2)
+    _lib.check(_lib.load().fluxb_mx_dequantize(q.data.data_ptr(), q._scales.data_ptr(), q.pitch, rows, q.k, fluxb_dtype(dtype), out.data_ptr(),
+                                               _cur_stream()))
+    return out
+
+
+def _check_operands(name: str, x: MXTensor, w: MXTensor, wdim: int, output_dtype: torch.dtype) -> None:
+    _check(isinstance(x, MXTensor) and isinstance(w, MXTensor) and x.data.dim() == 2 and w.data.dim() == wdim,
+           f"{name}: operands must be MXTensors, [rows, K] and {'[N, K]' if wdim == 2 else '[nexperts, N, K]'}")
+    _check(_on_device(x.data) and _on_device(w.data), f"{name}: operands must be on the current CUDA device")
+    if x.k != w.k:
+        raise RuntimeError(f"{name}: weight K {w.k} != input K {x.k}")
+    _check(output_dtype in _FLOATS, f"{name}: the output must be fp32, bf16 or fp16")
+
+
+def _output(name: str, output: Optional[torch.Tensor], rows: int, n: int, dtype: torch.dtype, device) -> torch.Tensor:
+    if output is None:
+        return torch.empty((rows, n), dtype=dtype, device=device)
+    _check(_on_device(output) and tuple(output.shape) == (rows, n) and output.dtype == dtype and output.is_contiguous(),
+           f"{name}: output has the wrong shape, dtype or layout")
+    return output
+
+
+def mx_gemm(x: MXTensor, w: MXTensor, bias: Optional[torch.Tensor] = None, output_dtype: torch.dtype = torch.bfloat16,
+            output: Optional[torch.Tensor] = None, tuning=None) -> torch.Tensor:
+    """y[M, N] = x[M, K] . w[N, K]^T (+ bias [N] of the output's type): exact products, summed in fp32, rounded once. M, N of
+    any size."""
+    _check_operands("mx_gemm", x, w, 2, output_dtype)
+    m, n = x.data.shape[0], w.data.shape[0]
+    if bias is not None:
+        _check(_on_device(bias) and bias.dtype == output_dtype and tuple(bias.shape) in ((n,), (1, n)) and bias.is_contiguous(),
+               "mx_gemm: bias must be a contiguous [N] tensor of the output's type")
+    out = _output("mx_gemm", output, m, n, output_dtype, x.data.device)
+    if n == 0:
+        return out
+    _lib.check(_lib.load().fluxb_mx_gemm(_comm().handle, x.data.data_ptr(), x._scales.data_ptr(), x.pitch, w.data.data_ptr(), w._scales.data_ptr(),
+                                         w.pitch, out.data_ptr(), m, n, x.k, fluxb_dtype(output_dtype), _ptr(bias), _tuning(tuning), _cur_stream()))
+    return out
+
+
+def mx_grouped_gemm(x: MXTensor, w: MXTensor, splits: torch.Tensor, output_dtype: torch.dtype = torch.bfloat16,
+                    output: Optional[torch.Tensor] = None, tuning=None) -> torch.Tensor:
+    """The experts' products: rows of x [rows, K] in the order of their experts, splits[e] of them for expert e (int32
+    [nexperts], on the GPU: nothing is read back), times w [nexperts, N, K]. Rows past sum(splits) are not written: they
+    stay as they were in a given `output`, and are undefined in a fresh one."""
+    _check_operands("mx_grouped_gemm", x, w, 3, output_dtype)
+    nexperts, n = w.data.shape[0], w.data.shape[1]
+    rows = x.data.shape[0]
+    if not (_on_device(splits) and splits.dtype == torch.int32 and splits.dim() == 1 and splits.numel() == nexperts and splits.is_contiguous()):
+        raise RuntimeError(f"mx_grouped_gemm: splits must be a contiguous int32 [{nexperts}] tensor on the current CUDA device")
+    out = _output("mx_grouped_gemm", output, rows, n, output_dtype, x.data.device)
+    if n == 0 or nexperts == 0:
+        return out
+    _lib.check(_lib.load().fluxb_mx_grouped_gemm(_comm().handle, x.data.data_ptr(), x._scales.data_ptr(), x.pitch, rows, w.data.data_ptr(),
+                                                 w._scales.data_ptr(), w.pitch, nexperts, splits.data_ptr(), out.data_ptr(), n, x.k,
+                                                 fluxb_dtype(output_dtype), _tuning(tuning), _cur_stream()))
+    return out

@@ -1,0 +1,70 @@
+"""Refusals of the microscaled operators: they need no GPU."""
+import ctypes as C
+
+import pytest
+import torch
+
+import flux_b200 as flux
+from flux_b200 import _lib
+
+
+def test_tensors_off_the_gpu_are_refused():
+    with pytest.raises(RuntimeError, match="mx_quantize: x must be"):
+        flux.mx_quantize(torch.zeros(4, 64))
+    with pytest.raises(RuntimeError, match="MXTensor: data and scales"):
+        flux.MXTensor(torch.zeros(4, 32, dtype=torch.uint8), torch.zeros(4, 2, dtype=torch.uint8))
+    with pytest.raises(RuntimeError, match="mx_gemm: operands"):
+        flux.mx_gemm(torch.zeros(4, 64), torch.zeros(8, 64))
+    with pytest.raises(RuntimeError, match="mx_grouped_gemm: operands"):
+        flux.mx_grouped_gemm(torch.zeros(4, 64), torch.zeros(2, 8, 64), torch.zeros(2, dtype=torch.int32))
+    with pytest.raises(RuntimeError, match="mx_dequantize: q"):
+        flux.mx_dequantize(torch.zeros(4, 64))
+
+
+P = C.c_void_p(256)  # never read: the calls are refused first
+
+
+@pytest.mark.parametrize("change,words", [
+    ({"dtype": _lib.E4M3}, "fp32, bf16 or fp16"), ({"rows": -1}, "rows=-1"), ({"k": 0}, "k=0"), ({"k": 48}, "k=48"), ({"pitch": 1}, "rows of scales"),
+    ({"splits": P}, "belong together"), ({"index": P}, "belong together"), ({"splits": P, "index": P, "topk": 0}, "topk=0"),
+    ({"splits": P, "index": P, "nexperts": 0}, "nexperts=0"), ({"splits": P, "index": P, "rows": 1 << 29}, "too many"),
+    ({"x": None}, "NULL"), ({"data": None}, "NULL"), ({"scales": None}, "NULL"), ({"x": C.c_void_p(257)}, "aligned"), ({"data": C.c_void_p(258)}, "aligned"),
+])
+def test_quantize_arguments(change, words):
+    a = {"x": P, "dtype": _lib.BF16, "rows": 4, "k": 64, "ldx": 64, "data": P, "scales": P, "pitch": 16, "splits": None, "nexperts": 8, "index": None,
+         "topk": 2, **change}
+    assert _lib.load().fluxb_mx_quantize(a["x"], a["dtype"], a["rows"], a["k"], a["ldx"], a["data"], a["scales"], a["pitch"], a["splits"], a["nexperts"],
+                                         a["index"], a["topk"], None) == _lib.FLUXB_ERR_INVALID
+    assert "mx_quantize" in _lib.last_error() and words in _lib.last_error()
+
+
+@pytest.mark.parametrize("change,words", [({"dtype": _lib.S8}, "fp32, bf16 or fp16"), ({"rows": -1}, "rows=-1"), ({"k": 33}, "k=33"), ({"pitch": 1}, "rows of scales"),
+                                          ({"data": None}, "NULL"), ({"data": C.c_void_p(258)}, "aligned"), ({"out": C.c_void_p(264)}, "aligned")])
+def test_dequantize_arguments(change, words):
+    a = {"data": P, "scales": P, "pitch": 16, "rows": 4, "k": 64, "dtype": _lib.BF16, "out": P, **change}
+    assert _lib.load().fluxb_mx_dequantize(a["data"], a["scales"], a["pitch"], a["rows"], a["k"], a["dtype"], a["out"], None) == _lib.FLUXB_ERR_INVALID
+    assert "mx_dequantize" in _lib.last_error() and words in _lib.last_error()
+
+
+@pytest.mark.parametrize("change,words", [
+    ({"comm": None}, "NULL"), ({"xq": None}, "NULL"), ({"out": None}, "NULL"), ({"k": 16}, "k=16"), ({"k": 80}, "k=80"), ({"n": 0}, "n=0"), ({"m": -1}, "=-1"),
+    ({"xp": 8}, "rows of scales"), ({"wp": 24}, "rows of scales"), ({"k": 544}, "rows of scales"), ({"xq": C.c_void_p(264)}, "16-byte"),
+    ({"ws": C.c_void_p(264)}, "16-byte"), ({"dtype": _lib.E5M2}, "not bf16/f16/f32"), ({"out": C.c_void_p(257)}, "aligned to its type"),
+    ({"dtype": _lib.F32, "out": C.c_void_p(258)}, "aligned to its type"),
+])
+def test_product_arguments(change, words):
+    a = {"comm": P, "xq": P, "xs": P, "xp": 16, "wq": P, "ws": P, "wp": 16, "out": P, "m": 4, "n": 8, "k": 64, "dtype": _lib.BF16, **change}
+    lib = _lib.load()
+    assert lib.fluxb_mx_gemm(a["comm"], a["xq"], a["xs"], a["xp"], a["wq"], a["ws"], a["wp"], a["out"], a["m"], a["n"], a["k"], a["dtype"], None, None,
+                             None) == _lib.FLUXB_ERR_INVALID
+    assert words in _lib.last_error()
+    assert lib.fluxb_mx_grouped_gemm(a["comm"], a["xq"], a["xs"], a["xp"], a["m"], a["wq"], a["ws"], a["wp"], 4, P, a["out"], a["n"], a["k"], a["dtype"], None,
+                                     None) == _lib.FLUXB_ERR_INVALID
+    assert words in _lib.last_error()
+
+
+def test_grouped_arguments():
+    lib = _lib.load()
+    for nexperts, n, splits, words in ((0, 8, P, "nexperts=0"), (1025, 8, P, "nexperts=1025"), (4, 8, None, "NULL"), (1024, 1 << 22, P, "too many")):
+        assert lib.fluxb_mx_grouped_gemm(P, P, P, 16, 4, P, P, 16, nexperts, splits, P, n, 64, _lib.BF16, None, None) == _lib.FLUXB_ERR_INVALID
+        assert words in _lib.last_error()

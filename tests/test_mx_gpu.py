@@ -1,0 +1,308 @@
+"""Microscaled 4-bit floating point (`mx_quantize`, `mx_dequantize`, `mx_gemm`, `mx_grouped_gemm`) against the format's
+definition in 64 bits.
+
+Quantisation is exact by its definition: bits are compared. Products: with scales of 1/2, 1 and 2 every term is a multiple
+of 2^-4 below 2^8, so that sums of up to 4096 terms fit into the 24 bits of fp32 and have to come out exactly, whatever
+their order. With scales of any size a sum of K terms in fp32, by adders that round or cut, is off by at most
+K 2^-23 sum|term|; the rounding to the output's type adds eps / 2 of the value."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+GRID = torch.tensor([0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0], dtype=torch.float64)
+# every kernel and tile: the library's choice, the few-token kernel, single CTAs, CTA pairs
+TILES = [None] + [{"block_n": b} for b in (16, 32, 64, 128)] + [{"block_n": b, "cta_group": 1} for b in (64, 128)] \
+    + [{"block_n": b, "cta_group": 2} for b in (64, 128, 192, 224)]
+
+
+def _values(data, scales):
+    """Packed values and scales as 64-bit numbers."""
+    data, scales = data.cpu(), scales.cpu().double()
+    code = torch.stack((data & 15, data >> 4), -1).view(*data.shape[:-1], -1).long()
+    v = GRID[code & 7] * torch.where(code >= 8, -1.0, 1.0).double()
+    s = torch.where(scales == 255, float("nan"), torch.exp2(scales - 127))
+    return v * s.repeat_interleave(32, -1)
+
+
+def _quantised64(x):
+    """(packed values, scales) of x by the definition, the nearest of eight magnitudes, ties to the even code."""
+    x = x.detach().cpu().double()
+    b = x.reshape(-1, 32)
+    bad = ~b.isfinite().all(1)
+    most = b.abs().amax(1)
+    e = torch.frexp(torch.where(bad | (most == 0), torch.ones_like(most), most)).exponent - 1 - 2
+    e = torch.where(most == 0, -127, e.clamp_min(-127))
+    a = torch.where(bad[:, None], torch.zeros_like(b), b / torch.exp2(e.double())[:, None])
+    mid = (GRID[1:] + GRID[:-1]) / 2
+    code = torch.zeros_like(a, dtype=torch.int64)
+    for c in range(7):
+        code += (a.abs() >= mid[c]) if c % 2 else (a.abs() > mid[c])
+    code += 8 * torch.signbit(a)
+    code[bad] = 0
+    code = code.view(*x.shape).to(torch.uint8)
+    scales = torch.where(bad, 255, e + 127).view(*x.shape[:-1], -1).to(torch.uint8)
+    return code[..., 0::2] | (code[..., 1::2] << 4), scales
+
+
+def _random_mx(shape, seed, low=126, high=128):
+    """Random codes with scales between two bytes."""
+    import flux_b200 as flux
+
+    g = torch.Generator().manual_seed(seed)
+    data = torch.randint(0, 256, (*shape[:-1], shape[-1] // 2), generator=g, dtype=torch.uint8)
+    scales = torch.randint(low, high + 1, (*shape[:-1], shape[-1] // 32), generator=g, dtype=torch.uint8)
+    return flux.MXTensor(data.cuda(), scales.cuda()), _values(data, scales)
+
+
+def _status():
+    import flux_b200 as flux
+
+    torch.cuda.synchronize()
+    flux.get_comm(None).check_status()
+
+
+# ---------------------------------------------------------------------------------------------------------- quantisation
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("rows,k", [(1, 32), (1, 4096), (3, 96), (7, 544), (130, 1024), (1001, 160)])
+def test_quantize_is_the_definition(rows, k, dtype):
+    import flux_b200 as flux
+
+    g = torch.Generator().manual_seed(rows + k)
+    x = (torch.randn(rows, k, generator=g) * torch.exp(3 * torch.randn(rows, k // 32, generator=g)).repeat_interleave(32, 1)).to(dtype)
+    q = flux.mx_quantize(x.cuda())
+    data, scales = _quantised64(x)
+    assert q.shape == (rows, k) and tuple(q.data.shape) == (rows, k // 2) and tuple(q.scales.shape) == (rows, k // 32)
+    assert torch.equal(q.scales.cpu(), scales)
+    assert torch.equal(q.data.cpu(), data)
+    for out in (torch.float32, torch.bfloat16, torch.float16):
+        got, want = q.dequantize(out).cpu(), _values(data, scales).to(out)
+        # (a block that overflowed fp16 before it came here is NaN)
+        assert torch.equal(got.isnan(), want.isnan()) and torch.equal(got[~got.isnan()], want[~want.isnan()])
+
+
+def test_quantize_at_every_border():
+    """All ties and their neighbours, both signs, at the ends of fp32's range and in between; zeros; what is no number."""
+    import flux_b200 as flux
+
+    marks = torch.tensor([0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0, 6.0, 7.0, 7.9999995], dtype=torch.float32)
+    near = torch.cat((marks, torch.nextafter(marks, torch.tensor(0.0)), torch.nextafter(marks, torch.tensor(8.0))))
+    block = torch.cat((near, torch.tensor([4.0, 0.0])))
+    signs = torch.where(torch.arange(32) % 3 == 0, -1.0, 1.0)
+    rows = [block * signs * 2.0 ** e for e in (0, 1, -1, 100, 125, -100, -120, -124, -126, -127, -140, -149)]
+    rows += [torch.zeros(32), -torch.zeros(32), torch.full((32,), 2.0 ** -149), torch.full((32,), torch.finfo(torch.float32).max)]
+    for bad in (float("inf"), -float("inf"), float("nan")):
+        r = block.clone()
+        r[5] = bad
+        rows.append(r)
+    x = torch.stack(rows).float()
+    q = flux.mx_quantize(x.cuda())
+    data, scales = _quantised64(x)
+    assert torch.equal(q.scales.cpu(), scales)
+    assert torch.equal(q.data.cpu(), data)
+    got, want = q.dequantize(torch.float32).cpu(), _values(data, scales).to(torch.float32)
+    assert torch.equal(got.isnan(), want.isnan()) and torch.equal(got.nan_to_num(0.0), want.nan_to_num(0.0))
+
+
+def test_quantize_layouts():
+    """Strided rows, columns that are not contiguous, addresses between the vectors' boundaries, three dimensions."""
+    import flux_b200 as flux
+
+    g = torch.Generator().manual_seed(2)
+    big = torch.randn(40, 200, generator=g).to(torch.bfloat16).cuda()
+    views = [big[:, 8:104], big[:, 3:131], big[::3, :64], big[:, ::2][:, :96], big.t()[:, :32], big[:1, :32].expand(5, 32),
+             big.reshape(-1)[1:32 * 64 + 1].view(32, 64), torch.randn(3, 5, 64, generator=g).cuda()]
+    for x in views:
+        q = flux.mx_quantize(x)
+        data, scales = _quantised64(x)
+        assert torch.equal(q.data.cpu(), data) and torch.equal(q.scales.cpu(), scales)
+
+
+def test_quantize_into_the_order_of_experts():
+    import flux_b200 as flux
+
+    g = torch.Generator().manual_seed(3)
+    for ntokens, topk, k in ((1, 1, 32), (33, 2, 544), (200, 5, 96)):
+        chosen = torch.rand(ntokens, 8, generator=g).topk(topk, dim=1).indices.to(torch.int32)
+        chosen[torch.rand(ntokens, topk, generator=g) < 0.2] = -1
+        si, splits = flux.calc_scatter_index(chosen.cuda(), torch.empty(8), return_splits=True)
+        x = torch.randn(ntokens, k, generator=g).to(torch.float16).cuda()
+        whole, q = flux.mx_quantize(x), flux.mx_quantize(x, splits, si)
+        assert torch.equal(q.data, flux.moe_permute(whole.data, splits, si))
+        assert torch.equal(q.scales, flux.moe_permute(whole.scales.contiguous(), splits, si))
+
+
+def test_dequantize_every_code_and_scale():
+    import flux_b200 as flux
+
+    data = (torch.arange(256 * 16) % 256).to(torch.uint8).view(256, 16)
+    scales = torch.arange(256, dtype=torch.int32).to(torch.uint8).view(256, 1)
+    q = flux.MXTensor(data.cuda(), scales.cuda())
+    want = _values(data, scales)
+    for out in (torch.float32, torch.bfloat16, torch.float16):
+        got = q.dequantize(out).cpu()
+        assert torch.equal(got.isnan(), want.isnan())
+        assert torch.equal(got.nan_to_num(0.0, 9.0, -9.0), want.to(out).nan_to_num(0.0, 9.0, -9.0))
+
+
+# -------------------------------------------------------------------------------------------------------------- products
+@pytest.mark.parametrize("tuning", TILES, ids=str)
+@pytest.mark.parametrize("m,n,k", [(1, 1, 32), (16, 128, 256), (5, 130, 288), (100, 257, 2080), (225, 513, 544), (300, 1000, 4096)])
+def test_product_is_exact(m, n, k, tuning):
+    import flux_b200 as flux
+
+    x, xv = _random_mx((m, k), m + k)
+    w, wv = _random_mx((n, k), n + k + 1)
+    y = flux.mx_gemm(x, w, output_dtype=torch.float32, tuning=tuning)
+    _status()
+    assert torch.equal(y.cpu().double(), xv @ wv.t())
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("m,n,k,bias", [(1, 3584, 8192, False), (48, 1031, 1024, True), (130, 96, 12288, True), (1000, 3588, 512, True)])
+def test_product_of_quantised_matrices(m, n, k, bias, dtype):
+    import flux_b200 as flux
+
+    g = torch.Generator().manual_seed(m)
+    x, w = torch.randn(m, k, generator=g), torch.randn(n, k, generator=g) * 0.02
+    b = (torch.randn(n, generator=g) * 0.1).to(dtype) if bias else None
+    xq, wq = flux.mx_quantize(x.to(torch.bfloat16).cuda()), flux.mx_quantize(w.to(torch.bfloat16).cuda())
+    y = flux.mx_gemm(xq, wq, bias=None if b is None else b.cuda(), output_dtype=dtype)
+    _status()
+    xv, wv = _values(xq.data, xq.scales), _values(wq.data, wq.scales)
+    want, size = xv @ wv.t(), xv.abs() @ wv.abs().t()
+    if bias:
+        want, size = want + b.double(), size + b.double().abs()
+    off = k * 2.0 ** -23 * size
+    off = off + torch.finfo(dtype).eps / 2 * (want.abs() + off)
+    assert bool(((y.cpu().double() - want).abs() <= off).all())
+
+
+def _grouped_want(xv, wv, splits):
+    parts, r = [], 0
+    for e, n in enumerate(splits):
+        parts.append(xv[r:r + n] @ wv[e].t())
+        r += n
+    return torch.cat(parts)
+
+
+@pytest.mark.parametrize("tuning", TILES, ids=str)
+@pytest.mark.parametrize("splits,n,k", [([3], 128, 256), ([0, 5, 0, 1, 40, 0], 130, 288), ([17, 300, 0, 64, 1, 33, 224], 257, 544),
+                                        ([1] * 100, 48, 96), ([0] * 40 + [200] + [0] * 300 + [7, 0], 70, 320), ([0, 0], 64, 64)])
+def test_grouped_product_is_exact(splits, n, k, tuning):
+    import flux_b200 as flux
+
+    rows = sum(splits) + 9  # rows behind the last expert's: left as they were
+    x, xv = _random_mx((rows, k), rows)
+    w, wv = _random_mx((len(splits), n, k), n)
+    out = torch.full((rows, n), -77.0, device="cuda")
+    flux.mx_grouped_gemm(x, w, torch.tensor(splits, dtype=torch.int32, device="cuda"), torch.float32, output=out, tuning=tuning)
+    _status()
+    got = out.cpu().double()
+    assert torch.equal(got[:sum(splits)], _grouped_want(xv, wv, splits))
+    assert bool((got[sum(splits):] == -77.0).all())
+
+
+def test_splits_that_do_not_fit_touch_nothing_outside():
+    import flux_b200 as flux
+
+    x, xv = _random_mx((50, 256), 1)
+    w, wv = _random_mx((4, 64, 256), 2)
+    for tuning in (None, {"block_n": 64, "cta_group": 2}):
+        for splits, real in (([20, 100, 5, 5], [20, 30, 0, 0]), ([-5, 20, -1, 2 ** 31 - 1], [0, 20, 0, 30]), ([2 ** 31 - 1] * 4, [50, 0, 0, 0])):
+            guard = torch.full((60, 64), -77.0, device="cuda")
+            flux.mx_grouped_gemm(x, w, torch.tensor(splits, dtype=torch.int32, device="cuda"), torch.float32, output=guard[:50], tuning=tuning)
+            _status()
+            assert torch.equal(guard[:50].cpu().double(), _grouped_want(xv, wv, real))
+            assert bool((guard[50:] == -77.0).all())
+
+
+def test_nan_stays_in_its_row():
+    """A block with the scale 255 makes its row (or column) of the result NaN and no other; scales at the ends of the range."""
+    import flux_b200 as flux
+
+    for tuning in (None, {"block_n": 64, "cta_group": 2}):
+        for k in (64, 544):
+            g = torch.Generator().manual_seed(k)
+            data = torch.randint(0, 256, (20, k // 2), generator=g, dtype=torch.uint8)
+            scales = torch.full((20, k // 32), 127, dtype=torch.uint8)
+            scales[3, -1], scales[7, 0], scales[9, :], scales[11, :] = 255, 255, 0, 190
+            x = flux.MXTensor(data.cuda(), scales.cuda())
+            w, wv = _random_mx((40, k), 5)
+            y = flux.mx_gemm(x, w, output_dtype=torch.float32, tuning=tuning).cpu().double()
+            _status()
+            bad = torch.zeros(20, dtype=torch.bool)
+            bad[3] = bad[7] = True
+            assert bool(y[bad].isnan().all()) and not bool(y[~bad].isnan().any())
+            want = _values(data, scales)[~bad] @ wv.t()
+            # row 9's terms are 2^-127 times multiples of 2^-4: fp32's subnormal steps hold them, rows of one scale are exact
+            assert torch.equal(y[~bad], want)
+
+
+def test_products_on_two_streams_and_in_graphs():
+    import flux_b200 as flux
+
+    x, xv = _random_mx((200, 2048), 1)
+    w, wv = _random_mx((700, 2048), 2)
+    few, fv = _random_mx((9, 2048), 3)
+    splits = torch.tensor([150, 50], dtype=torch.int32, device="cuda")
+    w2, w2v = _random_mx((2, 300, 2048), 4)
+    want, want_few, want_g = xv @ wv.t(), fv @ wv.t(), _grouped_want(xv, w2v, [150, 50])
+    f32 = torch.float32
+    flux.mx_gemm(x, w, output_dtype=f32)
+    a, b = torch.cuda.Stream(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    outs = []
+    for _ in range(4):
+        for s in (a, b):
+            with torch.cuda.stream(s):
+                outs.append((flux.mx_gemm(x, w, output_dtype=f32), flux.mx_gemm(few, w, output_dtype=f32), flux.mx_grouped_gemm(x, w2, splits, f32)))
+    _status()
+    for y, yf, yg in outs:
+        assert torch.equal(y.cpu().double(), want) and torch.equal(yf.cpu().double(), want_few) and torch.equal(yg.cpu().double(), want_g)
+    graphs, held = [], []
+    tokens = torch.randn(64, 2048, device="cuda")
+    for s in (a, b):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=s):
+            held.append((flux.mx_gemm(x, w, output_dtype=f32), flux.mx_gemm(flux.mx_quantize(tokens), w, output_dtype=f32),
+                         flux.mx_grouped_gemm(x, w2, splits, f32)))
+        graphs.append(g)
+    tokens.normal_()
+    splits.copy_(torch.tensor([30, 170], dtype=torch.int32))
+    for s, g in zip((a, b), graphs):
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            g.replay()
+    _status()
+    eager = flux.mx_gemm(flux.mx_quantize(tokens), w, output_dtype=f32)
+    for y, yt, yg in held:
+        assert torch.equal(y.cpu().double(), want) and torch.equal(yt, eager)
+        assert torch.equal(yg.cpu().double(), _grouped_want(xv, w2v, [30, 170]))
+
+
+def test_empty_operands_and_refusals():
+    import flux_b200 as flux
+
+    w = flux.mx_quantize(torch.randn(64, 96, device="cuda"))
+    x = flux.mx_quantize(torch.empty(0, 96, device="cuda"))
+    assert flux.mx_gemm(x, w).shape == (0, 64) and x.dequantize().shape == (0, 96)
+    one = flux.mx_quantize(torch.randn(3, 96, device="cuda"))
+    cases = [
+        (lambda: flux.mx_quantize(torch.randn(4, 40, device="cuda")), "multiple of 32"),
+        (lambda: flux.mx_quantize(torch.zeros(4, 64, dtype=torch.int32, device="cuda")), "fp32, bf16 or fp16"),
+        (lambda: flux.mx_quantize(torch.randn(4, 64, device="cuda", requires_grad=True)), "no gradient"),
+        (lambda: flux.mx_quantize(torch.randn(4, 64, device="cuda"), torch.zeros(4, dtype=torch.int32, device="cuda")), "belong together"),
+        (lambda: flux.mx_gemm(one, flux.mx_quantize(torch.randn(64, 64, device="cuda"))), "K 64 != input K 96"),
+        (lambda: flux.mx_gemm(one, w, output_dtype=torch.int32), "output must be"),
+        (lambda: flux.mx_gemm(one, w, bias=torch.zeros(64, device="cuda")), "bias"),
+        (lambda: flux.mx_gemm(one, w, output=torch.empty(3, 63, dtype=torch.bfloat16, device="cuda")), "output has"),
+        (lambda: flux.mx_gemm(one, w, tuning={"block_n": 48}), "block_n=48"),
+        (lambda: flux.mx_gemm(one, w, tuning={"block_n": 64, "cta_group": 3}), "cta_group=3"),
+        (lambda: flux.mx_grouped_gemm(one, w, torch.zeros(1, dtype=torch.int32, device="cuda")), "operands"),
+        (lambda: flux.MXTensor(torch.zeros(4, 24, dtype=torch.uint8, device="cuda"), torch.zeros(4, 1, dtype=torch.uint8, device="cuda")), "multiple of 32"),
+        (lambda: flux.MXTensor(torch.zeros(4, 16, dtype=torch.uint8, device="cuda"), torch.zeros(4, 2, dtype=torch.uint8, device="cuda")), "scales shape"),
+    ]
+    for call, words in cases:
+        with pytest.raises(RuntimeError, match=words):
+            call()
