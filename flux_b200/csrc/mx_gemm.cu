@@ -210,11 +210,11 @@ int fluxb_mx_grouped_gemm(fluxb_comm_t comm, const void* xq, const void* xs, lon
   FLUXB_REQUIRE(rows >= 0, "mx_grouped_gemm: rows=%d invalid", rows);
   FLUXB_REQUIRE(nexperts >= 1 && nexperts <= kMxMaxExperts, "mx_grouped_gemm: nexperts=%d out of [1,%d]", nexperts, kMxMaxExperts);
   if (rows == 0) return FLUXB_OK;
+  FLUXB_REQUIRE(splits_dev != nullptr, "mx_grouped_gemm: NULL argument");
+  FLUXB_REQUIRE(static_cast<long long>(nexperts) * n < (1ll << 31) - 256, "mx_grouped_gemm: %d experts of %d columns are too many", nexperts, n);
   MxParams p;
   const int rc = mx_fill("mx_grouped_gemm", comm, p, xq, xs, xs_pitch, wq, ws, ws_pitch, out, n, k, out_dtype);
   if (rc != FLUXB_OK) return rc;
-  FLUXB_REQUIRE(splits_dev != nullptr, "mx_grouped_gemm: NULL argument");
-  FLUXB_REQUIRE(static_cast<long long>(nexperts) * n < (1ll << 31) - 256, "mx_grouped_gemm: %d experts of %d columns are too many", nexperts, n);
   p.rows_w = nexperts * n;
   p.rows_x = rows;
   p.nexperts = nexperts;
