@@ -108,10 +108,12 @@ SIGNATURES = {
     "fluxb_moe_permute": (_i, [_vp, _i, _i, _ll, _vp, _i, _vp, _vp, _vp]),
     "fluxb_moe_unpermute": (_i, [_vp, _i, _i, _i, _i, _vp, _vp, _i, _vp, _vp]),
     "fluxb_moe_unpermute_backward": (_i, [_vp, _vp, _i, _i, _i, _i, _vp, _i, _vp, _vp, _i, _vp, _vp, _vp]),
-    "fluxb_mx_quantize": (_i, [_vp, _i, _i, _i, _ll, _vp, _vp, _ll, _vp, _i, _vp, _i, _vp]),
-    "fluxb_mx_dequantize": (_i, [_vp, _vp, _ll, _i, _i, _i, _vp, _vp]),
-    "fluxb_mx_gemm": (_i, [_vp, _vp, _vp, _ll, _vp, _vp, _ll, _vp, _i, _i, _i, _i, _vp, _tun, _vp]),
-    "fluxb_mx_grouped_gemm": (_i, [_vp, _vp, _vp, _ll, _i, _vp, _vp, _ll, _i, _vp, _vp, _i, _i, _i, _tun, _vp]),
+    "fluxb_mx_scale_bytes": (_sz, [_i, _i, _i]),
+    "fluxb_mx_grouped_workspace_bytes": (_sz, [_i, _i, _i]),
+    "fluxb_mx_quantize": (_i, [_vp, _i, _i, _i, _i, _ll, _vp, _vp, _vp, _i, _vp, _i, _vp]),
+    "fluxb_mx_dequantize": (_i, [_vp, _vp, _i, _i, _i, _i, _vp, _vp]),
+    "fluxb_mx_gemm": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _vp, _tun, _vp]),
+    "fluxb_mx_grouped_gemm": (_i, [_vp, _vp, _vp, _i, _vp, _vp, _i, _vp, _vp, _i, _i, _i, _vp, _tun, _vp]),
     "fluxb_moe_ag_scatter_workspace_bytes": (_sz, [_i, _i, _i, _i, _i]),
     "fluxb_moe_ag_scatter_create": (_i, [_vp, _i, _i, _i, _i, _i, _i, _i, _pp, _pp, _vp, _pp]),
     "fluxb_moe_ag_scatter_destroy": (_i, [_vp]),

@@ -172,6 +172,9 @@ int encode_tmap_2d(CUtensorMap* out, const void* base, int elt_dtype, long long 
 int encode_tmap_kn(CUtensorMap* out, const void* base, int elt_dtype, long long k, long long n, long long ld_bytes,
                    int box_k);
 
+// Rows of 32-bit words [rows, words] read as `box_rows` rows x 256 words, one after the other (no swizzle)
+int encode_tmap_words(CUtensorMap* out, const void* base, long long rows, long long words, int box_rows);
+
 // fp32 [rows, n] row-major matrix, 32 x 32 element boxes, 128-byte swizzle (reduce-scatter pushes)
 int encode_tmap_f32_store(CUtensorMap* out, const void* base, long long rows, long long n);
 int encode_tmap_b16_store(CUtensorMap* out, const void* base, long long rows, long long n);

@@ -102,34 +102,49 @@ static int mx_out_type(int out_dtype, int* ot) {
   }
 }
 
-// `per_group` = tokens that an expert gets on average (dense: all of them), `groups` = experts (dense: 1)
+// Scale blocks that a grouped launch's tokens can need: an expert without tokens needs none, one with tokens at most one
+// more than they fill (the same for tiles of `rows_per` tokens).
+static long long mx_most_blocks(int rows, int nexperts, int rows_per) { return static_cast<long long>(rows) / rows_per + (nexperts < rows ? nexperts : rows); }
+
+// `per_group` = tokens that an expert gets on average (dense: all of them)
 template <bool GROUPED>
-static int mx_run(fluxb_comm* comm, MxParams& p, const void* xq, const void* wq, int k, int per_group, int groups, const fluxb_tuning* tuning,
-                  cudaStream_t stream) {
+static int mx_run(fluxb_comm* comm, MxParams& p, const void* xq, const void* wq, const void* ws, void* workspace, int k, int per_group,
+                  const fluxb_tuning* tuning, cudaStream_t stream) {
   const int want_bn = tuning != nullptr ? tuning->block_n : 0, want_cg = tuning != nullptr ? tuning->cta_group : 0;
   const long long row_bytes = k / 2;
   const bool few = want_cg == 0 && (want_bn != 0 ? want_bn <= 128 : per_group <= 128);
   int bn = want_bn, cg = want_cg;
   if (few) {
     if (bn == 0) bn = per_group <= 16 ? 16 : per_group <= 32 ? 32 : per_group <= 64 ? 64 : 128;
+    // the scales of a tile must start at an even column of tensor memory, that is at a multiple of 64 rows of a block
+    // (an odd column raised a misaligned address); a grouped launch moves its tokens' scales to the tile's start
+    FLUXB_REQUIRE(GROUPED || bn >= 64 || p.rows_x <= bn, "mx_gemm: block_n=%d is for up to %d tokens", bn, bn);
     cg = 1;
   } else {
     if (cg == 0) cg = 2;
-    if (bn == 0) bn = 192;
+    if (bn == 0) bn = 256;
   }
   const int tile_n = cg * kBM;
+  const int groups = GROUPED ? p.nexperts : 1;
   p.n_tiles = (p.N + tile_n - 1) / tile_n;
   p.m_tiles = (p.rows_x + bn - 1) / bn;
-  // (an expert without tokens needs none, one with tokens at most one more than they fill)
-  const long long most_token_tiles = GROUPED ? static_cast<long long>(p.rows_x) / bn + (groups < p.rows_x ? groups : p.rows_x) : p.m_tiles;
-  const long long tiles = most_token_tiles * p.n_tiles;
+  p.w_blocks = (p.N + 127) / 128;
+  const long long tiles = (GROUPED ? mx_most_blocks(p.rows_x, groups, bn) : p.m_tiles) * p.n_tiles;
   FLUXB_REQUIRE(tiles < (1ll << 27), "mx_gemm: %d rows x %d columns have too many tiles", p.rows_x, p.N);
   p.band = tuning != nullptr && tuning->group_m > 0 ? tuning->group_m : 8;
   if (p.band > p.n_tiles) p.band = p.n_tiles;
-  int rc = encode_tmap_2d(&p.tmap_w, wq, FLUXB_S8, p.rows_w, row_bytes, row_bytes, kBM);
+  const long long words = static_cast<long long>(p.groups) * (kMxSfBytes / 4);
+  int rc = encode_tmap_2d(&p.tmap_w, wq, FLUXB_S8, static_cast<long long>(groups) * p.N, row_bytes, row_bytes, kBM);
   if (rc != FLUXB_OK) return rc;
   rc = encode_tmap_2d(&p.tmap_x, xq, FLUXB_S8, p.rows_x, row_bytes, row_bytes, bn / cg);
   if (rc != FLUXB_OK) return rc;
+  rc = encode_tmap_words(&p.tmap_sw, ws, static_cast<long long>(groups) * p.w_blocks, words, 1);
+  if (rc != FLUXB_OK) return rc;
+  if (!GROUPED || !few) {
+    const void* blocks = GROUPED ? workspace : p.sx;
+    rc = encode_tmap_words(&p.tmap_sx, blocks, GROUPED ? mx_most_blocks(p.rows_x, groups, 128) : (p.rows_x + 127) / 128, words, (bn + 127) / 128);
+    if (rc != FLUXB_OK) return rc;
+  }
   if (few) {
     p.split = mx_few_split(comm->sm_count, GROUPED ? static_cast<long long>(groups) * p.n_tiles : tiles, p.num_kb, bn);
     switch (bn) {
@@ -140,43 +155,38 @@ static int mx_run(fluxb_comm* comm, MxParams& p, const void* xq, const void* wq,
       default: FLUXB_FAIL(FLUXB_ERR_INVALID, "mx_gemm: block_n=%d not in {16,32,64,128} for few tokens", bn);
     }
   }
+  FLUXB_REQUIRE(cg == 2 ? bn == 64 || bn == 128 || bn == 192 || bn == 256 : cg == 1 && (bn == 64 || bn == 128),
+                "mx_gemm: block_n=%d cta_group=%d is not {64,128} with 1 or {64,128,192,256} with 2", bn, cg);
+  if (GROUPED) {
+    rc = launch_pdl(mx_regroup_kernel, static_cast<int>(mx_most_blocks(p.rows_x, groups, 128)), kMxRegroupThreads, stream, p.sx, p.rows_x, p.groups,
+                    p.splits, p.nexperts, static_cast<uint4*>(workspace));
+    if (rc != FLUXB_OK) return rc;
+  }
   const int num_ctas = tuning != nullptr ? tuning->num_ctas : 0;
   if (cg == 2) switch (bn) {
       case 64: return launch_mx_tiles<64, true, GROUPED>(comm, p, tiles, num_ctas, stream);
       case 128: return launch_mx_tiles<128, true, GROUPED>(comm, p, tiles, num_ctas, stream);
       case 192: return launch_mx_tiles<192, true, GROUPED>(comm, p, tiles, num_ctas, stream);
-      case 224: return launch_mx_tiles<224, true, GROUPED>(comm, p, tiles, num_ctas, stream);
-      default: FLUXB_FAIL(FLUXB_ERR_INVALID, "mx_gemm: block_n=%d not in {64,128,192,224} for CTA pairs", bn);
+      default: return launch_mx_tiles<256, true, GROUPED>(comm, p, tiles, num_ctas, stream);
     }
-  FLUXB_REQUIRE(cg == 1, "mx_gemm: cta_group=%d is not 1 or 2", cg);
-  switch (bn) {
-    case 64: return launch_mx_tiles<64, false, GROUPED>(comm, p, tiles, num_ctas, stream);
-    case 128: return launch_mx_tiles<128, false, GROUPED>(comm, p, tiles, num_ctas, stream);
-    default: FLUXB_FAIL(FLUXB_ERR_INVALID, "mx_gemm: block_n=%d not in {64,128} for single CTAs", bn);
-  }
+  return bn == 64 ? launch_mx_tiles<64, false, GROUPED>(comm, p, tiles, num_ctas, stream) : launch_mx_tiles<128, false, GROUPED>(comm, p, tiles, num_ctas, stream);
 }
 
-static int mx_fill(const char* who, fluxb_comm* comm, MxParams& p, const void* xq, const void* xs, long long xs_pitch, const void* wq, const void* ws,
-                   long long ws_pitch, const void* out, int n, int k, int out_dtype) {
+static int mx_fill(const char* who, fluxb_comm* comm, MxParams& p, const void* xq, const void* xs, const void* wq, const void* ws, const void* out, int n, int k,
+                   int out_dtype) {
   FLUXB_REQUIRE(comm != nullptr && xq != nullptr && xs != nullptr && wq != nullptr && ws != nullptr && out != nullptr, "%s: NULL argument", who);
   FLUXB_REQUIRE(k >= kMxBlock && k % kMxBlock == 0, "%s: k=%d must be a multiple of %d", who, k, kMxBlock);
   FLUXB_REQUIRE(n >= 1, "%s: n=%d invalid", who, n);
-  const long long least = static_cast<long long>((k + 2 * kMxStageK - 1) / (2 * kMxStageK)) * 16;
-  FLUXB_REQUIRE(xs_pitch >= least && ws_pitch >= least && xs_pitch % 16 == 0 && ws_pitch % 16 == 0,
-                "%s: rows of scales must be a multiple of 16 bytes apart, at least %lld (they are %lld and %lld)", who, least, xs_pitch, ws_pitch);
   FLUXB_REQUIRE(((reinterpret_cast<uintptr_t>(xq) | reinterpret_cast<uintptr_t>(xs) | reinterpret_cast<uintptr_t>(wq) | reinterpret_cast<uintptr_t>(ws)) & 15) == 0,
                 "%s: operands and their scales must be 16-byte aligned", who);
   memset(&p, 0, sizeof(p));
   int rc = mx_out_type(out_dtype, &p.out_type);
   if (rc != FLUXB_OK) return rc;
   FLUXB_REQUIRE((reinterpret_cast<uintptr_t>(out) & (p.out_type == kOutF32 ? 3 : 1)) == 0, "%s: the output is not aligned to its type", who);
-  p.sw = static_cast<const uint8_t*>(ws);
   p.sx = static_cast<const uint8_t*>(xs);
-  p.spw = ws_pitch;
-  p.spx = xs_pitch;
   p.N = n;
   p.num_kb = (k + kMxStageK - 1) / kMxStageK;
-  p.ksc = k / kMxBlock;
+  p.groups = (k + kMxGroupK - 1) / kMxGroupK;
   p.out = const_cast<void*>(out);
   p.ldo = n;
   p.timeout_ns = comm->timeout_ns;
@@ -190,37 +200,46 @@ using namespace fluxb;
 
 extern "C" {
 
-int fluxb_mx_gemm(fluxb_comm_t comm, const void* xq, const void* xs, long long xs_pitch, const void* wq, const void* ws, long long ws_pitch,
-                  void* out, int m, int n, int k, int out_dtype, const void* bias, const fluxb_tuning* tuning, fluxb_stream_t stream) {
+size_t fluxb_mx_scale_bytes(int batch, int rows, int k) {
+  if (batch < 0 || rows < 0 || k < 0) return 0;
+  return static_cast<size_t>(batch) * ((static_cast<size_t>(rows) + 127) / 128) * ((static_cast<size_t>(k) + kMxGroupK - 1) / kMxGroupK) * kMxSfBytes;
+}
+
+size_t fluxb_mx_grouped_workspace_bytes(int rows, int nexperts, int k) {
+  if (rows < 0 || nexperts < 0 || k < 0) return 0;
+  return static_cast<size_t>(mx_most_blocks(rows, nexperts, 128)) * ((static_cast<size_t>(k) + kMxGroupK - 1) / kMxGroupK) * kMxSfBytes;
+}
+
+int fluxb_mx_gemm(fluxb_comm_t comm, const void* xq, const void* xs, const void* wq, const void* ws, void* out, int m, int n, int k, int out_dtype,
+                  const void* bias, const fluxb_tuning* tuning, fluxb_stream_t stream) {
   FLUXB_REQUIRE(m >= 0, "mx_gemm: m=%d invalid", m);
   if (m == 0) return FLUXB_OK;
   MxParams p;
-  const int rc = mx_fill("mx_gemm", comm, p, xq, xs, xs_pitch, wq, ws, ws_pitch, out, n, k, out_dtype);
+  const int rc = mx_fill("mx_gemm", comm, p, xq, xs, wq, ws, out, n, k, out_dtype);
   if (rc != FLUXB_OK) return rc;
   FLUXB_REQUIRE((reinterpret_cast<uintptr_t>(bias) & (p.out_type == kOutF32 ? 3 : 1)) == 0, "mx_gemm: the bias is not aligned to its type");
-  p.rows_w = n;
   p.rows_x = m;
   p.bias = bias;
-  return mx_run<false>(comm, p, xq, wq, k, m, 1, tuning, static_cast<cudaStream_t>(stream));
+  return mx_run<false>(comm, p, xq, wq, ws, nullptr, k, m, tuning, static_cast<cudaStream_t>(stream));
 }
 
-int fluxb_mx_grouped_gemm(fluxb_comm_t comm, const void* xq, const void* xs, long long xs_pitch, int rows, const void* wq, const void* ws,
-                          long long ws_pitch, int nexperts, const int* splits_dev, void* out, int n, int k, int out_dtype,
-                          const fluxb_tuning* tuning, fluxb_stream_t stream) {
+int fluxb_mx_grouped_gemm(fluxb_comm_t comm, const void* xq, const void* xs, int rows, const void* wq, const void* ws, int nexperts,
+                          const int* splits_dev, void* out, int n, int k, int out_dtype, void* workspace, const fluxb_tuning* tuning,
+                          fluxb_stream_t stream) {
   FLUXB_REQUIRE(rows >= 0, "mx_grouped_gemm: rows=%d invalid", rows);
   FLUXB_REQUIRE(nexperts >= 1 && nexperts <= kMxMaxExperts, "mx_grouped_gemm: nexperts=%d out of [1,%d]", nexperts, kMxMaxExperts);
   if (rows == 0) return FLUXB_OK;
-  FLUXB_REQUIRE(splits_dev != nullptr, "mx_grouped_gemm: NULL argument");
+  FLUXB_REQUIRE(splits_dev != nullptr && workspace != nullptr, "mx_grouped_gemm: NULL argument");
+  FLUXB_REQUIRE((reinterpret_cast<uintptr_t>(workspace) & 15) == 0, "mx_grouped_gemm: the workspace must be 16-byte aligned");
   FLUXB_REQUIRE(static_cast<long long>(nexperts) * n < (1ll << 31) - 256, "mx_grouped_gemm: %d experts of %d columns are too many", nexperts, n);
   MxParams p;
-  const int rc = mx_fill("mx_grouped_gemm", comm, p, xq, xs, xs_pitch, wq, ws, ws_pitch, out, n, k, out_dtype);
+  const int rc = mx_fill("mx_grouped_gemm", comm, p, xq, xs, wq, ws, out, n, k, out_dtype);
   if (rc != FLUXB_OK) return rc;
-  p.rows_w = nexperts * n;
   p.rows_x = rows;
   p.nexperts = nexperts;
   p.splits = splits_dev;
   const int used = nexperts < rows ? nexperts : rows;
-  return mx_run<true>(comm, p, xq, wq, k, (rows + used - 1) / used, nexperts, tuning, static_cast<cudaStream_t>(stream));
+  return mx_run<true>(comm, p, xq, wq, ws, workspace, k, (rows + used - 1) / used, tuning, static_cast<cudaStream_t>(stream));
 }
 
 }  // extern "C"

@@ -7,37 +7,41 @@
 // its N dimension is the tokens, 16 to 256 of them: a tile is as narrow as there are tokens, the weights of an expert
 // with few tokens are not multiplied with padding, and a ragged end costs columns instead of 128-row boxes.
 //
-// A stage holds 256 values of K of every row of the tile: 128 bytes (swizzled, TMA) and 8 scale bytes. The scales stay
-// row-major in memory ([rows, pitch] bytes), which any producer can write and any row offset can start at; the tensor
-// cores want them in tensor memory, row r of a block of 128 in lane r % 32 of column r / 32, in all four quadrants.
-// Loader warps (one per block of 128 rows) bring them: a lane reads its four rows' bytes and writes them as one 16-byte
-// piece to shared memory, from where tcgen05.cp spreads 512 bytes (128 rows x 4 scales) at a time.
+// A stage holds 256 values of K of every row of the tile: 128 bytes (swizzled, TMA) and 8 scale bytes. The tensor cores
+// want the scales in tensor memory, row r of a block of 128 in lane r % 32 of column r / 32, four scales a cell, in all four
+// quadrants: what tcgen05.cp makes of 512 consecutive bytes. Scales are kept that way in memory, too (mx_format.cuh),
+// so that a copy brings them and no thread touches them. That matters because shared memory is the bound of these
+// kernels: a stage of a 256 x 256 pair tile is 512 clocks of tensor work, and 32 KB written by the copies and 32 KB read by
+// the tensor cores take all of them at 128 bytes a clock; barriers and loads of other warps wait behind that. (With
+// row-major scales that warps rearranged, through shared memory or by tcgen05.st, 8192 x 28672 x 8192 took 757 us at best,
+// in tiles of 192.)
 #pragma once
 #include "gemm_kernel.cuh"
+#include "mx_format.cuh"
 
 namespace fluxb {
 
-constexpr int kMxBlock = 32;           // values that share a scale
-constexpr int kMxStageK = 256;         // values of K per stage: 128 bytes
+constexpr int kMxStageK = 256;  // values of K per stage: 128 bytes
 constexpr int kMxMaxExperts = 1024;
 constexpr int kMxEpiWarps = 8;
 
 struct MxParams {
-  CUtensorMap tmap_w;  // weights [rows_w, K / 2 bytes]: 128 rows x 128 bytes
-  CUtensorMap tmap_x;  // tokens [rows_x, K / 2 bytes]: this CTA's share of a tile's tokens x 128 bytes
-  const uint8_t* sw;   // scales, `spw` / `spx` bytes a row (multiples of 16)
-  const uint8_t* sx;
-  long long spw, spx;
-  int rows_w, rows_x;  // rows that exist: experts x N, tokens
-  int N, num_kb, ksc;  // ksc = K / 32: scale bytes of a row that mean something
+  CUtensorMap tmap_w;   // weights [rows_w, K / 2 bytes]: 128 rows x 128 bytes
+  CUtensorMap tmap_x;   // tokens [rows_x, K / 2 bytes]: this CTA's share of a tile's tokens x 128 bytes
+  CUtensorMap tmap_sw;  // scale blocks, a row for every 128 rows: 1 x 1024 bytes (two groups of K)
+  CUtensorMap tmap_sx;  // ... for all blocks of a tile; grouped: every expert's rows start a block
+  const uint8_t* sx;    // few-token kernel, grouped: the tokens' scale blocks in row order
+  int rows_x;           // tokens
+  int N, num_kb, groups;  // groups = ceil(K / 128)
   int n_tiles, m_tiles, band;
-  int nexperts;        // grouped: experts, else 0
-  const int* splits;   // grouped: tokens per expert
+  int w_blocks;         // grouped: scale blocks of an expert's weights
+  int nexperts;         // grouped: experts, else 0
+  const int* splits;    // grouped: tokens per expert
   int out_type;
   void* out;
   long long ldo;
-  const void* bias;    // [N] of the output's type, or null
-  int split;           // few-token kernel: CTAs that share a tile's K
+  const void* bias;     // [N] of the output's type, or null
+  int split;            // few-token kernel: CTAs that share a tile's K
   unsigned long long timeout_ns;
   int* status;
 };
@@ -80,70 +84,46 @@ __device__ __forceinline__ void umma_mxf4(uint32_t d, uint64_t a, uint64_t b, ui
         : "memory");
 }
 
-// Arrival that hands over shared memory written by this warp to the CTA of the pair that issues the UMMAs, and its wait.
-__device__ __forceinline__ void mbar_arrive_release_cluster(uint32_t cluster_addr) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
-}
-__device__ __forceinline__ bool mbar_try_wait_acquire_cluster(uint32_t bar, uint32_t parity) {
-  uint32_t ok;
-  asm volatile(
-      "{\n\t.reg .pred P;\n\t"
-      "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 P, [%1], %2, %3;\n\t"
-      "selp.u32 %0, 1, 0, P;\n\t}"
-      : "=r"(ok)
-      : "r"(bar), "r"(parity), "r"(20000u)
-      : "memory");
-  return ok != 0;
-}
-__device__ __forceinline__ bool mbar_wait_acquire_cluster(uint32_t bar, uint32_t parity, const AbortWord& ab, int code, uint64_t budget_ns) {
-  if (mbar_try_wait_acquire_cluster(bar, parity)) return true;
-  const uint64_t t0 = globaltimer_ns();
-  uint32_t n = 0;
-  while (!mbar_try_wait_acquire_cluster(bar, parity)) {
-    if ((++n & 31u) == 0u) {
-      if (abort_seen(ab)) return false;
-      if (globaltimer_ns() - t0 > budget_ns) {
-        abort_raise(ab, code);
-        return false;
-      }
-    }
-  }
-  return true;
-}
-
 template <int BN, bool CTA2>
 struct MxLayout {
   static constexpr int kABytes = kBM * kRowBytes;
   static constexpr int kBRows = CTA2 ? BN / 2 : BN;
   static constexpr int kBBytes = kBRows * kRowBytes;
-  static constexpr int kSfBlocks = 1 + (BN + 127) / 128;  // blocks of 128 rows: the weights', the tokens' (all of them, in both CTAs of a pair)
+  static constexpr int kXBlocks = (BN + 127) / 128;  // scale blocks of the tokens: all of them, in both CTAs of a pair
   static constexpr int kSfOffset = kABytes + kBBytes;
-  static constexpr int kStageBytes = kSfOffset + kSfBlocks * 1024;
-  static constexpr int kStagesFit = (200 * 1024) / kStageBytes;
+  static constexpr int kStageBytes = kSfOffset + (1 + kXBlocks) * 2 * kMxSfBytes;
+  static constexpr int kStagesFit = (212 * 1024) / kStageBytes;
   static constexpr int kStages = kStagesFit > 8 ? 8 : kStagesFit;
-  static constexpr int kSfCols = kSfBlocks * 8;  // tensor memory columns of a stage's scales
-  static constexpr int kSlotsFit = (512 - 2 * BN) / kSfCols;
+  // Tensor memory: two accumulators and the scales of kSlots stages (for each of a stage's two groups of K four columns of
+  // the weights and four for every 128 tokens). 2 x 256 columns leave no room for scales: there the second accumulator
+  // starts kOverlap columns early, on the last columns of the first, which the epilogue reads before all others.
+  static constexpr int kSfCols = 2 * 4 * (1 + kXBlocks);
+  static constexpr int kSlotsFit = BN == 256 ? 4 : (512 - 2 * BN) / kSfCols;
   static constexpr int kSlots = kSlotsFit > kStages ? kStages : kSlotsFit;
-  static constexpr int kColsUsed = 2 * BN + kSlots * kSfCols;
+  static constexpr int kOverlap = BN == 256 ? kSlots * kSfCols : 0;
+  static constexpr int kAcc1 = BN - kOverlap;            // first column of the second accumulator
+  static constexpr int kSf = 2 * BN - kOverlap;          // ... of the scales
+  static constexpr int kColsUsed = kSf + kSlots * kSfCols;
   static constexpr uint32_t kTmemCols = kColsUsed <= 64 ? 64 : kColsUsed <= 128 ? 128 : kColsUsed <= 256 ? 256 : 512;
   static constexpr int kNumBars = 2 * kStages + 5;
   static constexpr int kBarOffset = kStages * kStageBytes;
   static constexpr int kMiscOffset = kBarOffset + kNumBars * 8;
   static constexpr int kGroupOffset = kMiscOffset + 64;
-  static constexpr int kGroupBytes = (2 * kMxMaxExperts + 2) * 4;
+  static constexpr int kGroupBytes = (3 * kMxMaxExperts + 1) * 4;
   static constexpr int total(bool grouped) { return kGroupOffset + (grouped ? kGroupBytes : 0) + 1024; }
-  static constexpr int kThreads = 64 + 32 * kMxEpiWarps + 32 * kSfBlocks;
-  static_assert(kStageBytes % 1024 == 0 && kSlots >= 2 && kStages >= 3, "layout");
+  static constexpr int kThreads = 64 + 32 * kMxEpiWarps;
+  static_assert(kStageBytes % 1024 == 0 && kSlots >= 2 && kStages >= 3 && kColsUsed <= 512, "layout");
 };
 
-// The groups of a grouped launch in shared memory: first row of every expert and the running number of token tiles, made
-// by one warp. Splits that are negative or run past the rows that exist are cut, so that nothing outside is touched.
-__device__ __forceinline__ void mx_group_table(const MxParams& p, int bn, int* row_first, int* tile_end, int lane) {
+// One warp's walk over the experts, 32 at a time: first row and end of expert e0 + lane, its tiles of `bn` tokens and its
+// scale blocks, and the numbers of both before it. Splits that are negative or run past the rows that exist are cut, so
+// that nothing outside is touched.
+struct MxExperts {
   long long rows = 0;
-  int tiles = 0;
-  for (int e0 = 0; e0 < p.nexperts; e0 += 32) {
-    const int e = e0 + lane;
-    long long m = e < p.nexperts ? p.splits[e] : 0;
+  int tiles = 0, blocks = 0;
+  int first, end, tiles_end, tiles_mine, blocks_before;
+  __device__ __forceinline__ void next(const int* splits, int nexperts, int rows_x, int bn, int e0, int lane) {
+    long long m = e0 + lane < nexperts ? splits[e0 + lane] : 0;
     if (m < 0) m = 0;
     long long incl = m;
 #pragma unroll
@@ -151,29 +131,32 @@ __device__ __forceinline__ void mx_group_table(const MxParams& p, int bn, int* r
       const long long v = __shfl_up_sync(0xffffffffu, incl, off);
       if (lane >= off) incl += v;
     }
-    long long first = rows + incl - m, end = rows + incl;
-    if (first > p.rows_x) first = p.rows_x;
-    if (end > p.rows_x) end = p.rows_x;
-    const int mine = (static_cast<int>(end - first) + bn - 1) / bn;
-    int tincl = mine;
+    const long long f = rows + incl - m, e = rows + incl;
+    first = static_cast<int>(f < rows_x ? f : rows_x);
+    end = static_cast<int>(e < rows_x ? e : rows_x);
+    tiles_mine = (end - first + bn - 1) / bn;
+    const int blocks_mine = (end - first + 127) >> 7;
+    int ti = tiles_mine, bi = blocks_mine;
 #pragma unroll
     for (int off = 1; off < 32; off <<= 1) {
-      const int v = __shfl_up_sync(0xffffffffu, tincl, off);
-      if (lane >= off) tincl += v;
+      const int t = __shfl_up_sync(0xffffffffu, ti, off), b = __shfl_up_sync(0xffffffffu, bi, off);
+      if (lane >= off) {
+        ti += t;
+        bi += b;
+      }
     }
-    if (e < p.nexperts) {
-      row_first[e] = static_cast<int>(first);
-      tile_end[e] = tiles + tincl;
-    }
+    tiles_end = tiles + ti;
+    blocks_before = blocks + bi - blocks_mine;
     rows += __shfl_sync(0xffffffffu, incl, 31);
-    tiles += __shfl_sync(0xffffffffu, tincl, 31);
-    if (e0 + 32 >= p.nexperts && lane == 31) row_first[p.nexperts] = static_cast<int>(rows < p.rows_x ? rows : p.rows_x);
+    tiles += __shfl_sync(0xffffffffu, ti, 31);
+    blocks += __shfl_sync(0xffffffffu, bi, 31);
   }
-}
+};
 
-// One output tile: rows [w_row, ...) of the weight matrix (n0 of its expert), tokens [m0, m_end).
+// One output tile: rows w_row ... of the weight matrix (column n0 of its expert), tokens [m0, m_end), and where their scale
+// blocks are; x_col = columns (32 tokens each) of its first block that are before the tile.
 struct MxTile {
-  int n0, w_row, m0, m_end;
+  int n0, w_row, w_block, m0, m_end, x_block, x_col;
 };
 // A run of `m_tiles` token tiles x n_tiles weight tiles, in bands of `band` weight tiles whose tiles go along the tokens:
 // the tiles in flight cover about as many rows of one operand as of the other.
@@ -184,59 +167,39 @@ __device__ __forceinline__ void mx_raster(int t, int n_tiles, int m_tiles, int b
   m_idx = r / h;
   n_idx = b * band + r - m_idx * h;
 }
+struct MxGroups {  // of a grouped launch, in shared memory
+  int *row_first, *tile_end, *block_first;
+};
 template <int BN, bool GROUPED>
-__device__ __forceinline__ bool mx_tile(const MxParams& p, int tile_rows, int t, const int* row_first, const int* tile_end, MxTile& out) {
+__device__ __forceinline__ bool mx_tile(const MxParams& p, int tile_rows, int t, const MxGroups& g, MxTile& out) {
   int n_idx, m_idx;
   if (!GROUPED) {
     if (t >= p.n_tiles * p.m_tiles) return false;
     mx_raster(t, p.n_tiles, p.m_tiles, p.band, n_idx, m_idx);
     out.n0 = out.w_row = n_idx * tile_rows;
+    out.w_block = out.n0 >> 7;
     out.m0 = m_idx * BN;
     out.m_end = p.rows_x;
-    return true;
-  }
-  const int g = t / p.n_tiles;  // token tiles before this one, if all experts had whole ones: finds the expert
-  int lo = 0, hi = p.nexperts;
-  while (lo < hi) {
-    const int mid = (lo + hi) >> 1;
-    if (tile_end[mid] > g) hi = mid; else lo = mid + 1;
-  }
-  if (lo == p.nexperts) return false;
-  const int before = lo > 0 ? tile_end[lo - 1] : 0;
-  mx_raster(t - before * p.n_tiles, p.n_tiles, tile_end[lo] - before, p.band, n_idx, m_idx);
-  out.n0 = n_idx * tile_rows;
-  out.w_row = lo * p.N + out.n0;
-  out.m0 = row_first[lo] + m_idx * BN;
-  out.m_end = row_first[lo + 1];
-  return true;
-}
-
-// The scales of four rows (first + lane, + 32, + 64, + 96) for one stage: 8 bytes each, zero for rows past `rows` and for
-// bytes past the row's end (a scale of 255 there would make NaN of the zeros it meets).
-struct MxScales {
-  uint2 v[4];
-};
-__device__ __forceinline__ void mx_load_scales(MxScales& s, const uint8_t* base, long long pitch, int first, int rows, int kb, int ksc, int lane) {
-#pragma unroll
-  for (int q = 0; q < 4; ++q) {
-    const int r = first + q * 32 + lane;
-    s.v[q] = r < rows ? __ldg(reinterpret_cast<const uint2*>(base + r * pitch + kb * 8)) : make_uint2(0u, 0u);
-  }
-  const int left = ksc - kb * 8;
-  if (left < 8) {
-    const uint32_t m0 = left >= 4 ? 0xFFFFFFFFu : left > 0 ? (1u << (8 * left)) - 1u : 0u;
-    const uint32_t m1 = left > 4 ? (1u << (8 * (left - 4))) - 1u : 0u;
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      s.v[q].x &= m0;
-      s.v[q].y &= m1;
+    out.x_block = out.m0 >> 7;
+  } else {
+    const int gt = t / p.n_tiles;
+    int lo = 0, hi = p.nexperts;  // the expert whose token tiles hold this one
+    while (lo < hi) {
+      const int mid = (lo + hi) >> 1;
+      if (g.tile_end[mid] > gt) hi = mid; else lo = mid + 1;
     }
+    if (lo == p.nexperts) return false;
+    const int before = lo > 0 ? g.tile_end[lo - 1] : 0;
+    mx_raster(t - before * p.n_tiles, p.n_tiles, g.tile_end[lo] - before, p.band, n_idx, m_idx);
+    out.n0 = n_idx * tile_rows;
+    out.w_row = lo * p.N + out.n0;
+    out.w_block = lo * p.w_blocks + (out.n0 >> 7);
+    out.m0 = g.row_first[lo] + m_idx * BN;
+    out.m_end = g.row_first[lo + 1];
+    out.x_block = g.block_first[lo] + ((m_idx * BN) >> 7);
   }
-}
-__device__ __forceinline__ void mx_store_scales(const MxScales& s, uint32_t dst, int lane) {
-  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst + lane * 16), "r"(s.v[0].x), "r"(s.v[1].x), "r"(s.v[2].x), "r"(s.v[3].x) : "memory");
-  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst + 512 + lane * 16), "r"(s.v[0].y), "r"(s.v[1].y), "r"(s.v[2].y), "r"(s.v[3].y)
-               : "memory");
+  out.x_col = ((m_idx * BN) & 127) >> 5;
+  return true;
 }
 
 __device__ __forceinline__ float mx_bias(const MxParams& p, int n) {
@@ -267,14 +230,15 @@ __device__ __forceinline__ void mx_store_column(const MxParams& p, const uint32_
   }
 }
 
-// Persistent kernel. Warp 0: TMA; warp 1: tensor memory and UMMA; kMxEpiWarps epilogue warps, two per quadrant; then the
-// loader warps of the scales. Two accumulators: the epilogue of a tile overlaps the main loop of the next.
+// Persistent kernel. Warp 0: TMA; warp 1: tensor memory and UMMA; kMxEpiWarps epilogue warps, two per quadrant. Two
+// accumulators: the epilogue of a tile overlaps the main loop of the next.
 template <int BN, bool CTA2, bool GROUPED>
 __global__ void __launch_bounds__(MxLayout<BN, CTA2>::kThreads, 1)
 mx_gemm_kernel(const __grid_constant__ MxParams p) {
   using L = MxLayout<BN, CTA2>;
   constexpr int STAGES = L::kStages, SLOTS = L::kSlots;
   constexpr int TILE_N = CTA2 ? 2 * kBM : kBM;
+  constexpr bool OVERLAP = L::kOverlap > 0;
   static_assert(L::total(GROUPED) <= 232448, "shared memory budget exceeded");
 
   extern __shared__ uint8_t smem_raw[];
@@ -288,8 +252,10 @@ mx_gemm_kernel(const __grid_constant__ MxParams p) {
   const uint32_t bar_retired = bar_base + 8u * (2 * STAGES + 4);
   uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(smem + L::kMiscOffset);
   volatile int* s_abort = reinterpret_cast<volatile int*>(smem + L::kMiscOffset + 8);
-  int* row_first = reinterpret_cast<int*>(smem + L::kGroupOffset);
-  int* tile_end = row_first + kMxMaxExperts + 1;
+  MxGroups groups;
+  groups.row_first = reinterpret_cast<int*>(smem + L::kGroupOffset);
+  groups.tile_end = groups.row_first + kMxMaxExperts + 1;
+  groups.block_first = groups.tile_end + kMxMaxExperts;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int half = CTA2 ? static_cast<int>(cluster_ctarank()) : 0;
   const bool leader = half == 0;
@@ -300,10 +266,7 @@ mx_gemm_kernel(const __grid_constant__ MxParams p) {
 
   if (warp == 0 && elect_one()) {
     *s_abort = 0;
-    for (int s = 0; s < STAGES; ++s) {
-      mbar_init(bar_full(s), 1 + (CTA2 ? 2 : 1) * L::kSfBlocks);  // the copies and the loader warps (of both CTAs)
-      mbar_init(bar_empty(s), 1);
-    }
+    for (int s = 0; s < 2 * STAGES; ++s) mbar_init(bar_base + 8u * s, 1);
     for (int a = 0; a < 2; ++a) {
       mbar_init(bar_tfull(a), 1);
       mbar_init(bar_tempty(a), (CTA2 ? 2 : 1) * kMxEpiWarps);
@@ -312,6 +275,8 @@ mx_gemm_kernel(const __grid_constant__ MxParams p) {
     mbar_init_fence();
     tma_prefetch_desc(&p.tmap_w);
     tma_prefetch_desc(&p.tmap_x);
+    tma_prefetch_desc(&p.tmap_sw);
+    tma_prefetch_desc(&p.tmap_sx);
   }
   if (warp == 1) {
     if (CTA2) {
@@ -324,7 +289,16 @@ mx_gemm_kernel(const __grid_constant__ MxParams p) {
   }
   if (GROUPED && warp == 2) {
     pdl_wait();
-    mx_group_table(p, BN, row_first, tile_end, lane);
+    MxExperts x;
+    for (int e0 = 0; e0 < p.nexperts; e0 += 32) {
+      x.next(p.splits, p.nexperts, p.rows_x, BN, e0, lane);
+      if (e0 + lane < p.nexperts) {
+        groups.row_first[e0 + lane] = x.first;
+        groups.tile_end[e0 + lane] = x.tiles_end;
+        groups.block_first[e0 + lane] = x.blocks_before;
+      }
+    }
+    if (lane == 0) groups.row_first[p.nexperts] = static_cast<int>(x.rows < p.rows_x ? x.rows : p.rows_x);
   }
   tc_fence_before();
   if (CTA2) cluster_sync_all(); else __syncthreads();
@@ -342,24 +316,23 @@ mx_gemm_kernel(const __grid_constant__ MxParams p) {
       const uint32_t full0 = CTA2 ? mapa_u32(bar_full(0), 0) : bar_full(0);
       const bool arms = !CTA2 || leader;
       MxTile tl;
-      for (int t = worker; ok && mx_tile<BN, GROUPED>(p, TILE_N, t, row_first, tile_end, tl); t += workers) {
+      for (int t = worker; ok && mx_tile<BN, GROUPED>(p, TILE_N, t, groups, tl); t += workers) {
         const int wrow = tl.w_row + half * kBM, xrow = tl.m0 + half * L::kBRows;
         for (int kb = 0; kb < p.num_kb; ++kb) {
           if (!mbar_wait(bar_empty(stage), phase ^ 1u, ab, kStatusTimeoutSmemEmpty, budget)) {
             ok = false;
             break;
           }
-          if (arms) mbar_arrive_expect_tx(bar_full(stage), (CTA2 ? 2 : 1) * (L::kABytes + L::kBBytes));
+          if (arms) mbar_arrive_expect_tx(bar_full(stage), (CTA2 ? 2 : 1) * L::kStageBytes);
           const uint32_t fb = full0 + 8u * stage;
           const uint32_t sa = smem_base + stage * L::kStageBytes;
-          const int k = kb * kRowBytes;
-          if (CTA2) {
-            tma_load_2d_2cta(sa, &p.tmap_w, fb, k, wrow);
-            tma_load_2d_2cta(sa + L::kABytes, &p.tmap_x, fb, k, xrow);
-          } else {
-            tma_load_2d(sa, &p.tmap_w, fb, k, wrow);
-            tma_load_2d(sa + L::kABytes, &p.tmap_x, fb, k, xrow);
-          }
+          auto load = [&](uint32_t dst, const void* map, int x, int y) {
+            if (CTA2) tma_load_2d_2cta(dst, map, fb, x, y); else tma_load_2d(dst, map, fb, x, y);
+          };
+          load(sa, &p.tmap_w, kb * kRowBytes, wrow);
+          load(sa + L::kABytes, &p.tmap_x, kb * kRowBytes, xrow);
+          load(sa + L::kSfOffset, &p.tmap_sw, kb * 256, tl.w_block + half);
+          load(sa + L::kSfOffset + 2 * kMxSfBytes, &p.tmap_sx, kb * 256, tl.x_block);
           if (++stage == STAGES) {
             stage = 0;
             phase ^= 1u;
@@ -377,29 +350,30 @@ mx_gemm_kernel(const __grid_constant__ MxParams p) {
     if (leader && elect_one()) {
       const uint64_t a_desc0 = make_kmajor_sw128_desc(smem_base), b_desc0 = make_kmajor_sw128_desc(smem_base + L::kABytes);
       const uint64_t sf_desc0 = mx_sf_desc(smem_base + L::kSfOffset);
-      const uint32_t sf_tmem0 = tmem_base + 2 * BN;
       constexpr uint32_t UM = CTA2 ? 256 : 128;
-      int stage = 0, slot = 0, it = 0, done = 0;  // `done` = stages issued so far, up to SLOTS
+      int stage = 0, slot = 0, it = 0, issued = 0;
       uint32_t phase = 0;
-      int old_stage = 0;                          // the stage that used this slot last, and its phase
+      int old_stage = 0;  // the stage that used this slot of scales last, and its phase
       uint32_t old_phase = 0;
       bool ok = true;
       MxTile tl;
-      for (int t = worker; ok && mx_tile<BN, GROUPED>(p, TILE_N, t, row_first, tile_end, tl); t += workers, ++it) {
+      for (int t = worker; ok && mx_tile<BN, GROUPED>(p, TILE_N, t, groups, tl); t += workers, ++it) {
         const int acc = it & 1;
-        if (!mbar_wait<CTA2>(bar_tempty(acc), ((it >> 1) & 1) ^ 1u, ab, kStatusTimeoutTmemEmpty, budget)) break;
+        // its accumulator has been read; overlapping ones: the columns that the tile before shares with this one
+        // (and with them everything of the tile before that)
+        const bool free = OVERLAP ? it == 0 || mbar_wait<CTA2>(bar_tempty(0), (it - 1) & 1, ab, kStatusTimeoutTmemEmpty, budget)
+                                  : mbar_wait<CTA2>(bar_tempty(acc), ((it >> 1) & 1) ^ 1u, ab, kStatusTimeoutTmemEmpty, budget);
+        if (!free) break;
         tc_fence_after();
-        const uint32_t d = tmem_base + static_cast<uint32_t>(acc * BN);
+        const uint32_t d = tmem_base + static_cast<uint32_t>(acc * L::kAcc1);
         for (int kb = 0; kb < p.num_kb; ++kb) {
-          const bool full = CTA2 ? mbar_wait_acquire_cluster(bar_full(stage), phase, ab, kStatusTimeoutSmemFull, budget)
-                                 : mbar_wait(bar_full(stage), phase, ab, kStatusTimeoutSmemFull, budget);
-          if (!full) {
+          if (!mbar_wait(bar_full(stage), phase, ab, kStatusTimeoutSmemFull, budget)) {
             ok = false;
             break;
           }
-          // the scales' tensor memory is used again once the UMMAs that read it have retired
+          // the scales' columns are used again once the UMMAs that read them have retired
           if (SLOTS < STAGES) {
-            if (done == SLOTS) {
+            if (issued == SLOTS) {
               if (!mbar_wait(bar_empty(old_stage), old_phase, ab, kStatusTimeoutSmemEmpty, budget)) {
                 ok = false;
                 break;
@@ -409,22 +383,23 @@ mx_gemm_kernel(const __grid_constant__ MxParams p) {
                 old_phase ^= 1u;
               }
             } else {
-              ++done;
+              ++issued;
             }
           }
           tc_fence_after();
           const uint32_t off = static_cast<uint32_t>(stage) * (L::kStageBytes >> 4);
-          const uint32_t sf = sf_tmem0 + static_cast<uint32_t>(slot * L::kSfCols);
-          // columns: per group of 128 values of K, 4 of the weights and 4 for every block of 128 tokens
+          const uint32_t sf = tmem_base + static_cast<uint32_t>(L::kSf + slot * L::kSfCols);
+          constexpr int GC = 4 * (1 + L::kXBlocks);  // columns per group of K
 #pragma unroll
           for (int g = 0; g < 2; ++g)
 #pragma unroll
-            for (int b = 0; b < L::kSfBlocks; ++b)
-              mx_copy_sf<CTA2>(sf + (g * L::kSfBlocks + b) * 4, sf_desc0 + off + static_cast<uint32_t>((b * 1024 + g * 512) >> 4));
+            for (int b = 0; b < 1 + L::kXBlocks; ++b)
+              mx_copy_sf<CTA2>(sf + g * GC + b * 4, sf_desc0 + off + static_cast<uint32_t>((b * 2 + g) * (kMxSfBytes >> 4)));
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
-            const uint32_t sfa = sf + (k >> 1) * L::kSfBlocks * 4;
-            umma_mxf4<CTA2>(d, a_desc0 + off + 2u * k, b_desc0 + off + 2u * k, mx_idesc(UM, BN, (k & 1) * 2), sfa, sfa + 4, (kb > 0 || k > 0) ? 1u : 0u);
+            const uint32_t sfa = sf + (k >> 1) * GC;
+            umma_mxf4<CTA2>(d, a_desc0 + off + 2u * k, b_desc0 + off + 2u * k, mx_idesc(UM, BN, (k & 1) * 2), sfa,
+                            sfa + 4 + (BN % 128 == 0 ? 0 : tl.x_col), (kb > 0 || k > 0) ? 1u : 0u);
           }
           if (CTA2) umma_commit_2cta(bar_empty(stage), 3); else umma_commit(bar_empty(stage));
           if (++stage == STAGES) {
@@ -442,73 +417,42 @@ mx_gemm_kernel(const __grid_constant__ MxParams p) {
         mbar_wait(bar_retired, 0, AbortWord{nullptr, 0u}, 0, 2000000ull);
       }
     }
-  } else if (warp < 2 + kMxEpiWarps) {
+  } else {
     // ------------------------------------------------------------- epilogue
     const int quad = warp & 3, first = (warp - 2) >> 2;
     const uint32_t tmem_quad = tmem_base + (static_cast<uint32_t>(quad * 32) << 16);
     const uint32_t tempty0 = CTA2 ? mapa_u32(bar_tempty(0), 0) : bar_tempty(0);
-    constexpr int CH = BN < 32 ? BN : 32;
+    constexpr int CHUNKS = BN / 32, SHARED = L::kOverlap / 32;
+    static_assert(BN % 32 == 0 && L::kOverlap % 32 == 0, "chunks");
     int it = 0;
     MxTile tl;
-    for (int t = worker; mx_tile<BN, GROUPED>(p, TILE_N, t, row_first, tile_end, tl); t += workers, ++it) {
+    for (int t = worker; mx_tile<BN, GROUPED>(p, TILE_N, t, groups, tl); t += workers, ++it) {
       const int acc = it & 1;
       const int n = tl.n0 + half * kBM + quad * 32 + lane;
       const float bias = mx_bias(p, n);
       if (!__all_sync(0xffffffffu, mbar_wait(bar_tfull(acc), (it >> 1) & 1, ab, kStatusTimeoutTmemFull, budget, 100))) break;
       tc_fence_after();
-      const uint32_t tacc = tmem_quad + static_cast<uint32_t>(acc * BN);
-#pragma unroll 1
-      for (int c = first * CH; c < BN && tl.m0 + c < tl.m_end; c += 2 * CH) {
-        uint32_t r[CH];
-        if constexpr (CH == 16) tmem_ld_32x16(tacc + c, r); else tmem_ld_32x32(tacc + c, r);
-        tmem_ld_wait();
-        mx_store_column<CH>(p, r, tl.m0 + c, tl.m_end - tl.m0 - c, n, bias);
-      }
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) {
-        if (CTA2) mbar_arrive_cluster(tempty0 + 8u * acc); else mbar_arrive(tempty0 + 8u * acc);
-      }
-    }
-  } else {
-    // --------------------------------------------------------------- scales
-    const int b = warp - 2 - kMxEpiWarps;  // block 0: the weights' rows of this CTA, then 128 tokens each
-    const uint32_t full0 = CTA2 ? mapa_u32(bar_full(0), 0) : bar_full(0);
-    const uint8_t* base = b == 0 ? p.sw : p.sx;
-    const long long pitch = b == 0 ? p.spw : p.spx;
-    const int rows_all = b == 0 ? p.rows_w : p.rows_x;
-    constexpr int UN = 4;  // stages whose loads are in flight together
-    int stage = 0;
-    uint32_t phase = 0;
-    bool ok = true;
-    MxTile tl;
-    for (int t = worker; ok && mx_tile<BN, GROUPED>(p, TILE_N, t, row_first, tile_end, tl); t += workers) {
-      const int first = b == 0 ? tl.w_row + half * kBM : tl.m0 + (b - 1) * 128;
-      const int rows = b == 0 ? rows_all : (rows_all < tl.m0 + BN ? rows_all : tl.m0 + BN);
-      for (int kb0 = 0; ok && kb0 < p.num_kb; kb0 += UN) {
-        MxScales s[UN];
-#pragma unroll
-        for (int u = 0; u < UN; ++u)
-          if (kb0 + u < p.num_kb) mx_load_scales(s[u], base, pitch, first, rows, kb0 + u, p.ksc, lane);
-#pragma unroll
-        for (int u = 0; u < UN; ++u) {
-          if (kb0 + u >= p.num_kb || !ok) break;
-          if (!__all_sync(0xffffffffu, mbar_wait(bar_empty(stage), phase ^ 1u, ab, kStatusTimeoutSmemEmpty, budget))) {
-            ok = false;
-            break;
-          }
-          mx_store_scales(s[u], smem_base + stage * L::kStageBytes + L::kSfOffset + b * 1024, lane);
-          fence_proxy_async_smem();
-          __syncwarp();
-          if (lane == 0) {
-            if (CTA2) mbar_arrive_release_cluster(full0 + 8u * stage); else mbar_arrive(full0 + 8u * stage);
-          }
-          if (++stage == STAGES) {
-            stage = 0;
-            phase ^= 1u;
-          }
+      const uint32_t tacc = tmem_quad + static_cast<uint32_t>(acc * L::kAcc1);
+      auto give_back = [&] {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          const uint32_t bar = tempty0 + (OVERLAP ? 0u : 8u * acc);
+          if (CTA2) mbar_arrive_cluster(bar); else mbar_arrive(bar);
         }
+      };
+#pragma unroll 1
+      for (int i = first; i < CHUNKS; i += 2) {
+        if (OVERLAP && (i == SHARED || i == SHARED + 1)) give_back();  // (its first chunk past the shared columns)
+        // the columns that the next tile's accumulator shares come first: the last ones of the first, the first of the second
+        const int c = (OVERLAP && acc == 0 ? CHUNKS - 1 - i : i) * 32;
+        if (tl.m0 + c >= tl.m_end) continue;
+        uint32_t r[32];
+        tmem_ld_32x32(tacc + c, r);
+        tmem_ld_wait();
+        mx_store_column<32>(p, r, tl.m0 + c, tl.m_end - tl.m0 - c, n, bias);
       }
+      if (!OVERLAP) give_back();
     }
   }
 
@@ -525,13 +469,55 @@ mx_gemm_kernel(const __grid_constant__ MxParams p) {
   }
 }
 
+// The tokens' scale blocks of a grouped launch: rows in the order of their experts, every expert's rows from a block's
+// start on. A CTA per block, as many as the experts could need; 16 bytes (four rows 32 apart) per thread and group of K.
+constexpr int kMxRegroupThreads = 256;
+__global__ void __launch_bounds__(kMxRegroupThreads)
+mx_regroup_kernel(const uint8_t* __restrict__ src, int rows, int groups, const int* __restrict__ splits, int nexperts, uint4* __restrict__ dst) {
+  __shared__ int s_first, s_end;
+  const int lane = threadIdx.x & 31;
+  pdl_wait();
+  if (threadIdx.x == 0) pdl_trigger();
+  if (threadIdx.x < 32) {
+    MxExperts x;
+    int first = 0, end = 0;
+    for (int e0 = 0; e0 < nexperts; e0 += 32) {
+      x.next(splits, nexperts, rows, 128, e0, lane);  // (tiles of 128 rows: blocks)
+      const unsigned has = __ballot_sync(0xffffffffu, x.tiles_end > static_cast<int>(blockIdx.x));
+      if (has == 0) continue;
+      const int from = __ffs(has) - 1;
+      first = __shfl_sync(0xffffffffu, x.first, from) + (static_cast<int>(blockIdx.x) - __shfl_sync(0xffffffffu, x.blocks_before, from)) * 128;
+      end = __shfl_sync(0xffffffffu, x.end, from);
+      break;
+    }
+    if (lane == 0) {
+      s_first = first;
+      s_end = end;
+    }
+  }
+  __syncthreads();
+  const int first = s_first, end = s_end;
+  if (first >= end) return;
+  for (int i = threadIdx.x; i < groups * 32; i += kMxRegroupThreads) {
+    const int kg = i >> 5;
+    uint32_t w[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const int r = first + q * 32 + lane;
+      w[q] = r < end ? __ldg(reinterpret_cast<const uint32_t*>(src + mx_sf_offset(r, kg, groups))) : 0u;
+    }
+    dst[(static_cast<long long>(blockIdx.x) * groups + kg) * 32 + lane] = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+}
+
 // ------------------------------------------------------------------------------------------------------- few tokens
 // Few tokens (up to 128, or a few per expert), where the time is that of reading the weights once and of getting started:
 // one output tile per cluster of `split` CTAs, which cut K. Each CTA leaves its accumulator in its own shared memory; after
 // a cluster barrier CTA r sums the tokens r * per ... of all parts, in rank order, through distributed shared memory: no
 // scratch, no counters, any number of launches side by side. A grouped launch has a cluster for every tile that the
-// experts could need (the counts are on the device); those that no expert needs leave at once.
-constexpr int kMxFewThreads = 256;  // warp 0 TMA, warp 1 UMMA + tensor memory, warps 2-5 read-out and output, 6-7 scales
+// experts could need (the counts are on the device); those that no expert needs leave at once. There a warp gathers the
+// tokens' scales, whose rows start anywhere in a block.
+constexpr int kMxFewThreads = 224;  // warp 0 TMA, warp 1 UMMA + tensor memory, warps 2-5 read-out and output, 6 scales of grouped tokens
 constexpr int kMxFewMaxSplit = 8;
 
 template <int BN>
@@ -539,7 +525,7 @@ struct MxFewLayout {
   static constexpr int kABytes = kBM * kRowBytes;
   static constexpr int kBBytes = BN * kRowBytes;
   static constexpr int kSfOffset = kABytes + kBBytes;
-  static constexpr int kStageBytes = kSfOffset + 2048;
+  static constexpr int kStageBytes = kSfOffset + 4 * kMxSfBytes;
   // up to 64 tokens a CTA takes half of an SM's shared memory, so that one CTA's prologue and reduction overlap another's loads
   static constexpr int kStages = BN == 16 ? 5 : BN <= 64 ? 4 : 6;
   static_assert(BN <= 128 && kStages * kStageBytes >= BN * kBM * 4, "the read-out must fit into the stages");
@@ -556,42 +542,20 @@ struct MxFewLayout {
 template <int BN>
 __device__ __forceinline__ bool mx_few_tile(const MxParams& p, int t, int lane, MxTile& out) {
   const int g = t / p.n_tiles;
-  long long rows = 0;
-  int tiles = 0;
+  MxExperts x;
   for (int e0 = 0; e0 < p.nexperts; e0 += 32) {
-    const int e = e0 + lane;
-    long long m = e < p.nexperts ? p.splits[e] : 0;
-    if (m < 0) m = 0;
-    long long incl = m;
-#pragma unroll
-    for (int off = 1; off < 32; off <<= 1) {
-      const long long v = __shfl_up_sync(0xffffffffu, incl, off);
-      if (lane >= off) incl += v;
-    }
-    long long first = rows + incl - m, end = rows + incl;
-    if (first > p.rows_x) first = p.rows_x;
-    if (end > p.rows_x) end = p.rows_x;
-    const int mine = (static_cast<int>(end - first) + BN - 1) / BN;
-    int tincl = mine;
-#pragma unroll
-    for (int off = 1; off < 32; off <<= 1) {
-      const int v = __shfl_up_sync(0xffffffffu, tincl, off);
-      if (lane >= off) tincl += v;
-    }
-    const unsigned has = __ballot_sync(0xffffffffu, tiles + tincl > g);
-    if (has != 0) {
-      const int src = __ffs(has) - 1;
-      const int f = __shfl_sync(0xffffffffu, static_cast<int>(first), src);
-      const int before = __shfl_sync(0xffffffffu, tiles + tincl - mine, src);
-      out.m_end = __shfl_sync(0xffffffffu, static_cast<int>(end), src);
-      const int n_idx = (t - before * p.n_tiles) % p.n_tiles, m_idx = g - before;
-      out.n0 = n_idx * kBM;
-      out.w_row = (e0 + src) * p.N + out.n0;
-      out.m0 = f + m_idx * BN;
-      return true;
-    }
-    rows += __shfl_sync(0xffffffffu, incl, 31);
-    tiles += __shfl_sync(0xffffffffu, tincl, 31);
+    x.next(p.splits, p.nexperts, p.rows_x, BN, e0, lane);
+    const unsigned has = __ballot_sync(0xffffffffu, x.tiles_end > g);
+    if (has == 0) continue;
+    const int from = __ffs(has) - 1;
+    const int before = __shfl_sync(0xffffffffu, x.tiles_end - x.tiles_mine, from);
+    out.n0 = (t - g * p.n_tiles) * kBM;
+    out.w_row = (e0 + from) * p.N + out.n0;
+    out.w_block = (e0 + from) * p.w_blocks + (out.n0 >> 7);
+    out.m0 = __shfl_sync(0xffffffffu, x.first, from) + (g - before) * BN;
+    out.m_end = __shfl_sync(0xffffffffu, x.end, from);
+    out.x_block = out.x_col = 0;
+    return true;
   }
   return false;
 }
@@ -661,7 +625,7 @@ mx_few_kernel(const __grid_constant__ MxParams p) {
   const uint32_t bar_done = bar_base + 8u * (2 * STAGES), bar_retired = bar_done + 8u;
   uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(smem + L::kMiscOffset);
   volatile int* s_abort = reinterpret_cast<volatile int*>(smem + L::kMiscOffset + 8);
-  volatile int* s_tile = reinterpret_cast<volatile int*>(smem + L::kMiscOffset + 16);  // n0, w_row, m0, m_end, K blocks
+  volatile int* s_tile = reinterpret_cast<volatile int*>(smem + L::kMiscOffset + 16);  // n0, m0, m_end, K blocks, x_col
   const AbortWord ab{s_abort, 0u};
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int split = p.split;
@@ -672,19 +636,20 @@ mx_few_kernel(const __grid_constant__ MxParams p) {
 
   auto load = [&](const MxTile& tl, int i, int stage) {  // K block i of this part
     const uint32_t bar = bar_base + 8u * stage, dst = smem_base + stage * L::kStageBytes;
-    const int k = (kb0 + i) * kRowBytes;
-    mbar_arrive_expect_tx(bar, L::kABytes + L::kBBytes);
-    tma_load_2d(dst, &p.tmap_w, bar, k, tl.w_row);
-    tma_load_2d(dst + L::kABytes, &p.tmap_x, bar, k, tl.m0);
+    mbar_arrive_expect_tx(bar, L::kABytes + L::kBBytes + (GROUPED ? 2 : 4) * kMxSfBytes);
+    tma_load_2d(dst, &p.tmap_w, bar, (kb0 + i) * kRowBytes, tl.w_row);
+    tma_load_2d(dst + L::kABytes, &p.tmap_x, bar, (kb0 + i) * kRowBytes, tl.m0);
+    tma_load_2d(dst + L::kSfOffset, &p.tmap_sw, bar, (kb0 + i) * 256, tl.w_block);
+    if (!GROUPED) tma_load_2d(dst + L::kSfOffset + 2 * kMxSfBytes, &p.tmap_sx, bar, (kb0 + i) * 256, tl.x_block);
   };
 
-  MxTile tl{0, 0, 0, 0};
+  MxTile tl{0, 0, 0, 0, 0, 0, 0};
   int nkb = kb1 - kb0;
   if (warp == 0) {
     if (elect_one()) {
       *s_abort = 0;
       for (int s = 0; s < STAGES; ++s) {
-        mbar_init(bar_base + 8u * s, 3);  // the copies and the two loader warps
+        mbar_init(bar_base + 8u * s, GROUPED ? 2 : 1);  // the copies and, grouped, the scale warp
         mbar_init(bar_base + 8u * (STAGES + s), 1);
       }
       mbar_init(bar_done, 1);
@@ -698,15 +663,18 @@ mx_few_kernel(const __grid_constant__ MxParams p) {
     } else {
       const int m_idx = tile / p.n_tiles;
       tl.n0 = tl.w_row = (tile - m_idx * p.n_tiles) * kBM;
+      tl.w_block = tl.n0 >> 7;
       tl.m0 = m_idx * BN;
       tl.m_end = p.rows_x;
+      tl.x_block = tl.m0 >> 7;
+      tl.x_col = (tl.m0 & 127) >> 5;
     }
     if (elect_one()) {
       s_tile[0] = tl.n0;
-      s_tile[1] = tl.w_row;
-      s_tile[2] = tl.m0;
-      s_tile[3] = tl.m_end;
-      s_tile[4] = nkb;
+      s_tile[1] = tl.m0;
+      s_tile[2] = tl.m_end;
+      s_tile[3] = nkb;
+      s_tile[4] = tl.x_col;
       // the first copies need no one else: they fly while tensor memory is allocated and the CTA meets
       for (int i = 0; i < STAGES && i < nkb; ++i) load(tl, i, i);
     }
@@ -721,10 +689,10 @@ mx_few_kernel(const __grid_constant__ MxParams p) {
   tc_fence_after();
   const uint32_t tmem_base = *tmem_holder;
   tl.n0 = s_tile[0];
-  tl.w_row = s_tile[1];
-  tl.m0 = s_tile[2];
-  tl.m_end = s_tile[3];
-  nkb = s_tile[4];
+  tl.m0 = s_tile[1];
+  tl.m_end = s_tile[2];
+  nkb = s_tile[3];
+  tl.x_col = s_tile[4];
   const int cnt = nkb == 0 ? 0 : imin(BN, tl.m_end - tl.m0);
   pdl_wait();  // (returns at once: warp 0 has been through it)
   if (threadIdx.x == 0) pdl_trigger();
@@ -764,15 +732,16 @@ mx_few_kernel(const __grid_constant__ MxParams p) {
           }
           tc_fence_after();
           const uint32_t off = static_cast<uint32_t>(stage) * (L::kStageBytes >> 4);
+          // (a slot of scales per stage: it is free when the stage is)
           const uint32_t sf = tmem_base + BN + static_cast<uint32_t>(stage * L::kSfCols);
 #pragma unroll
           for (int g = 0; g < 2; ++g)
 #pragma unroll
-            for (int b = 0; b < 2; ++b) mx_copy_sf<false>(sf + (g * 2 + b) * 4, sf_desc0 + off + static_cast<uint32_t>((b * 1024 + g * 512) >> 4));
+            for (int b = 0; b < 2; ++b) mx_copy_sf<false>(sf + (g * 2 + b) * 4, sf_desc0 + off + static_cast<uint32_t>((b * 2 + g) * (kMxSfBytes >> 4)));
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
             const uint32_t sfa = sf + (k >> 1) * 8;
-            umma_mxf4<false>(tmem_base, a_desc0 + off + 2u * k, b_desc0 + off + 2u * k, mx_idesc(128, BN, (k & 1) * 2), sfa, sfa + 4,
+            umma_mxf4<false>(tmem_base, a_desc0 + off + 2u * k, b_desc0 + off + 2u * k, mx_idesc(128, BN, (k & 1) * 2), sfa, sfa + 4 + tl.x_col,
                              (i > 0 || k > 0) ? 1u : 0u);
           }
           umma_commit(bar_base + 8u * (STAGES + stage));
@@ -806,18 +775,25 @@ mx_few_kernel(const __grid_constant__ MxParams p) {
         }
         tc_fence_before();
       }
-    } else {
-      const bool weights = warp == 6;
-      const int first = weights ? tl.w_row : tl.m0, rows = weights ? p.rows_w : tl.m0 + cnt;
+    } else if (GROUPED) {
+      // the scales of the tile's tokens, four rows (lane, lane + 32, ...) and two groups of K a stage
       constexpr int UN = 4;  // stages whose loads are in flight together
       int stage = 0;
       uint32_t phase = 1;
       bool ok = true;
       for (int i0 = 0; ok && i0 < nkb; i0 += UN) {
-        MxScales s[UN];
+        uint32_t w[UN][2][4];
 #pragma unroll
         for (int u = 0; u < UN; ++u)
-          if (i0 + u < nkb) mx_load_scales(s[u], weights ? p.sw : p.sx, weights ? p.spw : p.spx, first, rows, kb0 + i0 + u, p.ksc, lane);
+#pragma unroll
+          for (int g = 0; g < 2; ++g)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              const int kg = (kb0 + i0 + u) * 2 + g, r = q * 32 + lane;
+              w[u][g][q] = q * 32 < BN && r < cnt && i0 + u < nkb && kg < p.groups
+                               ? __ldg(reinterpret_cast<const uint32_t*>(p.sx + mx_sf_offset(tl.m0 + r, kg, p.groups)))
+                               : 0u;
+            }
 #pragma unroll
         for (int u = 0; u < UN; ++u) {
           if (i0 + u >= nkb || !ok) break;
@@ -825,7 +801,12 @@ mx_few_kernel(const __grid_constant__ MxParams p) {
             ok = false;
             break;
           }
-          mx_store_scales(s[u], smem_base + stage * L::kStageBytes + L::kSfOffset + (weights ? 0 : 1024), lane);
+          const uint32_t dst = smem_base + stage * L::kStageBytes + L::kSfOffset + 2 * kMxSfBytes + lane * 16;
+#pragma unroll
+          for (int g = 0; g < 2; ++g)
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst + g * kMxSfBytes), "r"(w[u][g][0]), "r"(w[u][g][1]), "r"(w[u][g][2]),
+                         "r"(w[u][g][3])
+                         : "memory");
           fence_proxy_async_smem();
           __syncwarp();
           if (lane == 0) mbar_arrive(bar_base + 8u * stage);

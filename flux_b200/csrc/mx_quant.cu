@@ -5,9 +5,10 @@
 // NaN has the scale 255, which makes all of it NaN.
 //
 // Bound by memory: 4 lanes share a block, 8 values each, so that a warp's loads are 512 contiguous bytes (16-bit types)
-// and its stores 128. Four such pieces of a thread are in flight together.
+// and its stores 128; the four scales of a cell (mx_format.cuh) are one store. Four such pieces of a thread are in flight
+// together.
 #include "internal.h"
-#include "mx_gemm.cuh"
+#include "mx_format.cuh"
 #include "plain_gemm.cuh"
 
 namespace fluxb {
@@ -18,18 +19,25 @@ constexpr int kQuantTailCtas = 148;
 
 struct QuantParams {
   const void* x;
-  long long ldx;      // elements between rows
-  int rows, units;    // units of 8 values in a row
-  FastDiv div;        // by units
-  long long total;    // rows * units
+  long long ldx;       // elements between rows
+  int rows, units;     // units of 8 values in a row
+  int groups;          // groups of 128 values in a row, started ones too: 16 units each
+  FastDiv div;         // by 16 * groups
+  FastDiv mat;         // by the rows of one matrix: every matrix starts a scale block
+  int row0;            // first row of this launch
   uint8_t* data;
   uint8_t* scales;
-  long long pitch;
   // quantised into the order of the experts: row t goes to the rows index[t, j]; else null
   const int* index;
   const int* splits;
   int topk, nexperts, main_ctas;
 };
+
+// row of the scale blocks that holds row r of the batch's matrices
+__device__ __forceinline__ long long quant_scale_row(const FastDiv& mat, int r) {
+  const int b = mat.quot(r);
+  return b * ((static_cast<long long>(mat.d) + 127) & ~127ll) + (r - b * static_cast<int>(mat.d));
+}
 
 // 8 values of one of the input types, 16 or 32 bytes
 template <class T>
@@ -107,14 +115,15 @@ mx_quantize_kernel(const __grid_constant__ QuantParams p, const int aligned) {
     for (int w = 0; w < kQuantThreads / 32; ++w) s += part[w];
     if (s < 0) s = 0;
     const long long rows = static_cast<long long>(p.rows) * p.topk;
-    for (long long r = s + static_cast<int>(blockIdx.x) - p.main_ctas; r < rows; r += static_cast<int>(gridDim.x) - p.main_ctas)
-      for (int u = threadIdx.x; u < p.units; u += kQuantThreads) {
-        reinterpret_cast<uint32_t*>(p.data)[r * p.units + u] = 0u;
-        if ((u & 3) == 0) p.scales[r * p.pitch + (u >> 2)] = 0;
-      }
+    for (long long r = s + static_cast<int>(blockIdx.x) - p.main_ctas; r < rows; r += static_cast<int>(gridDim.x) - p.main_ctas) {
+      for (int u = threadIdx.x; u < p.units; u += kQuantThreads) reinterpret_cast<uint32_t*>(p.data)[r * p.units + u] = 0u;
+      for (int g = threadIdx.x; g < p.groups; g += kQuantThreads) *reinterpret_cast<uint32_t*>(p.scales + mx_sf_offset(r, g, p.groups)) = 0u;
+    }
     return;
   }
   const int lane = threadIdx.x & 31;
+  const int per_row = p.groups * 16;
+  const long long total = static_cast<long long>(p.rows) * per_row;
   const long long u0 = static_cast<long long>(blockIdx.x) * (kQuantThreads * kQuantUnroll) + threadIdx.x;
   Eight<T> in[kQuantUnroll];
   int row[kQuantUnroll], unit[kQuantUnroll];
@@ -122,16 +131,18 @@ mx_quantize_kernel(const __grid_constant__ QuantParams p, const int aligned) {
   for (int i = 0; i < kQuantUnroll; ++i) {
     const long long u = u0 + i * kQuantThreads;
     row[i] = -1;
-    if (u < p.total) {
+    unit[i] = 0;
+    if (u < total) {
       row[i] = p.div.quot(static_cast<int>(u));
-      unit[i] = static_cast<int>(u) - row[i] * p.units;
-      eight_load(in[i], static_cast<const T*>(p.x) + row[i] * p.ldx + unit[i] * 8, aligned != 0);
+      unit[i] = static_cast<int>(u) - row[i] * per_row;
+      if (unit[i] < p.units) eight_load(in[i], static_cast<const T*>(p.x) + row[i] * p.ldx + unit[i] * 8, aligned != 0);
     }
   }
 #pragma unroll
   for (int i = 0; i < kQuantUnroll; ++i) {
+    const bool valid = row[i] >= 0 && unit[i] < p.units;
     float f[8];
-    if (row[i] >= 0) {
+    if (valid) {
       eight_floats(in[i], f);
     } else {
 #pragma unroll
@@ -152,15 +163,21 @@ mx_quantize_kernel(const __grid_constant__ QuantParams p, const int aligned) {
     uint32_t code = 0u, scale = 255u;
     if (field != 255u) {
       scale = field < 2u ? 0u : field - 2u;
-      const float inv = __uint_as_float((254u - scale) << 23);  // 2^(127 - scale): between 2^2 and 2^127, or 2^-125 and up
+      const float inv = __uint_as_float((254u - scale) << 23);  // 2^(127 - scale), from 2^-125 to 2^127
 #pragma unroll
       for (int j = 0; j < 8; ++j) f[j] *= inv;
       code = pack_e2m1(f);
     }
-    if (row[i] < 0) continue;
+    // the scales of 128 values (16 lanes, all of one row) as one word; those past the row's end are zero
+    uint32_t cell = valid ? scale << (2 * (lane & 12)) : 0u;
+    cell |= __shfl_xor_sync(0xffffffffu, cell, 4);
+    cell |= __shfl_xor_sync(0xffffffffu, cell, 8);
+    if (!valid) continue;
+    const int kg = unit[i] >> 4;
+    const bool writes_cell = (lane & 15) == 0;
     if (p.index == nullptr) {
-      reinterpret_cast<uint32_t*>(p.data)[static_cast<long long>(row[i]) * p.units + unit[i]] = code;
-      if ((lane & 3) == 0) p.scales[row[i] * p.pitch + (unit[i] >> 2)] = static_cast<uint8_t>(scale);
+      reinterpret_cast<uint32_t*>(p.data)[static_cast<long long>(p.row0 + row[i]) * p.units + unit[i]] = code;
+      if (writes_cell) *reinterpret_cast<uint32_t*>(p.scales + mx_sf_offset(quant_scale_row(p.mat, p.row0 + row[i]), kg, p.groups)) = cell;
     } else {
       const int* idx = p.index + static_cast<long long>(row[i]) * p.topk;
       const long long rows = static_cast<long long>(p.rows) * p.topk;
@@ -168,7 +185,7 @@ mx_quantize_kernel(const __grid_constant__ QuantParams p, const int aligned) {
         const long long r = __ldg(idx + j);
         if (r < 0 || r >= rows) continue;
         reinterpret_cast<uint32_t*>(p.data)[r * p.units + unit[i]] = code;
-        if ((lane & 3) == 0) p.scales[r * p.pitch + (unit[i] >> 2)] = static_cast<uint8_t>(scale);
+        if (writes_cell) *reinterpret_cast<uint32_t*>(p.scales + mx_sf_offset(r, kg, p.groups)) = cell;
       }
     }
   }
@@ -186,8 +203,8 @@ __device__ __forceinline__ __half mx_out(float v) { return __float2half_rn(v); }
 
 template <class T>
 __global__ void __launch_bounds__(kQuantThreads)
-mx_dequantize_kernel(const uint32_t* __restrict__ data, const uint8_t* __restrict__ scales, long long pitch, int units, FastDiv div,
-                     long long total, T* __restrict__ out) {
+mx_dequantize_kernel(const uint32_t* __restrict__ data, const uint8_t* __restrict__ scales, int row0, int units, int groups, const FastDiv div,
+                     const FastDiv mat, long long total, T* __restrict__ out) {
   pdl_wait();
   if (threadIdx.x == 0) pdl_trigger();
   const long long u0 = static_cast<long long>(blockIdx.x) * (kQuantThreads * kQuantUnroll) + threadIdx.x;
@@ -196,9 +213,9 @@ mx_dequantize_kernel(const uint32_t* __restrict__ data, const uint8_t* __restric
   for (int i = 0; i < kQuantUnroll; ++i) {
     const long long u = u0 + i * kQuantThreads;
     if (u < total) {
-      const int row = div.quot(static_cast<int>(u));
+      const int row = div.quot(static_cast<int>(u)), block = (static_cast<int>(u) - row * units) >> 2;
       code[i] = __ldg(data + u);
-      scale[i] = __ldg(scales + row * pitch + ((static_cast<int>(u) - row * units) >> 2));
+      scale[i] = __ldg(scales + mx_sf_offset(quant_scale_row(mat, row0 + row), block >> 2, groups) + (block & 3));
     }
   }
 #pragma unroll
@@ -228,89 +245,95 @@ static int mx_elt_bytes(int dt) { return dt == FLUXB_F32 ? 4 : dt == FLUXB_BF16 
 // Rows per launch: a unit's number is a 31-bit integer.
 static int mx_rows_per_launch(int units) { return static_cast<int>(((1ll << 31) - kQuantThreads * kQuantUnroll - 1) / units); }
 
+static int check_mx_matrices(const char* who, int batch, int rows, int k) {
+  FLUXB_REQUIRE(batch >= 0 && rows >= 0 && k >= kMxBlock && k % kMxBlock == 0, "%s: batch=%d rows=%d k=%d invalid (k must be a multiple of %d)", who, batch,
+                rows, k, kMxBlock);
+  FLUXB_REQUIRE(static_cast<long long>(batch) * rows < (1ll << 31), "%s: %d x %d rows are too many", who, batch, rows);
+  return FLUXB_OK;
+}
+
 }  // namespace fluxb
 
 using namespace fluxb;
 
 extern "C" {
 
-int fluxb_mx_quantize(const void* x, int dtype, int rows, int k, long long ldx, void* data, void* scales, long long scales_pitch,
-                      const int* splits_dev, int nexperts, const int* scatter_index_dev, int topk, fluxb_stream_t stream) {
+int fluxb_mx_quantize(const void* x, int dtype, int batch, int rows, int k, long long ldx, void* data, void* scales, const int* splits_dev,
+                      int nexperts, const int* scatter_index_dev, int topk, fluxb_stream_t stream) {
   const int eb = mx_elt_bytes(dtype);
   FLUXB_REQUIRE(eb != 0, "mx_quantize: the input must be fp32, bf16 or fp16");
-  FLUXB_REQUIRE(rows >= 0 && k >= kMxBlock && k % kMxBlock == 0, "mx_quantize: rows=%d k=%d invalid (k must be a multiple of %d)", rows, k, kMxBlock);
-  FLUXB_REQUIRE(scales_pitch >= k / kMxBlock, "mx_quantize: rows of scales are %lld bytes apart, fewer than they hold", scales_pitch);
+  int rc = check_mx_matrices("mx_quantize", batch, rows, k);
+  if (rc != FLUXB_OK) return rc;
   const bool scatter = scatter_index_dev != nullptr;
   FLUXB_REQUIRE(scatter == (splits_dev != nullptr), "mx_quantize: splits and scatter_index belong together");
-  FLUXB_REQUIRE(!scatter || (topk >= 1 && nexperts >= 1), "mx_quantize: topk=%d nexperts=%d invalid", topk, nexperts);
+  FLUXB_REQUIRE(!scatter || (batch == 1 && topk >= 1 && nexperts >= 1), "mx_quantize: batch=%d topk=%d nexperts=%d invalid", batch, topk, nexperts);
   FLUXB_REQUIRE(!scatter || static_cast<long long>(rows) * topk < (1ll << 30), "mx_quantize: too many routed rows");
-  if (rows == 0) return FLUXB_OK;
+  const int all = batch * rows;
+  if (all == 0) return FLUXB_OK;
   FLUXB_REQUIRE(x != nullptr && data != nullptr && scales != nullptr, "mx_quantize: NULL argument");
-  FLUXB_REQUIRE((reinterpret_cast<uintptr_t>(x) & (eb - 1)) == 0 && (reinterpret_cast<uintptr_t>(data) & 3) == 0,
-                "mx_quantize: the input must be aligned to its type, the packed values to 4 bytes");
-  const int units = k / 8;
-  const int most = mx_rows_per_launch(units);
-  FLUXB_REQUIRE(!scatter || rows <= most, "mx_quantize: too many values");
+  FLUXB_REQUIRE((reinterpret_cast<uintptr_t>(x) & (eb - 1)) == 0 && (reinterpret_cast<uintptr_t>(data) & 3) == 0 && (reinterpret_cast<uintptr_t>(scales) & 3) == 0,
+                "mx_quantize: the input must be aligned to its type, packed values and scales to 4 bytes");
+  QuantParams p;
+  memset(&p, 0, sizeof(p));
+  p.ldx = ldx;
+  p.units = k / 8;
+  p.groups = (k + kMxGroupK - 1) / kMxGroupK;
+  p.div.set(static_cast<uint32_t>(p.groups) * 16u);
+  p.mat.set(static_cast<uint32_t>(rows));
+  p.data = static_cast<uint8_t*>(data);
+  p.scales = static_cast<uint8_t*>(scales);
+  p.index = scatter_index_dev;
+  p.splits = splits_dev;
+  p.topk = topk;
+  p.nexperts = nexperts;
+  const int most = mx_rows_per_launch(p.groups * 16);
+  FLUXB_REQUIRE(!scatter || all <= most, "mx_quantize: too many values");
   const int aligned = ((reinterpret_cast<uintptr_t>(x) | static_cast<uintptr_t>(ldx * eb)) & 15) == 0 ? 1 : 0;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  for (int r0 = 0; r0 < rows; r0 += most) {
-    QuantParams p;
-    memset(&p, 0, sizeof(p));
-    p.x = static_cast<const uint8_t*>(x) + static_cast<long long>(r0) * ldx * eb;
-    p.ldx = ldx;
-    p.rows = rows - r0 < most ? rows - r0 : most;
-    p.units = units;
-    p.div.set(static_cast<uint32_t>(units));
-    p.total = static_cast<long long>(p.rows) * units;
-    p.data = static_cast<uint8_t*>(data) + static_cast<long long>(r0) * (k / 2);
-    p.scales = static_cast<uint8_t*>(scales) + r0 * scales_pitch;
-    p.pitch = scales_pitch;
-    p.index = scatter_index_dev;
-    p.splits = splits_dev;
-    p.topk = topk;
-    p.nexperts = nexperts;
-    p.main_ctas = static_cast<int>((p.total + kQuantThreads * kQuantUnroll - 1) / (kQuantThreads * kQuantUnroll));
+  for (long long r0 = 0; r0 < all; r0 += most) {
+    p.row0 = static_cast<int>(r0);
+    p.x = static_cast<const uint8_t*>(x) + r0 * ldx * eb;
+    p.rows = all - r0 < most ? static_cast<int>(all - r0) : most;
+    const long long total = static_cast<long long>(p.rows) * p.groups * 16;
+    p.main_ctas = static_cast<int>((total + kQuantThreads * kQuantUnroll - 1) / (kQuantThreads * kQuantUnroll));
     const long long out_rows = static_cast<long long>(rows) * topk;
     const int grid = p.main_ctas + (!scatter ? 0 : out_rows < kQuantTailCtas ? static_cast<int>(out_rows) : kQuantTailCtas);
-    const int rc = dtype == FLUXB_F32    ? launch_pdl(mx_quantize_kernel<float>, grid, kQuantThreads, s, p, aligned)
-                   : dtype == FLUXB_BF16 ? launch_pdl(mx_quantize_kernel<__nv_bfloat16>, grid, kQuantThreads, s, p, aligned)
-                                         : launch_pdl(mx_quantize_kernel<__half>, grid, kQuantThreads, s, p, aligned);
+    rc = dtype == FLUXB_F32    ? launch_pdl(mx_quantize_kernel<float>, grid, kQuantThreads, s, p, aligned)
+         : dtype == FLUXB_BF16 ? launch_pdl(mx_quantize_kernel<__nv_bfloat16>, grid, kQuantThreads, s, p, aligned)
+                               : launch_pdl(mx_quantize_kernel<__half>, grid, kQuantThreads, s, p, aligned);
     if (rc != FLUXB_OK) return rc;
-    if (rows - r0 <= most) break;
   }
   return FLUXB_OK;
 }
 
-int fluxb_mx_dequantize(const void* data, const void* scales, long long scales_pitch, int rows, int k, int out_dtype, void* out,
-                        fluxb_stream_t stream) {
+int fluxb_mx_dequantize(const void* data, const void* scales, int batch, int rows, int k, int out_dtype, void* out, fluxb_stream_t stream) {
   const int eb = mx_elt_bytes(out_dtype);
   FLUXB_REQUIRE(eb != 0, "mx_dequantize: the output must be fp32, bf16 or fp16");
-  FLUXB_REQUIRE(rows >= 0 && k >= kMxBlock && k % kMxBlock == 0, "mx_dequantize: rows=%d k=%d invalid (k must be a multiple of %d)", rows, k, kMxBlock);
-  FLUXB_REQUIRE(scales_pitch >= k / kMxBlock, "mx_dequantize: rows of scales are %lld bytes apart, fewer than they hold", scales_pitch);
-  if (rows == 0) return FLUXB_OK;
+  int rc = check_mx_matrices("mx_dequantize", batch, rows, k);
+  if (rc != FLUXB_OK) return rc;
+  const int all = batch * rows;
+  if (all == 0) return FLUXB_OK;
   FLUXB_REQUIRE(data != nullptr && scales != nullptr && out != nullptr, "mx_dequantize: NULL argument");
   FLUXB_REQUIRE((reinterpret_cast<uintptr_t>(data) & 3) == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0,
                 "mx_dequantize: the packed values must be 4-byte aligned, the output 16-byte");
-  const int units = k / 8;
+  const int units = k / 8, groups = (k + kMxGroupK - 1) / kMxGroupK;
   const int most = mx_rows_per_launch(units);
-  FastDiv div;
+  FastDiv div, mat;
   div.set(static_cast<uint32_t>(units));
+  mat.set(static_cast<uint32_t>(rows));
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  for (int r0 = 0; r0 < rows; r0 += most) {
-    const int n = rows - r0 < most ? rows - r0 : most;
-    const long long total = static_cast<long long>(n) * units;
-    const uint32_t* d = reinterpret_cast<const uint32_t*>(data) + static_cast<long long>(r0) * units;
-    const uint8_t* sc = static_cast<const uint8_t*>(scales) + r0 * scales_pitch;
-    uint8_t* o = static_cast<uint8_t*>(out) + static_cast<long long>(r0) * k * eb;
-    const int grid = static_cast<int>((total + kQuantThreads * kQuantUnroll - 1) / (kQuantThreads * kQuantUnroll));
-    const int rc =
-        out_dtype == FLUXB_F32    ? launch_pdl(mx_dequantize_kernel<float>, grid, kQuantThreads, s, d, sc, scales_pitch, units, div, total, reinterpret_cast<float*>(o))
-        : out_dtype == FLUXB_BF16 ? launch_pdl(mx_dequantize_kernel<__nv_bfloat16>, grid, kQuantThreads, s, d, sc, scales_pitch, units, div, total,
-                                               reinterpret_cast<__nv_bfloat16*>(o))
-                                  : launch_pdl(mx_dequantize_kernel<__half>, grid, kQuantThreads, s, d, sc, scales_pitch, units, div, total,
-                                               reinterpret_cast<__half*>(o));
+  const uint8_t* sc = static_cast<const uint8_t*>(scales);
+  for (long long r0 = 0; r0 < all; r0 += most) {
+    const long long total = (all - r0 < most ? all - r0 : most) * units;
+    const uint32_t* d = static_cast<const uint32_t*>(data) + r0 * units;
+    uint8_t* o = static_cast<uint8_t*>(out) + r0 * k * eb;
+    const int grid = static_cast<int>((total + kQuantThreads * kQuantUnroll - 1) / (kQuantThreads * kQuantUnroll)), row0 = static_cast<int>(r0);
+    rc = out_dtype == FLUXB_F32    ? launch_pdl(mx_dequantize_kernel<float>, grid, kQuantThreads, s, d, sc, row0, units, groups, div, mat, total, reinterpret_cast<float*>(o))
+         : out_dtype == FLUXB_BF16 ? launch_pdl(mx_dequantize_kernel<__nv_bfloat16>, grid, kQuantThreads, s, d, sc, row0, units, groups, div, mat, total,
+                                                reinterpret_cast<__nv_bfloat16*>(o))
+                                   : launch_pdl(mx_dequantize_kernel<__half>, grid, kQuantThreads, s, d, sc, row0, units, groups, div, mat, total,
+                                                reinterpret_cast<__half*>(o));
     if (rc != FLUXB_OK) return rc;
-    if (rows - r0 <= most) break;
   }
   return FLUXB_OK;
 }

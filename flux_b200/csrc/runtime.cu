@@ -81,6 +81,22 @@ int encode_tmap_kn(CUtensorMap* out, const void* base, int elt_dtype, long long 
   return FLUXB_OK;
 }
 
+int encode_tmap_words(CUtensorMap* out, const void* base, long long rows, long long words, int box_rows) {
+  EncodeTiledFn fn = get_encode_fn();
+  if (fn == nullptr) FLUXB_FAIL(FLUXB_ERR_CUDA, "cuTensorMapEncodeTiled is not available");
+  FLUXB_REQUIRE((reinterpret_cast<uintptr_t>(base) & 15) == 0 && words % 4 == 0 && rows > 0 && words > 0,
+                "word tensor map: base and row pitch must be 16-byte aligned (rows=%lld words=%lld)", rows, words);
+  cuuint64_t dims[2] = {static_cast<cuuint64_t>(words), static_cast<cuuint64_t>(rows)};
+  cuuint64_t strides[1] = {static_cast<cuuint64_t>(words) * 4};
+  cuuint32_t box[2] = {256, static_cast<cuuint32_t>(box_rows)};
+  cuuint32_t estr[2] = {1, 1};
+  CUresult r = fn(out, CU_TENSOR_MAP_DATA_TYPE_INT32, 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                  CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS)
+    FLUXB_FAIL(FLUXB_ERR_CUDA, "cuTensorMapEncodeTiled (words) failed with CUresult %d", static_cast<int>(r));
+  return FLUXB_OK;
+}
+
 int encode_tmap_f32_store(CUtensorMap* out, const void* base, long long rows, long long n) {
   EncodeTiledFn fn = get_encode_fn();
   if (fn == nullptr) FLUXB_FAIL(FLUXB_ERR_CUDA, "cuTensorMapEncodeTiled is not available");

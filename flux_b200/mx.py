@@ -37,42 +37,47 @@ def _comm() -> Comm:
     return c
 
 
-def _scale_pitch(k: int) -> int:
-    """Bytes between rows of scales: 16 for every 512 values, so that every stage of a product reads aligned pieces."""
-    return (k + 511) // 512 * 16
+def _blocks_shape(lead, rows: int, k: int):
+    return (*lead, (rows + 127) // 128, (k + 127) // 128, 512)
 
 
 class MXTensor:
-    """Values [..., K] as packed e2m1 and scales: `data` uint8 [..., K / 2], `scales` uint8 [..., K / 32]. The
-    constructor takes them as a checkpoint holds them and brings the scales into the layout that the products read (rows
-    a multiple of 16 bytes apart); `mx_quantize` makes them that way."""
+    """Matrices [..., N, K] as packed e2m1 values and scales. The constructor takes them as a checkpoint holds them, `data`
+    uint8 [..., N, K / 2] and `scales` uint8 [..., N, K / 32], and lays the scales out once, in the blocks of 128 rows x 4
+    scales that the tensor cores read (fluxb.h); `mx_quantize` makes them that way. `scales` gives them back row by row."""
 
-    __slots__ = ("data", "_scales", "k", "pitch")
+    __slots__ = ("data", "blocks", "k")
 
     def __init__(self, data: torch.Tensor, scales: torch.Tensor):
         _check(_on_device(data) and _on_device(scales), "MXTensor: data and scales must be on the current CUDA device")
         _check(data.dtype == torch.uint8 and scales.dtype == torch.uint8, "MXTensor: data and scales must be uint8")
         _check(data.dim() >= 2 and data.shape[-1] >= BLOCK // 2 and data.shape[-1] % (BLOCK // 2) == 0,
-               "MXTensor: data must be [..., K / 2] with K a multiple of 32")
+               "MXTensor: data must be [..., N, K / 2] with K a multiple of 32")
+        *lead, n, _ = data.shape
         k = data.shape[-1] * 2
-        if tuple(scales.shape) != (*data.shape[:-1], k // BLOCK):
-            raise RuntimeError(f"MXTensor: scales shape {tuple(scales.shape)} != {(*data.shape[:-1], k // BLOCK)}")
+        if tuple(scales.shape) != (*lead, n, k // BLOCK):
+            raise RuntimeError(f"MXTensor: scales shape {tuple(scales.shape)} != {(*lead, n, k // BLOCK)}")
         data = data.contiguous()
         if data.data_ptr() % 16:
             data = data.clone()
-        self.data, self.k, self.pitch = data, k, _scale_pitch(k)
-        self._scales = torch.zeros((*data.shape[:-1], self.pitch), dtype=torch.uint8, device=data.device)
-        self._scales[..., :k // BLOCK] = scales
+        shape = _blocks_shape(lead, n, k)
+        rows = torch.zeros((*lead, shape[-3] * 128, shape[-2] * 4), dtype=torch.uint8, device=data.device)
+        rows[..., :n, :k // BLOCK] = scales
+        # row = 128 block + 32 column + lane, scale = 4 group + s  ->  [block, group, lane, column, s]
+        self.blocks = rows.view(-1, shape[-3], 4, 32, shape[-2], 4).permute(0, 1, 4, 3, 2, 5).contiguous().view(shape)
+        self.data, self.k = data, k
 
     @classmethod
-    def _of(cls, data: torch.Tensor, padded_scales: torch.Tensor, k: int) -> "MXTensor":
+    def _of(cls, data: torch.Tensor, blocks: torch.Tensor, k: int) -> "MXTensor":
         t = cls.__new__(cls)
-        t.data, t._scales, t.k, t.pitch = data, padded_scales, k, padded_scales.shape[-1]
+        t.data, t.blocks, t.k = data, blocks, k
         return t
 
     @property
     def scales(self) -> torch.Tensor:
-        return self._scales[..., :self.k // BLOCK]
+        *lead, nb, groups, _ = self.blocks.shape
+        rows = self.blocks.view(-1, nb, groups, 32, 4, 4).permute(0, 1, 4, 3, 2, 5).reshape(*lead, nb * 128, groups * 4)
+        return rows[..., :self.data.shape[-2], :self.k // BLOCK].contiguous()
 
     @property
     def shape(self) -> torch.Size:
@@ -90,45 +95,45 @@ class MXTensor:
 
 
 def mx_quantize(x: torch.Tensor, splits: Optional[torch.Tensor] = None, scatter_index: Optional[torch.Tensor] = None) -> MXTensor:
-    """Quantise x [..., K] (fp32, bf16 or fp16; K a multiple of 32): scale 2^(floor(log2 max|x|) - 2) for every 32 values,
-    values rounded to nearest, ties to even, at most 6 in magnitude. A block with an infinity or a NaN becomes NaN.
+    """Quantise x [..., N, K] (fp32, bf16 or fp16; K a multiple of 32): scale 2^(floor(log2 max|x|) - 2) for every 32
+    values, values rounded to nearest, ties to even, at most 6 in magnitude. Values among which there is an infinity or a NaN
+    become NaN, all 32.
     With `splits` and `scatter_index` (as `calc_scatter_index` makes them) the tokens x [ntokens, K] go into the order of
     their experts on the way, as in `moe_permute`: the result has ntokens * topk rows, and the rows past sum(splits) are
     zero. Has no gradient."""
     if not (_on_device(x) and x.dim() >= 2 and x.dtype in _FLOATS and x.shape[-1] >= BLOCK and x.shape[-1] % BLOCK == 0):
-        raise RuntimeError("mx_quantize: x must be a fp32, bf16 or fp16 [..., K] tensor on the current CUDA device, K a multiple of 32")
+        raise RuntimeError("mx_quantize: x must be a fp32, bf16 or fp16 [..., N, K] tensor on the current CUDA device, K a multiple of 32")
     _check(not (x.requires_grad and torch.is_grad_enabled()), "mx_quantize has no gradient: detach x, or call it under torch.no_grad()")
-    k = x.shape[-1]
-    if x.dim() > 2 or x.stride(1) != 1:
-        x2 = x.contiguous().view(-1, k)
-    else:
-        x2 = x
-    rows = x2.shape[0]
-    topk = nexperts = 0
+    *lead, n, k = x.shape
+    if lead or x.stride(1) != 1:
+        x = x.contiguous()
+    batch, out_rows, topk, nexperts = 1, n, 0, 0
+    for b in lead:
+        batch *= b
     if scatter_index is None:
         _check(splits is None, "mx_quantize: splits and scatter_index belong together")
-        shape = x.shape[:-1]
     else:
-        _check(splits is not None and x.dim() == 2, "mx_quantize: into the order of experts go [ntokens, K] tokens, with splits and scatter_index")
-        _check_index("mx_quantize", splits, scatter_index, rows)
+        _check(splits is not None and not lead, "mx_quantize: into the order of experts go [ntokens, K] tokens, with splits and scatter_index")
+        _check_index("mx_quantize", splits, scatter_index, n)
         topk, nexperts = scatter_index.shape[1], splits.numel()
-        shape = (rows * topk,)
-    pitch = _scale_pitch(k)
-    data = torch.empty((*shape, k // 2), dtype=torch.uint8, device=x.device)
-    scales = torch.empty((*shape, pitch), dtype=torch.uint8, device=x.device)
-    _lib.check(_lib.load().fluxb_mx_quantize(x2.data_ptr(), fluxb_dtype(x.dtype), rows, k, x2.stride(0), data.data_ptr(), scales.data_ptr(), pitch,
+        out_rows = n * topk
+    data = torch.empty((*lead, out_rows, k // 2), dtype=torch.uint8, device=x.device)
+    blocks = torch.empty(_blocks_shape(lead, out_rows, k), dtype=torch.uint8, device=x.device)
+    _lib.check(_lib.load().fluxb_mx_quantize(x.data_ptr(), fluxb_dtype(x.dtype), batch, n, k, x.stride(-2), data.data_ptr(), blocks.data_ptr(),
                                              _ptr(splits), nexperts, _ptr(scatter_index), topk, _cur_stream()))
-    return MXTensor._of(data, scales, k)
+    return MXTensor._of(data, blocks, k)
 
 
 def mx_dequantize(q: MXTensor, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """The values that `q` stands for, as fp32, bf16 or fp16 (exact in bf16 but beyond its range)."""
     _check(isinstance(q, MXTensor) and _on_device(q.data), "mx_dequantize: q must be an MXTensor on the current CUDA device")
     _check(dtype in _FLOATS, "mx_dequantize: the output must be fp32, bf16 or fp16")
-    out = torch.empty((*q.data.shape[:-1], q.k), dtype=dtype, device=q.data.device)
-    rows = q.data.numel() // (q.k // 2)
-    _lib.check(_lib.load().fluxb_mx_dequantize(q.data.data_ptr(), q._scales.data_ptr(), q.pitch, rows, q.k, fluxb_dtype(dtype), out.data_ptr(),
-                                               _cur_stream()))
+    *lead, n, _ = q.data.shape
+    out = torch.empty((*lead, n, q.k), dtype=dtype, device=q.data.device)
+    batch = 1
+    for b in lead:
+        batch *= b
+    _lib.check(_lib.load().fluxb_mx_dequantize(q.data.data_ptr(), q.blocks.data_ptr(), batch, n, q.k, fluxb_dtype(dtype), out.data_ptr(), _cur_stream()))
     return out
 
 
@@ -161,8 +166,8 @@ def mx_gemm(x: MXTensor, w: MXTensor, bias: Optional[torch.Tensor] = None, outpu
     out = _output("mx_gemm", output, m, n, output_dtype, x.data.device)
     if n == 0:
         return out
-    _lib.check(_lib.load().fluxb_mx_gemm(_comm().handle, x.data.data_ptr(), x._scales.data_ptr(), x.pitch, w.data.data_ptr(), w._scales.data_ptr(),
-                                         w.pitch, out.data_ptr(), m, n, x.k, fluxb_dtype(output_dtype), _ptr(bias), _tuning(tuning), _cur_stream()))
+    _lib.check(_lib.load().fluxb_mx_gemm(_comm().handle, x.data.data_ptr(), x.blocks.data_ptr(), w.data.data_ptr(), w.blocks.data_ptr(), out.data_ptr(),
+                                         m, n, x.k, fluxb_dtype(output_dtype), _ptr(bias), _tuning(tuning), _cur_stream()))
     return out
 
 
@@ -179,7 +184,9 @@ def mx_grouped_gemm(x: MXTensor, w: MXTensor, splits: torch.Tensor, output_dtype
     out = _output("mx_grouped_gemm", output, rows, n, output_dtype, x.data.device)
     if n == 0 or nexperts == 0:
         return out
-    _lib.check(_lib.load().fluxb_mx_grouped_gemm(_comm().handle, x.data.data_ptr(), x._scales.data_ptr(), x.pitch, rows, w.data.data_ptr(),
-                                                 w._scales.data_ptr(), w.pitch, nexperts, splits.data_ptr(), out.data_ptr(), n, x.k,
-                                                 fluxb_dtype(output_dtype), _tuning(tuning), _cur_stream()))
+    lib = _lib.load()
+    workspace = torch.empty((lib.fluxb_mx_grouped_workspace_bytes(rows, nexperts, x.k),), dtype=torch.uint8, device=out.device)
+    _lib.check(lib.fluxb_mx_grouped_gemm(_comm().handle, x.data.data_ptr(), x.blocks.data_ptr(), rows, w.data.data_ptr(), w.blocks.data_ptr(), nexperts,
+                                         splits.data_ptr(), out.data_ptr(), n, x.k, fluxb_dtype(output_dtype), workspace.data_ptr(), _tuning(tuning),
+                                         _cur_stream()))
     return out

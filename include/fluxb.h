@@ -298,34 +298,42 @@ int fluxb_moe_scatter_gemm_static(fluxb_comm_t comm, const void* tokens, int nto
 
 /* ------------------------------------- microscaled 4-bit floating point
  * No counterpart in the reference (its narrowest type is fp8). MXFP4: 32 consecutive values along K share a power of two
- * (one byte, exponent + 127; 255 = NaN), the values are e2m1, two to a byte, the first in the low half. A matrix of `rows`
- * x k is packed values [rows, k / 2] (contiguous) and scales, rows `scales_pitch` bytes apart; k is a multiple of 32. The
- * products want operands 16-byte aligned and scales_pitch a multiple of 16, at least 16 for every started 512 values of K
- * (what lies past a row's k / 32 scales is never used).
+ * (one byte, exponent + 127; 255 = NaN), the values are e2m1, two to a byte, the first in the low half. k is a multiple
+ * of 32. A matrix [rows, k] is
+ *   packed values [rows, k / 2], contiguous, and
+ *   scale blocks [ceil(rows / 128)][ceil(k / 128)] of 512 bytes, each 128 rows x 4 scales: the scales of row r are the four
+ *   bytes from (r % 32) * 16 + r / 32 % 4 * 4 on. Scales past k / 32 must be zero; rows past the end may hold anything.
+ * A batch of matrices has their values, and their scale blocks, one after the other. The products want all of it
+ * 16-byte aligned.
  *
- * fluxb_mx_quantize: x [rows, k] of fp32, bf16 or fp16, rows `ldx` elements apart. Per block the scale is 2^(floor(log2
- * max|x|) - 2), at least 2^-127; values are rounded to nearest, ties to even, and cut at 6. A block that holds an infinity
- * or a NaN gets the scale 255. With splits_dev and scatter_index_dev [rows, topk] (else NULL) row t goes to the rows
- * scatter_index[t, j] of a result of rows * topk rows, as in fluxb_moe_permute; rows from sum(splits) on become zero.
+ * fluxb_mx_scale_bytes: size of the scale blocks.
+ * fluxb_mx_quantize: x [batch, rows, k] of fp32, bf16 or fp16, rows `ldx` elements apart. Per 32 values the scale is
+ * 2^(floor(log2 max|x|) - 2), at least 2^-127; values are rounded to nearest, ties to even, and cut at 6. Values among
+ * which there is an infinity or a NaN get the scale 255. With splits_dev and scatter_index_dev [rows, topk] (else NULL;
+ * batch 1) row t goes to the rows scatter_index[t, j] of a result of rows * topk rows, as in fluxb_moe_permute; rows from
+ * sum(splits) on become zero.
  * fluxb_mx_dequantize: the values, rounded once to fp32, bf16 or fp16.
  * fluxb_mx_gemm: out[m, n] = x[m, k] . w[n, k]^T + bias[n] (bias of the output's type, or NULL), summed in fp32; out is bf16,
  * fp16 or fp32, contiguous, and needs no more than its type's alignment.
  * fluxb_mx_grouped_gemm: x holds `rows` rows in the order of their experts, splits_dev[e] for expert e (on the device), w is
- * [nexperts, n, k]; rows from sum(splits) on are not written. nexperts <= 1024. Nothing here allocates; calls on
- * several streams and in captured graphs may run side by side.
+ * a batch of nexperts matrices [n, k]; rows from sum(splits) on are not written. nexperts <= 1024. workspace:
+ * fluxb_mx_grouped_workspace_bytes, 16-byte aligned, this call's own until it has run.
+ * Nothing here allocates; calls on several streams and in captured graphs may run side by side.
  * `comm`: a communicator of the current device (status word, time-out). tuning: cta_group 1 or 2 selects the tiled kernel
- * (block_n tokens: 64 or 128 with 1; 64, 128, 192 or 224 with 2), cta_group 0 with block_n 16, 32, 64 or 128 the few-token one. */
-int fluxb_mx_quantize(const void* x, int dtype, int rows, int k, long long ldx, void* data, void* scales,
-                      long long scales_pitch, const int* splits_dev, int nexperts, const int* scatter_index_dev,
-                      int topk, fluxb_stream_t stream);
-int fluxb_mx_dequantize(const void* data, const void* scales, long long scales_pitch, int rows, int k, int out_dtype,
-                        void* out, fluxb_stream_t stream);
-int fluxb_mx_gemm(fluxb_comm_t comm, const void* xq, const void* xs, long long xs_pitch, const void* wq, const void* ws,
-                  long long ws_pitch, void* out, int m, int n, int k, int out_dtype, const void* bias,
-                  const fluxb_tuning* tuning, fluxb_stream_t stream);
-int fluxb_mx_grouped_gemm(fluxb_comm_t comm, const void* xq, const void* xs, long long xs_pitch, int rows,
-                          const void* wq, const void* ws, long long ws_pitch, int nexperts, const int* splits_dev,
-                          void* out, int n, int k, int out_dtype, const fluxb_tuning* tuning, fluxb_stream_t stream);
+ * (block_n tokens: 64 or 128 with 1; 64, 128, 192 or 256 with 2), cta_group 0 with block_n 64 or 128, or 16 or
+ * 32 for no more tokens than that (grouped: any number), the few-token one. */
+size_t fluxb_mx_scale_bytes(int batch, int rows, int k);
+size_t fluxb_mx_grouped_workspace_bytes(int rows, int nexperts, int k);
+int fluxb_mx_quantize(const void* x, int dtype, int batch, int rows, int k, long long ldx, void* data, void* scales,
+                      const int* splits_dev, int nexperts, const int* scatter_index_dev, int topk,
+                      fluxb_stream_t stream);
+int fluxb_mx_dequantize(const void* data, const void* scales, int batch, int rows, int k, int out_dtype, void* out,
+                        fluxb_stream_t stream);
+int fluxb_mx_gemm(fluxb_comm_t comm, const void* xq, const void* xs, const void* wq, const void* ws, void* out, int m,
+                  int n, int k, int out_dtype, const void* bias, const fluxb_tuning* tuning, fluxb_stream_t stream);
+int fluxb_mx_grouped_gemm(fluxb_comm_t comm, const void* xq, const void* xs, int rows, const void* wq, const void* ws,
+                          int nexperts, const int* splits_dev, void* out, int n, int k, int out_dtype, void* workspace,
+                          const fluxb_tuning* tuning, fluxb_stream_t stream);
 
 /* ------------------------------------------------------ MoE gather + RS
  * Replaces GemmGroupedV3GatherRS

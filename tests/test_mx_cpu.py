@@ -25,46 +25,54 @@ P = C.c_void_p(256)  # never read: the calls are refused first
 
 
 @pytest.mark.parametrize("change,words", [
-    ({"dtype": _lib.E4M3}, "fp32, bf16 or fp16"), ({"rows": -1}, "rows=-1"), ({"k": 0}, "k=0"), ({"k": 48}, "k=48"), ({"pitch": 1}, "rows of scales"),
-    ({"splits": P}, "belong together"), ({"index": P}, "belong together"), ({"splits": P, "index": P, "topk": 0}, "topk=0"),
-    ({"splits": P, "index": P, "nexperts": 0}, "nexperts=0"), ({"splits": P, "index": P, "rows": 1 << 29}, "too many"),
-    ({"x": None}, "NULL"), ({"data": None}, "NULL"), ({"scales": None}, "NULL"), ({"x": C.c_void_p(257)}, "aligned"), ({"data": C.c_void_p(258)}, "aligned"),
+    ({"dtype": _lib.E4M3}, "fp32, bf16 or fp16"), ({"rows": -1}, "rows=-1"), ({"batch": -1}, "batch=-1"), ({"k": 0}, "k=0"), ({"k": 48}, "k=48"),
+    ({"batch": 1 << 16, "rows": 1 << 15}, "too many"), ({"splits": P}, "belong together"), ({"index": P}, "belong together"),
+    ({"splits": P, "index": P, "topk": 0}, "topk=0"), ({"splits": P, "index": P, "batch": 2}, "batch=2"), ({"splits": P, "index": P, "nexperts": 0}, "nexperts=0"),
+    ({"splits": P, "index": P, "rows": 1 << 29}, "too many"), ({"x": None}, "NULL"), ({"data": None}, "NULL"), ({"scales": None}, "NULL"),
+    ({"x": C.c_void_p(257)}, "aligned"), ({"data": C.c_void_p(258)}, "aligned"), ({"scales": C.c_void_p(258)}, "aligned"),
 ])
 def test_quantize_arguments(change, words):
-    a = {"x": P, "dtype": _lib.BF16, "rows": 4, "k": 64, "ldx": 64, "data": P, "scales": P, "pitch": 16, "splits": None, "nexperts": 8, "index": None,
+    a = {"x": P, "dtype": _lib.BF16, "batch": 1, "rows": 4, "k": 64, "ldx": 64, "data": P, "scales": P, "splits": None, "nexperts": 8, "index": None,
          "topk": 2, **change}
-    assert _lib.load().fluxb_mx_quantize(a["x"], a["dtype"], a["rows"], a["k"], a["ldx"], a["data"], a["scales"], a["pitch"], a["splits"], a["nexperts"],
+    assert _lib.load().fluxb_mx_quantize(a["x"], a["dtype"], a["batch"], a["rows"], a["k"], a["ldx"], a["data"], a["scales"], a["splits"], a["nexperts"],
                                          a["index"], a["topk"], None) == _lib.FLUXB_ERR_INVALID
     assert "mx_quantize" in _lib.last_error() and words in _lib.last_error()
 
 
-@pytest.mark.parametrize("change,words", [({"dtype": _lib.S8}, "fp32, bf16 or fp16"), ({"rows": -1}, "rows=-1"), ({"k": 33}, "k=33"), ({"pitch": 1}, "rows of scales"),
+@pytest.mark.parametrize("change,words", [({"dtype": _lib.S8}, "fp32, bf16 or fp16"), ({"rows": -1}, "rows=-1"), ({"k": 33}, "k=33"),
                                           ({"data": None}, "NULL"), ({"data": C.c_void_p(258)}, "aligned"), ({"out": C.c_void_p(264)}, "aligned")])
 def test_dequantize_arguments(change, words):
-    a = {"data": P, "scales": P, "pitch": 16, "rows": 4, "k": 64, "dtype": _lib.BF16, "out": P, **change}
-    assert _lib.load().fluxb_mx_dequantize(a["data"], a["scales"], a["pitch"], a["rows"], a["k"], a["dtype"], a["out"], None) == _lib.FLUXB_ERR_INVALID
+    a = {"data": P, "scales": P, "rows": 4, "k": 64, "dtype": _lib.BF16, "out": P, **change}
+    assert _lib.load().fluxb_mx_dequantize(a["data"], a["scales"], 1, a["rows"], a["k"], a["dtype"], a["out"], None) == _lib.FLUXB_ERR_INVALID
     assert "mx_dequantize" in _lib.last_error() and words in _lib.last_error()
 
 
 @pytest.mark.parametrize("change,words", [
     ({"comm": None}, "NULL"), ({"xq": None}, "NULL"), ({"out": None}, "NULL"), ({"k": 16}, "k=16"), ({"k": 80}, "k=80"), ({"n": 0}, "n=0"), ({"m": -1}, "=-1"),
-    ({"xp": 8}, "rows of scales"), ({"wp": 24}, "rows of scales"), ({"k": 544}, "rows of scales"), ({"xq": C.c_void_p(264)}, "16-byte"),
-    ({"ws": C.c_void_p(264)}, "16-byte"), ({"dtype": _lib.E5M2}, "not bf16/f16/f32"), ({"out": C.c_void_p(257)}, "aligned to its type"),
-    ({"dtype": _lib.F32, "out": C.c_void_p(258)}, "aligned to its type"),
+    ({"xq": C.c_void_p(264)}, "16-byte"), ({"ws": C.c_void_p(264)}, "16-byte"), ({"dtype": _lib.E5M2}, "not bf16/f16/f32"),
+    ({"out": C.c_void_p(257)}, "aligned to its type"), ({"dtype": _lib.F32, "out": C.c_void_p(258)}, "aligned to its type"),
 ])
 def test_product_arguments(change, words):
-    a = {"comm": P, "xq": P, "xs": P, "xp": 16, "wq": P, "ws": P, "wp": 16, "out": P, "m": 4, "n": 8, "k": 64, "dtype": _lib.BF16, **change}
+    a = {"comm": P, "xq": P, "xs": P, "wq": P, "ws": P, "out": P, "m": 4, "n": 8, "k": 64, "dtype": _lib.BF16, **change}
     lib = _lib.load()
-    assert lib.fluxb_mx_gemm(a["comm"], a["xq"], a["xs"], a["xp"], a["wq"], a["ws"], a["wp"], a["out"], a["m"], a["n"], a["k"], a["dtype"], None, None,
-                             None) == _lib.FLUXB_ERR_INVALID
+    assert lib.fluxb_mx_gemm(a["comm"], a["xq"], a["xs"], a["wq"], a["ws"], a["out"], a["m"], a["n"], a["k"], a["dtype"], None, None, None) == _lib.FLUXB_ERR_INVALID
     assert words in _lib.last_error()
-    assert lib.fluxb_mx_grouped_gemm(a["comm"], a["xq"], a["xs"], a["xp"], a["m"], a["wq"], a["ws"], a["wp"], 4, P, a["out"], a["n"], a["k"], a["dtype"], None,
+    assert lib.fluxb_mx_grouped_gemm(a["comm"], a["xq"], a["xs"], a["m"], a["wq"], a["ws"], 4, P, a["out"], a["n"], a["k"], a["dtype"], P, None,
                                      None) == _lib.FLUXB_ERR_INVALID
     assert words in _lib.last_error()
 
 
 def test_grouped_arguments():
     lib = _lib.load()
-    for nexperts, n, splits, words in ((0, 8, P, "nexperts=0"), (1025, 8, P, "nexperts=1025"), (4, 8, None, "NULL"), (1024, 1 << 22, P, "too many")):
-        assert lib.fluxb_mx_grouped_gemm(P, P, P, 16, 4, P, P, 16, nexperts, splits, P, n, 64, _lib.BF16, None, None) == _lib.FLUXB_ERR_INVALID
+    for nexperts, n, splits, ws, words in ((0, 8, P, P, "nexperts=0"), (1025, 8, P, P, "nexperts=1025"), (4, 8, None, P, "NULL"), (4, 8, P, None, "NULL"),
+                                           (4, 8, P, C.c_void_p(264), "workspace"), (1024, 1 << 22, P, P, "too many")):
+        assert lib.fluxb_mx_grouped_gemm(P, P, P, 4, P, P, nexperts, splits, P, n, 64, _lib.BF16, ws, None, None) == _lib.FLUXB_ERR_INVALID
         assert words in _lib.last_error()
+
+
+def test_sizes():
+    lib = _lib.load()
+    assert lib.fluxb_mx_scale_bytes(1, 1, 32) == 512 and lib.fluxb_mx_scale_bytes(3, 129, 160) == 3 * 2 * 2 * 512 and lib.fluxb_mx_scale_bytes(1, 0, 64) == 0
+    # every expert can start a block: 300 rows fill two and begin one more for each of 5 experts, 4 rows reach 4 of them
+    assert lib.fluxb_mx_grouped_workspace_bytes(300, 5, 256) == (2 + 5) * 2 * 512 and lib.fluxb_mx_grouped_workspace_bytes(4, 1024, 128) == 4 * 512
+    assert lib.fluxb_mx_scale_bytes(-1, 4, 64) == 0 and lib.fluxb_mx_grouped_workspace_bytes(4, -1, 64) == 0

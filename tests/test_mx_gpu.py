@@ -13,7 +13,7 @@ pytestmark = pytest.mark.gpu
 GRID = torch.tensor([0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0], dtype=torch.float64)
 # every kernel and tile: the library's choice, the few-token kernel, single CTAs, CTA pairs
 TILES = [None] + [{"block_n": b} for b in (16, 32, 64, 128)] + [{"block_n": b, "cta_group": 1} for b in (64, 128)] \
-    + [{"block_n": b, "cta_group": 2} for b in (64, 128, 192, 224)]
+    + [{"block_n": b, "cta_group": 2} for b in (64, 128, 192, 256)]
 
 
 def _values(data, scales):
@@ -110,7 +110,7 @@ def test_quantize_layouts():
 
     g = torch.Generator().manual_seed(2)
     big = torch.randn(40, 200, generator=g).to(torch.bfloat16).cuda()
-    views = [big[:, 8:104], big[:, 3:131], big[::3, :64], big[:, ::2][:, :96], big.t()[:, :32], big[:1, :32].expand(5, 32),
+    views = [torch.randn(2, 130, 160, generator=g).cuda(), torch.randn(2, 3, 7, 32, generator=g).cuda().half(), big[:, 8:104], big[:, 3:131], big[::3, :64], big[:, ::2][:, :96], big.t()[:, :32], big[:1, :32].expand(5, 32),
              big.reshape(-1)[1:32 * 64 + 1].view(32, 64), torch.randn(3, 5, 64, generator=g).cuda()]
     for x in views:
         q = flux.mx_quantize(x)
@@ -147,12 +147,16 @@ def test_dequantize_every_code_and_scale():
 
 # -------------------------------------------------------------------------------------------------------------- products
 @pytest.mark.parametrize("tuning", TILES, ids=str)
-@pytest.mark.parametrize("m,n,k", [(1, 1, 32), (16, 128, 256), (5, 130, 288), (100, 257, 2080), (225, 513, 544), (300, 1000, 4096)])
+@pytest.mark.parametrize("m,n,k", [(1, 1, 32), (16, 128, 256), (5, 130, 288), (100, 257, 2080), (225, 513, 544), (300, 1000, 4096), (1500, 2100, 1056)])
 def test_product_is_exact(m, n, k, tuning):
     import flux_b200 as flux
 
     x, xv = _random_mx((m, k), m + k)
     w, wv = _random_mx((n, k), n + k + 1)
+    if tuning in ({"block_n": 16}, {"block_n": 32}) and m > tuning["block_n"]:
+        with pytest.raises(RuntimeError, match="is for up to"):
+            flux.mx_gemm(x, w, output_dtype=torch.float32, tuning=tuning)
+        return
     y = flux.mx_gemm(x, w, output_dtype=torch.float32, tuning=tuning)
     _status()
     assert torch.equal(y.cpu().double(), xv @ wv.t())
