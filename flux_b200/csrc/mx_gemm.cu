@@ -36,9 +36,9 @@ static int mx_launch(Kern kern, const MxParams& p, int grid, int threads, int sm
 
 template <int BN, bool CTA2, bool GROUPED>
 static int launch_mx_tiles(const fluxb_comm* comm, const MxParams& p, long long most_tiles, int num_ctas, cudaStream_t stream) {
-  using L = MxLayout<BN, CTA2>;
+  using L = MxLayout<BN, CTA2, GROUPED>;
   auto kern = mx_gemm_kernel<BN, CTA2, GROUPED>;
-  constexpr int smem = L::total(GROUPED);
+  constexpr int smem = L::kTotal;
   static bool configured[64] = {};
   static int max_clusters[64] = {};
   const int dev = comm->device;
@@ -102,9 +102,9 @@ static int mx_out_type(int out_dtype, int* ot) {
   }
 }
 
-// Scale blocks that a grouped launch's tokens can need: an expert without tokens needs none, one with tokens at most one
-// more than they fill (the same for tiles of `rows_per` tokens).
-static long long mx_most_blocks(int rows, int nexperts, int rows_per) { return static_cast<long long>(rows) / rows_per + (nexperts < rows ? nexperts : rows); }
+// Tiles of `bn` tokens that a grouped launch can need: an expert without tokens needs none, one with tokens at most one
+// more than they fill.
+static long long mx_most_tiles(int rows, int nexperts, int bn) { return static_cast<long long>(rows) / bn + (nexperts < rows ? nexperts : rows); }
 
 // `per_group` = tokens that an expert gets on average (dense: all of them)
 template <bool GROUPED>
@@ -129,7 +129,7 @@ static int mx_run(fluxb_comm* comm, MxParams& p, const void* xq, const void* wq,
   p.n_tiles = (p.N + tile_n - 1) / tile_n;
   p.m_tiles = (p.rows_x + bn - 1) / bn;
   p.w_blocks = (p.N + 127) / 128;
-  const long long tiles = (GROUPED ? mx_most_blocks(p.rows_x, groups, bn) : p.m_tiles) * p.n_tiles;
+  const long long tiles = (GROUPED ? mx_most_tiles(p.rows_x, groups, bn) : p.m_tiles) * p.n_tiles;
   FLUXB_REQUIRE(tiles < (1ll << 27), "mx_gemm: %d rows x %d columns have too many tiles", p.rows_x, p.N);
   p.band = tuning != nullptr && tuning->group_m > 0 ? tuning->group_m : 8;
   if (p.band > p.n_tiles) p.band = p.n_tiles;
@@ -140,9 +140,10 @@ static int mx_run(fluxb_comm* comm, MxParams& p, const void* xq, const void* wq,
   if (rc != FLUXB_OK) return rc;
   rc = encode_tmap_words(&p.tmap_sw, ws, static_cast<long long>(groups) * p.w_blocks, words, 1);
   if (rc != FLUXB_OK) return rc;
+  const long long most_blocks = GROUPED ? mx_most_tiles(p.rows_x, groups, bn) * ((bn + 127) / 128) : 0;
   if (!GROUPED || !few) {
     const void* blocks = GROUPED ? workspace : p.sx;
-    rc = encode_tmap_words(&p.tmap_sx, blocks, GROUPED ? mx_most_blocks(p.rows_x, groups, 128) : (p.rows_x + 127) / 128, words, (bn + 127) / 128);
+    rc = encode_tmap_words(&p.tmap_sx, blocks, GROUPED ? most_blocks : (p.rows_x + 127) / 128, words, (bn + 127) / 128);
     if (rc != FLUXB_OK) return rc;
   }
   if (few) {
@@ -158,8 +159,8 @@ static int mx_run(fluxb_comm* comm, MxParams& p, const void* xq, const void* wq,
   FLUXB_REQUIRE(cg == 2 ? bn == 64 || bn == 128 || bn == 192 || bn == 256 : cg == 1 && (bn == 64 || bn == 128),
                 "mx_gemm: block_n=%d cta_group=%d is not {64,128} with 1 or {64,128,192,256} with 2", bn, cg);
   if (GROUPED) {
-    rc = launch_pdl(mx_regroup_kernel, static_cast<int>(mx_most_blocks(p.rows_x, groups, 128)), kMxRegroupThreads, stream, p.sx, p.rows_x, p.groups,
-                    p.splits, p.nexperts, static_cast<uint4*>(workspace));
+    rc = launch_pdl(mx_regroup_kernel, static_cast<int>(most_blocks), kMxRegroupThreads, stream, p.sx, p.rows_x, p.groups, bn, p.splits, p.nexperts,
+                    static_cast<uint4*>(workspace));
     if (rc != FLUXB_OK) return rc;
   }
   const int num_ctas = tuning != nullptr ? tuning->num_ctas : 0;
@@ -189,6 +190,7 @@ static int mx_fill(const char* who, fluxb_comm* comm, MxParams& p, const void* x
   p.groups = (k + kMxGroupK - 1) / kMxGroupK;
   p.out = const_cast<void*>(out);
   p.ldo = n;
+  p.out_blocks = p.out_type != kOutF32 && n % 8 == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0 ? 1 : 0;
   p.timeout_ns = comm->timeout_ns;
   p.status = comm->status_dev;
   return FLUXB_OK;
@@ -207,7 +209,9 @@ size_t fluxb_mx_scale_bytes(int batch, int rows, int k) {
 
 size_t fluxb_mx_grouped_workspace_bytes(int rows, int nexperts, int k) {
   if (rows < 0 || nexperts < 0 || k < 0) return 0;
-  return static_cast<size_t>(mx_most_blocks(rows, nexperts, 128)) * ((static_cast<size_t>(k) + kMxGroupK - 1) / kMxGroupK) * kMxSfBytes;
+  // the tile width that takes the most blocks: 64 (one for half as many rows), or 256 (two for an expert with one row)
+  const long long most = mx_most_tiles(rows, nexperts, 64) + (nexperts < rows ? nexperts : rows);
+  return static_cast<size_t>(most) * ((static_cast<size_t>(k) + kMxGroupK - 1) / kMxGroupK) * kMxSfBytes;
 }
 
 int fluxb_mx_gemm(fluxb_comm_t comm, const void* xq, const void* xs, const void* wq, const void* ws, void* out, int m, int n, int k, int out_dtype,

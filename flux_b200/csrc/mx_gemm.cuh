@@ -41,6 +41,7 @@ struct MxParams {
   void* out;
   long long ldo;
   const void* bias;     // [N] of the output's type, or null
+  int out_blocks;       // 16-bit output, rows 16-byte aligned
   int split;            // few-token kernel: CTAs that share a tile's K
   unsigned long long timeout_ns;
   int* status;
@@ -84,7 +85,7 @@ __device__ __forceinline__ void umma_mxf4(uint32_t d, uint64_t a, uint64_t b, ui
         : "memory");
 }
 
-template <int BN, bool CTA2>
+template <int BN, bool CTA2, bool GROUPED>
 struct MxLayout {
   static constexpr int kABytes = kBM * kRowBytes;
   static constexpr int kBRows = CTA2 ? BN / 2 : BN;
@@ -92,7 +93,9 @@ struct MxLayout {
   static constexpr int kXBlocks = (BN + 127) / 128;  // scale blocks of the tokens: all of them, in both CTAs of a pair
   static constexpr int kSfOffset = kABytes + kBBytes;
   static constexpr int kStageBytes = kSfOffset + (1 + kXBlocks) * 2 * kMxSfBytes;
-  static constexpr int kStagesFit = (212 * 1024) / kStageBytes;
+  static constexpr int kTableBytes = GROUPED ? (2 * kMxMaxExperts + 1) * 4 : 0;
+  static constexpr int kEpiBytes = kMxEpiWarps * 1024;  // 16 tokens x 32 columns of 16 bits and their neighbours, per epilogue warp
+  static constexpr int kStagesFit = (232448 - 2048 - kTableBytes - kEpiBytes) / kStageBytes;
   static constexpr int kStages = kStagesFit > 8 ? 8 : kStagesFit;
   // Tensor memory: two accumulators and the scales of kSlots stages (for each of a stage's two groups of K four columns of
   // the weights and four for every 128 tokens). 2 x 256 columns leave no room for scales: there the second accumulator
@@ -106,22 +109,22 @@ struct MxLayout {
   static constexpr int kColsUsed = kSf + kSlots * kSfCols;
   static constexpr uint32_t kTmemCols = kColsUsed <= 64 ? 64 : kColsUsed <= 128 ? 128 : kColsUsed <= 256 ? 256 : 512;
   static constexpr int kNumBars = 2 * kStages + 5;
-  static constexpr int kBarOffset = kStages * kStageBytes;
+  static constexpr int kEpiOffset = kStages * kStageBytes;
+  static constexpr int kBarOffset = kEpiOffset + kEpiBytes;
   static constexpr int kMiscOffset = kBarOffset + kNumBars * 8;
   static constexpr int kGroupOffset = kMiscOffset + 64;
-  static constexpr int kGroupBytes = (3 * kMxMaxExperts + 1) * 4;
-  static constexpr int total(bool grouped) { return kGroupOffset + (grouped ? kGroupBytes : 0) + 1024; }
+  static constexpr int kTotal = kGroupOffset + kTableBytes + 1024;
   static constexpr int kThreads = 64 + 32 * kMxEpiWarps;
   static_assert(kStageBytes % 1024 == 0 && kSlots >= 2 && kStages >= 3 && kColsUsed <= 512, "layout");
 };
 
-// One warp's walk over the experts, 32 at a time: first row and end of expert e0 + lane, its tiles of `bn` tokens and its
-// scale blocks, and the numbers of both before it. Splits that are negative or run past the rows that exist are cut, so
-// that nothing outside is touched.
+// One warp's walk over the experts, 32 at a time: first row and end of expert e0 + lane, its tiles of `bn` tokens, and the
+// number of tiles up to its end. Splits that are negative or run past the rows that exist are cut, so that nothing outside
+// is touched.
 struct MxExperts {
   long long rows = 0;
-  int tiles = 0, blocks = 0;
-  int first, end, tiles_end, tiles_mine, blocks_before;
+  int tiles = 0;
+  int first, end, tiles_end, tiles_mine;
   __device__ __forceinline__ void next(const int* splits, int nexperts, int rows_x, int bn, int e0, int lane) {
     long long m = e0 + lane < nexperts ? splits[e0 + lane] : 0;
     if (m < 0) m = 0;
@@ -135,21 +138,15 @@ struct MxExperts {
     first = static_cast<int>(f < rows_x ? f : rows_x);
     end = static_cast<int>(e < rows_x ? e : rows_x);
     tiles_mine = (end - first + bn - 1) / bn;
-    const int blocks_mine = (end - first + 127) >> 7;
-    int ti = tiles_mine, bi = blocks_mine;
+    int ti = tiles_mine;
 #pragma unroll
     for (int off = 1; off < 32; off <<= 1) {
-      const int t = __shfl_up_sync(0xffffffffu, ti, off), b = __shfl_up_sync(0xffffffffu, bi, off);
-      if (lane >= off) {
-        ti += t;
-        bi += b;
-      }
+      const int t = __shfl_up_sync(0xffffffffu, ti, off);
+      if (lane >= off) ti += t;
     }
     tiles_end = tiles + ti;
-    blocks_before = blocks + bi - blocks_mine;
     rows += __shfl_sync(0xffffffffu, incl, 31);
     tiles += __shfl_sync(0xffffffffu, ti, 31);
-    blocks += __shfl_sync(0xffffffffu, bi, 31);
   }
 };
 
@@ -168,7 +165,7 @@ __device__ __forceinline__ void mx_raster(int t, int n_tiles, int m_tiles, int b
   n_idx = b * band + r - m_idx * h;
 }
 struct MxGroups {  // of a grouped launch, in shared memory
-  int *row_first, *tile_end, *block_first;
+  int *row_first, *tile_end;
 };
 template <int BN, bool GROUPED>
 __device__ __forceinline__ bool mx_tile(const MxParams& p, int tile_rows, int t, const MxGroups& g, MxTile& out) {
@@ -196,7 +193,7 @@ __device__ __forceinline__ bool mx_tile(const MxParams& p, int tile_rows, int t,
     out.w_block = lo * p.w_blocks + (out.n0 >> 7);
     out.m0 = g.row_first[lo] + m_idx * BN;
     out.m_end = g.row_first[lo + 1];
-    out.x_block = g.block_first[lo] + ((m_idx * BN) >> 7);
+    out.x_block = before * ((BN + 127) / 128) + ((m_idx * BN) >> 7);  // (as mx_regroup_kernel lays them out)
   }
   out.x_col = ((m_idx * BN) & 127) >> 5;
   return true;
@@ -230,16 +227,53 @@ __device__ __forceinline__ void mx_store_column(const MxParams& p, const uint32_
   }
 }
 
+// The same for 16-bit outputs whose rows are 16-byte aligned. A lane has one column, and two bytes of a row are slow to store
+// (8192 x 14336 x 2048 took 190 us, most of it waiting for stores): the warp exchanges 16 tokens x 32 columns through 1 KB of
+// its own, two tokens' values in a word, so that a lane gets eight columns of two tokens. Pieces of 16 bytes are
+// exchanged in every other row, which keeps the reads off each other's banks.
+__device__ __forceinline__ void mx_store_block(const MxParams& p, const uint32_t (&r)[32], int m, int cnt, int n0, float bias, uint32_t buf, int lane) {
+  const bool bf16 = p.out_type == kOutBf16;
+  const int oct = lane & 3, pair = lane >> 2;
+  const bool cols = n0 + oct * 8 < p.N;  // (a multiple of 8)
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    if (h * 16 >= cnt) break;
+    __syncwarp();
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float a = __uint_as_float(r[h * 16 + 2 * j]) + bias, b = __uint_as_float(r[h * 16 + 2 * j + 1]) + bias;
+      const uint32_t w = bf16 ? pack_bf16(a, b) : pack_f16(a, b);
+      asm volatile("st.shared.b32 [%0], %1;" ::"r"(buf + j * 128 + ((((lane >> 2) ^ (j & 1)) << 4) | ((lane & 3) << 2))), "r"(w) : "memory");
+    }
+    __syncwarp();
+    uint32_t w[8];
+#pragma unroll
+    for (int q = 0; q < 2; ++q)
+      asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                   : "=r"(w[4 * q]), "=r"(w[4 * q + 1]), "=r"(w[4 * q + 2]), "=r"(w[4 * q + 3])
+                   : "r"(buf + pair * 128 + (((2 * oct + q) ^ (pair & 1)) << 4))
+                   : "memory");
+    const int t = h * 16 + 2 * pair;
+    uint16_t* o = static_cast<uint16_t*>(p.out) + (m + t) * p.ldo + n0 + oct * 8;
+    if (cols && t < cnt)
+      *reinterpret_cast<uint4*>(o) = make_uint4(__byte_perm(w[0], w[1], 0x5410), __byte_perm(w[2], w[3], 0x5410), __byte_perm(w[4], w[5], 0x5410),
+                                                __byte_perm(w[6], w[7], 0x5410));
+    if (cols && t + 1 < cnt)
+      *reinterpret_cast<uint4*>(o + p.ldo) = make_uint4(__byte_perm(w[0], w[1], 0x7632), __byte_perm(w[2], w[3], 0x7632), __byte_perm(w[4], w[5], 0x7632),
+                                                        __byte_perm(w[6], w[7], 0x7632));
+  }
+}
+
 // Persistent kernel. Warp 0: TMA; warp 1: tensor memory and UMMA; kMxEpiWarps epilogue warps, two per quadrant. Two
 // accumulators: the epilogue of a tile overlaps the main loop of the next.
 template <int BN, bool CTA2, bool GROUPED>
-__global__ void __launch_bounds__(MxLayout<BN, CTA2>::kThreads, 1)
+__global__ void __launch_bounds__(MxLayout<BN, CTA2, GROUPED>::kThreads, 1)
 mx_gemm_kernel(const __grid_constant__ MxParams p) {
-  using L = MxLayout<BN, CTA2>;
+  using L = MxLayout<BN, CTA2, GROUPED>;
   constexpr int STAGES = L::kStages, SLOTS = L::kSlots;
   constexpr int TILE_N = CTA2 ? 2 * kBM : kBM;
   constexpr bool OVERLAP = L::kOverlap > 0;
-  static_assert(L::total(GROUPED) <= 232448, "shared memory budget exceeded");
+  static_assert(L::kTotal <= 232448, "shared memory budget exceeded");
 
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
@@ -255,7 +289,6 @@ mx_gemm_kernel(const __grid_constant__ MxParams p) {
   MxGroups groups;
   groups.row_first = reinterpret_cast<int*>(smem + L::kGroupOffset);
   groups.tile_end = groups.row_first + kMxMaxExperts + 1;
-  groups.block_first = groups.tile_end + kMxMaxExperts;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int half = CTA2 ? static_cast<int>(cluster_ctarank()) : 0;
   const bool leader = half == 0;
@@ -295,7 +328,6 @@ mx_gemm_kernel(const __grid_constant__ MxParams p) {
       if (e0 + lane < p.nexperts) {
         groups.row_first[e0 + lane] = x.first;
         groups.tile_end[e0 + lane] = x.tiles_end;
-        groups.block_first[e0 + lane] = x.blocks_before;
       }
     }
     if (lane == 0) groups.row_first[p.nexperts] = static_cast<int>(x.rows < p.rows_x ? x.rows : p.rows_x);
@@ -422,6 +454,8 @@ mx_gemm_kernel(const __grid_constant__ MxParams p) {
     const int quad = warp & 3, first = (warp - 2) >> 2;
     const uint32_t tmem_quad = tmem_base + (static_cast<uint32_t>(quad * 32) << 16);
     const uint32_t tempty0 = CTA2 ? mapa_u32(bar_tempty(0), 0) : bar_tempty(0);
+    const uint32_t epi_buf = smem_base + L::kEpiOffset + (warp - 2) * 1024;
+    const bool blocks = p.out_blocks != 0;
     constexpr int CHUNKS = BN / 32, SHARED = L::kOverlap / 32;
     static_assert(BN % 32 == 0 && L::kOverlap % 32 == 0, "chunks");
     int it = 0;
@@ -441,16 +475,34 @@ mx_gemm_kernel(const __grid_constant__ MxParams p) {
           if (CTA2) mbar_arrive_cluster(bar); else mbar_arrive(bar);
         }
       };
+      auto store = [&](const uint32_t (&r)[32], int c) {
+        if (blocks) mx_store_block(p, r, tl.m0 + c, tl.m_end - tl.m0 - c, n - lane, bias, epi_buf, lane);
+        else mx_store_column<32>(p, r, tl.m0 + c, tl.m_end - tl.m0 - c, n, bias);
+      };
+      int i = first;
+      if constexpr (OVERLAP) {
+        // the columns that the next tile's accumulator shares, the last ones of the first and the first of the second, leave
+        // tensor memory before anything is stored: the UMMAs of that tile wait for them
+        static_assert(SHARED <= 4, "at most two chunks a warp");
+        uint32_t r0[32], r1[32];
+        const int c0 = (acc == 0 ? CHUNKS - 1 - first : first) * 32, c1 = (acc == 0 ? CHUNKS - 3 - first : first + 2) * 32;
+        const bool two = first + 2 < SHARED;
+        tmem_ld_32x32(tacc + c0, r0);
+        if (two) tmem_ld_32x32(tacc + c1, r1);
+        tmem_ld_wait();
+        give_back();
+        if (tl.m0 + c0 < tl.m_end) store(r0, c0);
+        if (two && tl.m0 + c1 < tl.m_end) store(r1, c1);
+        i += two ? 4 : 2;
+      }
 #pragma unroll 1
-      for (int i = first; i < CHUNKS; i += 2) {
-        if (OVERLAP && (i == SHARED || i == SHARED + 1)) give_back();  // (its first chunk past the shared columns)
-        // the columns that the next tile's accumulator shares come first: the last ones of the first, the first of the second
+      for (; i < CHUNKS; i += 2) {
         const int c = (OVERLAP && acc == 0 ? CHUNKS - 1 - i : i) * 32;
         if (tl.m0 + c >= tl.m_end) continue;
         uint32_t r[32];
         tmem_ld_32x32(tacc + c, r);
         tmem_ld_wait();
-        mx_store_column<32>(p, r, tl.m0 + c, tl.m_end - tl.m0 - c, n, bias);
+        store(r, c);
       }
       if (!OVERLAP) give_back();
     }
@@ -469,24 +521,27 @@ mx_gemm_kernel(const __grid_constant__ MxParams p) {
   }
 }
 
-// The tokens' scale blocks of a grouped launch: rows in the order of their experts, every expert's rows from a block's
-// start on. A CTA per block, as many as the experts could need; 16 bytes (four rows 32 apart) per thread and group of K.
+// The tokens' scale blocks of a grouped launch with tiles of `bn` tokens: every expert's rows from a block's start on, the
+// expert's blocks where its tiles, each of as many blocks as it has starts of 128 rows, begin. A CTA per block, as many as
+// the experts could need; 16 bytes (four rows 32 apart) per thread and group of K.
 constexpr int kMxRegroupThreads = 256;
-__global__ void __launch_bounds__(kMxRegroupThreads)
-mx_regroup_kernel(const uint8_t* __restrict__ src, int rows, int groups, const int* __restrict__ splits, int nexperts, uint4* __restrict__ dst) {
+static __global__ void __launch_bounds__(kMxRegroupThreads)
+mx_regroup_kernel(const uint8_t* __restrict__ src, int rows, int groups, int bn, const int* __restrict__ splits, int nexperts, uint4* __restrict__ dst) {
   __shared__ int s_first, s_end;
   const int lane = threadIdx.x & 31;
   pdl_wait();
   if (threadIdx.x == 0) pdl_trigger();
   if (threadIdx.x < 32) {
+    const int per = (bn + 127) / 128, tile = static_cast<int>(blockIdx.x) / per;
     MxExperts x;
     int first = 0, end = 0;
     for (int e0 = 0; e0 < nexperts; e0 += 32) {
-      x.next(splits, nexperts, rows, 128, e0, lane);  // (tiles of 128 rows: blocks)
-      const unsigned has = __ballot_sync(0xffffffffu, x.tiles_end > static_cast<int>(blockIdx.x));
+      x.next(splits, nexperts, rows, bn, e0, lane);
+      const unsigned has = __ballot_sync(0xffffffffu, x.tiles_end > tile);
       if (has == 0) continue;
       const int from = __ffs(has) - 1;
-      first = __shfl_sync(0xffffffffu, x.first, from) + (static_cast<int>(blockIdx.x) - __shfl_sync(0xffffffffu, x.blocks_before, from)) * 128;
+      const int before = __shfl_sync(0xffffffffu, x.tiles_end - x.tiles_mine, from);
+      first = __shfl_sync(0xffffffffu, x.first, from) + (static_cast<int>(blockIdx.x) - before * per) * 128;
       end = __shfl_sync(0xffffffffu, x.end, from);
       break;
     }

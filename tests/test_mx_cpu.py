@@ -73,6 +73,8 @@ def test_grouped_arguments():
 def test_sizes():
     lib = _lib.load()
     assert lib.fluxb_mx_scale_bytes(1, 1, 32) == 512 and lib.fluxb_mx_scale_bytes(3, 129, 160) == 3 * 2 * 2 * 512 and lib.fluxb_mx_scale_bytes(1, 0, 64) == 0
-    # every expert can start a block: 300 rows fill two and begin one more for each of 5 experts, 4 rows reach 4 of them
-    assert lib.fluxb_mx_grouped_workspace_bytes(300, 5, 256) == (2 + 5) * 2 * 512 and lib.fluxb_mx_grouped_workspace_bytes(4, 1024, 128) == 4 * 512
+    # for every tile width: the rows' whole tiles and one begun for each expert that can have rows, one or two blocks each
+    for rows, nexperts in ((300, 5), (4, 1024), (100000, 64), (1, 1)):
+        most = max((rows // bn + min(nexperts, rows)) * -(-bn // 128) for bn in (64, 128, 192, 256))
+        assert lib.fluxb_mx_grouped_workspace_bytes(rows, nexperts, 160) >= most * 2 * 512
     assert lib.fluxb_mx_scale_bytes(-1, 4, 64) == 0 and lib.fluxb_mx_grouped_workspace_bytes(4, -1, 64) == 0
