@@ -141,7 +141,7 @@ static int mx_run(fluxb_comm* comm, MxParams& p, const void* xq, const void* wq,
   rc = encode_tmap_words(&p.tmap_sw, ws, static_cast<long long>(groups) * p.w_blocks, words, 1);
   if (rc != FLUXB_OK) return rc;
   const long long most_blocks = GROUPED ? mx_most_tiles(p.rows_x, groups, bn) * ((bn + 127) / 128) : 0;
-  if (!GROUPED || !few) {
+  if (!GROUPED || cg == 2) {
     const void* blocks = GROUPED ? workspace : p.sx;
     rc = encode_tmap_words(&p.tmap_sx, blocks, GROUPED ? most_blocks : (p.rows_x + 127) / 128, words, (bn + 127) / 128);
     if (rc != FLUXB_OK) return rc;
@@ -158,9 +158,11 @@ static int mx_run(fluxb_comm* comm, MxParams& p, const void* xq, const void* wq,
   }
   FLUXB_REQUIRE(cg == 2 ? bn == 64 || bn == 128 || bn == 192 || bn == 256 : cg == 1 && (bn == 64 || bn == 128),
                 "mx_gemm: block_n=%d cta_group=%d is not {64,128} with 1 or {64,128,192,256} with 2", bn, cg);
-  if (GROUPED) {
-    rc = launch_pdl(mx_regroup_kernel, static_cast<int>(most_blocks), kMxRegroupThreads, stream, p.sx, p.rows_x, p.groups, bn, p.splits, p.nexperts,
-                    static_cast<uint4*>(workspace));
+  if (GROUPED && cg == 2) {
+    const int parts = (p.groups + kMxRegroupGroups - 1) / kMxRegroupGroups;
+    FLUXB_REQUIRE(most_blocks * parts < (1ll << 30), "mx_grouped_gemm: %d rows of %d groups are too many", p.rows_x, p.groups);
+    rc = launch_pdl(mx_regroup_kernel, static_cast<int>(most_blocks * parts), kMxRegroupThreads, stream, p.sx, p.rows_x, p.groups, parts, bn, p.splits,
+                    p.nexperts, static_cast<uint4*>(workspace));
     if (rc != FLUXB_OK) return rc;
   }
   const int num_ctas = tuning != nullptr ? tuning->num_ctas : 0;

@@ -114,7 +114,10 @@ struct MxLayout {
   static constexpr int kMiscOffset = kBarOffset + kNumBars * 8;
   static constexpr int kGroupOffset = kMiscOffset + 64;
   static constexpr int kTotal = kGroupOffset + kTableBytes + 1024;
-  static constexpr int kThreads = 64 + 32 * kMxEpiWarps;
+  // Grouped tokens start anywhere in a scale block. Single CTAs have a warp that gathers their scales; for pairs, whose two
+  // CTAs would have to hand them over, a launch before this one moves them (mx_regroup_kernel).
+  static constexpr bool kGather = GROUPED && !CTA2;
+  static constexpr int kThreads = 64 + 32 * kMxEpiWarps + (kGather ? 32 : 0);
   static_assert(kStageBytes % 1024 == 0 && kSlots >= 2 && kStages >= 3 && kColsUsed <= 512, "layout");
 };
 
@@ -125,9 +128,11 @@ struct MxExperts {
   long long rows = 0;
   int tiles = 0;
   int first, end, tiles_end, tiles_mine;
+  int ahead;  // the split of expert e0 + lane, loaded a step before it is used
+  __device__ __forceinline__ MxExperts(const int* splits, int nexperts, int lane) { ahead = lane < nexperts ? splits[lane] : 0; }
   __device__ __forceinline__ void next(const int* splits, int nexperts, int rows_x, int bn, int e0, int lane) {
-    long long m = e0 + lane < nexperts ? splits[e0 + lane] : 0;
-    if (m < 0) m = 0;
+    long long m = ahead > 0 ? ahead : 0;
+    ahead = e0 + 32 + lane < nexperts ? splits[e0 + 32 + lane] : 0;
     long long incl = m;
 #pragma unroll
     for (int off = 1; off < 32; off <<= 1) {
@@ -264,6 +269,25 @@ __device__ __forceinline__ void mx_store_block(const MxParams& p, const uint32_t
   }
 }
 
+// The scales of a grouped tile's tokens for one stage: of rows lane, lane + 32, ... the cells of two groups of K, zero past
+// the tile's tokens and past K; then as 16-byte pieces in the order of a scale block.
+template <int BN>
+__device__ __forceinline__ void mx_gather_scales(uint32_t (&w)[2][4], const MxParams& p, int m0, int m_end, int kb, int lane) {
+#pragma unroll
+  for (int g = 0; g < 2; ++g)
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const int kg = kb * 2 + g, r = m0 + q * 32 + lane;
+      w[g][q] = q * 32 < BN && r < m_end && kg < p.groups ? __ldg(reinterpret_cast<const uint32_t*>(p.sx + mx_sf_offset(r, kg, p.groups))) : 0u;
+    }
+}
+__device__ __forceinline__ void mx_put_scales(const uint32_t (&w)[2][4], uint32_t dst, int lane) {
+#pragma unroll
+  for (int g = 0; g < 2; ++g)
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst + g * kMxSfBytes + lane * 16), "r"(w[g][0]), "r"(w[g][1]), "r"(w[g][2]), "r"(w[g][3])
+                 : "memory");
+}
+
 // Persistent kernel. Warp 0: TMA; warp 1: tensor memory and UMMA; kMxEpiWarps epilogue warps, two per quadrant. Two
 // accumulators: the epilogue of a tile overlaps the main loop of the next.
 template <int BN, bool CTA2, bool GROUPED>
@@ -299,7 +323,10 @@ mx_gemm_kernel(const __grid_constant__ MxParams p) {
 
   if (warp == 0 && elect_one()) {
     *s_abort = 0;
-    for (int s = 0; s < 2 * STAGES; ++s) mbar_init(bar_base + 8u * s, 1);
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(bar_full(s), L::kGather ? 2 : 1);  // the copies, and the warp that gathers scales
+      mbar_init(bar_empty(s), 1);
+    }
     for (int a = 0; a < 2; ++a) {
       mbar_init(bar_tfull(a), 1);
       mbar_init(bar_tempty(a), (CTA2 ? 2 : 1) * kMxEpiWarps);
@@ -322,7 +349,7 @@ mx_gemm_kernel(const __grid_constant__ MxParams p) {
   }
   if (GROUPED && warp == 2) {
     pdl_wait();
-    MxExperts x;
+    MxExperts x(p.splits, p.nexperts, lane);
     for (int e0 = 0; e0 < p.nexperts; e0 += 32) {
       x.next(p.splits, p.nexperts, p.rows_x, BN, e0, lane);
       if (e0 + lane < p.nexperts) {
@@ -347,15 +374,19 @@ mx_gemm_kernel(const __grid_constant__ MxParams p) {
       bool ok = true;
       const uint32_t full0 = CTA2 ? mapa_u32(bar_full(0), 0) : bar_full(0);
       const bool arms = !CTA2 || leader;
-      MxTile tl;
-      for (int t = worker; ok && mx_tile<BN, GROUPED>(p, TILE_N, t, groups, tl); t += workers) {
+      MxTile tl, next;
+      int t = worker;
+      bool more = mx_tile<BN, GROUPED>(p, TILE_N, t, groups, next);
+      while (ok && more) {
+        tl = next;
         const int wrow = tl.w_row + half * kBM, xrow = tl.m0 + half * L::kBRows;
         for (int kb = 0; kb < p.num_kb; ++kb) {
+          if (kb == p.num_kb - 1) more = mx_tile<BN, GROUPED>(p, TILE_N, t += workers, groups, next);  // (while a stage is awaited)
           if (!mbar_wait(bar_empty(stage), phase ^ 1u, ab, kStatusTimeoutSmemEmpty, budget)) {
             ok = false;
             break;
           }
-          if (arms) mbar_arrive_expect_tx(bar_full(stage), (CTA2 ? 2 : 1) * L::kStageBytes);
+          if (arms) mbar_arrive_expect_tx(bar_full(stage), (CTA2 ? 2 : 1) * (L::kStageBytes - (L::kGather ? 2 * L::kXBlocks * kMxSfBytes : 0)));
           const uint32_t fb = full0 + 8u * stage;
           const uint32_t sa = smem_base + stage * L::kStageBytes;
           auto load = [&](uint32_t dst, const void* map, int x, int y) {
@@ -364,7 +395,7 @@ mx_gemm_kernel(const __grid_constant__ MxParams p) {
           load(sa, &p.tmap_w, kb * kRowBytes, wrow);
           load(sa + L::kABytes, &p.tmap_x, kb * kRowBytes, xrow);
           load(sa + L::kSfOffset, &p.tmap_sw, kb * 256, tl.w_block + half);
-          load(sa + L::kSfOffset + 2 * kMxSfBytes, &p.tmap_sx, kb * 256, tl.x_block);
+          if (!L::kGather) load(sa + L::kSfOffset + 2 * kMxSfBytes, &p.tmap_sx, kb * 256, tl.x_block);
           if (++stage == STAGES) {
             stage = 0;
             phase ^= 1u;
@@ -431,7 +462,7 @@ mx_gemm_kernel(const __grid_constant__ MxParams p) {
           for (int k = 0; k < 4; ++k) {
             const uint32_t sfa = sf + (k >> 1) * GC;
             umma_mxf4<CTA2>(d, a_desc0 + off + 2u * k, b_desc0 + off + 2u * k, mx_idesc(UM, BN, (k & 1) * 2), sfa,
-                            sfa + 4 + (BN % 128 == 0 ? 0 : tl.x_col), (kb > 0 || k > 0) ? 1u : 0u);
+                            sfa + 4 + (BN % 128 == 0 || L::kGather ? 0 : tl.x_col), (kb > 0 || k > 0) ? 1u : 0u);
           }
           if (CTA2) umma_commit_2cta(bar_empty(stage), 3); else umma_commit(bar_empty(stage));
           if (++stage == STAGES) {
@@ -449,7 +480,7 @@ mx_gemm_kernel(const __grid_constant__ MxParams p) {
         mbar_wait(bar_retired, 0, AbortWord{nullptr, 0u}, 0, 2000000ull);
       }
     }
-  } else {
+  } else if (warp < 2 + kMxEpiWarps) {
     // ------------------------------------------------------------- epilogue
     const int quad = warp & 3, first = (warp - 2) >> 2;
     const uint32_t tmem_quad = tmem_base + (static_cast<uint32_t>(quad * 32) << 16);
@@ -506,6 +537,55 @@ mx_gemm_kernel(const __grid_constant__ MxParams p) {
       }
       if (!OVERLAP) give_back();
     }
+  } else if constexpr (L::kGather) {
+    // ------------------------------------------------ scales of grouped tokens
+    // four stages at a time, the next four's words already on their way: a pair at a time, the warp's loads took as long as the
+    // stages' copies (64 experts of 6 tokens x 2048 x 2048 33.3 us)
+    static_assert(L::kXBlocks == 1, "one block of rows");
+    constexpr int UN = 4;
+    auto fetch = [&](uint32_t (&w)[UN][2][4], const MxTile& x, int kb) {
+#pragma unroll
+      for (int u = 0; u < UN; ++u) mx_gather_scales<BN>(w[u], p, x.m0, x.m_end, kb + u, lane);
+    };
+    int stage = 0, t = worker, kb = 0;
+    uint32_t phase = 1;
+    MxTile tl;
+    uint32_t cur[UN][2][4], nxt[UN][2][4];
+    bool more = mx_tile<BN, GROUPED>(p, TILE_N, t, groups, tl);
+    if (more) fetch(cur, tl, 0);
+    bool ok = true;
+    while (more && ok) {
+      const int n = p.num_kb - kb < UN ? p.num_kb - kb : UN;
+      kb += UN;
+      if (kb >= p.num_kb) {
+        kb = 0;
+        t += workers;
+        more = mx_tile<BN, GROUPED>(p, TILE_N, t, groups, tl);
+      }
+      if (more) fetch(nxt, tl, kb);
+#pragma unroll
+      for (int u = 0; u < UN; ++u) {
+        if (u >= n || !ok) break;
+        if (!__all_sync(0xffffffffu, mbar_wait(bar_empty(stage), phase, ab, kStatusTimeoutSmemEmpty, budget))) {
+          ok = false;
+          break;
+        }
+        mx_put_scales(cur[u], smem_base + stage * L::kStageBytes + L::kSfOffset + 2 * kMxSfBytes, lane);
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar_full(stage));
+        if (++stage == STAGES) {
+          stage = 0;
+          phase ^= 1u;
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < UN; ++u)
+#pragma unroll
+        for (int g = 0; g < 2; ++g)
+#pragma unroll
+          for (int q = 0; q < 4; ++q) cur[u][g][q] = nxt[u][g][q];
+    }
   }
 
   // ------------------------------------------------------------------ teardown
@@ -523,17 +603,19 @@ mx_gemm_kernel(const __grid_constant__ MxParams p) {
 
 // The tokens' scale blocks of a grouped launch with tiles of `bn` tokens: every expert's rows from a block's start on, the
 // expert's blocks where its tiles, each of as many blocks as it has starts of 128 rows, begin. A CTA per block, as many as
-// the experts could need; 16 bytes (four rows 32 apart) per thread and group of K.
-constexpr int kMxRegroupThreads = 256;
+// the experts could need, and 8 groups of K; 16 bytes (four rows 32 apart) per thread.
+constexpr int kMxRegroupThreads = 256, kMxRegroupGroups = kMxRegroupThreads / 32;
 static __global__ void __launch_bounds__(kMxRegroupThreads)
-mx_regroup_kernel(const uint8_t* __restrict__ src, int rows, int groups, int bn, const int* __restrict__ splits, int nexperts, uint4* __restrict__ dst) {
+mx_regroup_kernel(const uint8_t* __restrict__ src, int rows, int groups, int parts, int bn, const int* __restrict__ splits, int nexperts,
+                  uint4* __restrict__ dst) {
   __shared__ int s_first, s_end;
   const int lane = threadIdx.x & 31;
+  const int block = static_cast<int>(blockIdx.x) / parts, part = static_cast<int>(blockIdx.x) - block * parts;
   pdl_wait();
   if (threadIdx.x == 0) pdl_trigger();
   if (threadIdx.x < 32) {
-    const int per = (bn + 127) / 128, tile = static_cast<int>(blockIdx.x) / per;
-    MxExperts x;
+    const int per = (bn + 127) / 128, tile = block / per;
+    MxExperts x(splits, nexperts, lane);
     int first = 0, end = 0;
     for (int e0 = 0; e0 < nexperts; e0 += 32) {
       x.next(splits, nexperts, rows, bn, e0, lane);
@@ -541,7 +623,7 @@ mx_regroup_kernel(const uint8_t* __restrict__ src, int rows, int groups, int bn,
       if (has == 0) continue;
       const int from = __ffs(has) - 1;
       const int before = __shfl_sync(0xffffffffu, x.tiles_end - x.tiles_mine, from);
-      first = __shfl_sync(0xffffffffu, x.first, from) + (static_cast<int>(blockIdx.x) - before * per) * 128;
+      first = __shfl_sync(0xffffffffu, x.first, from) + (block - before * per) * 128;
       end = __shfl_sync(0xffffffffu, x.end, from);
       break;
     }
@@ -553,16 +635,15 @@ mx_regroup_kernel(const uint8_t* __restrict__ src, int rows, int groups, int bn,
   __syncthreads();
   const int first = s_first, end = s_end;
   if (first >= end) return;
-  for (int i = threadIdx.x; i < groups * 32; i += kMxRegroupThreads) {
-    const int kg = i >> 5;
-    uint32_t w[4];
+  const int kg = part * kMxRegroupGroups + static_cast<int>(threadIdx.x >> 5);
+  if (kg >= groups) return;
+  uint32_t w[4];
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const int r = first + q * 32 + lane;
-      w[q] = r < end ? __ldg(reinterpret_cast<const uint32_t*>(src + mx_sf_offset(r, kg, groups))) : 0u;
-    }
-    dst[(static_cast<long long>(blockIdx.x) * groups + kg) * 32 + lane] = make_uint4(w[0], w[1], w[2], w[3]);
+  for (int q = 0; q < 4; ++q) {
+    const int r = first + q * 32 + lane;
+    w[q] = r < end ? __ldg(reinterpret_cast<const uint32_t*>(src + mx_sf_offset(r, kg, groups))) : 0u;
   }
+  dst[(static_cast<long long>(block) * groups + kg) * 32 + lane] = make_uint4(w[0], w[1], w[2], w[3]);
 }
 
 // ------------------------------------------------------------------------------------------------------- few tokens
@@ -597,7 +678,7 @@ struct MxFewLayout {
 template <int BN>
 __device__ __forceinline__ bool mx_few_tile(const MxParams& p, int t, int lane, MxTile& out) {
   const int g = t / p.n_tiles;
-  MxExperts x;
+  MxExperts x(p.splits, p.nexperts, lane);
   for (int e0 = 0; e0 < p.nexperts; e0 += 32) {
     x.next(p.splits, p.nexperts, p.rows_x, BN, e0, lane);
     const unsigned has = __ballot_sync(0xffffffffu, x.tiles_end > g);
@@ -840,15 +921,7 @@ mx_few_kernel(const __grid_constant__ MxParams p) {
         uint32_t w[UN][2][4];
 #pragma unroll
         for (int u = 0; u < UN; ++u)
-#pragma unroll
-          for (int g = 0; g < 2; ++g)
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-              const int kg = (kb0 + i0 + u) * 2 + g, r = q * 32 + lane;
-              w[u][g][q] = q * 32 < BN && r < cnt && i0 + u < nkb && kg < p.groups
-                               ? __ldg(reinterpret_cast<const uint32_t*>(p.sx + mx_sf_offset(tl.m0 + r, kg, p.groups)))
-                               : 0u;
-            }
+          if (i0 + u < nkb) mx_gather_scales<BN>(w[u], p, tl.m0, tl.m0 + cnt, kb0 + i0 + u, lane);
 #pragma unroll
         for (int u = 0; u < UN; ++u) {
           if (i0 + u >= nkb || !ok) break;
@@ -856,12 +929,7 @@ mx_few_kernel(const __grid_constant__ MxParams p) {
             ok = false;
             break;
           }
-          const uint32_t dst = smem_base + stage * L::kStageBytes + L::kSfOffset + 2 * kMxSfBytes + lane * 16;
-#pragma unroll
-          for (int g = 0; g < 2; ++g)
-            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst + g * kMxSfBytes), "r"(w[u][g][0]), "r"(w[u][g][1]), "r"(w[u][g][2]),
-                         "r"(w[u][g][3])
-                         : "memory");
+          mx_put_scales(w[u], smem_base + stage * L::kStageBytes + L::kSfOffset + 2 * kMxSfBytes, lane);
           fence_proxy_async_smem();
           __syncwarp();
           if (lane == 0) mbar_arrive(bar_base + 8u * stage);
