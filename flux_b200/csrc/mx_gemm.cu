@@ -1,4 +1,6 @@
 // Host side of the microscaled 4-bit GEMMs (mx_gemm.cuh): checks, tensor maps, which kernel and tile a shape gets.
+#include <math.h>
+
 #include "internal.h"
 #include "mx_gemm.cuh"
 
@@ -84,13 +86,72 @@ static int launch_mx_few(const fluxb_comm* comm, const MxParams& p, long long ti
   return mx_launch(kern, p, static_cast<int>(tiles * p.split), kMxFewThreads, MxFewLayout<BN>::kTotal, p.split, comm->world == 1, stream);
 }
 
-// Into how many parts along K the tiles of a few-token launch are cut: as many as keep all CTAs resident (two per SM up to
-// 64 tokens, one above), with at least 2 K blocks each.
-static int mx_few_split(int sm_count, long long tiles, int num_kb, int bn) {
-  const long long slots = bn <= 64 ? 2 * sm_count : sm_count;
-  int split = 1;
-  while (split < kMxFewMaxSplit && 2 * split * tiles <= slots && num_kb / (2 * split) >= 2) split *= 2;
-  return split;
+// Which kernel and tile a launch gets: the one whose time, estimated from what it has to do, is the shortest. The estimates
+// are linear in the launch's numbers, with coefficients (us) fitted to measured times of all variants on 148 problems
+// (dense 1 .. 4096 x 1024 .. 28672 x 1024 .. 8192; 8 to 128 experts, 2 to 65536 rows, of 1024 .. 14336 x 1024 .. 8192;
+// weights from memory, launches back to back in a graph). Over those problems the choice takes 2% longer than the fastest
+// variant on average, 24% at worst (64 x 4096 x 4096 6.7 us against 5.4, grouped 11%); one variant for all would be far off
+// on either side: 256 x 4096 x 4096 takes 5.9 us in tiles of 64 and 9.7 in tiles of 256, 4096 x 8192 x 8192 160 and 90.
+//   tiled:      fixed + waves * (per_stage * K blocks + per_wave) + per_mb * MB of weights (+ grouped)
+//   few tokens: fixed + per_stage * K blocks of a part + per_cta * CTAs per slot + per_block * K blocks per slot
+//               + per_mb * MB of weights (+ grouped)
+struct MxTileCost {
+  int bn, cg;
+  float fixed, per_stage, per_wave, per_mb, grouped;
+};
+constexpr MxTileCost kMxTileCosts[] = {
+    {64, 1, 1.58f, 0.142f, 0.712f, 0.1007f, 2.83f},  {128, 1, 1.33f, 0.191f, 1.159f, 0.0981f, 3.77f}, {64, 2, 2.32f, 0.121f, 0.609f, 0.0989f, 5.35f},
+    {128, 2, 2.43f, 0.153f, 0.918f, 0.0844f, 4.94f}, {192, 2, 2.46f, 0.222f, 1.131f, 0.0729f, 5.13f}, {256, 2, 3.05f, 0.293f, 1.160f, 0.0543f, 4.71f},
+};
+struct MxFewCost {
+  int bn;
+  float fixed, per_stage, per_cta, per_block, per_mb, grouped;
+};
+constexpr MxFewCost kMxFewCosts[] = {
+    {16, 0.87f, 0.216f, 5.49f, 0.147f, 0.079f, 0.26f}, {32, 0.79f, 0.249f, 5.61f, 0.073f, 0.099f, 0.24f}, {64, 1.06f, 0.260f, 5.78f, 0.031f, 0.110f, 0.11f},
+};
+struct MxChoice {
+  int bn = 0, cg = 0, split = 0;  // split > 0: the few-token kernel
+};
+// `nexperts` 0: dense. `want_bn`, `want_cg`: the caller's choice of a kernel and tile, 0 = none.
+static MxChoice mx_choose(int sm_count, int nexperts, int rows, int n, int num_kb, double weight_mb, int want_bn, int want_cg) {
+  double used = 1.0, per = rows, longest = rows;
+  if (nexperts > 0) {
+    // experts that get rows if every row falls on one at random, and a good guess at what the longer of them get
+    used = nexperts > 1 ? nexperts * (1.0 - exp(rows * log1p(-1.0 / nexperts))) : 1.0;
+    per = rows / used;
+    longest = per + sqrt(per);
+  }
+  auto token_tiles = [&](int bn) {
+    if (nexperts == 0) return ceil(static_cast<double>(rows) / bn);
+    return longest <= 4.0 * bn ? used * ceil(longest / bn) : used * (per / bn + 0.5);
+  };
+  const double mb = used * weight_mb, grouped = nexperts > 0 ? 1.0 : 0.0;
+  MxChoice best;
+  double least = 0.0;
+  auto offer = [&](double us, int bn, int cg, int split) {
+    if (best.bn != 0 && us >= least) return;
+    best.bn = bn;
+    best.cg = cg;
+    best.split = split;
+    least = us;
+  };
+  for (const MxTileCost& c : kMxTileCosts) {
+    if ((want_bn != 0 || want_cg != 0) && (c.cg != want_cg || (want_bn != 0 && c.bn != want_bn))) continue;
+    const double tiles = token_tiles(c.bn) * ((n + kBM * c.cg - 1) / (kBM * c.cg));
+    const double waves = ceil(tiles / (sm_count / c.cg) - 1e-9);
+    offer(c.fixed + waves * (c.per_stage * num_kb + c.per_wave) + c.per_mb * mb + c.grouped * grouped, c.bn, c.cg, 0);
+  }
+  for (const MxFewCost& c : kMxFewCosts) {
+    if (want_cg != 0 || (want_bn != 0 ? c.bn != want_bn : per > 96)) continue;
+    if (nexperts == 0 && c.bn < 64 && rows > c.bn) continue;  // (see mx_run)
+    const double tiles = token_tiles(c.bn) * ((n + kBM - 1) / kBM);
+    for (int split = 1; split <= kMxFewMaxSplit && split <= num_kb; split *= 2)
+      offer(c.fixed + c.per_stage * num_kb / split + c.per_cta * tiles * split / (2 * sm_count) + c.per_block * tiles * num_kb / (2 * sm_count) + c.per_mb * mb +
+                c.grouped * grouped,
+            c.bn, 1, split);
+  }
+  return best;
 }
 
 static int mx_out_type(int out_dtype, int* ot) {
@@ -106,24 +167,18 @@ static int mx_out_type(int out_dtype, int* ot) {
 // more than they fill.
 static long long mx_most_tiles(int rows, int nexperts, int bn) { return static_cast<long long>(rows) / bn + (nexperts < rows ? nexperts : rows); }
 
-// `per_group` = tokens that an expert gets on average (dense: all of them)
 template <bool GROUPED>
-static int mx_run(fluxb_comm* comm, MxParams& p, const void* xq, const void* wq, const void* ws, void* workspace, int k, int per_group,
-                  const fluxb_tuning* tuning, cudaStream_t stream) {
+static int mx_run(fluxb_comm* comm, MxParams& p, const void* xq, const void* wq, const void* ws, void* workspace, int k, const fluxb_tuning* tuning,
+                  cudaStream_t stream) {
   const int want_bn = tuning != nullptr ? tuning->block_n : 0, want_cg = tuning != nullptr ? tuning->cta_group : 0;
   const long long row_bytes = k / 2;
-  const bool few = want_cg == 0 && (want_bn != 0 ? want_bn <= 128 : per_group <= 128);
-  int bn = want_bn, cg = want_cg;
-  if (few) {
-    if (bn == 0) bn = per_group <= 16 ? 16 : per_group <= 32 ? 32 : per_group <= 64 ? 64 : 128;
-    // the scales of a tile must start at an even column of tensor memory, that is at a multiple of 64 rows of a block
-    // (an odd column raised a misaligned address); a grouped launch moves its tokens' scales to the tile's start
-    FLUXB_REQUIRE(GROUPED || bn >= 64 || p.rows_x <= bn, "mx_gemm: block_n=%d is for up to %d tokens", bn, bn);
-    cg = 1;
-  } else {
-    if (cg == 0) cg = 2;
-    if (bn == 0) bn = 256;
-  }
+  // the scales of a tile must start at an even column of tensor memory, that is at a multiple of 64 rows of a block (an odd
+  // column raised a misaligned address); a grouped launch moves its tokens' scales to the tile's start
+  FLUXB_REQUIRE(GROUPED || want_cg != 0 || want_bn == 0 || want_bn >= 64 || p.rows_x <= want_bn, "mx_gemm: block_n=%d is for up to %d tokens", want_bn,
+                want_bn);
+  const MxChoice choice = mx_choose(comm->sm_count, p.nexperts, p.rows_x, p.N, p.num_kb, p.N * (row_bytes + k / kMxBlock) * 1e-6, want_bn, want_cg);
+  FLUXB_REQUIRE(choice.bn != 0, "mx_gemm: block_n=%d cta_group=%d is not {16,32,64} with 0, {64,128} with 1 or {64,128,192,256} with 2", want_bn, want_cg);
+  const int bn = choice.bn, cg = choice.cg;
   const int tile_n = cg * kBM;
   const int groups = GROUPED ? p.nexperts : 1;
   p.n_tiles = (p.N + tile_n - 1) / tile_n;
@@ -146,18 +201,12 @@ static int mx_run(fluxb_comm* comm, MxParams& p, const void* xq, const void* wq,
     rc = encode_tmap_words(&p.tmap_sx, blocks, GROUPED ? most_blocks : (p.rows_x + 127) / 128, words, (bn + 127) / 128);
     if (rc != FLUXB_OK) return rc;
   }
-  if (few) {
-    p.split = mx_few_split(comm->sm_count, GROUPED ? static_cast<long long>(groups) * p.n_tiles : tiles, p.num_kb, bn);
-    switch (bn) {
-      case 16: return launch_mx_few<16, GROUPED>(comm, p, tiles, stream);
-      case 32: return launch_mx_few<32, GROUPED>(comm, p, tiles, stream);
-      case 64: return launch_mx_few<64, GROUPED>(comm, p, tiles, stream);
-      case 128: return launch_mx_few<128, GROUPED>(comm, p, tiles, stream);
-      default: FLUXB_FAIL(FLUXB_ERR_INVALID, "mx_gemm: block_n=%d not in {16,32,64,128} for few tokens", bn);
-    }
+  p.split = choice.split;
+  if (p.split > 0) {
+    if (bn == 16) return launch_mx_few<16, GROUPED>(comm, p, tiles, stream);
+    if (bn == 32) return launch_mx_few<32, GROUPED>(comm, p, tiles, stream);
+    return launch_mx_few<64, GROUPED>(comm, p, tiles, stream);
   }
-  FLUXB_REQUIRE(cg == 2 ? bn == 64 || bn == 128 || bn == 192 || bn == 256 : cg == 1 && (bn == 64 || bn == 128),
-                "mx_gemm: block_n=%d cta_group=%d is not {64,128} with 1 or {64,128,192,256} with 2", bn, cg);
   if (GROUPED && cg == 2) {
     const int parts = (p.groups + kMxRegroupGroups - 1) / kMxRegroupGroups;
     FLUXB_REQUIRE(most_blocks * parts < (1ll << 30), "mx_grouped_gemm: %d rows of %d groups are too many", p.rows_x, p.groups);
@@ -226,7 +275,7 @@ int fluxb_mx_gemm(fluxb_comm_t comm, const void* xq, const void* xs, const void*
   FLUXB_REQUIRE((reinterpret_cast<uintptr_t>(bias) & (p.out_type == kOutF32 ? 3 : 1)) == 0, "mx_gemm: the bias is not aligned to its type");
   p.rows_x = m;
   p.bias = bias;
-  return mx_run<false>(comm, p, xq, wq, ws, nullptr, k, m, tuning, static_cast<cudaStream_t>(stream));
+  return mx_run<false>(comm, p, xq, wq, ws, nullptr, k, tuning, static_cast<cudaStream_t>(stream));
 }
 
 int fluxb_mx_grouped_gemm(fluxb_comm_t comm, const void* xq, const void* xs, int rows, const void* wq, const void* ws, int nexperts,
@@ -244,8 +293,7 @@ int fluxb_mx_grouped_gemm(fluxb_comm_t comm, const void* xq, const void* xs, int
   p.rows_x = rows;
   p.nexperts = nexperts;
   p.splits = splits_dev;
-  const int used = nexperts < rows ? nexperts : rows;
-  return mx_run<true>(comm, p, xq, wq, ws, workspace, k, (rows + used - 1) / used, tuning, static_cast<cudaStream_t>(stream));
+  return mx_run<true>(comm, p, xq, wq, ws, workspace, k, tuning, static_cast<cudaStream_t>(stream));
 }
 
 }  // extern "C"

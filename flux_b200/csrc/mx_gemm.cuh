@@ -647,7 +647,7 @@ mx_regroup_kernel(const uint8_t* __restrict__ src, int rows, int groups, int par
 }
 
 // ------------------------------------------------------------------------------------------------------- few tokens
-// Few tokens (up to 128, or a few per expert), where the time is that of reading the weights once and of getting started:
+// Few tokens (up to 64, or a few per expert), where the time is that of reading the weights once and of getting started:
 // one output tile per cluster of `split` CTAs, which cut K. Each CTA leaves its accumulator in its own shared memory; after
 // a cluster barrier CTA r sums the tokens r * per ... of all parts, in rank order, through distributed shared memory: no
 // scratch, no counters, any number of launches side by side. A grouped launch has a cluster for every tile that the
@@ -662,12 +662,13 @@ struct MxFewLayout {
   static constexpr int kBBytes = BN * kRowBytes;
   static constexpr int kSfOffset = kABytes + kBBytes;
   static constexpr int kStageBytes = kSfOffset + 4 * kMxSfBytes;
-  // up to 64 tokens a CTA takes half of an SM's shared memory, so that one CTA's prologue and reduction overlap another's loads
-  static constexpr int kStages = BN == 16 ? 5 : BN <= 64 ? 4 : 6;
-  static_assert(BN <= 128 && kStages * kStageBytes >= BN * kBM * 4, "the read-out must fit into the stages");
+  // a CTA takes half of an SM's shared memory, so that one CTA's prologue and reduction overlap another's loads
+  static constexpr int kStages = BN == 16 ? 5 : 4;
+  static_assert(BN <= 64 && kStages * kStageBytes >= BN * kBM * 4, "the read-out must fit into the stages");
   static constexpr int kSfCols = 16;
   static constexpr int kColsUsed = BN + kStages * kSfCols;
-  static constexpr uint32_t kTmemCols = kColsUsed <= 128 ? 128 : 256;
+  static constexpr uint32_t kTmemCols = 128;
+  static_assert(kColsUsed <= 128, "two CTAs' tensor memory");
   static constexpr int kNumBars = 2 * kStages + 2;  // full / empty per stage, accumulator complete, "UMMAs retired" (abort path)
   static constexpr int kBarOffset = kStages * kStageBytes;
   static constexpr int kMiscOffset = kBarOffset + kNumBars * 8;

@@ -320,8 +320,8 @@ int fluxb_moe_scatter_gemm_static(fluxb_comm_t comm, const void* tokens, int nto
  * fluxb_mx_grouped_workspace_bytes, 16-byte aligned, this call's own until it has run.
  * Nothing here allocates; calls on several streams and in captured graphs may run side by side.
  * `comm`: a communicator of the current device (status word, time-out). tuning: cta_group 1 or 2 selects the tiled kernel
- * (block_n tokens: 64 or 128 with 1; 64, 128, 192 or 256 with 2), cta_group 0 with block_n 64 or 128, or 16 or
- * 32 for no more tokens than that (grouped: any number), the few-token one. */
+ * (block_n tokens: 64 or 128 with 1; 64, 128, 192 or 256 with 2), cta_group 0 with block_n 64, or 16 or 32 for no more
+ * tokens than that (grouped: any number), the few-token one. */
 size_t fluxb_mx_scale_bytes(int batch, int rows, int k);
 size_t fluxb_mx_grouped_workspace_bytes(int rows, int nexperts, int k);
 int fluxb_mx_quantize(const void* x, int dtype, int batch, int rows, int k, long long ldx, void* data, void* scales,

@@ -12,7 +12,7 @@ pytestmark = pytest.mark.gpu
 
 GRID = torch.tensor([0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0], dtype=torch.float64)
 # every kernel and tile: the library's choice, the few-token kernel, single CTAs, CTA pairs
-TILES = [None] + [{"block_n": b} for b in (16, 32, 64, 128)] + [{"block_n": b, "cta_group": 1} for b in (64, 128)] \
+TILES = [None] + [{"block_n": b} for b in (16, 32, 64)] + [{"block_n": b, "cta_group": 1} for b in (64, 128)] \
     + [{"block_n": b, "cta_group": 2} for b in (64, 128, 192, 256)]
 
 
