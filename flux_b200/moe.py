@@ -63,7 +63,8 @@ _FLOATS = (torch.float32, torch.bfloat16, torch.float16)
 
 def _on_device(t: torch.Tensor) -> bool:
     """The library launches on the current device: tensors of another one are refused."""
-    return t.is_cuda and t.device.index == _cur_device()
+    d = t.get_device()  # -1 off the GPU
+    return d >= 0 and d == _cur_device()
 
 
 def _check_index(name: str, splits: torch.Tensor, scatter_index: torch.Tensor, ntokens: Optional[int] = None) -> None:
@@ -78,8 +79,8 @@ def _check_index(name: str, splits: torch.Tensor, scatter_index: torch.Tensor, n
 
 def _route_forward(logits: torch.Tensor, topk: int):
     ntokens, nexperts = logits.shape
-    chosen = torch.empty((ntokens, topk), dtype=torch.int32, device=logits.device)
-    weights = torch.empty((ntokens, topk), dtype=torch.float32, device=logits.device)
+    chosen = logits.new_empty((ntokens, topk), dtype=torch.int32)
+    weights = logits.new_empty((ntokens, topk), dtype=torch.float32)
     _lib.check(_lib.load().fluxb_moe_route(logits.data_ptr(), fluxb_dtype(logits.dtype), ntokens, nexperts, topk, chosen.data_ptr(),
                                            weights.data_ptr(), _cur_stream()))
     return chosen, weights
@@ -91,16 +92,19 @@ class _RouteFn(torch.autograd.Function):
         chosen, weights = _route_forward(logits, topk)
         ctx.save_for_backward(chosen, weights)
         ctx.mark_non_differentiable(chosen)
+        ctx.set_materialize_grads(False)  # no zeros in the place of the gradient that `chosen` does not have
         ctx.like = (logits.dtype, logits.shape[1])
         return chosen, weights
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, _, dweights):
+        if dweights is None:
+            return None, None
         chosen, weights = ctx.saved_tensors
         dtype, nexperts = ctx.like
         ntokens, topk = chosen.shape
-        dlogits = torch.empty((ntokens, nexperts), dtype=dtype, device=chosen.device)
+        dlogits = chosen.new_empty((ntokens, nexperts), dtype=dtype)
         _lib.check(_lib.load().fluxb_moe_route_backward(
             dweights.contiguous().data_ptr(), chosen.data_ptr(), weights.data_ptr(), fluxb_dtype(dtype), ntokens, nexperts, topk,
             dlogits.data_ptr(), _cur_stream()))
@@ -128,8 +132,9 @@ def _permute(tokens: torch.Tensor, splits: torch.Tensor, scatter_index: torch.Te
     ntokens, topk = scatter_index.shape
     if not tokens.is_contiguous():
         tokens = tokens.contiguous()
-    rows = torch.empty((ntokens * topk, tokens.shape[1]), dtype=tokens.dtype, device=tokens.device)
-    _lib.check(_lib.load().fluxb_moe_permute(tokens.data_ptr(), ntokens, topk, tokens.shape[1] * tokens.element_size(), splits.data_ptr(),
+    hidden = tokens.shape[1]
+    rows = tokens.new_empty((ntokens * topk, hidden))
+    _lib.check(_lib.load().fluxb_moe_permute(tokens.data_ptr(), ntokens, topk, hidden * tokens.element_size(), splits.data_ptr(),
                                              splits.numel(), scatter_index.data_ptr(), rows.data_ptr(), _cur_stream()))
     return rows
 
@@ -138,8 +143,9 @@ def _unpermute(rows: torch.Tensor, scatter_index: torch.Tensor, weights: Optiona
     ntokens, topk = scatter_index.shape
     if not rows.is_contiguous():
         rows = rows.contiguous()
-    out = torch.empty((ntokens, rows.shape[1]), dtype=rows.dtype, device=rows.device)
-    _lib.check(_lib.load().fluxb_moe_unpermute(rows.data_ptr(), fluxb_dtype(rows.dtype), ntokens, topk, rows.shape[1], scatter_index.data_ptr(),
+    hidden = rows.shape[1]
+    out = rows.new_empty((ntokens, hidden))
+    _lib.check(_lib.load().fluxb_moe_unpermute(rows.data_ptr(), fluxb_dtype(rows.dtype), ntokens, topk, hidden, scatter_index.data_ptr(),
                                                _ptr(weights), 0 if weights is None else fluxb_dtype(weights.dtype), out.data_ptr(), _cur_stream()))
     return out
 
@@ -175,10 +181,10 @@ class _UnpermuteFn(torch.autograd.Function):
         dout = dout.contiguous()
         drows = dweights = None
         if ctx.needs_input_grad[0]:
-            drows = torch.empty((ntokens * topk, hidden), dtype=dtype, device=dout.device)
+            drows = dout.new_empty((ntokens * topk, hidden))
         if ctx.needs_input_grad[3]:
             # pairs without an expert get a gradient of zero like the others get theirs: the kernel writes every entry
-            dweights = torch.empty((ntokens, topk), dtype=weights.dtype, device=dout.device)
+            dweights = torch.empty_like(weights)
             rows = rows.contiguous()
         else:
             rows = None

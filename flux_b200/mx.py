@@ -10,6 +10,7 @@ are e2m1 (0, 0.5, 1, 1.5, 2, 3, 4, 6 and their negatives), two to a byte, the fi
 """
 from __future__ import annotations
 
+import math
 from typing import Dict, Optional
 
 import torch
@@ -107,9 +108,7 @@ def mx_quantize(x: torch.Tensor, splits: Optional[torch.Tensor] = None, scatter_
     *lead, n, k = x.shape
     if lead or x.stride(1) != 1:
         x = x.contiguous()
-    batch, out_rows, topk, nexperts = 1, n, 0, 0
-    for b in lead:
-        batch *= b
+    batch, out_rows, topk, nexperts = math.prod(lead), n, 0, 0
     if scatter_index is None:
         _check(splits is None, "mx_quantize: splits and scatter_index belong together")
     else:
@@ -117,8 +116,8 @@ def mx_quantize(x: torch.Tensor, splits: Optional[torch.Tensor] = None, scatter_
         _check_index("mx_quantize", splits, scatter_index, n)
         topk, nexperts = scatter_index.shape[1], splits.numel()
         out_rows = n * topk
-    data = torch.empty((*lead, out_rows, k // 2), dtype=torch.uint8, device=x.device)
-    blocks = torch.empty(_blocks_shape(lead, out_rows, k), dtype=torch.uint8, device=x.device)
+    data = x.new_empty((*lead, out_rows, k // 2), dtype=torch.uint8)
+    blocks = x.new_empty(_blocks_shape(lead, out_rows, k), dtype=torch.uint8)
     _lib.check(_lib.load().fluxb_mx_quantize(x.data_ptr(), fluxb_dtype(x.dtype), batch, n, k, x.stride(-2), data.data_ptr(), blocks.data_ptr(),
                                              _ptr(splits), nexperts, _ptr(scatter_index), topk, _cur_stream()))
     return MXTensor._of(data, blocks, k)
@@ -129,26 +128,25 @@ def mx_dequantize(q: MXTensor, dtype: torch.dtype = torch.bfloat16) -> torch.Ten
     _check(isinstance(q, MXTensor) and _on_device(q.data), "mx_dequantize: q must be an MXTensor on the current CUDA device")
     _check(dtype in _FLOATS, "mx_dequantize: the output must be fp32, bf16 or fp16")
     *lead, n, _ = q.data.shape
-    out = torch.empty((*lead, n, q.k), dtype=dtype, device=q.data.device)
-    batch = 1
-    for b in lead:
-        batch *= b
-    _lib.check(_lib.load().fluxb_mx_dequantize(q.data.data_ptr(), q.blocks.data_ptr(), batch, n, q.k, fluxb_dtype(dtype), out.data_ptr(), _cur_stream()))
+    out = q.data.new_empty((*lead, n, q.k), dtype=dtype)
+    _lib.check(_lib.load().fluxb_mx_dequantize(q.data.data_ptr(), q.blocks.data_ptr(), math.prod(lead), n, q.k, fluxb_dtype(dtype), out.data_ptr(), _cur_stream()))
     return out
 
 
 def _check_operands(name: str, x: MXTensor, w: MXTensor, wdim: int, output_dtype: torch.dtype) -> None:
-    _check(isinstance(x, MXTensor) and isinstance(w, MXTensor) and x.data.dim() == 2 and w.data.dim() == wdim,
-           f"{name}: operands must be MXTensors, [rows, K] and {'[N, K]' if wdim == 2 else '[nexperts, N, K]'}")
-    _check(_on_device(x.data) and _on_device(w.data), f"{name}: operands must be on the current CUDA device")
+    if not (isinstance(x, MXTensor) and isinstance(w, MXTensor) and x.data.dim() == 2 and w.data.dim() == wdim):
+        raise RuntimeError(f"{name}: operands must be MXTensors, [rows, K] and {'[N, K]' if wdim == 2 else '[nexperts, N, K]'}")
+    if not (_on_device(x.data) and _on_device(w.data)):
+        raise RuntimeError(f"{name}: operands must be on the current CUDA device")
     if x.k != w.k:
         raise RuntimeError(f"{name}: weight K {w.k} != input K {x.k}")
-    _check(output_dtype in _FLOATS, f"{name}: the output must be fp32, bf16 or fp16")
+    if output_dtype not in _FLOATS:
+        raise RuntimeError(f"{name}: the output must be fp32, bf16 or fp16")
 
 
-def _output(name: str, output: Optional[torch.Tensor], rows: int, n: int, dtype: torch.dtype, device) -> torch.Tensor:
+def _output(name: str, output: Optional[torch.Tensor], rows: int, n: int, dtype: torch.dtype, like: torch.Tensor) -> torch.Tensor:
     if output is None:
-        return torch.empty((rows, n), dtype=dtype, device=device)
+        return like.new_empty((rows, n), dtype=dtype)
     _check(_on_device(output) and tuple(output.shape) == (rows, n) and output.dtype == dtype and output.is_contiguous(),
            f"{name}: output has the wrong shape, dtype or layout")
     return output
@@ -163,7 +161,7 @@ def mx_gemm(x: MXTensor, w: MXTensor, bias: Optional[torch.Tensor] = None, outpu
     if bias is not None:
         _check(_on_device(bias) and bias.dtype == output_dtype and tuple(bias.shape) in ((n,), (1, n)) and bias.is_contiguous(),
                "mx_gemm: bias must be a contiguous [N] tensor of the output's type")
-    out = _output("mx_gemm", output, m, n, output_dtype, x.data.device)
+    out = _output("mx_gemm", output, m, n, output_dtype, x.data)
     if n == 0:
         return out
     _lib.check(_lib.load().fluxb_mx_gemm(_comm().handle, x.data.data_ptr(), x.blocks.data_ptr(), w.data.data_ptr(), w.blocks.data_ptr(), out.data_ptr(),
@@ -181,11 +179,11 @@ def mx_grouped_gemm(x: MXTensor, w: MXTensor, splits: torch.Tensor, output_dtype
     rows = x.data.shape[0]
     if not (_on_device(splits) and splits.dtype == torch.int32 and splits.dim() == 1 and splits.numel() == nexperts and splits.is_contiguous()):
         raise RuntimeError(f"mx_grouped_gemm: splits must be a contiguous int32 [{nexperts}] tensor on the current CUDA device")
-    out = _output("mx_grouped_gemm", output, rows, n, output_dtype, x.data.device)
+    out = _output("mx_grouped_gemm", output, rows, n, output_dtype, x.data)
     if n == 0 or nexperts == 0:
         return out
     lib = _lib.load()
-    workspace = torch.empty((lib.fluxb_mx_grouped_workspace_bytes(rows, nexperts, x.k),), dtype=torch.uint8, device=out.device)
+    workspace = x.data.new_empty(lib.fluxb_mx_grouped_workspace_bytes(rows, nexperts, x.k))
     _lib.check(lib.fluxb_mx_grouped_gemm(_comm().handle, x.data.data_ptr(), x.blocks.data_ptr(), rows, w.data.data_ptr(), w.blocks.data_ptr(), nexperts,
                                          splits.data_ptr(), out.data_ptr(), n, x.k, fluxb_dtype(output_dtype), workspace.data_ptr(), _tuning(tuning),
                                          _cur_stream()))
