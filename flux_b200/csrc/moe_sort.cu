@@ -12,8 +12,9 @@ namespace fluxb {
 // ----------------------------------------------------------------------------------------------------------- route
 // z: logits of a token. chosen = the topk largest (ties: the lower expert), w = softmax over the chosen ones:
 //   w_j = exp(z_j - z_max) / sum_i exp(z_i - z_max),   dz_j = w_j (dw_j - sum_i w_i dw_i),   0 for the others.
-// One warp per token, its logits in registers as order-preserving integers; a choice is two warp-wide integer
-// reductions (the largest key, the lowest expert that has it), and only the lane that held it looks for its next one.
+// A group of G lanes per token, VPL logits a lane in registers as order-preserving integers: a choice is a maximum over
+// (key, lower expert first) among the lanes, and only the lane that held it looks for its next one. Bound by the latency
+// of that chain, so a warp takes as many tokens as it can: 32768 tokens of 8 experts top-2 took 9.0 us with a warp each.
 constexpr int kRouteThreads = 128;
 constexpr int kRouteMaxExperts = 1024;
 constexpr int kRouteMaxTopk = 32;
@@ -47,94 +48,116 @@ __device__ __forceinline__ float route_value(uint32_t key) {
   return __uint_as_float((key & 0x80000000u) ? key ^ 0x80000000u : ~key);
 }
 
-template <class T, int VPL>
+template <class T, int G, int VPL>
 __global__ void __launch_bounds__(kRouteThreads)
-moe_route_kernel(const T* __restrict__ logits, int ntokens, int nexperts, int topk, int* __restrict__ chosen, float* __restrict__ weights) {
-  const int lane = threadIdx.x & 31;
-  const int t = static_cast<int>((static_cast<long long>(blockIdx.x) * kRouteThreads + threadIdx.x) >> 5);
+moe_route_kernel(const T* __restrict__ logits, int ntokens, int nexperts, int topk, int vectors, int* __restrict__ chosen, float* __restrict__ weights) {
+  const int lane = threadIdx.x & (G - 1);
+  const int t = static_cast<int>((static_cast<long long>(blockIdx.x) * kRouteThreads + threadIdx.x) / G);
   pdl_wait();
   if (threadIdx.x == 0) pdl_trigger();
-  if (t >= ntokens) return;
-  const T* z = logits + static_cast<long long>(t) * nexperts;
+  const bool live = t < ntokens;  // (all lanes of a warp meet at the shuffles)
+  const T* z = logits + static_cast<long long>(live ? t : 0) * nexperts;
+  const int first = lane * VPL;  // this lane's experts
   uint32_t key[VPL];
+  constexpr int PER = 16 / static_cast<int>(sizeof(T));
+  if (VPL % PER == 0 && vectors) {
 #pragma unroll
-  for (int i = 0; i < VPL; ++i) key[i] = lane + 32 * i < nexperts ? route_key(to_f32(z[lane + 32 * i])) : 0u;
-  uint32_t best = 0;
-  int at = 0;
+    for (int i = 0; i < VPL / PER; ++i) {
+      union {
+        uint4 v;
+        T e[PER];
+      } x;
+      if (first + i * PER < nexperts) x.v = __ldg(reinterpret_cast<const uint4*>(z + first) + i);
+#pragma unroll
+      for (int j = 0; j < PER; ++j) key[i * PER + j] = first + i * PER + j < nexperts ? route_key(to_f32(x.e[j])) : 0u;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) key[i] = first + i < nexperts ? route_key(to_f32(z[first + i])) : 0u;
+  }
+  unsigned long long best = 0;  // key and expert of this lane's largest, the lower expert the larger
   auto look = [&] {
-    best = 0;
-    at = 0;
+    uint32_t k = 0;
+    int at = 0;
 #pragma unroll
     for (int i = 0; i < VPL; ++i)
-      if (key[i] > best) {
-        best = key[i];
+      if (key[i] > k) {
+        k = key[i];
         at = i;
       }
+    best = k == 0u ? 0ull : (static_cast<unsigned long long>(k) << 32) | (0xFFFFFFFFu - static_cast<uint32_t>(first + at));
   };
   look();
-  int mine = -1;         // lane j: choice j
+  int mine = -1;  // lane j: choice j
   uint32_t mine_key = 0;
   for (int j = 0; j < topk; ++j) {
-    const uint32_t top = __reduce_max_sync(0xffffffffu, best);
-    if (top == 0u) break;  // nothing left that may be chosen
-    const unsigned e = __reduce_min_sync(0xffffffffu, best == top ? static_cast<unsigned>(lane + 32 * at) : 0x7FFFFFFFu);
-    if (lane == j) {
-      mine = static_cast<int>(e);
-      mine_key = top;
+    unsigned long long top = best;
+#pragma unroll
+    for (int off = G / 2; off > 0; off >>= 1) {
+      const unsigned long long o = __shfl_xor_sync(0xffffffffu, top, off);
+      top = o > top ? o : top;
     }
-    if (static_cast<int>(e & 31u) == lane) {
+    if (top == 0ull) continue;  // nothing left that may be chosen (in this group)
+    const int e = static_cast<int>(0xFFFFFFFFu - static_cast<uint32_t>(top));
+    if (lane == j) {
+      mine = e;
+      mine_key = static_cast<uint32_t>(top >> 32);
+    }
+    if (best == top) {
 #pragma unroll
       for (int i = 0; i < VPL; ++i)
-        if (static_cast<int>(e >> 5) == i) key[i] = 0u;
+        if (first + i == e) key[i] = 0u;
       look();
     }
   }
   const float v = route_value(mine_key);
-  const float top_v = __shfl_sync(0xffffffffu, v, 0);
+  const float top_v = __shfl_sync(0xffffffffu, v, 0, G);
   const float p = mine >= 0 ? expf(v - top_v) : 0.0f;
   float sum = p;
 #pragma unroll
-  for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
-  if (lane < topk) {
+  for (int off = G / 2; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+  if (live && lane < topk) {
     const long long o = static_cast<long long>(t) * topk + lane;
     chosen[o] = mine;
     weights[o] = mine >= 0 ? p / sum : 0.0f;
   }
 }
 
-template <class T>
+// The row is cleared, then lane j writes the gradient of choice j: ordered by the warp's barrier.
+template <class T, int G>
 __global__ void __launch_bounds__(kRouteThreads)
 moe_route_backward_kernel(const float* __restrict__ dweights, const int* __restrict__ chosen, const float* __restrict__ weights,
-                          int ntokens, int nexperts, int topk, T* __restrict__ dlogits) {
-  const int lane = threadIdx.x & 31;
-  const int t = static_cast<int>((static_cast<long long>(blockIdx.x) * kRouteThreads + threadIdx.x) >> 5);
+                          int ntokens, int nexperts, int topk, int vectors, T* __restrict__ dlogits) {
+  const int lane = threadIdx.x & (G - 1);
+  const int t = static_cast<int>((static_cast<long long>(blockIdx.x) * kRouteThreads + threadIdx.x) / G);
   pdl_wait();
   if (threadIdx.x == 0) pdl_trigger();
-  if (t >= ntokens) return;
+  const bool live = t < ntokens;
+  T* out = dlogits + static_cast<long long>(live ? t : 0) * nexperts;
+  if (live) {
+    if (vectors) {
+      for (int i = lane; i < nexperts * static_cast<int>(sizeof(T)) / 16; i += G) reinterpret_cast<uint4*>(out)[i] = make_uint4(0u, 0u, 0u, 0u);
+    } else {
+      for (int e = lane; e < nexperts; e += G) out[e] = from_f32<T>(0.0f);
+    }
+  }
   int c = -1;
   float w = 0.0f, dw = 0.0f;
-  if (lane < topk) {
+  if (live && lane < topk) {
     const long long o = static_cast<long long>(t) * topk + lane;
     c = chosen[o];
-    if (c >= 0) {
+    if (c >= 0 && c < nexperts) {
       w = weights[o];
       dw = dweights[o];
+    } else {
+      c = -1;
     }
   }
   float s = w * dw;
 #pragma unroll
-  for (int off = 16; off > 0; off >>= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
-  const float g = w * (dw - s);
-  T* out = dlogits + static_cast<long long>(t) * nexperts;
-  for (int e0 = 0; e0 < nexperts; e0 += 32) {
-    float v = 0.0f;
-    for (int j = 0; j < topk; ++j) {
-      const int cj = __shfl_sync(0xffffffffu, c, j);
-      const float gj = __shfl_sync(0xffffffffu, g, j);
-      if (cj == e0 + lane) v = gj;
-    }
-    if (e0 + lane < nexperts) out[e0 + lane] = from_f32<T>(v);
-  }
+  for (int off = G / 2; off > 0; off >>= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
+  __syncwarp();
+  if (c >= 0) out[c] = from_f32<T>(w * (dw - s));
 }
 
 // ---------------------------------------------------------------------------------------------------- permute, unpermute
@@ -226,8 +249,9 @@ __device__ __forceinline__ float load_weight(const void* w, int dtype, long long
   return __half2float(static_cast<const __half*>(w)[i]);
 }
 
-// out[t] = sum_j w[t, j] rows[index[t, j]], j ascending, rounded once; without weights the plain sum
-template <class T, int VB>
+// out[t] = sum_j w[t, j] rows[index[t, j]], j ascending, rounded once; without weights the plain sum. UN rows of VU vectors
+// each are on their way together (8192 x 4096 bf16 top-2 with one vector of two rows a thread took 60 us, 3.3 TB/s).
+template <class T, int VB, int UN, int VU>
 __global__ void __launch_bounds__(kSortThreads)
 moe_unpermute_kernel(const typename RawVec<VB>::type* __restrict__ rows_in, int ntokens, int topk, int row_vecs, int width,
                      const int* __restrict__ index, const void* __restrict__ weights, int wdtype,
@@ -239,44 +263,56 @@ moe_unpermute_kernel(const typename RawVec<VB>::type* __restrict__ rows_in, int 
   const int per = kSortThreads / width;
   const long long t = static_cast<long long>(blockIdx.x) * per + static_cast<int>(threadIdx.x) / width;
   if (t >= ntokens) return;
-  const int* idx = index + t * topk;
-  constexpr int UN = 4;  // rows whose loads are in flight together
-  for (int v = static_cast<int>(threadIdx.x) & (width - 1); v < row_vecs; v += width) {
-    float acc[V::N];
+  int row[UN];
+  float w[UN];
+  auto choices = [&](int j0) {
 #pragma unroll
-    for (int i = 0; i < V::N; ++i) acc[i] = 0.0f;
+    for (int u = 0; u < UN; ++u) {
+      int r = j0 + u < topk ? __ldg(index + t * topk + j0 + u) : -1;
+      if (r >= rows) r = -1;
+      row[u] = r;
+      w[u] = r >= 0 && weights != nullptr ? load_weight(weights, wdtype, t * topk + j0 + u) : 1.0f;
+    }
+  };
+  choices(0);
+  for (int v0 = static_cast<int>(threadIdx.x) & (width - 1); v0 < row_vecs; v0 += VU * width) {
+    float acc[VU][V::N];
+#pragma unroll
+    for (int k = 0; k < VU; ++k)
+#pragma unroll
+      for (int i = 0; i < V::N; ++i) acc[k][i] = 0.0f;
     for (int j0 = 0; j0 < topk; j0 += UN) {
-      V x[UN];
-      float w[UN];
-      bool ok[UN];
-#pragma unroll
-      for (int u = 0; u < UN; ++u) {
-        const int r = j0 + u < topk ? idx[j0 + u] : -1;
-        ok[u] = r >= 0 && r < rows;
-        w[u] = 1.0f;
-        if (ok[u]) {
-          x[u].raw = __ldg(rows_in + static_cast<long long>(r) * row_vecs + v);
-          if (weights != nullptr) w[u] = load_weight(weights, wdtype, t * topk + j0 + u);
-        }
-      }
+      if (topk > UN) choices(j0);
+      V x[UN][VU];
 #pragma unroll
       for (int u = 0; u < UN; ++u)
-        if (ok[u]) {
 #pragma unroll
-          for (int i = 0; i < V::N; ++i) acc[i] = fmaf(w[u], to_f32(x[u].e[i]), acc[i]);
+        for (int k = 0; k < VU; ++k)
+          if (row[u] >= 0 && v0 + k * width < row_vecs) x[u][k].raw = __ldg(rows_in + static_cast<long long>(row[u]) * row_vecs + v0 + k * width);
+#pragma unroll
+      for (int u = 0; u < UN; ++u)
+        if (row[u] >= 0) {
+#pragma unroll
+          for (int k = 0; k < VU; ++k)
+#pragma unroll
+            for (int i = 0; i < V::N; ++i) acc[k][i] = fmaf(w[u], to_f32(x[u][k].e[i]), acc[k][i]);
         }
     }
-    V y;
 #pragma unroll
-    for (int i = 0; i < V::N; ++i) y.e[i] = from_f32<T>(acc[i]);
-    out[t * row_vecs + v] = y.raw;
+    for (int k = 0; k < VU; ++k)
+      if (v0 + k * width < row_vecs) {
+        V y;
+#pragma unroll
+        for (int i = 0; i < V::N; ++i) y.e[i] = from_f32<T>(acc[k][i]);
+        out[t * row_vecs + v0 + k * width] = y.raw;
+      }
   }
 }
 
-// drows[index[t, j]] = w[t, j] dout[t] and dw[t, j] = <dout[t], rows[index[t, j]]>, KC choices at a time: dout is read
-// once for them, their rows' loads are in flight together, and the products stay in fp32 until the token's threads add
-// them up. `rows_in` and `dweights` are null where only drows is wanted.
-template <class T, int VB, int KC>
+// drows[index[t, j]] = w[t, j] dout[t] and dw[t, j] = <dout[t], rows[index[t, j]]>, KC choices of VU vectors at a time: dout is
+// read once for them, their rows' loads are in flight together, and the products stay in fp32 until the token's threads
+// add them up. `rows_in` and `dweights` are null where only drows is wanted.
+template <class T, int VB, int KC, int VU>
 __global__ void __launch_bounds__(kSortThreads)
 moe_unpermute_backward_kernel(const typename RawVec<VB>::type* __restrict__ dout, const typename RawVec<VB>::type* __restrict__ rows_in,
                               int ntokens, int topk, int row_vecs, int width, int main_ctas, const int* __restrict__ splits, int nexperts,
@@ -301,33 +337,41 @@ moe_unpermute_backward_kernel(const typename RawVec<VB>::type* __restrict__ dout
     float w[KC], dot[KC];
 #pragma unroll
     for (int u = 0; u < KC; ++u) {
-      int r = live && j0 + u < topk ? index[t * topk + j0 + u] : -1;
+      int r = live && j0 + u < topk ? __ldg(index + t * topk + j0 + u) : -1;
       if (r >= rows) r = -1;
       row[u] = r;
       w[u] = r >= 0 ? load_weight(weights, wdtype, t * topk + j0 + u) : 0.0f;
       dot[u] = 0.0f;
     }
     if (live) {
-      for (int v = tid & (width - 1); v < row_vecs; v += width) {
-        V g, x[KC];
-        g.raw = __ldg(dout + t * row_vecs + v);
+      for (int v0 = tid & (width - 1); v0 < row_vecs; v0 += VU * width) {
+        V g[VU], x[KC][VU];
+#pragma unroll
+        for (int k = 0; k < VU; ++k)
+          if (v0 + k * width < row_vecs) g[k].raw = __ldg(dout + t * row_vecs + v0 + k * width);
         if (rows_in != nullptr) {
 #pragma unroll
           for (int u = 0; u < KC; ++u)
-            if (row[u] >= 0) x[u].raw = __ldg(rows_in + static_cast<long long>(row[u]) * row_vecs + v);
+#pragma unroll
+            for (int k = 0; k < VU; ++k)
+              if (row[u] >= 0 && v0 + k * width < row_vecs) x[u][k].raw = __ldg(rows_in + static_cast<long long>(row[u]) * row_vecs + v0 + k * width);
         }
 #pragma unroll
         for (int u = 0; u < KC; ++u) {
           if (row[u] < 0) continue;
-          if (rows_in != nullptr) {
 #pragma unroll
-            for (int i = 0; i < V::N; ++i) dot[u] = fmaf(to_f32(g.e[i]), to_f32(x[u].e[i]), dot[u]);
-          }
-          if (drows != nullptr) {
-            V d;
+          for (int k = 0; k < VU; ++k) {
+            if (v0 + k * width >= row_vecs) continue;
+            if (rows_in != nullptr) {
 #pragma unroll
-            for (int i = 0; i < V::N; ++i) d.e[i] = from_f32<T>(w[u] * to_f32(g.e[i]));
-            drows[static_cast<long long>(row[u]) * row_vecs + v] = d.raw;
+              for (int i = 0; i < V::N; ++i) dot[u] = fmaf(to_f32(g[k].e[i]), to_f32(x[u][k].e[i]), dot[u]);
+            }
+            if (drows != nullptr) {
+              V d;
+#pragma unroll
+              for (int i = 0; i < V::N; ++i) d.e[i] = from_f32<T>(w[u] * to_f32(g[k].e[i]));
+              drows[static_cast<long long>(row[u]) * row_vecs + v0 + k * width] = d.raw;
+            }
           }
         }
       }
@@ -361,9 +405,10 @@ static int sort_vec_bytes(long long row_bytes, int least, std::initializer_list<
   while (vb > least && (a & static_cast<uintptr_t>(vb - 1)) != 0) vb >>= 1;
   return vb;
 }
-static int sort_width(long long row_vecs) {
+// Threads per token that take `each` vectors of a row at a time.
+static int sort_width(long long row_vecs, int each) {
   int w = 32;
-  while (w < kSortThreads && w < row_vecs) w *= 2;
+  while (w < kSortThreads && static_cast<long long>(w) * each < row_vecs) w *= 2;
   return w;
 }
 
@@ -376,45 +421,70 @@ static bool is_float_type(int dt) { return dt == FLUXB_F32 || dt == FLUXB_BF16 |
 
 template <class T>
 static int launch_route(const void* logits, int ntokens, int nexperts, int topk, int* chosen, float* weights, cudaStream_t stream) {
-  const int grid = static_cast<int>((static_cast<long long>(ntokens) * 32 + kRouteThreads - 1) / kRouteThreads);
   const T* z = static_cast<const T*>(logits);
-#define FLUXB_ROUTE(V) \
-  if (nexperts <= 32 * V) return launch_pdl(moe_route_kernel<T, V>, grid, kRouteThreads, stream, z, ntokens, nexperts, topk, chosen, weights)
-  FLUXB_ROUTE(1);
-  FLUXB_ROUTE(2);
-  FLUXB_ROUTE(4);
-  FLUXB_ROUTE(8);
-  FLUXB_ROUTE(16);
-  FLUXB_ROUTE(32);
+  const int vectors = ((reinterpret_cast<uintptr_t>(logits) | static_cast<uintptr_t>(nexperts) * sizeof(T)) & 15) == 0 ? 1 : 0;
+#define FLUXB_ROUTE(G, V)                                                                                                                            \
+  if (nexperts <= G * V && topk <= G)                                                                                                                \
+  return launch_pdl(moe_route_kernel<T, G, V>, static_cast<int>((static_cast<long long>(ntokens) * G + kRouteThreads - 1) / kRouteThreads), kRouteThreads, \
+                    stream, z, ntokens, nexperts, topk, vectors, chosen, weights)
+  FLUXB_ROUTE(8, 1);
+  FLUXB_ROUTE(8, 4);
+  FLUXB_ROUTE(8, 8);
+  FLUXB_ROUTE(16, 8);
+  FLUXB_ROUTE(16, 16);
+  FLUXB_ROUTE(32, 8);
+  FLUXB_ROUTE(32, 32);
 #undef FLUXB_ROUTE
-  FLUXB_FAIL(FLUXB_ERR_INVALID, "moe_route: nexperts=%d above %d", nexperts, kRouteMaxExperts);
+  FLUXB_FAIL(FLUXB_ERR_INVALID, "moe_route: nexperts=%d topk=%d not supported", nexperts, topk);
 }
 
+template <class T>
+static int launch_route_backward(const float* dweights, const int* chosen, const float* weights, int ntokens, int nexperts, int topk, void* dlogits,
+                                 cudaStream_t stream) {
+  const int vectors = ((reinterpret_cast<uintptr_t>(dlogits) | static_cast<uintptr_t>(nexperts) * sizeof(T)) & 15) == 0 ? 1 : 0;
+  const int g = topk <= 8 && nexperts <= 64 ? 8 : topk <= 16 && nexperts <= 256 ? 16 : 32;
+  const int grid = static_cast<int>((static_cast<long long>(ntokens) * g + kRouteThreads - 1) / kRouteThreads);
+  auto kern = g == 8 ? moe_route_backward_kernel<T, 8> : g == 16 ? moe_route_backward_kernel<T, 16> : moe_route_backward_kernel<T, 32>;
+  return launch_pdl(kern, grid, kRouteThreads, stream, dweights, chosen, weights, ntokens, nexperts, topk, vectors, static_cast<T*>(dlogits));
+}
+
+// 8 vectors' loads in flight per thread, as rows x vectors of a row
+template <class T, int VB, int UN>
+static int launch_unpermute_rows(const void* rows, int ntokens, int topk, int row_vecs, const int* index, const void* weights, int wdtype, void* out,
+                                 cudaStream_t stream) {
+  using R = typename RawVec<VB>::type;
+  constexpr int VU = 8 / UN;
+  const int width = sort_width(row_vecs, VU), per = kSortThreads / width;
+  return launch_pdl(moe_unpermute_kernel<T, VB, UN, VU>, (ntokens + per - 1) / per, kSortThreads, stream, static_cast<const R*>(rows), ntokens, topk,
+                    row_vecs, width, index, weights, wdtype, static_cast<R*>(out));
+}
 template <class T, int VB>
 static int launch_unpermute(const void* rows, int ntokens, int topk, int row_vecs, const int* index, const void* weights, int wdtype, void* out,
                             cudaStream_t stream) {
-  using R = typename RawVec<VB>::type;
-  const int width = sort_width(row_vecs), per = kSortThreads / width;
-  return launch_pdl(moe_unpermute_kernel<T, VB>, (ntokens + per - 1) / per, kSortThreads, stream, static_cast<const R*>(rows), ntokens, topk, row_vecs,
-                    width, index, weights, wdtype, static_cast<R*>(out));
+  if (topk <= 2) return launch_unpermute_rows<T, VB, 2>(rows, ntokens, topk, row_vecs, index, weights, wdtype, out, stream);
+  if (topk <= 4) return launch_unpermute_rows<T, VB, 4>(rows, ntokens, topk, row_vecs, index, weights, wdtype, out, stream);
+  return launch_unpermute_rows<T, VB, 8>(rows, ntokens, topk, row_vecs, index, weights, wdtype, out, stream);
 }
 
-template <class T, int VB>
-static int launch_unpermute_backward(const void* dout, const void* rows, int ntokens, int topk, int row_vecs, const int* splits, int nexperts,
-                                     const int* index, const void* weights, int wdtype, void* drows, void* dweights, cudaStream_t stream) {
+template <class T, int VB, int KC>
+static int launch_unpermute_backward_rows(const void* dout, const void* rows, int ntokens, int topk, int row_vecs, const int* splits, int nexperts,
+                                          const int* index, const void* weights, int wdtype, void* drows, void* dweights, cudaStream_t stream) {
   using R = typename RawVec<VB>::type;
-  const int width = sort_width(row_vecs), per = kSortThreads / width;
+  constexpr int VU = 8 / KC;
+  const int width = sort_width(row_vecs, VU), per = kSortThreads / width;
   const int main_ctas = (ntokens + per - 1) / per;
   const long long total = static_cast<long long>(ntokens) * topk;
   const int tail = total < kSortTailCtas ? static_cast<int>(total) : kSortTailCtas;
   const int grid = main_ctas + (drows != nullptr ? tail : 0);
-#define FLUXB_UNPERMUTE_BWD(KC)                                                                                                                    \
-  return launch_pdl(moe_unpermute_backward_kernel<T, VB, KC>, grid, kSortThreads, stream, static_cast<const R*>(dout), static_cast<const R*>(rows), \
-                    ntokens, topk, row_vecs, width, main_ctas, splits, nexperts, index, weights, wdtype, static_cast<R*>(drows), dweights)
-  if (topk <= 2) FLUXB_UNPERMUTE_BWD(2);
-  if (topk <= 4) FLUXB_UNPERMUTE_BWD(4);
-  FLUXB_UNPERMUTE_BWD(8);
-#undef FLUXB_UNPERMUTE_BWD
+  return launch_pdl(moe_unpermute_backward_kernel<T, VB, KC, VU>, grid, kSortThreads, stream, static_cast<const R*>(dout), static_cast<const R*>(rows),
+                    ntokens, topk, row_vecs, width, main_ctas, splits, nexperts, index, weights, wdtype, static_cast<R*>(drows), dweights);
+}
+template <class T, int VB>
+static int launch_unpermute_backward(const void* dout, const void* rows, int ntokens, int topk, int row_vecs, const int* splits, int nexperts,
+                                     const int* index, const void* weights, int wdtype, void* drows, void* dweights, cudaStream_t stream) {
+  if (topk <= 2) return launch_unpermute_backward_rows<T, VB, 2>(dout, rows, ntokens, topk, row_vecs, splits, nexperts, index, weights, wdtype, drows, dweights, stream);
+  if (topk <= 4) return launch_unpermute_backward_rows<T, VB, 4>(dout, rows, ntokens, topk, row_vecs, splits, nexperts, index, weights, wdtype, drows, dweights, stream);
+  return launch_unpermute_backward_rows<T, VB, 8>(dout, rows, ntokens, topk, row_vecs, splits, nexperts, index, weights, wdtype, drows, dweights, stream);
 }
 
 }  // namespace fluxb
@@ -448,14 +518,10 @@ int fluxb_moe_route_backward(const float* dweights, const int* chosen, const flo
   if (rc != FLUXB_OK) return rc;
   if (ntokens == 0) return FLUXB_OK;
   FLUXB_REQUIRE(dweights != nullptr && chosen != nullptr && weights != nullptr && dlogits != nullptr, "moe_route_backward: NULL argument");
-  const int grid = static_cast<int>((static_cast<long long>(ntokens) * 32 + kRouteThreads - 1) / kRouteThreads);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (dtype == FLUXB_F32)
-    return launch_pdl(moe_route_backward_kernel<float>, grid, kRouteThreads, s, dweights, chosen, weights, ntokens, nexperts, topk, static_cast<float*>(dlogits));
-  if (dtype == FLUXB_BF16)
-    return launch_pdl(moe_route_backward_kernel<__nv_bfloat16>, grid, kRouteThreads, s, dweights, chosen, weights, ntokens, nexperts, topk,
-                      static_cast<__nv_bfloat16*>(dlogits));
-  return launch_pdl(moe_route_backward_kernel<__half>, grid, kRouteThreads, s, dweights, chosen, weights, ntokens, nexperts, topk, static_cast<__half*>(dlogits));
+  if (dtype == FLUXB_F32) return launch_route_backward<float>(dweights, chosen, weights, ntokens, nexperts, topk, dlogits, s);
+  if (dtype == FLUXB_BF16) return launch_route_backward<__nv_bfloat16>(dweights, chosen, weights, ntokens, nexperts, topk, dlogits, s);
+  return launch_route_backward<__half>(dweights, chosen, weights, ntokens, nexperts, topk, dlogits, s);
 }
 
 int fluxb_moe_permute(const void* tokens, int ntokens, int topk, long long row_bytes, const int* splits, int nexperts, const int* scatter_index,
@@ -468,7 +534,7 @@ int fluxb_moe_permute(const void* tokens, int ntokens, int topk, long long row_b
   FLUXB_REQUIRE(tokens != nullptr && splits != nullptr && scatter_index != nullptr && rows_out != nullptr, "moe_permute: NULL argument");
   const int vb = sort_vec_bytes(row_bytes, 1, {tokens, rows_out});
   const long long row_vecs = row_bytes / vb;
-  const int width = sort_width(row_vecs), per = kSortThreads / width;
+  const int width = sort_width(row_vecs, 4), per = kSortThreads / width;
   const int main_ctas = (ntokens + per - 1) / per;
   const long long total = static_cast<long long>(ntokens) * topk;
   const int grid = main_ctas + (total < kSortTailCtas ? static_cast<int>(total) : kSortTailCtas);

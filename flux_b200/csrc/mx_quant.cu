@@ -227,13 +227,20 @@ mx_dequantize_kernel(const uint32_t* __restrict__ data, const uint8_t* __restric
       uint4 v[sizeof(T) / 2];
       T e[8];
     } o;
+    uint32_t h[4];  // pairs of fp16, which holds every e2m1 value
+    asm("{\n\t.reg .b8 a, b, c, d;\n\t"
+        "mov.b32 {a, b, c, d}, %4;\n\t"
+        "cvt.rn.f16x2.e2m1x2 %0, a;\n\t"
+        "cvt.rn.f16x2.e2m1x2 %1, b;\n\t"
+        "cvt.rn.f16x2.e2m1x2 %2, c;\n\t"
+        "cvt.rn.f16x2.e2m1x2 %3, d;\n\t}"
+        : "=r"(h[0]), "=r"(h[1]), "=r"(h[2]), "=r"(h[3])
+        : "r"(code[i]));
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const uint32_t c = (code[i] >> (4 * j)) & 15u;
-      // e2m1: 2^(e - 1) (1 + m / 2), or m / 2 where e = 0
-      const uint32_t e = (c >> 1) & 3u, m = c & 1u;
-      const float mag = e == 0u ? 0.5f * static_cast<float>(m) : __uint_as_float(((126u + e) << 23) | (m << 22));
-      o.e[j] = mx_out<T>((c & 8u) ? -mag * s : mag * s);
+    for (int j = 0; j < 4; ++j) {
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h[j]));
+      o.e[2 * j] = mx_out<T>(f.x * s);
+      o.e[2 * j + 1] = mx_out<T>(f.y * s);
     }
 #pragma unroll
     for (int j = 0; j < static_cast<int>(sizeof(T) / 2); ++j) reinterpret_cast<uint4*>(out + u * 8)[j] = o.v[j];
