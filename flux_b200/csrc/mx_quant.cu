@@ -4,9 +4,9 @@
 // Dividing by the power of two is exact, so every q is the correctly rounded value. A block that holds an infinity or a
 // NaN has the scale 255, which makes all of it NaN.
 //
-// Bound by memory: 4 lanes share a block, 8 values each, so that a warp's loads are 512 contiguous bytes (16-bit types)
-// and its stores 128; the four scales of a cell (mx_format.cuh) are one store. Four such pieces of a thread are in flight
-// together.
+// Bound by memory, and by instructions next (75% of the issue slots with 8 values a thread and everything in fp32): two lanes
+// share 32 values, 16 each, the largest is found in the input's own type, two values at a time, and bf16 is scaled so, too,
+// which is exact. The four scales of a cell (mx_format.cuh) are one store. Two pieces of a thread are in flight together.
 #include "internal.h"
 #include "mx_format.cuh"
 #include "plain_gemm.cuh"
@@ -14,20 +14,22 @@
 namespace fluxb {
 
 constexpr int kQuantThreads = 256;
-constexpr int kQuantUnroll = 4;
+constexpr int kQuantUnroll = 2;
+constexpr int kQuantUnit = 16;  // values of a thread at a time
 constexpr int kQuantTailCtas = 148;
+constexpr int kDequantUnroll = 4;
 
 struct QuantParams {
   const void* x;
   long long ldx;       // elements between rows
-  int rows, units;     // units of 8 values in a row
-  int groups;          // groups of 128 values in a row, started ones too: 16 units each
-  FastDiv div;         // by 16 * groups
+  int rows, units;     // units in a row
+  int groups;          // groups of 128 values in a row, started ones too: 8 units each
+  FastDiv div;         // by 8 * groups
   FastDiv mat;         // by the rows of one matrix: every matrix starts a scale block
   int row0;            // first row of this launch
   uint8_t* data;
   uint8_t* scales;
-  // quantised into the order of the experts: row t goes to the rows index[t, j]; else null
+  // quantised into the order of the experts: row t goes to the rows index[t, j]
   const int* index;
   const int* splits;
   int topk, nexperts, main_ctas;
@@ -39,46 +41,74 @@ __device__ __forceinline__ long long quant_scale_row(const FastDiv& mat, int r) 
   return b * ((static_cast<long long>(mat.d) + 127) & ~127ll) + (r - b * static_cast<int>(mat.d));
 }
 
-// 8 values of one of the input types, 16 or 32 bytes
+// 16 values of one of the input types, as words
 template <class T>
-struct Eight {
-  uint4 v[sizeof(T) / 2];
+struct QuantValues {
+  static constexpr int W = 16 * sizeof(T) / 4;
+  uint32_t w[W];
+  __device__ __forceinline__ void load(const T* p, bool aligned) {
+    if (aligned) {
+#pragma unroll
+      for (int i = 0; i < W / 4; ++i) {
+        const uint4 v = __ldg(reinterpret_cast<const uint4*>(p) + i);
+        w[4 * i] = v.x;
+        w[4 * i + 1] = v.y;
+        w[4 * i + 2] = v.z;
+        w[4 * i + 3] = v.w;
+      }
+    } else if (sizeof(T) == 4) {
+#pragma unroll
+      for (int i = 0; i < W; ++i) w[i] = __float_as_uint(reinterpret_cast<const float*>(p)[i]);
+    } else {
+      const uint16_t* h = reinterpret_cast<const uint16_t*>(p);
+#pragma unroll
+      for (int i = 0; i < W; ++i) w[i] = h[2 * i] | (static_cast<uint32_t>(h[2 * i + 1]) << 16);
+    }
+  }
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int i = 0; i < W; ++i) w[i] = 0u;
+  }
 };
-template <class T>
-__device__ __forceinline__ void eight_load(Eight<T>& e, const T* p, bool aligned) {
-  if (aligned) {
+// Bits of the largest magnitude as a float's; magnitudes are compared as integers, where infinities and NaN come out on top.
+__device__ __forceinline__ uint32_t quant_most16(const uint32_t (&w)[8]) {
+  uint32_t m = w[0] & 0x7FFF7FFFu;
 #pragma unroll
-    for (int i = 0; i < static_cast<int>(sizeof(T) / 2); ++i) e.v[i] = __ldg(reinterpret_cast<const uint4*>(p) + i);
-  } else {
-    T* t = reinterpret_cast<T*>(e.v);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) t[i] = p[i];
-  }
+  for (int i = 1; i < 8; ++i) m = __vmaxu2(m, w[i] & 0x7FFF7FFFu);
+  return max(m & 0xFFFFu, m >> 16);
 }
-__device__ __forceinline__ void eight_floats(const Eight<float>& e, float (&f)[8]) {
+__device__ __forceinline__ uint32_t quant_most(const QuantValues<float>& x) {
+  uint32_t m = 0;
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    f[4 * i] = __uint_as_float(e.v[i].x);
-    f[4 * i + 1] = __uint_as_float(e.v[i].y);
-    f[4 * i + 2] = __uint_as_float(e.v[i].z);
-    f[4 * i + 3] = __uint_as_float(e.v[i].w);
-  }
+  for (int i = 0; i < 16; ++i) m = max(m, x.w[i] & 0x7FFFFFFFu);
+  return m;
 }
-__device__ __forceinline__ void eight_floats(const Eight<__nv_bfloat16>& e, float (&f)[8]) {
-  const uint32_t w[4] = {e.v[0].x, e.v[0].y, e.v[0].z, e.v[0].w};
+__device__ __forceinline__ uint32_t quant_most(const QuantValues<__nv_bfloat16>& x) { return quant_most16(x.w) << 16; }
+__device__ __forceinline__ uint32_t quant_most(const QuantValues<__half>& x) {
+  return __float_as_uint(__half2float(__ushort_as_half(static_cast<uint16_t>(quant_most16(x.w)))));
+}
+// The eight values from word 8 h (fp32) or 4 h on, times a power of two.
+__device__ __forceinline__ void quant_scaled(const QuantValues<float>& x, int h, float inv, float (&f)[8]) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) f[i] = __uint_as_float(x.w[8 * h + i]) * inv;
+}
+__device__ __forceinline__ void quant_scaled(const QuantValues<__nv_bfloat16>& x, int h, float inv, float (&f)[8]) {
+  // exact: the products are at most 8, and those below bf16's normal numbers, which may be rounded, become zeros
+  const __nv_bfloat162 s = __bfloat162bfloat162(__float2bfloat16_rn(inv));
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    f[2 * i] = __uint_as_float(w[i] << 16);
-    f[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+    const __nv_bfloat162 v = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&x.w[4 * h + i]), s);
+    const uint32_t b = *reinterpret_cast<const uint32_t*>(&v);
+    f[2 * i] = __uint_as_float(b << 16);
+    f[2 * i + 1] = __uint_as_float(b & 0xFFFF0000u);
   }
 }
-__device__ __forceinline__ void eight_floats(const Eight<__half>& e, float (&f)[8]) {
-  const uint32_t w[4] = {e.v[0].x, e.v[0].y, e.v[0].z, e.v[0].w};
+__device__ __forceinline__ void quant_scaled(const QuantValues<__half>& x, int h, float inv, float (&f)[8]) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
-    f[2 * i] = v.x;
-    f[2 * i + 1] = v.y;
+    const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&x.w[4 * h + i]));
+    f[2 * i] = v.x * inv;
+    f[2 * i + 1] = v.y * inv;
   }
 }
 
@@ -96,12 +126,12 @@ __device__ __forceinline__ uint32_t pack_e2m1(const float (&f)[8]) {
   return r;
 }
 
-template <class T>
+template <class T, bool SCATTER>
 __global__ void __launch_bounds__(kQuantThreads)
 mx_quantize_kernel(const __grid_constant__ QuantParams p, const int aligned) {
   pdl_wait();
   if (threadIdx.x == 0) pdl_trigger();
-  if (static_cast<int>(blockIdx.x) >= p.main_ctas) {
+  if (SCATTER && static_cast<int>(blockIdx.x) >= p.main_ctas) {
     // the rows that belong to no expert: zeros
     __shared__ long long part[kQuantThreads / 32];
     long long s = 0;
@@ -116,67 +146,49 @@ mx_quantize_kernel(const __grid_constant__ QuantParams p, const int aligned) {
     if (s < 0) s = 0;
     const long long rows = static_cast<long long>(p.rows) * p.topk;
     for (long long r = s + static_cast<int>(blockIdx.x) - p.main_ctas; r < rows; r += static_cast<int>(gridDim.x) - p.main_ctas) {
-      for (int u = threadIdx.x; u < p.units; u += kQuantThreads) reinterpret_cast<uint32_t*>(p.data)[r * p.units + u] = 0u;
+      for (int u = threadIdx.x; u < p.units; u += kQuantThreads) reinterpret_cast<uint2*>(p.data)[r * p.units + u] = make_uint2(0u, 0u);
       for (int g = threadIdx.x; g < p.groups; g += kQuantThreads) *reinterpret_cast<uint32_t*>(p.scales + mx_sf_offset(r, g, p.groups)) = 0u;
     }
     return;
   }
   const int lane = threadIdx.x & 31;
-  const int per_row = p.groups * 16;
-  const long long total = static_cast<long long>(p.rows) * per_row;
+  const int per_row = p.groups * 8;
   const long long u0 = static_cast<long long>(blockIdx.x) * (kQuantThreads * kQuantUnroll) + threadIdx.x;
-  Eight<T> in[kQuantUnroll];
+  QuantValues<T> in[kQuantUnroll];
   int row[kQuantUnroll], unit[kQuantUnroll];
 #pragma unroll
   for (int i = 0; i < kQuantUnroll; ++i) {
-    const long long u = u0 + i * kQuantThreads;
-    row[i] = -1;
-    unit[i] = 0;
-    if (u < total) {
-      row[i] = p.div.quot(static_cast<int>(u));
-      unit[i] = static_cast<int>(u) - row[i] * per_row;
-      if (unit[i] < p.units) eight_load(in[i], static_cast<const T*>(p.x) + row[i] * p.ldx + unit[i] * 8, aligned != 0);
-    }
+    row[i] = p.div.quot(static_cast<int>(u0) + i * kQuantThreads);  // (past the last row: p.rows or more)
+    unit[i] = static_cast<int>(u0) + i * kQuantThreads - row[i] * per_row;
+    if (row[i] < p.rows && unit[i] < p.units) in[i].load(static_cast<const T*>(p.x) + row[i] * p.ldx + unit[i] * kQuantUnit, aligned != 0);
+    else in[i].clear();
   }
 #pragma unroll
   for (int i = 0; i < kQuantUnroll; ++i) {
-    const bool valid = row[i] >= 0 && unit[i] < p.units;
-    float f[8];
-    if (valid) {
-      eight_floats(in[i], f);
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) f[j] = 0.0f;
-    }
-    uint32_t most = 0;  // |x| as integers: infinities and NaN come out on top
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const uint32_t b = __float_as_uint(f[j]) & 0x7FFFFFFFu;
-      most = b > most ? b : most;
-    }
-#pragma unroll
-    for (int off = 1; off < 4; off <<= 1) {
-      const uint32_t o = __shfl_xor_sync(0xffffffffu, most, off);
-      most = o > most ? o : most;
-    }
+    const bool valid = row[i] < p.rows && unit[i] < p.units;
+    uint32_t most = quant_most(in[i]);
+    most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
     const uint32_t field = most >> 23;
-    uint32_t code = 0u, scale = 255u;
+    uint2 code = make_uint2(0u, 0u);
+    uint32_t scale = 255u;
     if (field != 255u) {
       scale = field < 2u ? 0u : field - 2u;
       const float inv = __uint_as_float((254u - scale) << 23);  // 2^(127 - scale), from 2^-125 to 2^127
-#pragma unroll
-      for (int j = 0; j < 8; ++j) f[j] *= inv;
-      code = pack_e2m1(f);
+      float f[8];
+      quant_scaled(in[i], 0, inv, f);
+      code.x = pack_e2m1(f);
+      quant_scaled(in[i], 1, inv, f);
+      code.y = pack_e2m1(f);
     }
-    // the scales of 128 values (16 lanes, all of one row) as one word; those past the row's end are zero
-    uint32_t cell = valid ? scale << (2 * (lane & 12)) : 0u;
+    // the scales of 128 values (8 lanes, all of one row) as one word; those past the row's end are zero
+    uint32_t cell = valid ? scale << (4 * (lane & 6)) : 0u;
+    cell |= __shfl_xor_sync(0xffffffffu, cell, 2);
     cell |= __shfl_xor_sync(0xffffffffu, cell, 4);
-    cell |= __shfl_xor_sync(0xffffffffu, cell, 8);
     if (!valid) continue;
-    const int kg = unit[i] >> 4;
-    const bool writes_cell = (lane & 15) == 0;
-    if (p.index == nullptr) {
-      reinterpret_cast<uint32_t*>(p.data)[static_cast<long long>(p.row0 + row[i]) * p.units + unit[i]] = code;
+    const int kg = unit[i] >> 3;
+    const bool writes_cell = (lane & 7) == 0;
+    if (!SCATTER) {
+      reinterpret_cast<uint2*>(p.data)[static_cast<long long>(p.row0 + row[i]) * p.units + unit[i]] = code;
       if (writes_cell) *reinterpret_cast<uint32_t*>(p.scales + mx_sf_offset(quant_scale_row(p.mat, p.row0 + row[i]), kg, p.groups)) = cell;
     } else {
       const int* idx = p.index + static_cast<long long>(row[i]) * p.topk;
@@ -184,7 +196,7 @@ mx_quantize_kernel(const __grid_constant__ QuantParams p, const int aligned) {
       for (int j = 0; j < p.topk; ++j) {
         const long long r = __ldg(idx + j);
         if (r < 0 || r >= rows) continue;
-        reinterpret_cast<uint32_t*>(p.data)[r * p.units + unit[i]] = code;
+        reinterpret_cast<uint2*>(p.data)[r * p.units + unit[i]] = code;
         if (writes_cell) *reinterpret_cast<uint32_t*>(p.scales + mx_sf_offset(r, kg, p.groups)) = cell;
       }
     }
@@ -207,10 +219,10 @@ mx_dequantize_kernel(const uint32_t* __restrict__ data, const uint8_t* __restric
                      const FastDiv mat, long long total, T* __restrict__ out) {
   pdl_wait();
   if (threadIdx.x == 0) pdl_trigger();
-  const long long u0 = static_cast<long long>(blockIdx.x) * (kQuantThreads * kQuantUnroll) + threadIdx.x;
-  uint32_t code[kQuantUnroll], scale[kQuantUnroll];
+  const long long u0 = static_cast<long long>(blockIdx.x) * (kQuantThreads * kDequantUnroll) + threadIdx.x;
+  uint32_t code[kDequantUnroll], scale[kDequantUnroll];
 #pragma unroll
-  for (int i = 0; i < kQuantUnroll; ++i) {
+  for (int i = 0; i < kDequantUnroll; ++i) {
     const long long u = u0 + i * kQuantThreads;
     if (u < total) {
       const int row = div.quot(static_cast<int>(u)), block = (static_cast<int>(u) - row * units) >> 2;
@@ -219,7 +231,7 @@ mx_dequantize_kernel(const uint32_t* __restrict__ data, const uint8_t* __restric
     }
   }
 #pragma unroll
-  for (int i = 0; i < kQuantUnroll; ++i) {
+  for (int i = 0; i < kDequantUnroll; ++i) {
     const long long u = u0 + i * kQuantThreads;
     if (u >= total) break;
     const float s = scale[i] == 255u ? __uint_as_float(0x7FC00000u) : scale[i] == 0u ? __uint_as_float(0x00400000u) : __uint_as_float(scale[i] << 23);
@@ -250,7 +262,7 @@ mx_dequantize_kernel(const uint32_t* __restrict__ data, const uint8_t* __restric
 static int mx_elt_bytes(int dt) { return dt == FLUXB_F32 ? 4 : dt == FLUXB_BF16 || dt == FLUXB_F16 ? 2 : 0; }
 
 // Rows per launch: a unit's number is a 31-bit integer.
-static int mx_rows_per_launch(int units) { return static_cast<int>(((1ll << 31) - kQuantThreads * kQuantUnroll - 1) / units); }
+static int mx_rows_per_launch(int units) { return static_cast<int>(((1ll << 31) - kQuantThreads * kDequantUnroll - 1) / units); }
 
 static int check_mx_matrices(const char* who, int batch, int rows, int k) {
   FLUXB_REQUIRE(batch >= 0 && rows >= 0 && k >= kMxBlock && k % kMxBlock == 0, "%s: batch=%d rows=%d k=%d invalid (k must be a multiple of %d)", who, batch,
@@ -278,14 +290,14 @@ int fluxb_mx_quantize(const void* x, int dtype, int batch, int rows, int k, long
   const int all = batch * rows;
   if (all == 0) return FLUXB_OK;
   FLUXB_REQUIRE(x != nullptr && data != nullptr && scales != nullptr, "mx_quantize: NULL argument");
-  FLUXB_REQUIRE((reinterpret_cast<uintptr_t>(x) & (eb - 1)) == 0 && (reinterpret_cast<uintptr_t>(data) & 3) == 0 && (reinterpret_cast<uintptr_t>(scales) & 3) == 0,
-                "mx_quantize: the input must be aligned to its type, packed values and scales to 4 bytes");
+  FLUXB_REQUIRE((reinterpret_cast<uintptr_t>(x) & (eb - 1)) == 0 && (reinterpret_cast<uintptr_t>(data) & 7) == 0 && (reinterpret_cast<uintptr_t>(scales) & 3) == 0,
+                "mx_quantize: the input must be aligned to its type, packed values to 8 bytes, scales to 4");
   QuantParams p;
   memset(&p, 0, sizeof(p));
   p.ldx = ldx;
-  p.units = k / 8;
+  p.units = k / kQuantUnit;
   p.groups = (k + kMxGroupK - 1) / kMxGroupK;
-  p.div.set(static_cast<uint32_t>(p.groups) * 16u);
+  p.div.set(static_cast<uint32_t>(p.groups) * 8u);
   p.mat.set(static_cast<uint32_t>(rows));
   p.data = static_cast<uint8_t*>(data);
   p.scales = static_cast<uint8_t*>(scales);
@@ -293,7 +305,7 @@ int fluxb_mx_quantize(const void* x, int dtype, int batch, int rows, int k, long
   p.splits = splits_dev;
   p.topk = topk;
   p.nexperts = nexperts;
-  const int most = mx_rows_per_launch(p.groups * 16);
+  const int most = mx_rows_per_launch(p.groups * 8);
   FLUXB_REQUIRE(!scatter || all <= most, "mx_quantize: too many values");
   const int aligned = ((reinterpret_cast<uintptr_t>(x) | static_cast<uintptr_t>(ldx * eb)) & 15) == 0 ? 1 : 0;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
@@ -301,13 +313,14 @@ int fluxb_mx_quantize(const void* x, int dtype, int batch, int rows, int k, long
     p.row0 = static_cast<int>(r0);
     p.x = static_cast<const uint8_t*>(x) + r0 * ldx * eb;
     p.rows = all - r0 < most ? static_cast<int>(all - r0) : most;
-    const long long total = static_cast<long long>(p.rows) * p.groups * 16;
+    const long long total = static_cast<long long>(p.rows) * p.groups * 8;
     p.main_ctas = static_cast<int>((total + kQuantThreads * kQuantUnroll - 1) / (kQuantThreads * kQuantUnroll));
     const long long out_rows = static_cast<long long>(rows) * topk;
     const int grid = p.main_ctas + (!scatter ? 0 : out_rows < kQuantTailCtas ? static_cast<int>(out_rows) : kQuantTailCtas);
-    rc = dtype == FLUXB_F32    ? launch_pdl(mx_quantize_kernel<float>, grid, kQuantThreads, s, p, aligned)
-         : dtype == FLUXB_BF16 ? launch_pdl(mx_quantize_kernel<__nv_bfloat16>, grid, kQuantThreads, s, p, aligned)
-                               : launch_pdl(mx_quantize_kernel<__half>, grid, kQuantThreads, s, p, aligned);
+#define FLUXB_QUANTIZE(T) \
+  (scatter ? launch_pdl(mx_quantize_kernel<T, true>, grid, kQuantThreads, s, p, aligned) : launch_pdl(mx_quantize_kernel<T, false>, grid, kQuantThreads, s, p, aligned))
+    rc = dtype == FLUXB_F32 ? FLUXB_QUANTIZE(float) : dtype == FLUXB_BF16 ? FLUXB_QUANTIZE(__nv_bfloat16) : FLUXB_QUANTIZE(__half);
+#undef FLUXB_QUANTIZE
     if (rc != FLUXB_OK) return rc;
   }
   return FLUXB_OK;
@@ -334,7 +347,7 @@ int fluxb_mx_dequantize(const void* data, const void* scales, int batch, int row
     const long long total = (all - r0 < most ? all - r0 : most) * units;
     const uint32_t* d = static_cast<const uint32_t*>(data) + r0 * units;
     uint8_t* o = static_cast<uint8_t*>(out) + r0 * k * eb;
-    const int grid = static_cast<int>((total + kQuantThreads * kQuantUnroll - 1) / (kQuantThreads * kQuantUnroll)), row0 = static_cast<int>(r0);
+    const int grid = static_cast<int>((total + kQuantThreads * kDequantUnroll - 1) / (kQuantThreads * kDequantUnroll)), row0 = static_cast<int>(r0);
     rc = out_dtype == FLUXB_F32    ? launch_pdl(mx_dequantize_kernel<float>, grid, kQuantThreads, s, d, sc, row0, units, groups, div, mat, total, reinterpret_cast<float*>(o))
          : out_dtype == FLUXB_BF16 ? launch_pdl(mx_dequantize_kernel<__nv_bfloat16>, grid, kQuantThreads, s, d, sc, row0, units, groups, div, mat, total,
                                                 reinterpret_cast<__nv_bfloat16*>(o))

@@ -29,7 +29,7 @@ P = C.c_void_p(256)  # never read: the calls are refused first
     ({"batch": 1 << 16, "rows": 1 << 15}, "too many"), ({"splits": P}, "belong together"), ({"index": P}, "belong together"),
     ({"splits": P, "index": P, "topk": 0}, "topk=0"), ({"splits": P, "index": P, "batch": 2}, "batch=2"), ({"splits": P, "index": P, "nexperts": 0}, "nexperts=0"),
     ({"splits": P, "index": P, "rows": 1 << 29}, "too many"), ({"x": None}, "NULL"), ({"data": None}, "NULL"), ({"scales": None}, "NULL"),
-    ({"x": C.c_void_p(257)}, "aligned"), ({"data": C.c_void_p(258)}, "aligned"), ({"scales": C.c_void_p(258)}, "aligned"),
+    ({"x": C.c_void_p(257)}, "aligned"), ({"data": C.c_void_p(260)}, "aligned"), ({"scales": C.c_void_p(258)}, "aligned"),
 ])
 def test_quantize_arguments(change, words):
     a = {"x": P, "dtype": _lib.BF16, "batch": 1, "rows": 4, "k": 64, "ldx": 64, "data": P, "scales": P, "splits": None, "nexperts": 8, "index": None,
