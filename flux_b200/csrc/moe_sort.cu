@@ -250,7 +250,9 @@ __device__ __forceinline__ float load_weight(const void* w, int dtype, long long
 }
 
 // out[t] = sum_j w[t, j] rows[index[t, j]], j ascending, rounded once; without weights the plain sum. UN rows of VU vectors
-// each are on their way together (8192 x 4096 bf16 top-2 with one vector of two rows a thread took 60 us, 3.3 TB/s).
+// each are on their way together, and the next token's index and weights with them: what a token waits for is one trip to
+// memory, not two (8192 x 4096 bf16 top-2: 60 us with one vector of two rows a thread and a launch of short CTAs, 48 with four
+// vectors).
 template <class T, int VB, int UN, int VU>
 __global__ void __launch_bounds__(kSortThreads)
 moe_unpermute_kernel(const typename RawVec<VB>::type* __restrict__ rows_in, int ntokens, int topk, int row_vecs, int width,
@@ -261,51 +263,58 @@ moe_unpermute_kernel(const typename RawVec<VB>::type* __restrict__ rows_in, int 
   pdl_wait();
   if (threadIdx.x == 0) pdl_trigger();
   const int per = kSortThreads / width;
-  const long long t = static_cast<long long>(blockIdx.x) * per + static_cast<int>(threadIdx.x) / width;
-  if (t >= ntokens) return;
-  int row[UN];
-  float w[UN];
-  auto choices = [&](int j0) {
+  const int step = static_cast<int>(gridDim.x) * per;
+  int row[UN], next_row[UN];
+  float w[UN], next_w[UN];
+  auto choices = [&](int (&r)[UN], float (&f)[UN], long long t, int j0) {
 #pragma unroll
     for (int u = 0; u < UN; ++u) {
-      int r = j0 + u < topk ? __ldg(index + t * topk + j0 + u) : -1;
-      if (r >= rows) r = -1;
-      row[u] = r;
-      w[u] = r >= 0 && weights != nullptr ? load_weight(weights, wdtype, t * topk + j0 + u) : 1.0f;
+      r[u] = t < ntokens && j0 + u < topk ? __ldg(index + t * topk + j0 + u) : -1;
+      f[u] = weights != nullptr && t < ntokens && j0 + u < topk ? load_weight(weights, wdtype, t * topk + j0 + u) : 1.0f;
     }
   };
-  choices(0);
-  for (int v0 = static_cast<int>(threadIdx.x) & (width - 1); v0 < row_vecs; v0 += VU * width) {
-    float acc[VU][V::N];
+  long long t = static_cast<long long>(blockIdx.x) * per + static_cast<int>(threadIdx.x) / width;
+  choices(next_row, next_w, t, 0);
+  for (; t < ntokens; t += step) {
 #pragma unroll
-    for (int k = 0; k < VU; ++k)
+    for (int u = 0; u < UN; ++u) {
+      row[u] = next_row[u];
+      w[u] = next_w[u];
+    }
+    choices(next_row, next_w, t + step, 0);
+    for (int v0 = static_cast<int>(threadIdx.x) & (width - 1); v0 < row_vecs; v0 += VU * width) {
+      float acc[VU][V::N];
 #pragma unroll
-      for (int i = 0; i < V::N; ++i) acc[k][i] = 0.0f;
-    for (int j0 = 0; j0 < topk; j0 += UN) {
-      if (topk > UN) choices(j0);
-      V x[UN][VU];
+      for (int k = 0; k < VU; ++k)
 #pragma unroll
-      for (int u = 0; u < UN; ++u)
+        for (int i = 0; i < V::N; ++i) acc[k][i] = 0.0f;
+      for (int j0 = 0; j0 < topk; j0 += UN) {
+        if (topk > UN) choices(row, w, t, j0);
+        V x[UN][VU];
 #pragma unroll
-        for (int k = 0; k < VU; ++k)
-          if (row[u] >= 0 && v0 + k * width < row_vecs) x[u][k].raw = __ldg(rows_in + static_cast<long long>(row[u]) * row_vecs + v0 + k * width);
-#pragma unroll
-      for (int u = 0; u < UN; ++u)
-        if (row[u] >= 0) {
+        for (int u = 0; u < UN; ++u)
 #pragma unroll
           for (int k = 0; k < VU; ++k)
+            if (row[u] >= 0 && row[u] < rows && v0 + k * width < row_vecs)
+              x[u][k].raw = __ldg(rows_in + static_cast<long long>(row[u]) * row_vecs + v0 + k * width);
 #pragma unroll
-            for (int i = 0; i < V::N; ++i) acc[k][i] = fmaf(w[u], to_f32(x[u][k].e[i]), acc[k][i]);
+        for (int u = 0; u < UN; ++u)
+          if (row[u] >= 0 && row[u] < rows) {
+#pragma unroll
+            for (int k = 0; k < VU; ++k)
+#pragma unroll
+              for (int i = 0; i < V::N; ++i) acc[k][i] = fmaf(w[u], to_f32(x[u][k].e[i]), acc[k][i]);
+          }
+      }
+#pragma unroll
+      for (int k = 0; k < VU; ++k)
+        if (v0 + k * width < row_vecs) {
+          V y;
+#pragma unroll
+          for (int i = 0; i < V::N; ++i) y.e[i] = from_f32<T>(acc[k][i]);
+          out[t * row_vecs + v0 + k * width] = y.raw;
         }
     }
-#pragma unroll
-    for (int k = 0; k < VU; ++k)
-      if (v0 + k * width < row_vecs) {
-        V y;
-#pragma unroll
-        for (int i = 0; i < V::N; ++i) y.e[i] = from_f32<T>(acc[k][i]);
-        out[t * row_vecs + v0 + k * width] = y.raw;
-      }
   }
 }
 
@@ -448,15 +457,38 @@ static int launch_route_backward(const float* dweights, const int* chosen, const
   return launch_pdl(kern, grid, kRouteThreads, stream, dweights, chosen, weights, ntokens, nexperts, topk, vectors, static_cast<T*>(dlogits));
 }
 
+// CTAs of `kern` that the current device holds at a time
+template <class Kern>
+static int sort_resident_ctas(Kern kern, int* ctas) {
+  static int known[64] = {};
+  int dev = 0;
+  FLUXB_CUDA(cudaGetDevice(&dev));
+  FLUXB_REQUIRE(dev < 64, "device index %d not supported", dev);
+  if (known[dev] == 0) {
+    int per_sm = 0, sms = 0;
+    FLUXB_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kern, kSortThreads, 0));
+    FLUXB_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
+    known[dev] = (per_sm > 0 ? per_sm : 1) * sms;
+  }
+  *ctas = known[dev];
+  return FLUXB_OK;
+}
+
 // 8 vectors' loads in flight per thread, as rows x vectors of a row
+constexpr int kSortInFlight = 8;
 template <class T, int VB, int UN>
 static int launch_unpermute_rows(const void* rows, int ntokens, int topk, int row_vecs, const int* index, const void* weights, int wdtype, void* out,
                                  cudaStream_t stream) {
   using R = typename RawVec<VB>::type;
-  constexpr int VU = 8 / UN;
+  constexpr int VU = kSortInFlight / UN;
+  auto kern = moe_unpermute_kernel<T, VB, UN, VU>;
   const int width = sort_width(row_vecs, VU), per = kSortThreads / width;
-  return launch_pdl(moe_unpermute_kernel<T, VB, UN, VU>, (ntokens + per - 1) / per, kSortThreads, stream, static_cast<const R*>(rows), ntokens, topk,
-                    row_vecs, width, index, weights, wdtype, static_cast<R*>(out));
+  int ctas = 0;
+  const int rc = sort_resident_ctas(kern, &ctas);
+  if (rc != FLUXB_OK) return rc;
+  const int need = (ntokens + per - 1) / per;
+  return launch_pdl(kern, need < ctas ? need : ctas, kSortThreads, stream, static_cast<const R*>(rows), ntokens, topk, row_vecs, width, index, weights, wdtype,
+                    static_cast<R*>(out));
 }
 template <class T, int VB>
 static int launch_unpermute(const void* rows, int ntokens, int topk, int row_vecs, const int* index, const void* weights, int wdtype, void* out,
