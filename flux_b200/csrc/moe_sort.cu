@@ -249,39 +249,179 @@ __device__ __forceinline__ float load_weight(const void* w, int dtype, long long
   return __half2float(static_cast<const __half*>(w)[i]);
 }
 
-// out[t] = sum_j w[t, j] rows[index[t, j]], j ascending, rounded once; without weights the plain sum. UN rows of VU vectors
-// each are on their way together, and the next token's index and weights with them: what a token waits for is one trip to
-// memory, not two (8192 x 4096 bf16 top-2: 60 us with one vector of two rows a thread and a launch of short CTAs, 48 with four
-// vectors).
-template <class T, int VB, int UN, int VU>
-__global__ void __launch_bounds__(kSortThreads)
+// What a thread gathers from several rows comes through shared memory, by asynchronous copies of its own that it waits for
+// in order: no thread reads what another has copied, so there are no barriers, and what is on its way is bound by shared
+// memory (about 190 KB an SM) instead of registers. An item is UN choices of VU vectors of one token; items follow each
+// other through the CTA's tokens, a ring of D items is in flight. Items of 128 bytes (one vector of two rows, 32 bytes, spent
+// more on the way from item to item than on memory: 8192 x 4096 bf16 top-2 46 us).
+constexpr int kGatherSmem = 96 * 1024;  // a CTA's share, two CTAs an SM
+constexpr int gather_vectors(int vb, int un) { return (vb == 16 ? 8 : 16) / un; }
+constexpr int gather_depth(int vb, int un) { return kGatherSmem / (kSortThreads * vb * un * gather_vectors(vb, un)); }
+template <int VB>
+__device__ __forceinline__ void copy_async(uint32_t dst, const void* src) {
+  if constexpr (VB == 16)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+  else
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copy_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+template <int VB>
+__device__ __forceinline__ typename RawVec<VB>::type read_shared(uint32_t addr) {
+  typename RawVec<VB>::type v;
+  if constexpr (VB == 16)
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
+  else
+    asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(addr) : "memory");
+  return v;
+}
+
+// Where a thread is among its items: token, vector column, first choice. Choices change fastest.
+struct GatherAt {
+  int t, v, j;
+  template <int UN>
+  __device__ __forceinline__ void next(int step, int width, int vecs, int row_vecs, int topk) {
+    j += UN;
+    if (j < topk) return;
+    j = 0;
+    v += width * vecs;
+    if (v < row_vecs) return;
+    v &= width - 1;
+    t += step;
+  }
+};
+template <int UN>
+__device__ __forceinline__ void gather_index(int (&r)[UN], const int* index, const GatherAt& at, int ntokens, int topk, int rows) {
+#pragma unroll
+  for (int u = 0; u < UN; ++u) {
+    r[u] = at.t < ntokens && at.j + u < topk ? __ldg(index + static_cast<long long>(at.t) * topk + at.j + u) : -1;
+    if (r[u] >= rows) r[u] = -1;
+  }
+}
+template <int UN>
+__device__ __forceinline__ void gather_weights(float (&w)[UN], const void* weights, int wdtype, const GatherAt& at, int ntokens, int topk) {
+#pragma unroll
+  for (int u = 0; u < UN; ++u)
+    w[u] = weights != nullptr && at.t < ntokens && at.j + u < topk ? load_weight(weights, wdtype, static_cast<long long>(at.t) * topk + at.j + u) : 1.0f;
+}
+
+// out[t] = sum_j w[t, j] rows[index[t, j]], j ascending, rounded once; without weights the plain sum.
+// (8192 x 4096 bf16: top-2 with one vector of two rows a thread and a CTA for every token 60 us, with eight vectors in
+// registers and resident CTAs 38.)
+template <class T, int VB, int UN>
+__global__ void __launch_bounds__(kSortThreads, 2)
 moe_unpermute_kernel(const typename RawVec<VB>::type* __restrict__ rows_in, int ntokens, int topk, int row_vecs, int width,
                      const int* __restrict__ index, const void* __restrict__ weights, int wdtype,
                      typename RawVec<VB>::type* __restrict__ out) {
   using V = SortVec<T, VB>;
-  const long long rows = static_cast<long long>(ntokens) * topk;
+  constexpr int VU = gather_vectors(VB, UN), D = gather_depth(VB, UN);
+  extern __shared__ __align__(16) uint8_t gather_smem[];
+  const uint32_t slots = smem_u32(gather_smem) + threadIdx.x * VB;  // [D][UN][VU][threads] vectors
+  const int rows = ntokens * topk;
   pdl_wait();
   if (threadIdx.x == 0) pdl_trigger();
-  const int per = kSortThreads / width;
-  const int step = static_cast<int>(gridDim.x) * per;
-  int row[UN], next_row[UN];
-  float w[UN], next_w[UN];
-  auto choices = [&](int (&r)[UN], float (&f)[UN], long long t, int j0) {
+  const int per = kSortThreads / width, step = static_cast<int>(gridDim.x) * per;
+  GatherAt put{static_cast<int>(blockIdx.x) * per + static_cast<int>(threadIdx.x) / width, static_cast<int>(threadIdx.x) & (width - 1), 0};
+  if (put.v >= row_vecs) return;
+  GatherAt get = put, ahead = put;
+  int row[UN];
+  gather_index<UN>(row, index, put, ntokens, topk, rows);
+  int stage_put = 0;
+  auto issue = [&] {
 #pragma unroll
-    for (int u = 0; u < UN; ++u) {
-      r[u] = t < ntokens && j0 + u < topk ? __ldg(index + t * topk + j0 + u) : -1;
-      f[u] = weights != nullptr && t < ntokens && j0 + u < topk ? load_weight(weights, wdtype, t * topk + j0 + u) : 1.0f;
-    }
+    for (int u = 0; u < UN; ++u)
+      if (row[u] >= 0) {
+        const auto* src = rows_in + static_cast<long long>(row[u]) * row_vecs + put.v;
+#pragma unroll
+        for (int k = 0; k < VU; ++k)
+          if (put.v + k * width < row_vecs) copy_async<VB>(slots + ((stage_put * UN + u) * VU + k) * (kSortThreads * VB), src + k * width);
+      }
+    copy_commit();
+    if (++stage_put == D) stage_put = 0;
+    put.next<UN>(step, width, VU, row_vecs, topk);
+    gather_index<UN>(row, index, put, ntokens, topk, rows);
   };
-  long long t = static_cast<long long>(blockIdx.x) * per + static_cast<int>(threadIdx.x) / width;
-  choices(next_row, next_w, t, 0);
-  for (; t < ntokens; t += step) {
+#pragma unroll 1
+  for (int i = 0; i < D - 1; ++i) issue();
+  int cur[UN], nxt[UN];
+  float w[UN], nxt_w[UN];
+  gather_index<UN>(nxt, index, ahead, ntokens, topk, rows);
+  gather_weights<UN>(nxt_w, weights, wdtype, ahead, ntokens, topk);
+  float acc[VU][V::N];
+  int stage = 0;
+  while (get.t < ntokens) {
 #pragma unroll
     for (int u = 0; u < UN; ++u) {
-      row[u] = next_row[u];
-      w[u] = next_w[u];
+      cur[u] = nxt[u];
+      w[u] = nxt_w[u];
     }
-    choices(next_row, next_w, t + step, 0);
+    ahead.next<UN>(step, width, VU, row_vecs, topk);
+    gather_index<UN>(nxt, index, ahead, ntokens, topk, rows);
+    gather_weights<UN>(nxt_w, weights, wdtype, ahead, ntokens, topk);
+    issue();
+    copy_wait<D - 1>();
+    if (get.j == 0) {
+#pragma unroll
+      for (int k = 0; k < VU; ++k)
+#pragma unroll
+        for (int i = 0; i < V::N; ++i) acc[k][i] = 0.0f;
+    }
+#pragma unroll
+    for (int u = 0; u < UN; ++u)
+      if (cur[u] >= 0) {
+#pragma unroll
+        for (int k = 0; k < VU; ++k) {
+          V x;  // (vectors past the row's end were not copied, and are not stored)
+          x.raw = read_shared<VB>(slots + ((stage * UN + u) * VU + k) * (kSortThreads * VB));
+#pragma unroll
+          for (int i = 0; i < V::N; ++i) acc[k][i] = fmaf(w[u], to_f32(x.e[i]), acc[k][i]);
+        }
+      }
+    if (get.j + UN >= topk) {
+#pragma unroll
+      for (int k = 0; k < VU; ++k)
+        if (get.v + k * width < row_vecs) {
+          V y;
+#pragma unroll
+          for (int i = 0; i < V::N; ++i) y.e[i] = from_f32<T>(acc[k][i]);
+          out[static_cast<long long>(get.t) * row_vecs + get.v + k * width] = y.raw;
+        }
+    }
+    if (++stage == D) stage = 0;
+    get.next<UN>(step, width, VU, row_vecs, topk);
+  }
+  copy_wait<0>();
+}
+
+// The same for vectors of 2 and 4 bytes (odd row lengths), with UN rows of VU vectors in registers: asynchronous copies do
+// not know 2 bytes, and take an instruction for every 4 (4096 x 4097 fp32 top-2 53 us through the ring, 43 here).
+template <class T, int VB, int UN, int VU>
+__global__ void __launch_bounds__(kSortThreads)
+moe_unpermute_narrow_kernel(const typename RawVec<VB>::type* __restrict__ rows_in, int ntokens, int topk, int row_vecs, int width,
+                            const int* __restrict__ index, const void* __restrict__ weights, int wdtype,
+                            typename RawVec<VB>::type* __restrict__ out) {
+  using V = SortVec<T, VB>;
+  const int rows = ntokens * topk;
+  pdl_wait();
+  if (threadIdx.x == 0) pdl_trigger();
+  const int per = kSortThreads / width, step = static_cast<int>(gridDim.x) * per;
+  int row[UN], nxt[UN];
+  float w[UN], nxt_w[UN];
+  GatherAt at{static_cast<int>(blockIdx.x) * per + static_cast<int>(threadIdx.x) / width, 0, 0};
+  gather_index<UN>(nxt, index, at, ntokens, topk, rows);
+  gather_weights<UN>(nxt_w, weights, wdtype, at, ntokens, topk);
+  for (int t = at.t; t < ntokens; t += step) {
+#pragma unroll
+    for (int u = 0; u < UN; ++u) {
+      row[u] = nxt[u];
+      w[u] = nxt_w[u];
+    }
+    at = {t + step, 0, 0};
+    gather_index<UN>(nxt, index, at, ntokens, topk, rows);
+    gather_weights<UN>(nxt_w, weights, wdtype, at, ntokens, topk);
     for (int v0 = static_cast<int>(threadIdx.x) & (width - 1); v0 < row_vecs; v0 += VU * width) {
       float acc[VU][V::N];
 #pragma unroll
@@ -289,17 +429,20 @@ moe_unpermute_kernel(const typename RawVec<VB>::type* __restrict__ rows_in, int 
 #pragma unroll
         for (int i = 0; i < V::N; ++i) acc[k][i] = 0.0f;
       for (int j0 = 0; j0 < topk; j0 += UN) {
-        if (topk > UN) choices(row, w, t, j0);
+        if (topk > UN) {
+          at = {t, 0, j0};
+          gather_index<UN>(row, index, at, ntokens, topk, rows);
+          gather_weights<UN>(w, weights, wdtype, at, ntokens, topk);
+        }
         V x[UN][VU];
 #pragma unroll
         for (int u = 0; u < UN; ++u)
 #pragma unroll
           for (int k = 0; k < VU; ++k)
-            if (row[u] >= 0 && row[u] < rows && v0 + k * width < row_vecs)
-              x[u][k].raw = __ldg(rows_in + static_cast<long long>(row[u]) * row_vecs + v0 + k * width);
+            if (row[u] >= 0 && v0 + k * width < row_vecs) x[u][k].raw = __ldg(rows_in + static_cast<long long>(row[u]) * row_vecs + v0 + k * width);
 #pragma unroll
         for (int u = 0; u < UN; ++u)
-          if (row[u] >= 0 && row[u] < rows) {
+          if (row[u] >= 0) {
 #pragma unroll
             for (int k = 0; k < VU; ++k)
 #pragma unroll
@@ -312,21 +455,153 @@ moe_unpermute_kernel(const typename RawVec<VB>::type* __restrict__ rows_in, int 
           V y;
 #pragma unroll
           for (int i = 0; i < V::N; ++i) y.e[i] = from_f32<T>(acc[k][i]);
-          out[t * row_vecs + v0 + k * width] = y.raw;
+          out[static_cast<long long>(t) * row_vecs + v0 + k * width] = y.raw;
         }
     }
   }
 }
 
-// drows[index[t, j]] = w[t, j] dout[t] and dw[t, j] = <dout[t], rows[index[t, j]]>, KC choices of VU vectors at a time: dout is
-// read once for them, their rows' loads are in flight together, and the products stay in fp32 until the token's threads
-// add them up. `rows_in` and `dweights` are null where only drows is wanted.
-template <class T, int VB, int KC, int VU>
-__global__ void __launch_bounds__(kSortThreads)
+// drows[index[t, j]] = w[t, j] dout[t] and dw[t, j] = <dout[t], rows[index[t, j]]>, KC choices at a time, whose rows and dout come
+// through the ring: dout is read once for them, and the products stay in fp32 until the token's threads add them up.
+// `rows_in` and `dweights` are null where only drows is wanted. An item is VU vectors; vectors change fastest, then choices.
+// (8192 x 2048 bf16 top-6 with the rows in registers 125 us, 3.5 TB/s.)
+constexpr int scatter_vectors(int vb, int kc) { return (vb == 16 ? 1 : 2) * (kc == 2 ? 2 : 1); }
+constexpr int scatter_depth(int vb, int kc) { return kGatherSmem / (kSortThreads * vb * (kc + 1) * scatter_vectors(vb, kc)); }
+template <class T, int VB, int KC>
+__global__ void __launch_bounds__(kSortThreads, 2)
 moe_unpermute_backward_kernel(const typename RawVec<VB>::type* __restrict__ dout, const typename RawVec<VB>::type* __restrict__ rows_in,
                               int ntokens, int topk, int row_vecs, int width, int main_ctas, const int* __restrict__ splits, int nexperts,
                               const int* __restrict__ index, const void* __restrict__ weights, int wdtype,
                               typename RawVec<VB>::type* __restrict__ drows, void* __restrict__ dweights) {
+  using V = SortVec<T, VB>;
+  constexpr int VU = scatter_vectors(VB, KC), D = scatter_depth(VB, KC);
+  __shared__ float part[2][kSortThreads / 32][KC];
+  extern __shared__ __align__(16) uint8_t gather_smem[];
+  const uint32_t slots = smem_u32(gather_smem) + threadIdx.x * VB;  // [D][KC + 1][VU][threads] vectors, dout first
+  const int rows = ntokens * topk;
+  pdl_wait();
+  if (threadIdx.x == 0) pdl_trigger();
+  if (static_cast<int>(blockIdx.x) >= main_ctas) {
+    if (drows != nullptr)
+      sort_clear_tail<VB>(drows, rows, row_vecs, splits, nexperts, static_cast<int>(blockIdx.x) - main_ctas, static_cast<int>(gridDim.x) - main_ctas);
+    return;
+  }
+  const int tid = static_cast<int>(threadIdx.x), warp = tid >> 5, lane = tid & 31, v_first = tid & (width - 1);
+  const int per = kSortThreads / width, step = main_ctas * per;
+  const int columns = (row_vecs + width * VU - 1) / (width * VU);  // items of a token and KC choices
+  struct At {
+    int t, j, c;
+  };
+  auto next = [&](At& at) {
+    if (++at.c < columns) return;
+    at.c = 0;
+    at.j += KC;
+    if (at.j < topk) return;
+    at.j = 0;
+    at.t += step;
+  };
+  auto choices = [&](int (&r)[KC], const At& at) { gather_index<KC>(r, index, GatherAt{at.t, 0, at.j}, ntokens, topk, rows); };
+  At put{static_cast<int>(blockIdx.x) * per + tid / width, 0, 0}, get = put, ahead = put;
+  int base = static_cast<int>(blockIdx.x) * per;  // the CTA's first token: all its threads meet at the sums
+  int row[KC];
+  choices(row, put);
+  int stage_put = 0;
+  auto issue = [&] {
+    if (put.t < ntokens) {
+#pragma unroll
+      for (int k = 0; k < VU; ++k) {
+        const int v = v_first + (put.c * VU + k) * width;
+        if (v >= row_vecs) continue;
+        const uint32_t dst = slots + (stage_put * (KC + 1) * VU + k) * (kSortThreads * VB);
+        copy_async<VB>(dst, dout + static_cast<long long>(put.t) * row_vecs + v);
+        if (rows_in != nullptr) {
+#pragma unroll
+          for (int u = 0; u < KC; ++u)
+            if (row[u] >= 0) copy_async<VB>(dst + (u + 1) * VU * (kSortThreads * VB), rows_in + static_cast<long long>(row[u]) * row_vecs + v);
+        }
+      }
+    }
+    copy_commit();
+    if (++stage_put == D) stage_put = 0;
+    next(put);
+    choices(row, put);
+  };
+#pragma unroll 1
+  for (int i = 0; i < D - 1; ++i) issue();
+  int cur[KC], nxt[KC];
+  float w[KC], nxt_w[KC], dot[KC];
+  choices(nxt, ahead);
+  gather_weights<KC>(nxt_w, weights, wdtype, GatherAt{ahead.t, 0, ahead.j}, ntokens, topk);
+  int stage = 0, turn = 0;
+  while (base < ntokens) {
+#pragma unroll
+    for (int u = 0; u < KC; ++u) {
+      cur[u] = nxt[u];
+      w[u] = nxt_w[u];
+      if (get.c == 0) dot[u] = 0.0f;
+    }
+    next(ahead);
+    choices(nxt, ahead);
+    gather_weights<KC>(nxt_w, weights, wdtype, GatherAt{ahead.t, 0, ahead.j}, ntokens, topk);
+    issue();
+    copy_wait<D - 1>();
+#pragma unroll
+    for (int k = 0; k < VU; ++k) {
+      const int v = v_first + (get.c * VU + k) * width;
+      if (v >= row_vecs) continue;
+      const uint32_t src = slots + (stage * (KC + 1) * VU + k) * (kSortThreads * VB);
+      V g;
+      g.raw = read_shared<VB>(src);
+#pragma unroll
+      for (int u = 0; u < KC; ++u) {
+        if (cur[u] < 0) continue;
+        if (rows_in != nullptr) {
+          V x;
+          x.raw = read_shared<VB>(src + (u + 1) * VU * (kSortThreads * VB));
+#pragma unroll
+          for (int i = 0; i < V::N; ++i) dot[u] = fmaf(to_f32(g.e[i]), to_f32(x.e[i]), dot[u]);
+        }
+        if (drows != nullptr) {
+          V d;
+#pragma unroll
+          for (int i = 0; i < V::N; ++i) d.e[i] = from_f32<T>(w[u] * to_f32(g.e[i]));
+          drows[static_cast<long long>(cur[u]) * row_vecs + v] = d.raw;
+        }
+      }
+    }
+    if (++stage == D) stage = 0;
+    if (get.c == columns - 1 && dweights != nullptr) {
+#pragma unroll
+      for (int u = 0; u < KC; ++u) {
+#pragma unroll
+        for (int off = 16; off > 0; off >>= 1) dot[u] += __shfl_xor_sync(0xffffffffu, dot[u], off);
+        if (lane == 0) part[turn][warp][u] = dot[u];
+      }
+      __syncthreads();  // (one: the next sums go to the other half)
+      if (get.t < ntokens && v_first < KC && get.j + v_first < topk) {
+        float s = 0.0f;
+        for (int k = 0; k < width / 32; ++k) s += part[turn][tid / width * (width / 32) + k][v_first];
+        const long long o = static_cast<long long>(get.t) * topk + get.j + v_first;
+        if (wdtype == FLUXB_F32) static_cast<float*>(dweights)[o] = s;
+        else if (wdtype == FLUXB_BF16) static_cast<__nv_bfloat16*>(dweights)[o] = __float2bfloat16_rn(s);
+        else static_cast<__half*>(dweights)[o] = __float2half_rn(s);
+      }
+      turn ^= 1;
+    }
+    const int t_before = get.t;
+    next(get);
+    base += get.t - t_before;
+  }
+  copy_wait<0>();
+}
+
+// The same for vectors of 2 and 4 bytes, KC choices of VU vectors in registers.
+template <class T, int VB, int KC, int VU>
+__global__ void __launch_bounds__(kSortThreads)
+moe_unpermute_backward_narrow_kernel(const typename RawVec<VB>::type* __restrict__ dout, const typename RawVec<VB>::type* __restrict__ rows_in,
+                                     int ntokens, int topk, int row_vecs, int width, int main_ctas, const int* __restrict__ splits, int nexperts,
+                                     const int* __restrict__ index, const void* __restrict__ weights, int wdtype,
+                                     typename RawVec<VB>::type* __restrict__ drows, void* __restrict__ dweights) {
   using V = SortVec<T, VB>;
   __shared__ float part[kSortThreads / 32][KC];
   const long long rows = static_cast<long long>(ntokens) * topk;
@@ -457,16 +732,16 @@ static int launch_route_backward(const float* dweights, const int* chosen, const
   return launch_pdl(kern, grid, kRouteThreads, stream, dweights, chosen, weights, ntokens, nexperts, topk, vectors, static_cast<T*>(dlogits));
 }
 
-// CTAs of `kern` that the current device holds at a time
+// CTAs of `kern` with `smem` bytes that the current device holds at a time; `known` is the kernel's own
 template <class Kern>
-static int sort_resident_ctas(Kern kern, int* ctas) {
-  static int known[64] = {};
+static int sort_resident_ctas(Kern kern, int smem, int (&known)[64], int* ctas) {
   int dev = 0;
   FLUXB_CUDA(cudaGetDevice(&dev));
   FLUXB_REQUIRE(dev < 64, "device index %d not supported", dev);
   if (known[dev] == 0) {
     int per_sm = 0, sms = 0;
-    FLUXB_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kern, kSortThreads, 0));
+    FLUXB_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    FLUXB_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kern, kSortThreads, smem));
     FLUXB_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
     known[dev] = (per_sm > 0 ? per_sm : 1) * sms;
   }
@@ -474,21 +749,24 @@ static int sort_resident_ctas(Kern kern, int* ctas) {
   return FLUXB_OK;
 }
 
-// 8 vectors' loads in flight per thread, as rows x vectors of a row
-constexpr int kSortInFlight = 8;
 template <class T, int VB, int UN>
 static int launch_unpermute_rows(const void* rows, int ntokens, int topk, int row_vecs, const int* index, const void* weights, int wdtype, void* out,
                                  cudaStream_t stream) {
   using R = typename RawVec<VB>::type;
-  constexpr int VU = kSortInFlight / UN;
-  auto kern = moe_unpermute_kernel<T, VB, UN, VU>;
+  constexpr bool NARROW = VB < 8;
+  constexpr int VU = NARROW ? 8 / UN : gather_vectors(VB, UN), SMEM = NARROW ? 0 : gather_depth(VB, UN) * UN * VU * VB * kSortThreads;
+  auto kern = [] {
+    if constexpr (NARROW) return moe_unpermute_narrow_kernel<T, VB, UN, VU>;
+    else return moe_unpermute_kernel<T, VB, UN>;
+  }();
   const int width = sort_width(row_vecs, VU), per = kSortThreads / width;
+  static int known[64] = {};
   int ctas = 0;
-  const int rc = sort_resident_ctas(kern, &ctas);
+  const int rc = sort_resident_ctas(kern, SMEM, known, &ctas);
   if (rc != FLUXB_OK) return rc;
   const int need = (ntokens + per - 1) / per;
-  return launch_pdl(kern, need < ctas ? need : ctas, kSortThreads, stream, static_cast<const R*>(rows), ntokens, topk, row_vecs, width, index, weights, wdtype,
-                    static_cast<R*>(out));
+  return launch_pdl_cluster(kern, need < ctas ? need : ctas, kSortThreads, SMEM, 0, stream, static_cast<const R*>(rows), ntokens, topk, row_vecs, width, index,
+                            weights, wdtype, static_cast<R*>(out));
 }
 template <class T, int VB>
 static int launch_unpermute(const void* rows, int ntokens, int topk, int row_vecs, const int* index, const void* weights, int wdtype, void* out,
@@ -502,14 +780,24 @@ template <class T, int VB, int KC>
 static int launch_unpermute_backward_rows(const void* dout, const void* rows, int ntokens, int topk, int row_vecs, const int* splits, int nexperts,
                                           const int* index, const void* weights, int wdtype, void* drows, void* dweights, cudaStream_t stream) {
   using R = typename RawVec<VB>::type;
-  constexpr int VU = 8 / KC;
+  constexpr bool NARROW = VB < 8;
+  constexpr int VU = NARROW ? 8 / KC : scatter_vectors(VB, KC), SMEM = NARROW ? 0 : scatter_depth(VB, KC) * (KC + 1) * VU * VB * kSortThreads;
+  auto kern = [] {
+    if constexpr (NARROW) return moe_unpermute_backward_narrow_kernel<T, VB, KC, VU>;
+    else return moe_unpermute_backward_kernel<T, VB, KC>;
+  }();
   const int width = sort_width(row_vecs, VU), per = kSortThreads / width;
-  const int main_ctas = (ntokens + per - 1) / per;
+  static int known[64] = {};
+  int ctas = 0;
+  const int rc = sort_resident_ctas(kern, SMEM, known, &ctas);
+  if (rc != FLUXB_OK) return rc;
+  int main_ctas = (ntokens + per - 1) / per;
+  if (!NARROW && main_ctas > ctas) main_ctas = ctas;
   const long long total = static_cast<long long>(ntokens) * topk;
   const int tail = total < kSortTailCtas ? static_cast<int>(total) : kSortTailCtas;
   const int grid = main_ctas + (drows != nullptr ? tail : 0);
-  return launch_pdl(moe_unpermute_backward_kernel<T, VB, KC, VU>, grid, kSortThreads, stream, static_cast<const R*>(dout), static_cast<const R*>(rows),
-                    ntokens, topk, row_vecs, width, main_ctas, splits, nexperts, index, weights, wdtype, static_cast<R*>(drows), dweights);
+  return launch_pdl_cluster(kern, grid, kSortThreads, SMEM, 0, stream, static_cast<const R*>(dout), static_cast<const R*>(rows), ntokens, topk, row_vecs,
+                            width, main_ctas, splits, nexperts, index, weights, wdtype, static_cast<R*>(drows), dweights);
 }
 template <class T, int VB>
 static int launch_unpermute_backward(const void* dout, const void* rows, int ntokens, int topk, int row_vecs, const int* splits, int nexperts,
