@@ -12,9 +12,11 @@ namespace fluxb {
 // ----------------------------------------------------------------------------------------------------------- route
 // z: logits of a token. chosen = the topk largest (ties: the lower expert), w = softmax over the chosen ones:
 //   w_j = exp(z_j - z_max) / sum_i exp(z_i - z_max),   dz_j = w_j (dw_j - sum_i w_i dw_i),   0 for the others.
-// A group of G lanes per token, VPL logits a lane in registers as order-preserving integers: a choice is a maximum over
-// (key, lower expert first) among the lanes, and only the lane that held it looks for its next one. Bound by the latency
-// of that chain, so a warp takes as many tokens as it can: 32768 tokens of 8 experts top-2 took 9.0 us with a warp each.
+// A group of G lanes per token, VPL logits a lane in registers as order-preserving integers. A choice is a maximum over the
+// lanes, ties to the lower expert, and only the lane that held it looks for its next one. 16-bit logits leave room for the
+// expert in the same word, so that one maximum finds both; for fp32 a vote finds the lowest lane (its experts are lower)
+// that has the largest key. Bound by instructions, so a warp takes as many tokens as it can (32768 x 8 experts top-2 took
+// 9.0 us with a warp per token, 32768 x 128 top-8 22.5 us with maxima over 64-bit pairs of key and expert).
 constexpr int kRouteThreads = 128;
 constexpr int kRouteMaxExperts = 1024;
 constexpr int kRouteMaxTopk = 32;
@@ -47,10 +49,29 @@ __device__ __forceinline__ float route_value(uint32_t key) {
   if (key == 0xFFFFFFFFu) return __uint_as_float(0x7FC00000u);
   return __uint_as_float((key & 0x80000000u) ? key ^ 0x80000000u : ~key);
 }
+// The same for 16-bit logits, in the upper half of a word; in the lower half the expert, lower ones larger.
+template <class T>
+__device__ __forceinline__ uint32_t route_key16(T x, int expert) {
+  const float v = to_f32(x);
+  if (v == -INFINITY) return 0u;
+  uint32_t u = *reinterpret_cast<const uint16_t*>(&x);
+  if (v == 0.0f) u = 0u;
+  u = (u & 0x8000u) ? ~u & 0xFFFFu : u | 0x8000u;
+  if (v != v) u = 0xFFFFu;
+  return (u << 16) | (0xFFFFu - static_cast<uint32_t>(expert));
+}
+template <class T>
+__device__ __forceinline__ float route_value16(uint32_t key) {
+  const uint32_t u = key >> 16;
+  if (u == 0xFFFFu) return __uint_as_float(0x7FC00000u);
+  const uint16_t bits = static_cast<uint16_t>((u & 0x8000u) ? u ^ 0x8000u : ~u);
+  return to_f32(*reinterpret_cast<const T*>(&bits));
+}
 
 template <class T, int G, int VPL>
 __global__ void __launch_bounds__(kRouteThreads)
 moe_route_kernel(const T* __restrict__ logits, int ntokens, int nexperts, int topk, int vectors, int* __restrict__ chosen, float* __restrict__ weights) {
+  constexpr bool PACKED = sizeof(T) == 2;
   const int lane = threadIdx.x & (G - 1);
   const int t = static_cast<int>((static_cast<long long>(blockIdx.x) * kRouteThreads + threadIdx.x) / G);
   pdl_wait();
@@ -59,6 +80,11 @@ moe_route_kernel(const T* __restrict__ logits, int ntokens, int nexperts, int to
   const T* z = logits + static_cast<long long>(live ? t : 0) * nexperts;
   const int first = lane * VPL;  // this lane's experts
   uint32_t key[VPL];
+  auto key_of = [&](T x, int e) -> uint32_t {
+    if (e >= nexperts) return 0u;
+    if constexpr (PACKED) return route_key16<T>(x, e);
+    else return route_key(x);
+  };
   constexpr int PER = 16 / static_cast<int>(sizeof(T));
   if (VPL % PER == 0 && vectors) {
 #pragma unroll
@@ -67,50 +93,61 @@ moe_route_kernel(const T* __restrict__ logits, int ntokens, int nexperts, int to
         uint4 v;
         T e[PER];
       } x;
-      if (first + i * PER < nexperts) x.v = __ldg(reinterpret_cast<const uint4*>(z + first) + i);
+      x.v = first + i * PER < nexperts ? __ldg(reinterpret_cast<const uint4*>(z + first) + i) : make_uint4(0u, 0u, 0u, 0u);
 #pragma unroll
-      for (int j = 0; j < PER; ++j) key[i * PER + j] = first + i * PER + j < nexperts ? route_key(to_f32(x.e[j])) : 0u;
+      for (int j = 0; j < PER; ++j) key[i * PER + j] = key_of(x.e[j], first + i * PER + j);
     }
   } else {
 #pragma unroll
-    for (int i = 0; i < VPL; ++i) key[i] = first + i < nexperts ? route_key(to_f32(z[first + i])) : 0u;
+    for (int i = 0; i < VPL; ++i) key[i] = key_of(first + i < nexperts ? z[first + i] : from_f32<T>(0.0f), first + i);
   }
-  unsigned long long best = 0;  // key and expert of this lane's largest, the lower expert the larger
+  uint32_t best = 0;  // this lane's largest
+  int at = 0;         // (fp32) where it is
   auto look = [&] {
-    uint32_t k = 0;
-    int at = 0;
+    best = key[0];
+    at = 0;
 #pragma unroll
-    for (int i = 0; i < VPL; ++i)
-      if (key[i] > k) {
-        k = key[i];
+    for (int i = 1; i < VPL; ++i) {
+      if constexpr (PACKED) {
+        best = max(best, key[i]);
+      } else if (key[i] > best) {
+        best = key[i];
         at = i;
       }
-    best = k == 0u ? 0ull : (static_cast<unsigned long long>(k) << 32) | (0xFFFFFFFFu - static_cast<uint32_t>(first + at));
+    }
   };
   look();
   int mine = -1;  // lane j: choice j
   uint32_t mine_key = 0;
   for (int j = 0; j < topk; ++j) {
-    unsigned long long top = best;
+    uint32_t top = best;
 #pragma unroll
-    for (int off = G / 2; off > 0; off >>= 1) {
-      const unsigned long long o = __shfl_xor_sync(0xffffffffu, top, off);
-      top = o > top ? o : top;
+    for (int off = G / 2; off > 0; off >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, off));
+    int e;
+    bool held;
+    if constexpr (PACKED) {
+      e = static_cast<int>(0xFFFFu - (top & 0xFFFFu));
+      held = best == top && top != 0u;
+    } else {
+      const int group = static_cast<int>(threadIdx.x) & 31 & ~(G - 1);  // the group's first lane in its warp
+      const unsigned has = __ballot_sync(0xffffffffu, best == top) >> group;
+      const int from = group + __ffs(static_cast<int>(has)) - 1;
+      e = __shfl_sync(0xffffffffu, first + at, from);
+      held = (static_cast<int>(threadIdx.x) & 31) == from && top != 0u;
     }
-    if (top == 0ull) continue;  // nothing left that may be chosen (in this group)
-    const int e = static_cast<int>(0xFFFFFFFFu - static_cast<uint32_t>(top));
-    if (lane == j) {
+    if (lane == j && top != 0u) {  // (0: nothing left that may be chosen)
       mine = e;
-      mine_key = static_cast<uint32_t>(top >> 32);
+      mine_key = top;
     }
-    if (best == top) {
+    if (held) {
 #pragma unroll
       for (int i = 0; i < VPL; ++i)
         if (first + i == e) key[i] = 0u;
       look();
     }
   }
-  const float v = route_value(mine_key);
+  float v;
+  if constexpr (PACKED) v = route_value16<T>(mine_key); else v = route_value(mine_key);
   const float top_v = __shfl_sync(0xffffffffu, v, 0, G);
   const float p = mine >= 0 ? expf(v - top_v) : 0.0f;
   float sum = p;
