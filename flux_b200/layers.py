@@ -28,6 +28,7 @@ import torch
 import torch.distributed as dist
 
 from . import moe as _moe
+from . import mx as _mx
 from . import ops as _ops
 from .shm import get_comm
 
@@ -317,3 +318,93 @@ class MoEMLP(torch.nn.Module):
             return self._l1._forward(act, self.w_down, None, splits, scatter_index.reshape(-1), output_vec_scale=row_scale)
         return self._l1.forward_gather_rs(act, self.w_down, splits.cpu(), scatter_index.reshape(-1),
                                           output_vec_scale=row_scale)
+
+
+class MXLinear(torch.nn.Module):
+    """y = x . W^T (+ bias) with microscaled 4-bit weights, for serving: the weight [out_features, in_features] is quantised
+    once (a tensor, or an `MXTensor` from a checkpoint), x [..., in_features] at every call (`mx_quantize`, `mx_gemm`). The
+    output has the type of x unless `output_dtype` says otherwise; the bias has it, too. No gradients."""
+
+    def __init__(self, weight, bias: Optional[torch.Tensor] = None, output_dtype: Optional[torch.dtype] = None):
+        super().__init__()
+        w = weight if isinstance(weight, _mx.MXTensor) else _mx.mx_quantize(weight.detach())
+        if w.data.dim() != 2:
+            raise RuntimeError("MXLinear: the weight must be [out_features, in_features]")
+        self.out_features, self.in_features = w.shape
+        self.output_dtype = output_dtype
+        self.register_buffer("weight_data", w.data)
+        self.register_buffer("weight_blocks", w.blocks)
+        self.register_buffer("bias", None if bias is None else bias.detach())
+
+    @classmethod
+    def from_linear(cls, linear, output_dtype: Optional[torch.dtype] = None) -> "MXLinear":
+        """From a `torch.nn.Linear`, or a `ColumnParallelLinear` / `RowParallelLinear` of one rank."""
+        if getattr(linear, "world", 1) != 1:
+            raise RuntimeError("MXLinear: the weights of a tensor-parallel layer of several ranks are not supported")
+        return cls(linear.weight, linear.bias, output_dtype)
+
+    @torch.no_grad()
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        w = _mx.MXTensor._of(self.weight_data, self.weight_blocks, self.in_features)
+        y = _mx.mx_gemm(_mx.mx_quantize(x.reshape(-1, x.shape[-1])), w, bias=self.bias, output_dtype=self.output_dtype or x.dtype)
+        return y.view(*x.shape[:-1], self.out_features)
+
+
+class MXMoEMLP(torch.nn.Module):
+    """Mixture-of-experts MLP of one rank with microscaled 4-bit expert weights (serving forward), the counterpart of
+    `MoEMLP`. Per call:
+
+      1. router logits in fp32 and `moe_route`: experts and weights of every token;
+      2. `calc_scatter_index`: the row of every (token, choice) pair in the order of the experts;
+      3. `mx_quantize` of the tokens straight into that order;
+      4. `mx_grouped_gemm` with the up projection (gated: gate and up projection as one weight [E, 2 ffn, hidden]);
+      5. activation, `mx_quantize`, `mx_grouped_gemm` with the down projection;
+      6. `moe_unpermute`: the weighted sum of every token's rows.
+
+    `w_up` [E, ffn, hidden], `w_gate` the same or None, `w_down` [E, hidden, ffn] are tensors or, but for a gated layer's
+    `w_up` and `w_gate`, `MXTensor`s."""
+
+    def __init__(self, router: torch.Tensor, w_up, w_down, topk: int, w_gate: Optional[torch.Tensor] = None,
+                 activation: Optional[Callable[[torch.Tensor], torch.Tensor]] = None):
+        super().__init__()
+        self.gated = w_gate is not None
+        if self.gated:
+            w_up = torch.cat((w_gate.detach(), w_up.detach()), dim=1)
+        quantised = [w if isinstance(w, _mx.MXTensor) else _mx.mx_quantize(w.detach()) for w in (w_up, w_down)]
+        up, down = quantised
+        if not (up.data.dim() == 3 and down.data.dim() == 3 and router.dim() == 2):
+            raise RuntimeError("MXMoEMLP: the router must be [E, hidden], the experts' weights [E, ffn, hidden] and [E, hidden, ffn]")
+        nexperts, up_rows, hidden = up.shape
+        self.nexperts, self.hidden, self.ffn_hidden = nexperts, hidden, up_rows // 2 if self.gated else up_rows
+        if tuple(down.shape) != (nexperts, hidden, self.ffn_hidden) or tuple(router.shape) != (nexperts, hidden):
+            raise RuntimeError(f"MXMoEMLP: router {tuple(router.shape)}, up {tuple(up.shape)} and down {tuple(down.shape)} do not fit together")
+        self.topk = int(topk)
+        self.register_buffer("router", router.detach().float())
+        for name, w in (("up", up), ("down", down)):
+            self.register_buffer(f"{name}_data", w.data)
+            self.register_buffer(f"{name}_blocks", w.blocks)
+        if activation is None:
+            activation = torch.nn.functional.silu if self.gated else torch.nn.functional.gelu
+        self.activation = activation
+
+    @classmethod
+    def from_moe(cls, moe: MoEMLP) -> "MXMoEMLP":
+        """From a `MoEMLP` of one rank."""
+        if moe.world != 1:
+            raise RuntimeError("MXMoEMLP: the weights of a tensor-parallel layer of several ranks are not supported")
+        return cls(moe.router, moe.w_up, moe.w_down, moe.topk, moe.w_gate, moe.activation)
+
+    @torch.no_grad()
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        tokens = x.reshape(-1, self.hidden)
+        chosen, weights = _moe.moe_route(tokens.float() @ self.router.t(), self.topk)
+        scatter_index, splits = _scatter_index(chosen, self.nexperts)
+        up = _mx.MXTensor._of(self.up_data, self.up_blocks, self.hidden)
+        down = _mx.MXTensor._of(self.down_data, self.down_blocks, self.ffn_hidden)
+        h = _mx.mx_grouped_gemm(_mx.mx_quantize(tokens, splits, scatter_index), up, splits, output_dtype=x.dtype)
+        if self.gated:
+            h = self.activation(h[:, :self.ffn_hidden]) * h[:, self.ffn_hidden:]
+        else:
+            h = self.activation(h)
+        y = _mx.mx_grouped_gemm(_mx.mx_quantize(h), down, splits, output_dtype=x.dtype)
+        return _moe.moe_unpermute(y, splits, scatter_index, weights).view(x.shape)

@@ -79,7 +79,8 @@ def test_route(dtype, ntokens, nexperts, topk):
     _within(dz, want, bound + _half_step(dtype) * (want.abs() + bound) + low)
 
 
-def test_route_masks_ties_and_values_that_are_no_numbers():
+@pytest.mark.parametrize("dtype", FLOATS)
+def test_route_masks_ties_and_values_that_are_no_numbers(dtype):
     import flux_b200 as flux
 
     inf, nan = float("inf"), float("nan")
@@ -92,7 +93,9 @@ def test_route_masks_ties_and_values_that_are_no_numbers():
         [0.0, nan, 1.0, -inf, 2.0],            # NaN is the largest, and spreads
         [0.0, inf, 1.0, 5.0, 2.0],
         [1e-40, 2e-40, 0.0, -1e-40, -inf],     # subnormal differences count
-    ])
+    ]).to(dtype)
+    if dtype != torch.float32:
+        z[4] = torch.finfo(dtype).min
     chosen, w = flux.moe_route(z.cuda(), 3)
     want_c, want_w = _route64(z, 3)
     assert torch.equal(chosen.cpu(), want_c)
