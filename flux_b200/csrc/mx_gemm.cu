@@ -241,6 +241,7 @@ static int mx_fill(const char* who, fluxb_comm* comm, MxParams& p, const void* x
   p.groups = (k + kMxGroupK - 1) / kMxGroupK;
   p.out = const_cast<void*>(out);
   p.ldo = n;
+  FLUXB_REQUIRE(comm->ranks_on_gpu <= 1, "%s: not while several ranks share the GPU", who);  // (calls only queue their work then)
   p.out_blocks = p.out_type != kOutF32 && n % 8 == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0 ? 1 : 0;
   p.timeout_ns = comm->timeout_ns;
   p.status = comm->status_dev;

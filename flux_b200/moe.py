@@ -73,6 +73,8 @@ def _check_index(name: str, splits: torch.Tensor, scatter_index: torch.Tensor, n
     if not (_on_device(scatter_index) and scatter_index.dtype == torch.int32 and scatter_index.dim() == 2 and scatter_index.shape[1] >= 1
             and scatter_index.is_contiguous()):
         raise RuntimeError(f"{name}: scatter_index must be a contiguous int32 [ntokens, topk] tensor on the current CUDA device")
+    if scatter_index.numel() >= 1 << 30:
+        raise RuntimeError(f"{name}: {scatter_index.numel()} routed rows are too many")
     if ntokens is not None and scatter_index.shape[0] != ntokens:
         raise RuntimeError(f"{name}: scatter_index has {scatter_index.shape[0]} tokens, not {ntokens}")
 
@@ -119,8 +121,8 @@ def moe_route(logits: torch.Tensor, topk: int):
     if not (_on_device(logits) and logits.dim() == 2 and logits.dtype in _FLOATS):
         raise RuntimeError("moe_route: logits must be a fp32, bf16 or fp16 [ntokens, nexperts] tensor on the current CUDA device")
     topk = int(topk)
-    if not 1 <= topk <= logits.shape[1]:
-        raise RuntimeError(f"moe_route: topk={topk} for {logits.shape[1]} experts")
+    if not 1 <= topk <= logits.shape[1] or logits.shape[0] * topk >= 1 << 30:
+        raise RuntimeError(f"moe_route: topk={topk} for {logits.shape[0]} tokens and {logits.shape[1]} experts")
     if not logits.is_contiguous():
         logits = logits.contiguous()
     if logits.requires_grad and torch.is_grad_enabled():
@@ -196,8 +198,8 @@ class _UnpermuteFn(torch.autograd.Function):
 
 def moe_permute(tokens: torch.Tensor, splits: torch.Tensor, scatter_index: torch.Tensor) -> torch.Tensor:
     """Tokens in the order of their experts: rows [ntokens * topk, hidden] with rows[scatter_index[t, j]] = tokens[t], for
-    `splits` and `scatter_index` as `calc_scatter_index` makes them. Pairs without an expert (entry -1) have no row; the
-    rows past sum(splits) are zero. Any element type; differentiable in floating-point tokens."""
+    `splits` and `scatter_index` as `calc_scatter_index` makes them: every row from 0 to sum(splits) - 1 is named once. Pairs
+    without an expert (entry -1, or any other that is no row) have no row; the rows past sum(splits) are zero. Any element type; differentiable in floating-point tokens."""
     _check(_on_device(tokens) and tokens.dim() == 2 and tokens.shape[1] >= 1, "moe_permute: tokens must be a [ntokens, hidden] tensor on the current CUDA device")
     _check_index("moe_permute", splits, scatter_index, tokens.shape[0])
     if tokens.requires_grad and torch.is_grad_enabled():

@@ -25,16 +25,16 @@ _COMMS: Dict[int, Comm] = {}
 
 
 def _comm() -> Comm:
-    """A communicator of the current device (its status word and time-out): the process's own, or one of one rank."""
+    """A communicator of the current device, for its status word and time-out: the default one (made if there is none yet),
+    or, beside a default of another device, one that this module keeps."""
     dev = _cur_device()
-    if _LAST and _LAST[0].device.index == dev:
+    if not _LAST:
+        get_comm(None)
+    if _LAST[0].device.index == dev:
         return _LAST[0]
     c = _COMMS.get(dev)
     if c is None:
-        c = get_comm(None)
-        if c.device.index != dev:
-            c = Comm(None)
-        _COMMS[dev] = c
+        c = _COMMS[dev] = Comm(None)
     return c
 
 
@@ -109,6 +109,8 @@ def mx_quantize(x: torch.Tensor, splits: Optional[torch.Tensor] = None, scatter_
     if lead or x.stride(1) != 1:
         x = x.contiguous()
     batch, out_rows, topk, nexperts = math.prod(lead), n, 0, 0
+    if batch * n >= 1 << 31:
+        raise RuntimeError(f"mx_quantize: {batch * n} rows are too many")
     if scatter_index is None:
         _check(splits is None, "mx_quantize: splits and scatter_index belong together")
     else:
@@ -140,6 +142,8 @@ def _check_operands(name: str, x: MXTensor, w: MXTensor, wdim: int, output_dtype
         raise RuntimeError(f"{name}: operands must be on the current CUDA device")
     if x.k != w.k:
         raise RuntimeError(f"{name}: weight K {w.k} != input K {x.k}")
+    if x.data.shape[0] >= 1 << 31 or w.data.shape[-2] >= 1 << 31:
+        raise RuntimeError(f"{name}: {x.data.shape[0]} x {w.data.shape[-2]} is too large")
     if output_dtype not in _FLOATS:
         raise RuntimeError(f"{name}: the output must be fp32, bf16 or fp16")
 

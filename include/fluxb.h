@@ -225,7 +225,8 @@ int fluxb_moe_gather_index(const int* scatter_index, int ntokens, int topk, int*
  * fluxb_moe_unpermute_backward: drows[scatter_index[t, j]] = weights[t, j] * dout[t] and
  * dweights[t, j] = <dout[t], rows[scatter_index[t, j]]>; drows may be NULL, and `rows` with `dweights`.
  * The row matrices have ntokens * topk rows. `splits` and `scatter_index` belong together as fluxb_moe_scatter_index makes
- * them: entries outside [0, ntokens * topk) are skipped, rows from sum(splits) on are written as zero. */
+ * them: every row below sum(splits) is named once, entries outside [0, ntokens * topk) are skipped, rows from sum(splits) on
+ * are written as zero. */
 int fluxb_moe_route(const void* logits, int dtype, int ntokens, int nexperts, int topk, int* chosen_out,
                     float* weights_out, fluxb_stream_t stream);
 int fluxb_moe_route_backward(const float* dweights, const int* chosen, const float* weights, int dtype, int ntokens,
@@ -318,7 +319,8 @@ int fluxb_moe_scatter_gemm_static(fluxb_comm_t comm, const void* tokens, int nto
  * fluxb_mx_grouped_gemm: x holds `rows` rows in the order of their experts, splits_dev[e] for expert e (on the device), w is
  * a batch of nexperts matrices [n, k]; rows from sum(splits) on are not written. nexperts <= 1024. workspace:
  * fluxb_mx_grouped_workspace_bytes, 16-byte aligned, this call's own until it has run.
- * Nothing here allocates; calls on several streams and in captured graphs may run side by side.
+ * Nothing here allocates; calls on several streams and in captured graphs may run side by side. Not available while
+ * several ranks share a GPU (fluxb_comm_set_ranks_on_gpu).
  * `comm`: a communicator of the current device (status word, time-out). tuning: cta_group 1 or 2 selects the tiled kernel
  * (block_n tokens: 64 or 128 with 1; 64, 128, 192 or 256 with 2), cta_group 0 with block_n 64, or 16 or 32 for no more
  * tokens than that (grouped: any number), the few-token one. */
