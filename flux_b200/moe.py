@@ -67,16 +67,17 @@ def _on_device(t: torch.Tensor) -> bool:
     return d >= 0 and d == _cur_device()
 
 
-def _check_index(name: str, splits: torch.Tensor, scatter_index: torch.Tensor, ntokens: Optional[int] = None) -> None:
-    if not (_on_device(splits) and splits.dtype == torch.int32 and splits.dim() == 1 and splits.numel() >= 1 and splits.is_contiguous()):
+def _check_index(name: str, dev: int, splits: torch.Tensor, scatter_index: torch.Tensor) -> torch.Size:
+    """Shape [ntokens, topk] of an index whose tensors, like the call's others, are on device `dev`, the current one."""
+    if not (splits.get_device() == dev and splits.dtype is torch.int32 and len(splits.shape) == 1 and splits.shape[0] >= 1 and splits.is_contiguous()):
         raise RuntimeError(f"{name}: splits must be a contiguous int32 [nexperts] tensor on the current CUDA device")
-    if not (_on_device(scatter_index) and scatter_index.dtype == torch.int32 and scatter_index.dim() == 2 and scatter_index.shape[1] >= 1
+    shape = scatter_index.shape
+    if not (scatter_index.get_device() == dev and scatter_index.dtype is torch.int32 and len(shape) == 2 and shape[1] >= 1
             and scatter_index.is_contiguous()):
         raise RuntimeError(f"{name}: scatter_index must be a contiguous int32 [ntokens, topk] tensor on the current CUDA device")
-    if scatter_index.numel() >= 1 << 30:
-        raise RuntimeError(f"{name}: {scatter_index.numel()} routed rows are too many")
-    if ntokens is not None and scatter_index.shape[0] != ntokens:
-        raise RuntimeError(f"{name}: scatter_index has {scatter_index.shape[0]} tokens, not {ntokens}")
+    if shape[0] * shape[1] >= 1 << 30:
+        raise RuntimeError(f"{name}: {shape[0]} x {shape[1]} routed rows are too many")
+    return shape
 
 
 def _route_forward(logits: torch.Tensor, topk: int):
@@ -200,8 +201,12 @@ def moe_permute(tokens: torch.Tensor, splits: torch.Tensor, scatter_index: torch
     """Tokens in the order of their experts: rows [ntokens * topk, hidden] with rows[scatter_index[t, j]] = tokens[t], for
     `splits` and `scatter_index` as `calc_scatter_index` makes them: every row from 0 to sum(splits) - 1 is named once. Pairs
     without an expert (entry -1, or any other that is no row) have no row; the rows past sum(splits) are zero. Any element type; differentiable in floating-point tokens."""
-    _check(_on_device(tokens) and tokens.dim() == 2 and tokens.shape[1] >= 1, "moe_permute: tokens must be a [ntokens, hidden] tensor on the current CUDA device")
-    _check_index("moe_permute", splits, scatter_index, tokens.shape[0])
+    shape = tokens.shape
+    if not (_on_device(tokens) and len(shape) == 2 and shape[1] >= 1):
+        raise RuntimeError("moe_permute: tokens must be a [ntokens, hidden] tensor on the current CUDA device")
+    ntokens, _ = _check_index("moe_permute", tokens.get_device(), splits, scatter_index)
+    if ntokens != shape[0]:
+        raise RuntimeError(f"moe_permute: scatter_index has {ntokens} tokens, not {shape[0]}")
     if tokens.requires_grad and torch.is_grad_enabled():
         _check(tokens.dtype in _FLOATS, "moe_permute: only fp32, bf16 and fp16 tokens have gradients")
         return _PermuteFn.apply(tokens, splits, scatter_index)
@@ -213,14 +218,16 @@ def moe_unpermute(rows: torch.Tensor, splits: torch.Tensor, scatter_index: torch
     """The way back: out[t] = sum over j of weights[t, j] * rows[scatter_index[t, j]], summed in fp32 in the order of j and
     rounded once. `rows` [ntokens * topk, hidden] and `weights` [ntokens, topk] (None: all 1) are fp32, bf16 or fp16 each.
     A token none of whose choices has a row gets zeros. Differentiable in the rows and in the weights."""
-    if not (_on_device(rows) and rows.dim() == 2 and rows.shape[1] >= 1 and rows.dtype in _FLOATS):
+    shape = rows.shape
+    if not (_on_device(rows) and len(shape) == 2 and shape[1] >= 1 and rows.dtype in _FLOATS):
         raise RuntimeError("moe_unpermute: rows must be a fp32, bf16 or fp16 [ntokens * topk, hidden] tensor on the current CUDA device")
-    _check_index("moe_unpermute", splits, scatter_index)
-    if rows.shape[0] != scatter_index.numel():
-        raise RuntimeError(f"moe_unpermute: {rows.shape[0]} rows for {scatter_index.numel()} entries of scatter_index")
+    dev = rows.get_device()
+    ntokens, topk = _check_index("moe_unpermute", dev, splits, scatter_index)
+    if shape[0] != ntokens * topk:
+        raise RuntimeError(f"moe_unpermute: {shape[0]} rows for {ntokens} x {topk} entries of scatter_index")
     if weights is not None:
-        _check(_on_device(weights) and weights.dtype in _FLOATS and weights.shape == scatter_index.shape,
-               "moe_unpermute: weights must be a fp32, bf16 or fp16 [ntokens, topk] tensor on the current CUDA device")
+        if not (weights.get_device() == dev and weights.dtype in _FLOATS and weights.shape == scatter_index.shape):
+            raise RuntimeError("moe_unpermute: weights must be a fp32, bf16 or fp16 [ntokens, topk] tensor on the current CUDA device")
         if not weights.is_contiguous():
             weights = weights.contiguous()
     if torch.is_grad_enabled() and (rows.requires_grad or (weights is not None and weights.requires_grad)):

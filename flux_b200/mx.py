@@ -102,24 +102,33 @@ def mx_quantize(x: torch.Tensor, splits: Optional[torch.Tensor] = None, scatter_
     With `splits` and `scatter_index` (as `calc_scatter_index` makes them) the tokens x [ntokens, K] go into the order of
     their experts on the way, as in `moe_permute`: the result has ntokens * topk rows, and the rows past sum(splits) are
     zero. Has no gradient."""
-    if not (_on_device(x) and x.dim() >= 2 and x.dtype in _FLOATS and x.shape[-1] >= BLOCK and x.shape[-1] % BLOCK == 0):
+    shape = x.shape
+    if not (_on_device(x) and len(shape) >= 2 and x.dtype in _FLOATS and shape[-1] >= BLOCK and shape[-1] % BLOCK == 0):
         raise RuntimeError("mx_quantize: x must be a fp32, bf16 or fp16 [..., N, K] tensor on the current CUDA device, K a multiple of 32")
-    _check(not (x.requires_grad and torch.is_grad_enabled()), "mx_quantize has no gradient: detach x, or call it under torch.no_grad()")
-    *lead, n, k = x.shape
-    if lead or x.stride(1) != 1:
+    if x.requires_grad and torch.is_grad_enabled():
+        raise RuntimeError("mx_quantize has no gradient: detach x, or call it under torch.no_grad()")
+    n, k = shape[-2:]
+    lead, batch = (), 1
+    if len(shape) > 2:
+        lead = shape[:-2]
+        batch = math.prod(lead)
         x = x.contiguous()
-    batch, out_rows, topk, nexperts = math.prod(lead), n, 0, 0
+    elif x.stride(1) != 1:
+        x = x.contiguous()
     if batch * n >= 1 << 31:
         raise RuntimeError(f"mx_quantize: {batch * n} rows are too many")
-    if scatter_index is None:
-        _check(splits is None, "mx_quantize: splits and scatter_index belong together")
-    else:
-        _check(splits is not None and not lead, "mx_quantize: into the order of experts go [ntokens, K] tokens, with splits and scatter_index")
-        _check_index("mx_quantize", splits, scatter_index, n)
-        topk, nexperts = scatter_index.shape[1], splits.numel()
-        out_rows = n * topk
+    out_rows, topk, nexperts = n, 0, 0
+    if scatter_index is not None:
+        if splits is None or lead:
+            raise RuntimeError("mx_quantize: into the order of experts go [ntokens, K] tokens, with splits and scatter_index")
+        ntokens, topk = _check_index("mx_quantize", x.get_device(), splits, scatter_index)
+        if ntokens != n:
+            raise RuntimeError(f"mx_quantize: scatter_index has {ntokens} tokens, not {n}")
+        out_rows, nexperts = n * topk, splits.shape[0]
+    elif splits is not None:
+        raise RuntimeError("mx_quantize: splits and scatter_index belong together")
     data = x.new_empty((*lead, out_rows, k // 2), dtype=torch.uint8)
-    blocks = x.new_empty(_blocks_shape(lead, out_rows, k), dtype=torch.uint8)
+    blocks = data.new_empty(_blocks_shape(lead, out_rows, k))
     _lib.check(_lib.load().fluxb_mx_quantize(x.data_ptr(), fluxb_dtype(x.dtype), batch, n, k, x.stride(-2), data.data_ptr(), blocks.data_ptr(),
                                              _ptr(splits), nexperts, _ptr(scatter_index), topk, _cur_stream()))
     return MXTensor._of(data, blocks, k)
