@@ -15,8 +15,8 @@ namespace fluxb {
 // A group of G lanes per token, VPL logits a lane in registers as order-preserving integers. A choice is a maximum over the
 // lanes, ties to the lower expert, and only the lane that held it looks for its next one. 16-bit logits leave room for the
 // expert in the same word, so that one maximum finds both; for fp32 a vote finds the lowest lane (its experts are lower)
-// that has the largest key. Bound by instructions, so a warp takes as many tokens as it can (32768 x 8 experts top-2 took
-// 9.0 us with a warp per token, 32768 x 128 top-8 22.5 us with maxima over 64-bit pairs of key and expert).
+// that has the largest key. Bound by instructions, so a warp takes as many tokens as it can: 32768 x 8 bf16 top-2 2.8 us (a
+// warp per token 9.0), 16384 x 64 bf16 top-6 4.4, 32768 x 128 fp32 top-8 17.7 (maxima over 64-bit pairs of key and expert 22.5).
 constexpr int kRouteThreads = 128;
 constexpr int kRouteMaxExperts = 1024;
 constexpr int kRouteMaxTopk = 32;
@@ -246,6 +246,7 @@ __device__ __forceinline__ void sort_clear_tail(typename RawVec<VB>::type* rows_
 }
 
 // `width` threads (a power of two from 32 to 256) take one token: each vector is read once and stored to the token's rows.
+// 8192 x 4096 bf16 top-2 33 us, 6.1 TB/s; rows of odd length go two or one bytes at a time (4096 x 1001 bf16 9.3 us, 2.7 TB/s).
 template <int VB>
 __global__ void __launch_bounds__(kSortThreads)
 moe_permute_kernel(const typename RawVec<VB>::type* __restrict__ tokens, int ntokens, int topk, int row_vecs, int width, int main_ctas,
@@ -346,8 +347,8 @@ __device__ __forceinline__ void gather_weights(float (&w)[UN], const void* weigh
 }
 
 // out[t] = sum_j w[t, j] rows[index[t, j]], j ascending, rounded once; without weights the plain sum.
-// (8192 x 4096 bf16: top-2 with one vector of two rows a thread and a CTA for every token 60 us, with eight vectors in
-// registers and resident CTAs 38.)
+// 8192 x 4096 bf16 top-2 32.6 us, 6.2 TB/s (one vector of two rows a thread and a CTA for every token 60, eight vectors in
+// registers and resident CTAs 38); 8192 x 2048 top-6 47 us, 5.0 TB/s (72, 65).
 template <class T, int VB, int UN>
 __global__ void __launch_bounds__(kSortThreads, 2)
 moe_unpermute_kernel(const typename RawVec<VB>::type* __restrict__ rows_in, int ntokens, int topk, int row_vecs, int width,
@@ -501,7 +502,7 @@ moe_unpermute_narrow_kernel(const typename RawVec<VB>::type* __restrict__ rows_i
 // drows[index[t, j]] = w[t, j] dout[t] and dw[t, j] = <dout[t], rows[index[t, j]]>, KC choices at a time, whose rows and dout come
 // through the ring: dout is read once for them, and the products stay in fp32 until the token's threads add them up.
 // `rows_in` and `dweights` are null where only drows is wanted. An item is VU vectors; vectors change fastest, then choices.
-// (8192 x 2048 bf16 top-6 with the rows in registers 125 us, 3.5 TB/s.)
+// 8192 x 4096 bf16 top-2 56.5 us, 5.9 TB/s; 8192 x 2048 top-6 76 us, 5.7 TB/s (with the rows in registers 125).
 constexpr int scatter_vectors(int vb, int kc) { return (vb == 16 ? 1 : 2) * (kc == 2 ? 2 : 1); }
 constexpr int scatter_depth(int vb, int kc) { return kGatherSmem / (kSortThreads * vb * (kc + 1) * scatter_vectors(vb, kc)); }
 template <class T, int VB, int KC>

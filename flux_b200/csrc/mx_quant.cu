@@ -7,6 +7,7 @@
 // Bound by memory, and by instructions next (75% of the issue slots with 8 values a thread and everything in fp32): two lanes
 // share 32 values, 16 each, the largest is found in the input's own type, two values at a time, and bf16 is scaled so, too,
 // which is exact. The four scales of a cell (mx_format.cuh) are one store. Two pieces of a thread are in flight together.
+// 14336 x 12288 bf16 74 us, 6.0 TB/s (129 before); back to bf16 72 us, 6.2 TB/s (144 with codes taken apart by shifts).
 #include "internal.h"
 #include "mx_format.cuh"
 #include "plain_gemm.cuh"

@@ -397,6 +397,8 @@ class MXMoEMLP(torch.nn.Module):
     @torch.no_grad()
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         tokens = x.reshape(-1, self.hidden)
+        if tokens.shape[0] == 0:
+            return torch.empty_like(x)
         chosen, weights = _moe.moe_route(tokens.float() @ self.router.t(), self.topk)
         scatter_index, splits = _scatter_index(chosen, self.nexperts)
         up = _mx.MXTensor._of(self.up_data, self.up_blocks, self.hidden)

@@ -131,7 +131,8 @@ def test_route_gradient_against_differences():
 
 
 # ----------------------------------------------------------------------------------------------------- permute, unpermute
-SIZES = [(1, 4, 1, 1), (1, 8, 2, 4096), (3, 8, 2, 2), (7, 16, 5, 33), (130, 8, 2, 64), (33, 64, 9, 130), (257, 32, 4, 1000), (20, 300, 12, 4100)]
+SIZES = [(1, 4, 1, 1), (1, 8, 2, 4096), (3, 8, 2, 2), (7, 16, 5, 33), (130, 8, 2, 64), (33, 64, 9, 130), (257, 32, 4, 1000), (20, 300, 12, 4100),
+         (5000, 16, 3, 264), (6000, 8, 2, 36), (3001, 64, 10, 16)]
 
 
 def _pairs(si):

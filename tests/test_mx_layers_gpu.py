@@ -112,6 +112,16 @@ def test_moe_layer_captured_and_replayed():
     flux.get_comm(None).check_status()
 
 
+def test_no_tokens():
+    import flux_b200 as flux
+
+    layer = flux.MXMoEMLP.from_moe(flux.MoEMLP(128, 64, 4, 2, 8, None, dtype=torch.bfloat16))
+    x = torch.empty(0, 128, device="cuda", dtype=torch.bfloat16)
+    assert layer(x).shape == (0, 128)
+    assert flux.MXLinear(torch.randn(48, 128, device="cuda"))(x).shape == (0, 48)
+    torch.cuda.synchronize()
+
+
 def test_layers_refuse_what_does_not_fit():
     import flux_b200 as flux
 
