@@ -328,7 +328,7 @@ class MXLinear(torch.nn.Module):
     def __init__(self, weight, bias: Optional[torch.Tensor] = None, output_dtype: Optional[torch.dtype] = None):
         super().__init__()
         w = weight if isinstance(weight, _mx.MXTensor) else _mx.mx_quantize(weight.detach())
-        if w.data.dim() != 2:
+        if w.lead:
             raise RuntimeError("MXLinear: the weight must be [out_features, in_features]")
         self.out_features, self.in_features = w.shape
         self.output_dtype = output_dtype
@@ -345,7 +345,7 @@ class MXLinear(torch.nn.Module):
 
     @torch.no_grad()
     def forward(self, x: torch.Tensor) -> torch.Tensor:
-        w = _mx.MXTensor._of(self.weight_data, self.weight_blocks, self.in_features)
+        w = _mx.MXTensor._of(self.weight_data, self.weight_blocks)
         y = _mx.mx_gemm(_mx.mx_quantize(x.reshape(-1, x.shape[-1])), w, bias=self.bias, output_dtype=self.output_dtype or x.dtype)
         return y.view(*x.shape[:-1], self.out_features)
 
@@ -372,7 +372,7 @@ class MXMoEMLP(torch.nn.Module):
             w_up = torch.cat((w_gate.detach(), w_up.detach()), dim=1)
         quantised = [w if isinstance(w, _mx.MXTensor) else _mx.mx_quantize(w.detach()) for w in (w_up, w_down)]
         up, down = quantised
-        if not (up.data.dim() == 3 and down.data.dim() == 3 and router.dim() == 2):
+        if not (len(up.lead) == 1 and len(down.lead) == 1 and router.dim() == 2):
             raise RuntimeError("MXMoEMLP: the router must be [E, hidden], the experts' weights [E, ffn, hidden] and [E, hidden, ffn]")
         nexperts, up_rows, hidden = up.shape
         self.nexperts, self.hidden, self.ffn_hidden = nexperts, hidden, up_rows // 2 if self.gated else up_rows
@@ -401,8 +401,8 @@ class MXMoEMLP(torch.nn.Module):
             return torch.empty_like(x)
         chosen, weights = _moe.moe_route(tokens.float() @ self.router.t(), self.topk)
         scatter_index, splits = _scatter_index(chosen, self.nexperts)
-        up = _mx.MXTensor._of(self.up_data, self.up_blocks, self.hidden)
-        down = _mx.MXTensor._of(self.down_data, self.down_blocks, self.ffn_hidden)
+        up = _mx.MXTensor._of(self.up_data, self.up_blocks)
+        down = _mx.MXTensor._of(self.down_data, self.down_blocks)
         h = _mx.mx_grouped_gemm(_mx.mx_quantize(tokens, splits, scatter_index), up, splits, output_dtype=x.dtype)
         if self.gated:
             h = self.activation(h[:, :self.ffn_hidden]) * h[:, self.ffn_hidden:]

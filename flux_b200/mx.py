@@ -45,9 +45,13 @@ def _blocks_shape(lead, rows: int, k: int):
 class MXTensor:
     """Matrices [..., N, K] as packed e2m1 values and scales. The constructor takes them as a checkpoint holds them, `data`
     uint8 [..., N, K / 2] and `scales` uint8 [..., N, K / 32], and lays the scales out once, in the blocks of 128 rows x 4
-    scales that the tensor cores read (fluxb.h); `mx_quantize` makes them that way. `scales` gives them back row by row."""
+    scales that the tensor cores read (fluxb.h); `mx_quantize` makes them that way. `data`, `blocks` (the laid-out scales)
+    and `scales` (row by row again, a copy) are tensors.
 
-    __slots__ = ("data", "blocks", "k")
+    What a product needs of it is kept as plain numbers, and `mx_quantize` puts values and scales into one allocation, of
+    which `data` and `blocks` are views made when asked for: a call's tensor bookkeeping took as long as its launch."""
+
+    __slots__ = ("lead", "rows", "k", "_dev", "_store", "_data", "_blocks", "_data_ptr", "_blocks_ptr")
 
     def __init__(self, data: torch.Tensor, scales: torch.Tensor):
         _check(_on_device(data) and _on_device(scales), "MXTensor: data and scales must be on the current CUDA device")
@@ -65,28 +69,46 @@ class MXTensor:
         rows = torch.zeros((*lead, shape[-3] * 128, shape[-2] * 4), dtype=torch.uint8, device=data.device)
         rows[..., :n, :k // BLOCK] = scales
         # row = 128 block + 32 column + lane, scale = 4 group + s  ->  [block, group, lane, column, s]
-        self.blocks = rows.view(-1, shape[-3], 4, 32, shape[-2], 4).permute(0, 1, 4, 3, 2, 5).contiguous().view(shape)
-        self.data, self.k = data, k
+        self._set(data, rows.view(-1, shape[-3], 4, 32, shape[-2], 4).permute(0, 1, 4, 3, 2, 5).contiguous().view(shape))
+
+    def _set(self, data: torch.Tensor, blocks: torch.Tensor) -> None:
+        *lead, self.rows, half = data.shape
+        self.lead, self.k, self._dev = tuple(lead), half * 2, data.get_device()
+        self._store, self._data, self._blocks = None, data, blocks
+        self._data_ptr, self._blocks_ptr = data.data_ptr(), blocks.data_ptr()
 
     @classmethod
-    def _of(cls, data: torch.Tensor, blocks: torch.Tensor, k: int) -> "MXTensor":
+    def _of(cls, data: torch.Tensor, blocks: torch.Tensor) -> "MXTensor":
         t = cls.__new__(cls)
-        t.data, t.blocks, t.k = data, blocks, k
+        t._set(data, blocks)
         return t
+
+    @property
+    def data(self) -> torch.Tensor:
+        if self._data is None:
+            n = math.prod(self.lead) * self.rows * (self.k // 2)
+            self._data = self._store[:n].view(*self.lead, self.rows, self.k // 2)
+        return self._data
+
+    @property
+    def blocks(self) -> torch.Tensor:
+        if self._blocks is None:
+            self._blocks = self._store[self._blocks_ptr - self._data_ptr:].view(_blocks_shape(self.lead, self.rows, self.k))
+        return self._blocks
 
     @property
     def scales(self) -> torch.Tensor:
         *lead, nb, groups, _ = self.blocks.shape
         rows = self.blocks.view(-1, nb, groups, 32, 4, 4).permute(0, 1, 4, 3, 2, 5).reshape(*lead, nb * 128, groups * 4)
-        return rows[..., :self.data.shape[-2], :self.k // BLOCK].contiguous()
+        return rows[..., :self.rows, :self.k // BLOCK].contiguous()
 
     @property
     def shape(self) -> torch.Size:
-        return torch.Size((*self.data.shape[:-1], self.k))
+        return torch.Size((*self.lead, self.rows, self.k))
 
     @property
     def device(self) -> torch.device:
-        return self.data.device
+        return torch.device("cuda", self._dev)
 
     def dequantize(self, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
         return mx_dequantize(self, dtype)
@@ -110,7 +132,7 @@ def mx_quantize(x: torch.Tensor, splits: Optional[torch.Tensor] = None, scatter_
     n, k = shape[-2:]
     lead, batch = (), 1
     if len(shape) > 2:
-        lead = shape[:-2]
+        lead = tuple(shape[:-2])
         batch = math.prod(lead)
         x = x.contiguous()
     elif x.stride(1) != 1:
@@ -127,32 +149,42 @@ def mx_quantize(x: torch.Tensor, splits: Optional[torch.Tensor] = None, scatter_
         out_rows, nexperts = n * topk, splits.shape[0]
     elif splits is not None:
         raise RuntimeError("mx_quantize: splits and scatter_index belong together")
-    data = x.new_empty((*lead, out_rows, k // 2), dtype=torch.uint8)
-    blocks = data.new_empty(_blocks_shape(lead, out_rows, k))
-    _lib.check(_lib.load().fluxb_mx_quantize(x.data_ptr(), fluxb_dtype(x.dtype), batch, n, k, x.stride(-2), data.data_ptr(), blocks.data_ptr(),
+    t = MXTensor.__new__(MXTensor)
+    t.lead, t.rows, t.k, t._dev = lead, out_rows, k, x.get_device()
+    at = (batch * out_rows * (k // 2) + 15) & ~15  # where the scales start
+    t._store = x.new_empty(at + batch * ((out_rows + 127) // 128) * ((k + 127) // 128) * 512, dtype=torch.uint8)
+    t._data = t._blocks = None
+    t._data_ptr = t._store.data_ptr()
+    t._blocks_ptr = t._data_ptr + at
+    _lib.check(_lib.load().fluxb_mx_quantize(x.data_ptr(), fluxb_dtype(x.dtype), batch, n, k, x.stride(-2), t._data_ptr, t._blocks_ptr,
                                              _ptr(splits), nexperts, _ptr(scatter_index), topk, _cur_stream()))
-    return MXTensor._of(data, blocks, k)
+    return t
+
+
+def _like(q: MXTensor) -> torch.Tensor:
+    return q._data if q._store is None else q._store
 
 
 def mx_dequantize(q: MXTensor, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """The values that `q` stands for, as fp32, bf16 or fp16 (exact in bf16 but beyond its range)."""
-    _check(isinstance(q, MXTensor) and _on_device(q.data), "mx_dequantize: q must be an MXTensor on the current CUDA device")
-    _check(dtype in _FLOATS, "mx_dequantize: the output must be fp32, bf16 or fp16")
-    *lead, n, _ = q.data.shape
-    out = q.data.new_empty((*lead, n, q.k), dtype=dtype)
-    _lib.check(_lib.load().fluxb_mx_dequantize(q.data.data_ptr(), q.blocks.data_ptr(), math.prod(lead), n, q.k, fluxb_dtype(dtype), out.data_ptr(), _cur_stream()))
+    if not (isinstance(q, MXTensor) and q._dev == _cur_device()):
+        raise RuntimeError("mx_dequantize: q must be an MXTensor on the current CUDA device")
+    if dtype not in _FLOATS:
+        raise RuntimeError("mx_dequantize: the output must be fp32, bf16 or fp16")
+    out = _like(q).new_empty((*q.lead, q.rows, q.k), dtype=dtype)
+    _lib.check(_lib.load().fluxb_mx_dequantize(q._data_ptr, q._blocks_ptr, math.prod(q.lead), q.rows, q.k, fluxb_dtype(dtype), out.data_ptr(), _cur_stream()))
     return out
 
 
 def _check_operands(name: str, x: MXTensor, w: MXTensor, wdim: int, output_dtype: torch.dtype) -> None:
-    if not (isinstance(x, MXTensor) and isinstance(w, MXTensor) and x.data.dim() == 2 and w.data.dim() == wdim):
+    if not (isinstance(x, MXTensor) and isinstance(w, MXTensor) and not x.lead and len(w.lead) == wdim - 2):
         raise RuntimeError(f"{name}: operands must be MXTensors, [rows, K] and {'[N, K]' if wdim == 2 else '[nexperts, N, K]'}")
-    if not (_on_device(x.data) and _on_device(w.data)):
+    if not x._dev == w._dev == _cur_device():
         raise RuntimeError(f"{name}: operands must be on the current CUDA device")
     if x.k != w.k:
         raise RuntimeError(f"{name}: weight K {w.k} != input K {x.k}")
-    if x.data.shape[0] >= 1 << 31 or w.data.shape[-2] >= 1 << 31:
-        raise RuntimeError(f"{name}: {x.data.shape[0]} x {w.data.shape[-2]} is too large")
+    if x.rows >= 1 << 31 or w.rows >= 1 << 31:
+        raise RuntimeError(f"{name}: {x.rows} x {w.rows} is too large")
     if output_dtype not in _FLOATS:
         raise RuntimeError(f"{name}: the output must be fp32, bf16 or fp16")
 
@@ -170,15 +202,15 @@ def mx_gemm(x: MXTensor, w: MXTensor, bias: Optional[torch.Tensor] = None, outpu
     """y[M, N] = x[M, K] . w[N, K]^T (+ bias [N] of the output's type): exact products, summed in fp32, rounded once. M, N of
     any size."""
     _check_operands("mx_gemm", x, w, 2, output_dtype)
-    m, n = x.data.shape[0], w.data.shape[0]
+    m, n = x.rows, w.rows
     if bias is not None:
         _check(_on_device(bias) and bias.dtype == output_dtype and tuple(bias.shape) in ((n,), (1, n)) and bias.is_contiguous(),
                "mx_gemm: bias must be a contiguous [N] tensor of the output's type")
-    out = _output("mx_gemm", output, m, n, output_dtype, x.data)
+    out = _output("mx_gemm", output, m, n, output_dtype, _like(x))
     if n == 0:
         return out
-    _lib.check(_lib.load().fluxb_mx_gemm(_comm().handle, x.data.data_ptr(), x.blocks.data_ptr(), w.data.data_ptr(), w.blocks.data_ptr(), out.data_ptr(),
-                                         m, n, x.k, fluxb_dtype(output_dtype), _ptr(bias), _tuning(tuning), _cur_stream()))
+    _lib.check(_lib.load().fluxb_mx_gemm(_comm().handle, x._data_ptr, x._blocks_ptr, w._data_ptr, w._blocks_ptr, out.data_ptr(), m, n, x.k,
+                                         fluxb_dtype(output_dtype), _ptr(bias), _tuning(tuning), _cur_stream()))
     return out
 
 
@@ -188,16 +220,15 @@ def mx_grouped_gemm(x: MXTensor, w: MXTensor, splits: torch.Tensor, output_dtype
     [nexperts], on the GPU: nothing is read back), times w [nexperts, N, K]. Rows past sum(splits) are not written: they
     stay as they were in a given `output`, and are undefined in a fresh one."""
     _check_operands("mx_grouped_gemm", x, w, 3, output_dtype)
-    nexperts, n = w.data.shape[0], w.data.shape[1]
-    rows = x.data.shape[0]
-    if not (_on_device(splits) and splits.dtype == torch.int32 and splits.dim() == 1 and splits.numel() == nexperts and splits.is_contiguous()):
+    nexperts, n, rows = w.lead[0], w.rows, x.rows
+    if not (splits.get_device() == x._dev and splits.dtype is torch.int32 and tuple(splits.shape) == (nexperts,) and splits.is_contiguous()):
         raise RuntimeError(f"mx_grouped_gemm: splits must be a contiguous int32 [{nexperts}] tensor on the current CUDA device")
-    out = _output("mx_grouped_gemm", output, rows, n, output_dtype, x.data)
+    out = _output("mx_grouped_gemm", output, rows, n, output_dtype, _like(x))
     if n == 0 or nexperts == 0:
         return out
     lib = _lib.load()
-    workspace = x.data.new_empty(lib.fluxb_mx_grouped_workspace_bytes(rows, nexperts, x.k))
-    _lib.check(lib.fluxb_mx_grouped_gemm(_comm().handle, x.data.data_ptr(), x.blocks.data_ptr(), rows, w.data.data_ptr(), w.blocks.data_ptr(), nexperts,
+    workspace = _like(x).new_empty(lib.fluxb_mx_grouped_workspace_bytes(rows, nexperts, x.k))
+    _lib.check(lib.fluxb_mx_grouped_gemm(_comm().handle, x._data_ptr, x._blocks_ptr, rows, w._data_ptr, w._blocks_ptr, nexperts,
                                          splits.data_ptr(), out.data_ptr(), n, x.k, fluxb_dtype(output_dtype), workspace.data_ptr(), _tuning(tuning),
                                          _cur_stream()))
     return out
