@@ -792,6 +792,10 @@ mx_few_kernel(const __grid_constant__ MxParams p) {
       mbar_init(bar_done, 1);
       mbar_init(bar_retired, 1);
       mbar_init_fence();
+      tma_prefetch_desc(&p.tmap_w);
+      tma_prefetch_desc(&p.tmap_x);
+      tma_prefetch_desc(&p.tmap_sw);
+      if (!GROUPED) tma_prefetch_desc(&p.tmap_sx);
     }
     __syncwarp();
     pdl_wait();  // nothing before this line reads global memory
