@@ -503,8 +503,8 @@ moe_unpermute_narrow_kernel(const typename RawVec<VB>::type* __restrict__ rows_i
 // through the ring: dout is read once for them, and the products stay in fp32 until the token's threads add them up.
 // `rows_in` and `dweights` are null where only drows is wanted. An item is VU vectors; vectors change fastest, then choices.
 // 8192 x 4096 bf16 top-2 56.5 us, 5.9 TB/s; 8192 x 2048 top-6 76 us, 5.7 TB/s (with the rows in registers 125).
-constexpr int scatter_vectors(int vb, int kc) { return (vb == 16 ? 1 : 2) * (kc == 2 ? 2 : 1); }
-constexpr int scatter_depth(int vb, int kc) { return kGatherSmem / (kSortThreads * vb * (kc + 1) * scatter_vectors(vb, kc)); }
+constexpr int scatter_vectors(int kc) { return kc == 2 ? 2 : 1; }
+constexpr int scatter_depth(int vb, int kc) { return kGatherSmem / (kSortThreads * vb * (kc + 1) * scatter_vectors(kc)); }
 template <class T, int VB, int KC>
 __global__ void __launch_bounds__(kSortThreads, 2)
 moe_unpermute_backward_kernel(const typename RawVec<VB>::type* __restrict__ dout, const typename RawVec<VB>::type* __restrict__ rows_in,
@@ -512,7 +512,7 @@ moe_unpermute_backward_kernel(const typename RawVec<VB>::type* __restrict__ dout
                               const int* __restrict__ index, const void* __restrict__ weights, int wdtype,
                               typename RawVec<VB>::type* __restrict__ drows, void* __restrict__ dweights) {
   using V = SortVec<T, VB>;
-  constexpr int VU = scatter_vectors(VB, KC), D = scatter_depth(VB, KC);
+  constexpr int VU = scatter_vectors(KC), D = scatter_depth(VB, KC);
   __shared__ float part[2][kSortThreads / 32][KC];
   extern __shared__ __align__(16) uint8_t gather_smem[];
   const uint32_t slots = smem_u32(gather_smem) + threadIdx.x * VB;  // [D][KC + 1][VU][threads] vectors, dout first
@@ -633,7 +633,9 @@ moe_unpermute_backward_kernel(const typename RawVec<VB>::type* __restrict__ dout
   copy_wait<0>();
 }
 
-// The same for vectors of 2 and 4 bytes, KC choices of VU vectors in registers.
+// The same for vectors below 16 bytes, KC choices of VU vectors in registers. Vectors of 8 bytes (widths that 8 does not divide) against
+// the ring, which has to copy twice as often for the same bytes: 8192 x 4100 bf16 top-2 70 and 85 us, 8192 x 2052 top-6 105 and 133,
+// 2000 x 5124 fp16 top-4 38 and 41. (The sum above reads only, and is faster from the ring: top-6 82 against 152.)
 template <class T, int VB, int KC, int VU>
 __global__ void __launch_bounds__(kSortThreads)
 moe_unpermute_backward_narrow_kernel(const typename RawVec<VB>::type* __restrict__ dout, const typename RawVec<VB>::type* __restrict__ rows_in,
@@ -818,8 +820,8 @@ template <class T, int VB, int KC>
 static int launch_unpermute_backward_rows(const void* dout, const void* rows, int ntokens, int topk, int row_vecs, const int* splits, int nexperts,
                                           const int* index, const void* weights, int wdtype, void* drows, void* dweights, cudaStream_t stream) {
   using R = typename RawVec<VB>::type;
-  constexpr bool NARROW = VB < 8;
-  constexpr int VU = NARROW ? 8 / KC : scatter_vectors(VB, KC), SMEM = NARROW ? 0 : scatter_depth(VB, KC) * (KC + 1) * VU * VB * kSortThreads;
+  constexpr bool NARROW = VB < 16;
+  constexpr int VU = NARROW ? 8 / KC : scatter_vectors(KC), SMEM = NARROW ? 0 : scatter_depth(VB, KC) * (KC + 1) * VU * VB * kSortThreads;
   auto kern = [] {
     if constexpr (NARROW) return moe_unpermute_backward_narrow_kernel<T, VB, KC, VU>;
     else return moe_unpermute_backward_kernel<T, VB, KC>;
