@@ -135,8 +135,11 @@ def mx_quantize(x: torch.Tensor, splits: Optional[torch.Tensor] = None, scatter_
         lead = tuple(shape[:-2])
         batch = math.prod(lead)
         x = x.contiguous()
-    elif x.stride(1) != 1:
-        x = x.contiguous()
+        ldx = k  # (a contiguous tensor's stride along a dimension of one row may be any number)
+    else:
+        if x.stride(1) != 1:
+            x = x.contiguous()
+        ldx = x.stride(0) if n > 1 else k
     if batch * n >= 1 << 31:
         raise RuntimeError(f"mx_quantize: {batch * n} rows are too many")
     out_rows, topk, nexperts = n, 0, 0
@@ -156,7 +159,7 @@ def mx_quantize(x: torch.Tensor, splits: Optional[torch.Tensor] = None, scatter_
     t._data = t._blocks = None
     t._data_ptr = t._store.data_ptr()
     t._blocks_ptr = t._data_ptr + at
-    _lib.check(_lib.load().fluxb_mx_quantize(x.data_ptr(), fluxb_dtype(x.dtype), batch, n, k, x.stride(-2), t._data_ptr, t._blocks_ptr,
+    _lib.check(_lib.load().fluxb_mx_quantize(x.data_ptr(), fluxb_dtype(x.dtype), batch, n, k, ldx, t._data_ptr, t._blocks_ptr,
                                              _ptr(splits), nexperts, _ptr(scatter_index), topk, _cur_stream()))
     return t
 

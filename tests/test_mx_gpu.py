@@ -118,6 +118,19 @@ def test_quantize_layouts():
         assert torch.equal(q.data.cpu(), data) and torch.equal(q.scales.cpu(), scales)
 
 
+def test_quantize_matrices_of_one_row():
+    """Contiguous by torch's rules whatever the stride along the row that there is one of."""
+    import flux_b200 as flux
+
+    g = torch.Generator().manual_seed(8)
+    for x in (torch.randn(3, 64, 1, generator=g).transpose(1, 2), torch.randn(2, 3, 96, 1, generator=g).transpose(2, 3),
+              torch.randn(64, 1, generator=g).t(), torch.randn(5, 64, generator=g)[:, None, :]):
+        x = x.cuda()
+        q = flux.mx_quantize(x)
+        data, scales = _quantised64(x)
+        assert q.shape == x.shape and torch.equal(q.data.cpu(), data) and torch.equal(q.scales.cpu(), scales)
+
+
 def test_quantize_into_the_order_of_experts():
     import flux_b200 as flux
 
