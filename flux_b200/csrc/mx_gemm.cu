@@ -154,6 +154,9 @@ static MxChoice mx_choose(int sm_count, int nexperts, int rows, int n, int num_k
   return best;
 }
 
+// A tile's last row is a 31-bit integer, too.
+constexpr int kMxMostRows = 0x7FFFFFFF - 512;
+
 static int mx_out_type(int out_dtype, int* ot) {
   switch (out_dtype) {
     case FLUXB_BF16: *ot = kOutBf16; return FLUXB_OK;
@@ -228,7 +231,7 @@ static int mx_fill(const char* who, fluxb_comm* comm, MxParams& p, const void* x
                    int out_dtype) {
   FLUXB_REQUIRE(comm != nullptr && xq != nullptr && xs != nullptr && wq != nullptr && ws != nullptr && out != nullptr, "%s: NULL argument", who);
   FLUXB_REQUIRE(k >= kMxBlock && k % kMxBlock == 0, "%s: k=%d must be a multiple of %d", who, k, kMxBlock);
-  FLUXB_REQUIRE(n >= 1, "%s: n=%d invalid", who, n);
+  FLUXB_REQUIRE(n >= 1 && n <= kMxMostRows, "%s: n=%d invalid", who, n);
   FLUXB_REQUIRE(((reinterpret_cast<uintptr_t>(xq) | reinterpret_cast<uintptr_t>(xs) | reinterpret_cast<uintptr_t>(wq) | reinterpret_cast<uintptr_t>(ws)) & 15) == 0,
                 "%s: operands and their scales must be 16-byte aligned", who);
   memset(&p, 0, sizeof(p));
@@ -268,7 +271,7 @@ size_t fluxb_mx_grouped_workspace_bytes(int rows, int nexperts, int k) {
 
 int fluxb_mx_gemm(fluxb_comm_t comm, const void* xq, const void* xs, const void* wq, const void* ws, void* out, int m, int n, int k, int out_dtype,
                   const void* bias, const fluxb_tuning* tuning, fluxb_stream_t stream) {
-  FLUXB_REQUIRE(m >= 0, "mx_gemm: m=%d invalid", m);
+  FLUXB_REQUIRE(m >= 0 && m <= kMxMostRows, "mx_gemm: m=%d invalid", m);
   if (m == 0) return FLUXB_OK;
   MxParams p;
   const int rc = mx_fill("mx_gemm", comm, p, xq, xs, wq, ws, out, n, k, out_dtype);
@@ -282,7 +285,7 @@ int fluxb_mx_gemm(fluxb_comm_t comm, const void* xq, const void* xs, const void*
 int fluxb_mx_grouped_gemm(fluxb_comm_t comm, const void* xq, const void* xs, int rows, const void* wq, const void* ws, int nexperts,
                           const int* splits_dev, void* out, int n, int k, int out_dtype, void* workspace, const fluxb_tuning* tuning,
                           fluxb_stream_t stream) {
-  FLUXB_REQUIRE(rows >= 0, "mx_grouped_gemm: rows=%d invalid", rows);
+  FLUXB_REQUIRE(rows >= 0 && rows <= kMxMostRows, "mx_grouped_gemm: rows=%d invalid", rows);
   FLUXB_REQUIRE(nexperts >= 1 && nexperts <= kMxMaxExperts, "mx_grouped_gemm: nexperts=%d out of [1,%d]", nexperts, kMxMaxExperts);
   if (rows == 0) return FLUXB_OK;
   FLUXB_REQUIRE(splits_dev != nullptr && workspace != nullptr, "mx_grouped_gemm: NULL argument");

@@ -62,6 +62,16 @@ def test_product_arguments(change, words):
     assert words in _lib.last_error()
 
 
+@pytest.mark.parametrize("change", [{"m": (1 << 31) - 1}, {"m": (1 << 31) - 512}, {"n": (1 << 31) - 1}])
+def test_rows_whose_tiles_would_pass_31_bits(change):
+    a = {"m": 4, "n": 8, **change}
+    lib = _lib.load()
+    assert lib.fluxb_mx_gemm(P, P, P, P, P, P, a["m"], a["n"], 32, _lib.BF16, None, None, None) == _lib.FLUXB_ERR_INVALID
+    assert "invalid" in _lib.last_error()
+    assert lib.fluxb_mx_grouped_gemm(P, P, P, a["m"], P, P, 1, P, P, a["n"], 32, _lib.BF16, P, None, None) == _lib.FLUXB_ERR_INVALID
+    assert "invalid" in _lib.last_error() or "too many" in _lib.last_error()
+
+
 def test_grouped_arguments():
     lib = _lib.load()
     for nexperts, n, splits, ws, words in ((0, 8, P, P, "nexperts=0"), (1025, 8, P, P, "nexperts=1025"), (4, 8, None, P, "NULL"), (4, 8, P, None, "NULL"),
