@@ -209,6 +209,8 @@ def mx_gemm(x: MXTensor, w: MXTensor, bias: Optional[torch.Tensor] = None, outpu
     if bias is not None:
         _check(_on_device(bias) and bias.dtype == output_dtype and tuple(bias.shape) in ((n,), (1, n)) and bias.is_contiguous(),
                "mx_gemm: bias must be a contiguous [N] tensor of the output's type")
+        if bias.requires_grad and torch.is_grad_enabled():
+            raise RuntimeError("mx_gemm has no gradient: detach the bias, or call it under torch.no_grad()")
     out = _output("mx_gemm", output, m, n, output_dtype, _like(x))
     if n == 0:
         return out

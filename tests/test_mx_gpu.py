@@ -323,3 +323,14 @@ def test_empty_operands_and_refusals():
     for call, words in cases:
         with pytest.raises(RuntimeError, match=words):
             call()
+
+
+def test_a_bias_with_a_gradient_is_refused():
+    import flux_b200 as flux
+
+    x, w = (flux.mx_quantize(torch.randn(n, 96, device="cuda")) for n in (3, 64))
+    bias = torch.zeros(64, dtype=torch.bfloat16, device="cuda", requires_grad=True)
+    with pytest.raises(RuntimeError, match="no gradient"):
+        flux.mx_gemm(x, w, bias=bias)
+    with torch.no_grad():
+        assert torch.equal(flux.mx_gemm(x, w, bias=bias), flux.mx_gemm(x, w))
