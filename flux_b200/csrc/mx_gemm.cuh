@@ -422,12 +422,8 @@ mx_gemm_kernel(const __grid_constant__ MxParams p) {
       MxTile tl;
       for (int t = worker; ok && mx_tile<BN, GROUPED>(p, TILE_N, t, groups, tl); t += workers, ++it) {
         const int acc = it & 1;
-        // its accumulator has been read; overlapping ones: the columns that the tile before shares with this one
-        // (and with them everything of the tile before that)
-        const bool free = OVERLAP ? it == 0 || mbar_wait<CTA2>(bar_tempty(0), (it - 1) & 1, ab, kStatusTimeoutTmemEmpty, budget)
-                                  : mbar_wait<CTA2>(bar_tempty(acc), ((it >> 1) & 1) ^ 1u, ab, kStatusTimeoutTmemEmpty, budget);
-        if (!free) break;
-        tc_fence_after();
+        // its accumulator has been read
+        if (!OVERLAP && !mbar_wait<CTA2>(bar_tempty(acc), ((it >> 1) & 1) ^ 1u, ab, kStatusTimeoutTmemEmpty, budget)) break;
         const uint32_t d = tmem_base + static_cast<uint32_t>(acc * L::kAcc1);
         for (int kb = 0; kb < p.num_kb; ++kb) {
           if (!mbar_wait(bar_full(stage), phase, ab, kStatusTimeoutSmemFull, budget)) {
@@ -458,6 +454,15 @@ mx_gemm_kernel(const __grid_constant__ MxParams p) {
 #pragma unroll
             for (int b = 0; b < 1 + L::kXBlocks; ++b)
               mx_copy_sf<CTA2>(sf + g * GC + b * 4, sf_desc0 + off + static_cast<uint32_t>((b * 2 + g) * (kMxSfBytes >> 4)));
+          if (OVERLAP && kb == 0 && it > 0) {
+            // the columns that the tile before shares with this one have been read (and with them everything of the tile before
+            // that); the first stage's scales are on their way by then
+            if (!mbar_wait<CTA2>(bar_tempty(0), (it - 1) & 1, ab, kStatusTimeoutTmemEmpty, budget)) {
+              ok = false;
+              break;
+            }
+            tc_fence_after();
+          }
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
             const uint32_t sfa = sf + (k >> 1) * GC;
