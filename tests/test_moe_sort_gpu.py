@@ -349,3 +349,40 @@ def test_results_do_not_change_from_run_to_run():
         runs.append((out,) + torch.autograd.grad(out, (y, w), dout))
     for other in runs[1:]:
         assert all(torch.equal(a, b) for a, b in zip(runs[0], other))
+
+
+@pytest.mark.parametrize("hidden", [4096, 4100, 4097])
+def test_more_than_31_bits_of_values(hidden):
+    import flux_b200 as flux
+
+    ntokens, topk, dtype = 66000, 8, torch.bfloat16
+    si, splits, _ = _routing(ntokens, 16, topk, 0.01, hidden)
+    last = int(splits.sum())
+    g = torch.Generator(device="cuda").manual_seed(hidden)
+    x = torch.randn(ntokens, hidden, generator=g, device="cuda", dtype=dtype)
+    dout = torch.randn(ntokens, hidden, generator=g, device="cuda", dtype=dtype)
+    w = torch.rand(ntokens, topk, generator=g, device="cuda").requires_grad_(True)
+    rows = flux.moe_permute(x, splits, si).requires_grad_(True)
+    out = flux.moe_unpermute(rows, splits, si, w)
+    drows, dw = torch.autograd.grad(out, (rows, w), dout)
+    (dx,) = torch.autograd.grad(flux.moe_permute(x.requires_grad_(True), splits, si), x, drows)
+    assert int(rows[last:].count_nonzero()) == 0 and int(drows[last:].count_nonzero()) == 0
+    half, low = _half_step(dtype), torch.finfo(dtype).smallest_normal
+    for at in (slice(0, 100), slice(ntokens // 2, ntokens // 2 + 100), slice(ntokens - 100, ntokens)):
+        t, j, r = _pairs(si[at])
+        xs, gs, ws = x[at].detach().cpu(), dout[at].cpu().double(), w[at].detach().cpu().double()
+        here = r.cuda()
+        assert torch.equal(rows[here].cpu(), xs[t])
+        total = torch.zeros(100, dtype=torch.float64).index_add_(0, t, ws[t, j])[:, None]
+        want = xs.double() * total
+        _within(out[at].detach(), want, 2 * topk * U * want.abs() + half * want.abs() * 1.001 + low)
+        want = gs[t] * ws[t, j][:, None]
+        _within(drows[here], want, (U + half) * want.abs() * 1.001 + low)
+        term = xs[t].double() * gs[t]
+        want, size = torch.zeros(100, topk, dtype=torch.float64), torch.zeros(100, topk, dtype=torch.float64)
+        want[t, j], size[t, j] = term.sum(1), term.abs().sum(1)
+        _within(dw[at], want, (hidden + 2) * U * size)
+        term = drows[here].cpu().double()
+        want = torch.zeros(100, hidden, dtype=torch.float64).index_add_(0, t, term)
+        size = torch.zeros(100, hidden, dtype=torch.float64).index_add_(0, t, term.abs())
+        _within(dx[at], want, topk * U * size + half * (want.abs() + topk * U * size) + low)

@@ -334,3 +334,39 @@ def test_a_bias_with_a_gradient_is_refused():
         flux.mx_gemm(x, w, bias=bias)
     with torch.no_grad():
         assert torch.equal(flux.mx_gemm(x, w, bias=bias), flux.mx_gemm(x, w))
+
+
+# ------------------------------------------------------------------------------------------------ offsets beyond 32 bits
+@pytest.mark.parametrize("n,tuning", [(32768, None), (32771, None), (32768, {"block_n": 128, "cta_group": 1}), (32771, {"block_n": 64})], ids=str)
+def test_products_of_more_than_31_bits_of_values(n, tuning):
+    import flux_b200 as flux
+
+    m, splits = 66000, [9000, 0, 20001, 36998]
+    x, xv = _random_mx((m, 32), 1)
+    w, wv = _random_mx((n, 32), 2)
+    w3, w3v = _random_mx((4, n, 32), 3)
+    y = flux.mx_gemm(x, w, tuning=tuning)
+    _status()
+    for r in (slice(0, 40), slice(m // 2, m // 2 + 40), slice(m - 40, m)):
+        assert torch.equal(y[r].cpu(), (xv[r] @ wv.t()).to(torch.bfloat16))
+    y = flux.mx_grouped_gemm(x, w3, torch.tensor(splits, dtype=torch.int32, device="cuda"), output=y, tuning=tuning)
+    _status()
+    for e, r in ((0, slice(0, 40)), (0, slice(8960, 9000)), (2, slice(9000, 9040)), (3, slice(m - 41, m - 1))):
+        assert torch.equal(y[r].cpu(), (xv[r] @ w3v[e].t()).to(torch.bfloat16))
+    assert torch.equal(y[-1].cpu(), (xv[-1] @ wv.t()).to(torch.bfloat16))  # the row past the last expert's is the one from before
+
+
+def test_quantise_more_than_32_bits_of_values():
+    import flux_b200 as flux
+
+    rows, k = 540000, 8192
+    x = torch.empty(rows, k, dtype=torch.bfloat16, device="cuda")
+    part = torch.randn(1000, k, generator=torch.Generator().manual_seed(4)).to(torch.bfloat16)
+    for r in range(0, rows, 1000):
+        torch.mul(part.cuda(), 1.0 + r / rows, out=x[r:r + 1000])
+    q = flux.mx_quantize(x)
+    y = q.dequantize()
+    for r in (slice(0, 30), slice(rows // 2 + 7, rows // 2 + 40), slice(rows - 30, rows)):
+        data, scales = _quantised64(x[r])
+        assert torch.equal(q.data[r].cpu(), data)
+        assert torch.equal(y[r].cpu().double(), _values(data, scales))
