@@ -243,6 +243,10 @@ __device__ __forceinline__ void tma_load_2d(uint32_t smem_dst, const void* tmap,
       : "r"(smem_dst), "l"(reinterpret_cast<uint64_t>(tmap)), "r"(bar), "r"(x), "r"(y)
       : "memory");
 }
+// The same box into the L2 only: a hint, which orders nothing.
+__device__ __forceinline__ void tma_prefetch_2d(const void* tmap, int x, int y) {
+  asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global [%0, {%1, %2}];" ::"l"(reinterpret_cast<uint64_t>(tmap)), "r"(x), "r"(y) : "memory");
+}
 // Four independent rows (y0..y3) of one 2-D tensor, `box_x` elements each,
 // land as four consecutive smem rows.
 __device__ __forceinline__ void tma_gather4_2d(uint32_t smem_dst, const void* tmap, uint32_t bar,
