@@ -851,120 +851,122 @@ mx_few_kernel(const __grid_constant__ MxParams p) {
   tl.m_end = s_tile[2];
   nkb = s_tile[3];
   tl.x_col = s_tile[4];
-  const int cnt = nkb == 0 ? 0 : imin(BN, tl.m_end - tl.m0);
+  const int cnt = imin(BN, tl.m_end - tl.m0);
   pdl_wait();  // (returns at once: warp 0 has been through it)
   if (threadIdx.x == 0) pdl_trigger();
+  if (GROUPED && nkb == 0) {  // no expert has this tile (all CTAs of the cluster see that)
+    if (warp == 1) tmem_dealloc(tmem_base, L::kTmemCols);
+    return;
+  }
 
-  if (nkb > 0) {
-    if (warp == 0) {
-      if (elect_one()) {
-        int stage = 0;
-        uint32_t phase = 0;
-        int i = STAGES;
-        for (; i < nkb; ++i) {
-          if (!mbar_wait(bar_base + 8u * (STAGES + stage), phase, ab, kStatusTimeoutSmemEmpty, p.timeout_ns)) break;
-          load(tl, i, stage);
-          if (++stage == STAGES) {
-            stage = 0;
-            phase ^= 1u;
-          }
-        }
-        if (*s_abort != 0) {
-          // give the copies in flight their time to land (1 ms per stage at most): none may outlive the CTA
-          const AbortWord none{nullptr, 0u};
-          for (int s = 0; s < STAGES && s < nkb; ++s)
-            mbar_wait(bar_base + 8u * s, static_cast<uint32_t>(((i - 1 - s) / STAGES) & 1), none, 0, 1000000ull);
-        }
-      }
-    } else if (warp == 1) {
-      if (elect_one()) {
-        const uint64_t a_desc0 = make_kmajor_sw128_desc(smem_base), b_desc0 = make_kmajor_sw128_desc(smem_base + L::kABytes);
-        const uint64_t sf_desc0 = mx_sf_desc(smem_base + L::kSfOffset);
-        int stage = 0;
-        uint32_t phase = 0;
-        bool ok = true;
-        for (int i = 0; i < nkb; ++i) {
-          if (!mbar_wait(bar_base + 8u * stage, phase, ab, kStatusTimeoutSmemFull, p.timeout_ns)) {
-            ok = false;
-            break;
-          }
-          tc_fence_after();
-          const uint32_t off = static_cast<uint32_t>(stage) * (L::kStageBytes >> 4);
-          // (a slot of scales per stage: it is free when the stage is)
-          const uint32_t sf = tmem_base + BN + static_cast<uint32_t>(stage * L::kSfCols);
-#pragma unroll
-          for (int g = 0; g < 2; ++g)
-#pragma unroll
-            for (int b = 0; b < 2; ++b) mx_copy_sf<false>(sf + (g * 2 + b) * 4, sf_desc0 + off + static_cast<uint32_t>((b * 2 + g) * (kMxSfBytes >> 4)));
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const uint32_t sfa = sf + (k >> 1) * 8;
-            umma_mxf4<false>(tmem_base, a_desc0 + off + 2u * k, b_desc0 + off + 2u * k, mx_idesc(128, BN, (k & 1) * 2), sfa, sfa + 4 + tl.x_col,
-                             (i > 0 || k > 0) ? 1u : 0u);
-          }
-          umma_commit(bar_base + 8u * (STAGES + stage));
-          if (++stage == STAGES) {
-            stage = 0;
-            phase ^= 1u;
-          }
-        }
-        if (ok) umma_commit(bar_done);
-        if (*s_abort != 0) {  // UMMAs in flight still read shared memory and write tensor memory
-          umma_commit(bar_retired);
-          mbar_wait(bar_retired, 0, AbortWord{nullptr, 0u}, 0, 2000000ull);
-        }
-      }
-    } else if (warp < 6) {
-      // this CTA's accumulator, tokens x 128 output columns, into its shared memory (all loads have landed and all UMMAs
-      // have retired by then, so the stages are free)
-      const int quad = warp & 3;
-      const int row = quad * 32 + lane;
-      if (__all_sync(0xffffffffu, mbar_wait(bar_done, 0, ab, kStatusTimeoutTmemFull, p.timeout_ns))) {
-        tc_fence_after();
-        const uint32_t t0 = tmem_base + (static_cast<uint32_t>(quad * 32) << 16);
-        constexpr int CH = BN < 32 ? BN : 32;
-#pragma unroll 1
-        for (int c = 0; c < BN && c < cnt; c += CH) {
-          uint32_t r[CH];
-          if constexpr (CH == 16) tmem_ld_32x16(t0 + c, r); else tmem_ld_32x32(t0 + c, r);
-          tmem_ld_wait();
-#pragma unroll
-          for (int j = 0; j < CH; ++j) *reinterpret_cast<uint32_t*>(smem + ((c + j) * kBM + row) * 4) = r[j];
-        }
-        tc_fence_before();
-      }
-    } else if (GROUPED) {
-      // the scales of the tile's tokens, four rows (lane, lane + 32, ...) and two groups of K a stage
-      constexpr int UN = 4;  // stages whose loads are in flight together
+  if (warp == 0) {
+    if (elect_one()) {
       int stage = 0;
-      uint32_t phase = 1;
+      uint32_t phase = 0;
+      int i = STAGES;
+      for (; i < nkb; ++i) {
+        if (!mbar_wait(bar_base + 8u * (STAGES + stage), phase, ab, kStatusTimeoutSmemEmpty, p.timeout_ns)) break;
+        load(tl, i, stage);
+        if (++stage == STAGES) {
+          stage = 0;
+          phase ^= 1u;
+        }
+      }
+      if (*s_abort != 0) {
+        // give the copies in flight their time to land (1 ms per stage at most): none may outlive the CTA
+        const AbortWord none{nullptr, 0u};
+        for (int s = 0; s < STAGES && s < nkb; ++s)
+          mbar_wait(bar_base + 8u * s, static_cast<uint32_t>(((i - 1 - s) / STAGES) & 1), none, 0, 1000000ull);
+      }
+    }
+  } else if (warp == 1) {
+    if (elect_one()) {
+      const uint64_t a_desc0 = make_kmajor_sw128_desc(smem_base), b_desc0 = make_kmajor_sw128_desc(smem_base + L::kABytes);
+      const uint64_t sf_desc0 = mx_sf_desc(smem_base + L::kSfOffset);
+      int stage = 0;
+      uint32_t phase = 0;
       bool ok = true;
-      for (int i0 = 0; ok && i0 < nkb; i0 += UN) {
-        uint32_t w[UN][2][4];
+      for (int i = 0; i < nkb; ++i) {
+        if (!mbar_wait(bar_base + 8u * stage, phase, ab, kStatusTimeoutSmemFull, p.timeout_ns)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        const uint32_t off = static_cast<uint32_t>(stage) * (L::kStageBytes >> 4);
+        // (a slot of scales per stage: it is free when the stage is)
+        const uint32_t sf = tmem_base + BN + static_cast<uint32_t>(stage * L::kSfCols);
 #pragma unroll
-        for (int u = 0; u < UN; ++u)
-          if (i0 + u < nkb) mx_gather_scales<BN>(w[u], p, tl.m0, tl.m0 + cnt, kb0 + i0 + u, lane);
+        for (int g = 0; g < 2; ++g)
 #pragma unroll
-        for (int u = 0; u < UN; ++u) {
-          if (i0 + u >= nkb || !ok) break;
-          if (!__all_sync(0xffffffffu, mbar_wait(bar_base + 8u * (STAGES + stage), phase, ab, kStatusTimeoutSmemEmpty, p.timeout_ns))) {
-            ok = false;
-            break;
-          }
-          mx_put_scales(w[u], smem_base + stage * L::kStageBytes + L::kSfOffset + 2 * kMxSfBytes, lane);
-          fence_proxy_async_smem();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(bar_base + 8u * stage);
-          if (++stage == STAGES) {
-            stage = 0;
-            phase ^= 1u;
-          }
+          for (int b = 0; b < 2; ++b) mx_copy_sf<false>(sf + (g * 2 + b) * 4, sf_desc0 + off + static_cast<uint32_t>((b * 2 + g) * (kMxSfBytes >> 4)));
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const uint32_t sfa = sf + (k >> 1) * 8;
+          umma_mxf4<false>(tmem_base, a_desc0 + off + 2u * k, b_desc0 + off + 2u * k, mx_idesc(128, BN, (k & 1) * 2), sfa, sfa + 4 + tl.x_col,
+                           (i > 0 || k > 0) ? 1u : 0u);
+        }
+        umma_commit(bar_base + 8u * (STAGES + stage));
+        if (++stage == STAGES) {
+          stage = 0;
+          phase ^= 1u;
+        }
+      }
+      if (ok) umma_commit(bar_done);
+      if (*s_abort != 0) {  // UMMAs in flight still read shared memory and write tensor memory
+        umma_commit(bar_retired);
+        mbar_wait(bar_retired, 0, AbortWord{nullptr, 0u}, 0, 2000000ull);
+      }
+    }
+  } else if (warp < 6) {
+    // this CTA's accumulator, tokens x 128 output columns, into its shared memory (all loads have landed and all UMMAs
+    // have retired by then, so the stages are free)
+    const int quad = warp & 3;
+    const int row = quad * 32 + lane;
+    if (__all_sync(0xffffffffu, mbar_wait(bar_done, 0, ab, kStatusTimeoutTmemFull, p.timeout_ns))) {
+      tc_fence_after();
+      const uint32_t t0 = tmem_base + (static_cast<uint32_t>(quad * 32) << 16);
+      constexpr int CH = BN < 32 ? BN : 32;
+#pragma unroll 1
+      for (int c = 0; c < BN && c < cnt; c += CH) {
+        uint32_t r[CH];
+        if constexpr (CH == 16) tmem_ld_32x16(t0 + c, r); else tmem_ld_32x32(t0 + c, r);
+        tmem_ld_wait();
+#pragma unroll
+        for (int j = 0; j < CH; ++j) *reinterpret_cast<uint32_t*>(smem + ((c + j) * kBM + row) * 4) = r[j];
+      }
+      tc_fence_before();
+    }
+  } else if (GROUPED) {
+    // the scales of the tile's tokens, four rows (lane, lane + 32, ...) and two groups of K a stage
+    constexpr int UN = 4;  // stages whose loads are in flight together
+    int stage = 0;
+    uint32_t phase = 1;
+    bool ok = true;
+    for (int i0 = 0; ok && i0 < nkb; i0 += UN) {
+      uint32_t w[UN][2][4];
+#pragma unroll
+      for (int u = 0; u < UN; ++u)
+        if (i0 + u < nkb) mx_gather_scales<BN>(w[u], p, tl.m0, tl.m0 + cnt, kb0 + i0 + u, lane);
+#pragma unroll
+      for (int u = 0; u < UN; ++u) {
+        if (i0 + u >= nkb || !ok) break;
+        if (!__all_sync(0xffffffffu, mbar_wait(bar_base + 8u * (STAGES + stage), phase, ab, kStatusTimeoutSmemEmpty, p.timeout_ns))) {
+          ok = false;
+          break;
+        }
+        mx_put_scales(w[u], smem_base + stage * L::kStageBytes + L::kSfOffset + 2 * kMxSfBytes, lane);
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar_base + 8u * stage);
+        if (++stage == STAGES) {
+          stage = 0;
+          phase ^= 1u;
         }
       }
     }
   }
   cluster_sync_all();
-  if (warp >= 2 && warp < 6 && cnt > 0 && *s_abort == 0) {
+  if (warp >= 2 && warp < 6 && *s_abort == 0) {
     const int t = static_cast<int>(threadIdx.x) - 64;
     if (split == 1) mx_few_reduce<1, 8>(p, smem_base, tl, cnt, part, t);
     else if (split == 2) mx_few_reduce<2, 8>(p, smem_base, tl, cnt, part, t);
