@@ -90,8 +90,9 @@ static int launch_mx_few(const fluxb_comm* comm, const MxParams& p, long long ti
 // are linear in the launch's numbers, with coefficients (us) fitted to measured times of all variants on 148 problems
 // (dense 1 .. 4096 x 1024 .. 28672 x 1024 .. 8192; 8 to 128 experts, 2 to 65536 rows, of 1024 .. 14336 x 1024 .. 8192;
 // weights from memory, launches back to back in a graph). Over those problems the choice takes 2% longer than the fastest
-// variant on average, 24% at worst (64 x 4096 x 4096 6.7 us against 5.4, grouped 11%); one variant for all would be far off
-// on either side: 256 x 4096 x 4096 takes 5.9 us in tiles of 64 and 9.7 in tiles of 256, 4096 x 8192 x 8192 160 and 90.
+// variant on average, 24% at worst (64 x 4096 x 4096 6.7 us against 5.4, grouped 11%); over 297 others, down to 512 x 416, 3%
+// and, among launches of a few us, up to 42% (64 x 1000 x 416 5.4 us against 3.8). One variant for all would be far off on
+// either side: 256 x 4096 x 4096 takes 5.9 us in tiles of 64 and 9.7 in tiles of 256, 4096 x 8192 x 8192 160 and 90.
 //   tiled:      fixed + waves * (per_stage * K blocks + per_wave) + per_mb * MB of weights (+ grouped)
 //   few tokens: fixed + per_stage * K blocks of a part + per_cta * CTAs per slot + per_block * K blocks per slot
 //               + per_mb * MB of weights (+ grouped)
