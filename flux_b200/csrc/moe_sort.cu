@@ -249,18 +249,18 @@ __device__ __forceinline__ void sort_clear_tail(typename RawVec<VB>::type* rows_
 // 8192 x 4096 bf16 top-2 33 us, 6.1 TB/s; rows of odd length go two or one bytes at a time (4096 x 1001 bf16 9.3 us, 2.7 TB/s).
 template <int VB>
 __global__ void __launch_bounds__(kSortThreads)
-moe_permute_kernel(const typename RawVec<VB>::type* __restrict__ tokens, int ntokens, int topk, int row_vecs, int width, int main_ctas,
+moe_permute_kernel(const typename RawVec<VB>::type* __restrict__ tokens, int ntokens, int topk, int row_vecs, int width, int tail_ctas,
                    const int* __restrict__ splits, int nexperts, const int* __restrict__ index,
                    typename RawVec<VB>::type* __restrict__ rows_out) {
   const long long rows = static_cast<long long>(ntokens) * topk;
   pdl_wait();
   if (threadIdx.x == 0) pdl_trigger();
-  if (static_cast<int>(blockIdx.x) >= main_ctas) {
-    sort_clear_tail<VB>(rows_out, rows, row_vecs, splits, nexperts, static_cast<int>(blockIdx.x) - main_ctas, static_cast<int>(gridDim.x) - main_ctas);
+  if (static_cast<int>(blockIdx.x) < tail_ctas) {
+    sort_clear_tail<VB>(rows_out, rows, row_vecs, splits, nexperts, static_cast<int>(blockIdx.x), tail_ctas);
     return;
   }
   const int per = kSortThreads / width;
-  const long long t = static_cast<long long>(blockIdx.x) * per + static_cast<int>(threadIdx.x) / width;
+  const long long t = static_cast<long long>(static_cast<int>(blockIdx.x) - tail_ctas) * per + static_cast<int>(threadIdx.x) / width;
   if (t >= ntokens) return;
   const auto* src = tokens + t * row_vecs;
   const int* idx = index + t * topk;
@@ -895,13 +895,13 @@ int fluxb_moe_permute(const void* tokens, int ntokens, int topk, long long row_b
   const int vb = sort_vec_bytes(row_bytes, 1, {tokens, rows_out});
   const long long row_vecs = row_bytes / vb;
   const int width = sort_width(row_vecs, 4), per = kSortThreads / width;
-  const int main_ctas = (ntokens + per - 1) / per;
   const long long total = static_cast<long long>(ntokens) * topk;
-  const int grid = main_ctas + (total < kSortTailCtas ? static_cast<int>(total) : kSortTailCtas);
+  const int tail = total < kSortTailCtas ? static_cast<int>(total) : kSortTailCtas;  // (first: they work beside the others)
+  const int grid = tail + (ntokens + per - 1) / per;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
 #define FLUXB_PERMUTE(VB)                                                                                                                       \
   return launch_pdl(moe_permute_kernel<VB>, grid, kSortThreads, s, static_cast<const RawVec<VB>::type*>(tokens), ntokens, topk,                  \
-                    static_cast<int>(row_vecs), width, main_ctas, splits, nexperts, scatter_index, static_cast<RawVec<VB>::type*>(rows_out))
+                    static_cast<int>(row_vecs), width, tail, splits, nexperts, scatter_index, static_cast<RawVec<VB>::type*>(rows_out))
   switch (vb) {
     case 16: FLUXB_PERMUTE(16);
     case 8: FLUXB_PERMUTE(8);
