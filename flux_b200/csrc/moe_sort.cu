@@ -639,7 +639,7 @@ moe_unpermute_backward_kernel(const typename RawVec<VB>::type* __restrict__ dout
 template <class T, int VB, int KC, int VU>
 __global__ void __launch_bounds__(kSortThreads)
 moe_unpermute_backward_narrow_kernel(const typename RawVec<VB>::type* __restrict__ dout, const typename RawVec<VB>::type* __restrict__ rows_in,
-                                     int ntokens, int topk, int row_vecs, int width, int main_ctas, const int* __restrict__ splits, int nexperts,
+                                     int ntokens, int topk, int row_vecs, int width, int tail_ctas, const int* __restrict__ splits, int nexperts,
                                      const int* __restrict__ index, const void* __restrict__ weights, int wdtype,
                                      typename RawVec<VB>::type* __restrict__ drows, void* __restrict__ dweights) {
   using V = SortVec<T, VB>;
@@ -647,14 +647,13 @@ moe_unpermute_backward_narrow_kernel(const typename RawVec<VB>::type* __restrict
   const long long rows = static_cast<long long>(ntokens) * topk;
   pdl_wait();
   if (threadIdx.x == 0) pdl_trigger();
-  if (static_cast<int>(blockIdx.x) >= main_ctas) {
-    if (drows != nullptr)
-      sort_clear_tail<VB>(drows, rows, row_vecs, splits, nexperts, static_cast<int>(blockIdx.x) - main_ctas, static_cast<int>(gridDim.x) - main_ctas);
+  if (static_cast<int>(blockIdx.x) < tail_ctas) {
+    sort_clear_tail<VB>(drows, rows, row_vecs, splits, nexperts, static_cast<int>(blockIdx.x), tail_ctas);
     return;
   }
   const int per = kSortThreads / width;
   const int tid = static_cast<int>(threadIdx.x), warp = tid >> 5, lane = tid & 31;
-  const long long t = static_cast<long long>(blockIdx.x) * per + tid / width;
+  const long long t = static_cast<long long>(static_cast<int>(blockIdx.x) - tail_ctas) * per + tid / width;
   const bool live = t < ntokens;  // (all threads of the CTA meet at the barriers)
   for (int j0 = 0; j0 < topk; j0 += KC) {
     int row[KC];
@@ -831,13 +830,11 @@ static int launch_unpermute_backward_rows(const void* dout, const void* rows, in
   int ctas = 0;
   const int rc = sort_resident_ctas(kern, SMEM, known, &ctas);
   if (rc != FLUXB_OK) return rc;
-  int main_ctas = (ntokens + per - 1) / per;
-  if (!NARROW && main_ctas > ctas) main_ctas = ctas;
   const long long total = static_cast<long long>(ntokens) * topk;
-  const int tail = total < kSortTailCtas ? static_cast<int>(total) : kSortTailCtas;
-  const int grid = main_ctas + (drows != nullptr ? tail : 0);
-  return launch_pdl_cluster(kern, grid, kSortThreads, SMEM, 0, stream, static_cast<const R*>(dout), static_cast<const R*>(rows), ntokens, topk, row_vecs,
-                            width, main_ctas, splits, nexperts, index, weights, wdtype, static_cast<R*>(drows), dweights);
+  const int need = (ntokens + per - 1) / per, main_ctas = NARROW || need < ctas ? need : ctas;
+  const int tail = drows == nullptr ? 0 : total < kSortTailCtas ? static_cast<int>(total) : kSortTailCtas;
+  return launch_pdl_cluster(kern, main_ctas + tail, kSortThreads, SMEM, 0, stream, static_cast<const R*>(dout), static_cast<const R*>(rows), ntokens, topk, row_vecs,
+                            width, NARROW ? tail : main_ctas, splits, nexperts, index, weights, wdtype, static_cast<R*>(drows), dweights);
 }
 template <class T, int VB>
 static int launch_unpermute_backward(const void* dout, const void* rows, int ntokens, int topk, int row_vecs, const int* splits, int nexperts,
