@@ -137,3 +137,45 @@ def test_layers_refuse_what_does_not_fit():
         flux.MXMoEMLP(moe.router, moe.w_up, moe.w_up, 2)
     with pytest.raises(RuntimeError, match="must be"):
         flux.MXLinear(moe.w_up)
+
+
+def test_the_path_from_several_threads():
+    """Each thread with a stream and sizes of its own; what it gets the first time, alone or not, it gets every time."""
+    import threading
+
+    import flux_b200 as flux
+
+    flux.init_flux_shm(None)
+    wrong = []
+
+    def work(i):
+        try:
+            g = torch.Generator(device="cuda")
+            with torch.cuda.stream(torch.cuda.Stream()):
+                first = None
+                for _ in range(12):
+                    g.manual_seed(i)
+                    tokens, hidden = 50 + 37 * i, 512 + 32 * i
+                    x = torch.randn(tokens, hidden, device="cuda", generator=g).bfloat16().requires_grad_(True)
+                    chosen, weights = flux.moe_route(torch.randn(tokens, 8, device="cuda", generator=g), 2)
+                    si, splits = flux.calc_scatter_index(chosen, torch.empty(8), return_splits=True)
+                    rows = flux.moe_permute(x, splits, si)
+                    out = flux.moe_unpermute(rows, splits, si, weights)
+                    (dx,) = torch.autograd.grad(out, x, torch.ones_like(out))
+                    up = flux.mx_quantize(torch.randn(8, 300 + i, hidden, device="cuda", generator=g))
+                    w = flux.mx_quantize(torch.randn(700 + i, hidden, device="cuda", generator=g))
+                    got = [chosen, weights, rows.detach(), out.detach(), dx, flux.mx_grouped_gemm(flux.mx_quantize(x.detach(), splits, si), up, splits),
+                           flux.mx_gemm(flux.mx_quantize(x.detach()), w)]
+                    first = first or got
+                    wrong.extend((i, n) for n, (a, b) in enumerate(zip(first, got)) if not torch.equal(a, b))
+        except Exception as e:  # (an exception in a thread is not pytest's)
+            wrong.append((i, repr(e)))
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    flux.get_comm(None).check_status()
+    assert wrong == []
