@@ -290,7 +290,7 @@ __device__ __forceinline__ float load_weight(const void* w, int dtype, long long
 // What a thread gathers from several rows comes through shared memory, by asynchronous copies of its own that it waits for
 // in order: no thread reads what another has copied, so there are no barriers, and what is on its way is bound by shared
 // memory (about 190 KB an SM) instead of registers. An item is UN choices of VU vectors of one token; items follow each
-// other through the CTA's tokens, a ring of D items is in flight. Items of 128 bytes (one vector of two rows, 32 bytes, spent
+// other, a ring of D items is in flight. Items of 128 bytes (one vector of two rows, 32 bytes, spent
 // more on the way from item to item than on memory: 8192 x 4096 bf16 top-2 46 us).
 constexpr int kGatherSmem = 96 * 1024;  // a CTA's share, two CTAs an SM
 constexpr int gather_vectors(int vb, int un) { return (vb == 16 ? 8 : 16) / un; }
@@ -317,19 +317,9 @@ __device__ __forceinline__ typename RawVec<VB>::type read_shared(uint32_t addr) 
   return v;
 }
 
-// Where a thread is among its items: token, vector column, first choice. Choices change fastest.
+// Where a thread is: token, first vector, first choice.
 struct GatherAt {
   int t, v, j;
-  template <int UN>
-  __device__ __forceinline__ void next(int step, int width, int vecs, int row_vecs, int topk) {
-    j += UN;
-    if (j < topk) return;
-    j = 0;
-    v += width * vecs;
-    if (v < row_vecs) return;
-    v &= width - 1;
-    t += step;
-  }
 };
 template <int UN>
 __device__ __forceinline__ void gather_index(int (&r)[UN], const int* index, const GatherAt& at, int ntokens, int topk, int rows) {
@@ -347,11 +337,13 @@ __device__ __forceinline__ void gather_weights(float (&w)[UN], const void* weigh
 }
 
 // out[t] = sum_j w[t, j] rows[index[t, j]], j ascending, rounded once; without weights the plain sum.
-// 8192 x 4096 bf16 top-2 32.6 us, 6.2 TB/s (one vector of two rows a thread and a CTA for every token 60, eight vectors in
-// registers and resident CTAs 38); 8192 x 2048 top-6 47 us, 5.0 TB/s (72, 65).
+// 8192 x 4096 bf16 top-2 32 us, 6.3 TB/s (one vector of two rows a thread and a CTA for every token 60, eight vectors in
+// registers and resident CTAs 38); 8192 x 2048 top-6 46 us, 5.1 TB/s (72, 65). Rows are shared out by the warp's 32 * VU vectors:
+// as many threads to a token as a power of two has left half of them without work where a row is a little longer
+// (8192 x 4100 top-2 34 us against 44, 8192 x 2052 top-6 53 against 82, 2000 x 5120 fp16 top-4 18 against 20).
 template <class T, int VB, int UN>
 __global__ void __launch_bounds__(kSortThreads, 2)
-moe_unpermute_kernel(const typename RawVec<VB>::type* __restrict__ rows_in, int ntokens, int topk, int row_vecs, int width,
+moe_unpermute_kernel(const typename RawVec<VB>::type* __restrict__ rows_in, int ntokens, int topk, int row_vecs,
                      const int* __restrict__ index, const void* __restrict__ weights, int wdtype,
                      typename RawVec<VB>::type* __restrict__ out) {
   using V = SortVec<T, VB>;
@@ -361,9 +353,21 @@ moe_unpermute_kernel(const typename RawVec<VB>::type* __restrict__ rows_in, int 
   const int rows = ntokens * topk;
   pdl_wait();
   if (threadIdx.x == 0) pdl_trigger();
-  const int per = kSortThreads / width, step = static_cast<int>(gridDim.x) * per;
-  GatherAt put{static_cast<int>(blockIdx.x) * per + static_cast<int>(threadIdx.x) / width, static_cast<int>(threadIdx.x) & (width - 1), 0};
-  if (put.v >= row_vecs) return;
+  // a warp's units: 32 * VU vectors of a token, units of all tokens one after the other
+  const int unit = 32 * VU, units = (row_vecs + unit - 1) / unit, all_vecs = units * unit;
+  const int start = static_cast<int>(blockIdx.x) * (kSortThreads / 32) + (static_cast<int>(threadIdx.x) >> 5);
+  const int step = static_cast<int>(gridDim.x) * (kSortThreads / 32), step_t = step / units, step_v = (step - step_t * units) * unit;
+  auto next = [&](GatherAt& at) {  // choices change fastest
+    at.j += UN;
+    if (at.j < topk) return;
+    at.j = 0;
+    at.t += step_t;
+    at.v += step_v;
+    if (at.v < all_vecs) return;
+    at.v -= all_vecs;
+    ++at.t;
+  };
+  GatherAt put{start / units, start % units * unit + (static_cast<int>(threadIdx.x) & 31), 0};
   GatherAt get = put, ahead = put;
   int row[UN];
   gather_index<UN>(row, index, put, ntokens, topk, rows);
@@ -375,11 +379,11 @@ moe_unpermute_kernel(const typename RawVec<VB>::type* __restrict__ rows_in, int 
         const auto* src = rows_in + static_cast<long long>(row[u]) * row_vecs + put.v;
 #pragma unroll
         for (int k = 0; k < VU; ++k)
-          if (put.v + k * width < row_vecs) copy_async<VB>(slots + ((stage_put * UN + u) * VU + k) * (kSortThreads * VB), src + k * width);
+          if (put.v + k * 32 < row_vecs) copy_async<VB>(slots + ((stage_put * UN + u) * VU + k) * (kSortThreads * VB), src + k * 32);
       }
     copy_commit();
     if (++stage_put == D) stage_put = 0;
-    put.next<UN>(step, width, VU, row_vecs, topk);
+    next(put);
     gather_index<UN>(row, index, put, ntokens, topk, rows);
   };
 #pragma unroll 1
@@ -396,7 +400,7 @@ moe_unpermute_kernel(const typename RawVec<VB>::type* __restrict__ rows_in, int 
       cur[u] = nxt[u];
       w[u] = nxt_w[u];
     }
-    ahead.next<UN>(step, width, VU, row_vecs, topk);
+    next(ahead);
     gather_index<UN>(nxt, index, ahead, ntokens, topk, rows);
     gather_weights<UN>(nxt_w, weights, wdtype, ahead, ntokens, topk);
     issue();
@@ -421,15 +425,15 @@ moe_unpermute_kernel(const typename RawVec<VB>::type* __restrict__ rows_in, int 
     if (get.j + UN >= topk) {
 #pragma unroll
       for (int k = 0; k < VU; ++k)
-        if (get.v + k * width < row_vecs) {
+        if (get.v + k * 32 < row_vecs) {
           V y;
 #pragma unroll
           for (int i = 0; i < V::N; ++i) y.e[i] = from_f32<T>(acc[k][i]);
-          out[static_cast<long long>(get.t) * row_vecs + get.v + k * width] = y.raw;
+          out[static_cast<long long>(get.t) * row_vecs + get.v + k * 32] = y.raw;
         }
     }
     if (++stage == D) stage = 0;
-    get.next<UN>(step, width, VU, row_vecs, topk);
+    next(get);
   }
   copy_wait<0>();
 }
@@ -634,8 +638,8 @@ moe_unpermute_backward_kernel(const typename RawVec<VB>::type* __restrict__ dout
 }
 
 // The same for vectors below 16 bytes, KC choices of VU vectors in registers. Vectors of 8 bytes (widths that 8 does not divide) against
-// the ring, which has to copy twice as often for the same bytes: 8192 x 4100 bf16 top-2 70 and 85 us, 8192 x 2052 top-6 105 and 133,
-// 2000 x 5124 fp16 top-4 38 and 41. (The sum above reads only, and is faster from the ring: top-6 82 against 152.)
+// the ring, which has to copy twice as often for the same bytes: 8192 x 4100 bf16 top-2 60 and 85 us, 8192 x 2052 top-6 91 and 133,
+// 2000 x 5124 fp16 top-4 35 and 41. (The sum above reads only, and is faster from the ring: top-6 53 against 152.)
 template <class T, int VB, int KC, int VU>
 __global__ void __launch_bounds__(kSortThreads)
 moe_unpermute_backward_narrow_kernel(const typename RawVec<VB>::type* __restrict__ dout, const typename RawVec<VB>::type* __restrict__ rows_in,
@@ -734,6 +738,19 @@ static int sort_width(long long row_vecs, int each) {
   while (w < kSortThreads && static_cast<long long>(w) * each < row_vecs) w *= 2;
   return w;
 }
+// The same, or fewer, 64 at least, where that leaves the `ctas` that run side by side with less to do one after the other: rows a
+// little longer than a power of two fill half of their places. Backward of 8192 x 4100 bf16 top-2 60 us (69 without), 8192 x 2052
+// top-6 90 (103), 4096 x 1028 top-3 16 (25), but 4096 x 4098 fp32 top-2 61.5 (59.4); down to 32 threads that takes 66.5.
+static int sort_width_even(int ntokens, long long row_vecs, int each, int ctas) {
+  int w = sort_width(row_vecs, each);
+  auto turns = [&](int width) {
+    const long long at_once = static_cast<long long>(ctas) * (kSortThreads / width);
+    return (ntokens + at_once - 1) / at_once * ((row_vecs + width * each - 1) / (width * each));
+  };
+  for (int fewer = w / 2; fewer >= 64; fewer /= 2)
+    if (turns(fewer) < turns(w)) w = fewer;
+  return w;
+}
 
 static int check_sort(const char* what, int ntokens, int topk, int hidden) {
   FLUXB_REQUIRE(ntokens >= 0 && topk >= 1 && hidden >= 1 && hidden < (1 << 28), "%s: ntokens=%d topk=%d hidden=%d invalid", what, ntokens, topk, hidden);
@@ -792,20 +809,25 @@ template <class T, int VB, int UN>
 static int launch_unpermute_rows(const void* rows, int ntokens, int topk, int row_vecs, const int* index, const void* weights, int wdtype, void* out,
                                  cudaStream_t stream) {
   using R = typename RawVec<VB>::type;
-  constexpr bool NARROW = VB < 8;
-  constexpr int VU = NARROW ? 8 / UN : gather_vectors(VB, UN), SMEM = NARROW ? 0 : gather_depth(VB, UN) * UN * VU * VB * kSortThreads;
-  auto kern = [] {
-    if constexpr (NARROW) return moe_unpermute_narrow_kernel<T, VB, UN, VU>;
-    else return moe_unpermute_kernel<T, VB, UN>;
-  }();
-  const int width = sort_width(row_vecs, VU), per = kSortThreads / width;
   static int known[64] = {};
   int ctas = 0;
-  const int rc = sort_resident_ctas(kern, SMEM, known, &ctas);
-  if (rc != FLUXB_OK) return rc;
-  const int need = (ntokens + per - 1) / per;
-  return launch_pdl_cluster(kern, need < ctas ? need : ctas, kSortThreads, SMEM, 0, stream, static_cast<const R*>(rows), ntokens, topk, row_vecs, width, index,
-                            weights, wdtype, static_cast<R*>(out));
+  if constexpr (VB < 8) {
+    constexpr int VU = 8 / UN;
+    auto kern = moe_unpermute_narrow_kernel<T, VB, UN, VU>;
+    const int rc = sort_resident_ctas(kern, 0, known, &ctas);
+    if (rc != FLUXB_OK) return rc;
+    const int width = sort_width(row_vecs, VU), per = kSortThreads / width, need = (ntokens + per - 1) / per;
+    return launch_pdl(kern, need < ctas ? need : ctas, kSortThreads, stream, static_cast<const R*>(rows), ntokens, topk, row_vecs, width, index, weights, wdtype,
+                      static_cast<R*>(out));
+  } else {
+    constexpr int VU = gather_vectors(VB, UN), SMEM = gather_depth(VB, UN) * UN * VU * VB * kSortThreads;
+    auto kern = moe_unpermute_kernel<T, VB, UN>;
+    const int rc = sort_resident_ctas(kern, SMEM, known, &ctas);
+    if (rc != FLUXB_OK) return rc;
+    const long long warps = static_cast<long long>(ntokens) * ((row_vecs + 32 * VU - 1) / (32 * VU)), need = (warps + kSortThreads / 32 - 1) / (kSortThreads / 32);
+    return launch_pdl_cluster(kern, need < ctas ? static_cast<int>(need) : ctas, kSortThreads, SMEM, 0, stream, static_cast<const R*>(rows), ntokens, topk,
+                              row_vecs, index, weights, wdtype, static_cast<R*>(out));
+  }
 }
 template <class T, int VB>
 static int launch_unpermute(const void* rows, int ntokens, int topk, int row_vecs, const int* index, const void* weights, int wdtype, void* out,
@@ -825,11 +847,11 @@ static int launch_unpermute_backward_rows(const void* dout, const void* rows, in
     if constexpr (NARROW) return moe_unpermute_backward_narrow_kernel<T, VB, KC, VU>;
     else return moe_unpermute_backward_kernel<T, VB, KC>;
   }();
-  const int width = sort_width(row_vecs, VU), per = kSortThreads / width;
   static int known[64] = {};
   int ctas = 0;
   const int rc = sort_resident_ctas(kern, SMEM, known, &ctas);
   if (rc != FLUXB_OK) return rc;
+  const int width = NARROW ? sort_width_even(ntokens, row_vecs, VU, ctas) : sort_width(row_vecs, VU), per = kSortThreads / width;
   const long long total = static_cast<long long>(ntokens) * topk;
   const int need = (ntokens + per - 1) / per, main_ctas = NARROW || need < ctas ? need : ctas;
   const int tail = drows == nullptr ? 0 : total < kSortTailCtas ? static_cast<int>(total) : kSortTailCtas;
