@@ -338,9 +338,9 @@ __device__ __forceinline__ void gather_weights(float (&w)[UN], const void* weigh
 
 // out[t] = sum_j w[t, j] rows[index[t, j]], j ascending, rounded once; without weights the plain sum.
 // 8192 x 4096 bf16 top-2 32 us, 6.3 TB/s (one vector of two rows a thread and a CTA for every token 60, eight vectors in
-// registers and resident CTAs 38); 8192 x 2048 top-6 46 us, 5.1 TB/s (72, 65). Rows are shared out by the warp's 32 * VU vectors:
-// as many threads to a token as a power of two has left half of them without work where a row is a little longer
-// (8192 x 4100 top-2 34 us against 44, 8192 x 2052 top-6 53 against 82, 2000 x 5120 fp16 top-4 18 against 20).
+// registers and resident CTAs 38); 8192 x 2048 top-6 39 us, 6.0 TB/s (72, 65; eight choices an item 46). Rows are shared out by
+// the warp's 32 * VU vectors: as many threads to a token as a power of two has left half of them without work where a row is a
+// little longer (8192 x 4100 top-2 34 us against 44, 8192 x 2052 top-6 45 against 82, 2000 x 5120 fp16 top-4 18 against 20).
 template <class T, int VB, int UN>
 __global__ void __launch_bounds__(kSortThreads, 2)
 moe_unpermute_kernel(const typename RawVec<VB>::type* __restrict__ rows_in, int ntokens, int topk, int row_vecs,
@@ -439,67 +439,74 @@ moe_unpermute_kernel(const typename RawVec<VB>::type* __restrict__ rows_in, int 
 }
 
 // The same for vectors of 2 and 4 bytes (odd row lengths), with UN rows of VU vectors in registers: asynchronous copies do
-// not know 2 bytes, and take an instruction for every 4 (4096 x 4097 fp32 top-2 53 us through the ring, 43 here).
+// not know 2 bytes, and take an instruction for every 4. 16 vectors in flight (8 or 32 are slower): 4096 x 4097 bf16 top-2 25 us,
+// 4.0 TB/s; 4096 x 2049 fp16 top-8 43 (a token at a time by a power of two of threads, 8 vectors 39 and 83).
 template <class T, int VB, int UN, int VU>
 __global__ void __launch_bounds__(kSortThreads)
-moe_unpermute_narrow_kernel(const typename RawVec<VB>::type* __restrict__ rows_in, int ntokens, int topk, int row_vecs, int width,
+moe_unpermute_narrow_kernel(const typename RawVec<VB>::type* __restrict__ rows_in, int ntokens, int topk, int row_vecs,
                             const int* __restrict__ index, const void* __restrict__ weights, int wdtype,
                             typename RawVec<VB>::type* __restrict__ out) {
   using V = SortVec<T, VB>;
   const int rows = ntokens * topk;
   pdl_wait();
   if (threadIdx.x == 0) pdl_trigger();
-  const int per = kSortThreads / width, step = static_cast<int>(gridDim.x) * per;
+  const int unit = 32 * VU, units = (row_vecs + unit - 1) / unit, all_vecs = units * unit;
+  const int start = static_cast<int>(blockIdx.x) * (kSortThreads / 32) + (static_cast<int>(threadIdx.x) >> 5);
+  const int step = static_cast<int>(gridDim.x) * (kSortThreads / 32), step_t = step / units, step_v = (step - step_t * units) * unit;
+  GatherAt at{start / units, start % units * unit + (static_cast<int>(threadIdx.x) & 31), 0};
   int row[UN], nxt[UN];
   float w[UN], nxt_w[UN];
-  GatherAt at{static_cast<int>(blockIdx.x) * per + static_cast<int>(threadIdx.x) / width, 0, 0};
   gather_index<UN>(nxt, index, at, ntokens, topk, rows);
   gather_weights<UN>(nxt_w, weights, wdtype, at, ntokens, topk);
-  for (int t = at.t; t < ntokens; t += step) {
+  while (at.t < ntokens) {
 #pragma unroll
     for (int u = 0; u < UN; ++u) {
       row[u] = nxt[u];
       w[u] = nxt_w[u];
     }
-    at = {t + step, 0, 0};
+    const int t = at.t, v0 = at.v;
+    at.t += step_t;
+    at.v += step_v;
+    if (at.v >= all_vecs) {
+      at.v -= all_vecs;
+      ++at.t;
+    }
     gather_index<UN>(nxt, index, at, ntokens, topk, rows);
     gather_weights<UN>(nxt_w, weights, wdtype, at, ntokens, topk);
-    for (int v0 = static_cast<int>(threadIdx.x) & (width - 1); v0 < row_vecs; v0 += VU * width) {
-      float acc[VU][V::N];
+    float acc[VU][V::N];
 #pragma unroll
-      for (int k = 0; k < VU; ++k)
+    for (int k = 0; k < VU; ++k)
 #pragma unroll
-        for (int i = 0; i < V::N; ++i) acc[k][i] = 0.0f;
-      for (int j0 = 0; j0 < topk; j0 += UN) {
-        if (topk > UN) {
-          at = {t, 0, j0};
-          gather_index<UN>(row, index, at, ntokens, topk, rows);
-          gather_weights<UN>(w, weights, wdtype, at, ntokens, topk);
-        }
-        V x[UN][VU];
+      for (int i = 0; i < V::N; ++i) acc[k][i] = 0.0f;
+    for (int j0 = 0; j0 < topk; j0 += UN) {
+      if (topk > UN) {
+        const GatherAt more{t, 0, j0};
+        gather_index<UN>(row, index, more, ntokens, topk, rows);
+        gather_weights<UN>(w, weights, wdtype, more, ntokens, topk);
+      }
+      V x[UN][VU];
 #pragma unroll
-        for (int u = 0; u < UN; ++u)
+      for (int u = 0; u < UN; ++u)
+#pragma unroll
+        for (int k = 0; k < VU; ++k)
+          if (row[u] >= 0 && v0 + k * 32 < row_vecs) x[u][k].raw = __ldg(rows_in + static_cast<long long>(row[u]) * row_vecs + v0 + k * 32);
+#pragma unroll
+      for (int u = 0; u < UN; ++u)
+        if (row[u] >= 0) {
 #pragma unroll
           for (int k = 0; k < VU; ++k)
-            if (row[u] >= 0 && v0 + k * width < row_vecs) x[u][k].raw = __ldg(rows_in + static_cast<long long>(row[u]) * row_vecs + v0 + k * width);
 #pragma unroll
-        for (int u = 0; u < UN; ++u)
-          if (row[u] >= 0) {
-#pragma unroll
-            for (int k = 0; k < VU; ++k)
-#pragma unroll
-              for (int i = 0; i < V::N; ++i) acc[k][i] = fmaf(w[u], to_f32(x[u][k].e[i]), acc[k][i]);
-          }
-      }
-#pragma unroll
-      for (int k = 0; k < VU; ++k)
-        if (v0 + k * width < row_vecs) {
-          V y;
-#pragma unroll
-          for (int i = 0; i < V::N; ++i) y.e[i] = from_f32<T>(acc[k][i]);
-          out[static_cast<long long>(t) * row_vecs + v0 + k * width] = y.raw;
+            for (int i = 0; i < V::N; ++i) acc[k][i] = fmaf(w[u], to_f32(x[u][k].e[i]), acc[k][i]);
         }
     }
+#pragma unroll
+    for (int k = 0; k < VU; ++k)
+      if (v0 + k * 32 < row_vecs) {
+        V y;
+#pragma unroll
+        for (int i = 0; i < V::N; ++i) y.e[i] = from_f32<T>(acc[k][i]);
+        out[static_cast<long long>(t) * row_vecs + v0 + k * 32] = y.raw;
+      }
   }
 }
 
@@ -507,7 +514,7 @@ moe_unpermute_narrow_kernel(const typename RawVec<VB>::type* __restrict__ rows_i
 // through the ring: dout is read once for them, and the products stay in fp32 until the token's threads add them up.
 // `rows_in` and `dweights` are null where only drows is wanted. An item is VU vectors; vectors change fastest, then choices.
 // 8192 x 4096 bf16 top-2 56.5 us, 5.9 TB/s; 8192 x 2048 top-6 76 us, 5.7 TB/s (with the rows in registers 125).
-constexpr int scatter_vectors(int kc) { return kc == 2 ? 2 : 1; }
+constexpr int scatter_vectors(int kc) { return kc <= 4 ? 2 : 1; }
 constexpr int scatter_depth(int vb, int kc) { return kGatherSmem / (kSortThreads * vb * (kc + 1) * scatter_vectors(kc)); }
 template <class T, int VB, int KC>
 __global__ void __launch_bounds__(kSortThreads, 2)
@@ -812,13 +819,13 @@ static int launch_unpermute_rows(const void* rows, int ntokens, int topk, int ro
   static int known[64] = {};
   int ctas = 0;
   if constexpr (VB < 8) {
-    constexpr int VU = 8 / UN;
+    constexpr int VU = 16 / UN;
     auto kern = moe_unpermute_narrow_kernel<T, VB, UN, VU>;
     const int rc = sort_resident_ctas(kern, 0, known, &ctas);
     if (rc != FLUXB_OK) return rc;
-    const int width = sort_width(row_vecs, VU), per = kSortThreads / width, need = (ntokens + per - 1) / per;
-    return launch_pdl(kern, need < ctas ? need : ctas, kSortThreads, stream, static_cast<const R*>(rows), ntokens, topk, row_vecs, width, index, weights, wdtype,
-                      static_cast<R*>(out));
+    const long long warps = static_cast<long long>(ntokens) * ((row_vecs + 32 * VU - 1) / (32 * VU)), need = (warps + kSortThreads / 32 - 1) / (kSortThreads / 32);
+    return launch_pdl(kern, need < ctas ? static_cast<int>(need) : ctas, kSortThreads, stream, static_cast<const R*>(rows), ntokens, topk, row_vecs, index, weights,
+                      wdtype, static_cast<R*>(out));
   } else {
     constexpr int VU = gather_vectors(VB, UN), SMEM = gather_depth(VB, UN) * UN * VU * VB * kSortThreads;
     auto kern = moe_unpermute_kernel<T, VB, UN>;
@@ -833,8 +840,7 @@ template <class T, int VB>
 static int launch_unpermute(const void* rows, int ntokens, int topk, int row_vecs, const int* index, const void* weights, int wdtype, void* out,
                             cudaStream_t stream) {
   if (topk <= 2) return launch_unpermute_rows<T, VB, 2>(rows, ntokens, topk, row_vecs, index, weights, wdtype, out, stream);
-  if (topk <= 4) return launch_unpermute_rows<T, VB, 4>(rows, ntokens, topk, row_vecs, index, weights, wdtype, out, stream);
-  return launch_unpermute_rows<T, VB, 8>(rows, ntokens, topk, row_vecs, index, weights, wdtype, out, stream);
+  return launch_unpermute_rows<T, VB, 4>(rows, ntokens, topk, row_vecs, index, weights, wdtype, out, stream);
 }
 
 template <class T, int VB, int KC>
