@@ -245,11 +245,13 @@ __device__ __forceinline__ void sort_clear_tail(typename RawVec<VB>::type* rows_
     for (long long v = threadIdx.x; v < row_vecs; v += kSortThreads) rows_out[r * row_vecs + v] = zero;
 }
 
-// `width` threads (a power of two from 32 to 256) take one token: each vector is read once and stored to the token's rows.
-// 8192 x 4096 bf16 top-2 33 us, 6.1 TB/s; rows of odd length go two or one bytes at a time (4096 x 1001 bf16 9.3 us, 2.7 TB/s).
+// A warp takes 32 * UN vectors of a token: each is read once and stored to the token's rows.
+// 8192 x 4096 bf16 top-2 33 us, 6.1 TB/s; 512 x 7168 top-8 10.6 (with four vectors 12.3, with a power of two of threads a token
+// 11.8); rows of odd length go two or one bytes at a time, four of them (4096 x 4097 bf16 top-2 24 us, 4.2 TB/s; two of them 39).
+constexpr int permute_vectors(int vb) { return vb == 16 ? 2 : 4; }
 template <int VB>
 __global__ void __launch_bounds__(kSortThreads)
-moe_permute_kernel(const typename RawVec<VB>::type* __restrict__ tokens, int ntokens, int topk, int row_vecs, int width, int tail_ctas,
+moe_permute_kernel(const typename RawVec<VB>::type* __restrict__ tokens, int ntokens, int topk, int row_vecs, int units, int tail_ctas,
                    const int* __restrict__ splits, int nexperts, const int* __restrict__ index,
                    typename RawVec<VB>::type* __restrict__ rows_out) {
   const long long rows = static_cast<long long>(ntokens) * topk;
@@ -259,25 +261,24 @@ moe_permute_kernel(const typename RawVec<VB>::type* __restrict__ tokens, int nto
     sort_clear_tail<VB>(rows_out, rows, row_vecs, splits, nexperts, static_cast<int>(blockIdx.x), tail_ctas);
     return;
   }
-  const int per = kSortThreads / width;
-  const long long t = static_cast<long long>(static_cast<int>(blockIdx.x) - tail_ctas) * per + static_cast<int>(threadIdx.x) / width;
+  constexpr int UN = permute_vectors(VB);
+  const int unit = (static_cast<int>(blockIdx.x) - tail_ctas) * (kSortThreads / 32) + (static_cast<int>(threadIdx.x) >> 5);
+  const int t = unit / units;
   if (t >= ntokens) return;
-  const auto* src = tokens + t * row_vecs;
-  const int* idx = index + t * topk;
-  constexpr int UN = 4;
-  for (int v0 = static_cast<int>(threadIdx.x) & (width - 1); v0 < row_vecs; v0 += UN * width) {
-    typename RawVec<VB>::type x[UN];
+  const int v0 = (unit - t * units) * (32 * UN) + (static_cast<int>(threadIdx.x) & 31);
+  const auto* src = tokens + static_cast<long long>(t) * row_vecs;
+  const int* idx = index + static_cast<long long>(t) * topk;
+  typename RawVec<VB>::type x[UN];
+#pragma unroll
+  for (int u = 0; u < UN; ++u)
+    if (v0 + u * 32 < row_vecs) x[u] = __ldg(src + v0 + u * 32);
+  for (int j = 0; j < topk; ++j) {
+    const int r = __ldg(idx + j);
+    if (r < 0 || r >= rows) continue;
+    auto* dst = rows_out + static_cast<long long>(r) * row_vecs;
 #pragma unroll
     for (int u = 0; u < UN; ++u)
-      if (v0 + u * width < row_vecs) x[u] = __ldg(src + v0 + u * width);
-    for (int j = 0; j < topk; ++j) {
-      const int r = idx[j];
-      if (r < 0 || r >= rows) continue;
-      auto* dst = rows_out + static_cast<long long>(r) * row_vecs;
-#pragma unroll
-      for (int u = 0; u < UN; ++u)
-        if (v0 + u * width < row_vecs) dst[v0 + u * width] = x[u];
-    }
+      if (v0 + u * 32 < row_vecs) dst[v0 + u * 32] = x[u];
   }
 }
 
@@ -919,14 +920,15 @@ int fluxb_moe_permute(const void* tokens, int ntokens, int topk, long long row_b
   FLUXB_REQUIRE(tokens != nullptr && splits != nullptr && scatter_index != nullptr && rows_out != nullptr, "moe_permute: NULL argument");
   const int vb = sort_vec_bytes(row_bytes, 1, {tokens, rows_out});
   const long long row_vecs = row_bytes / vb;
-  const int width = sort_width(row_vecs, 4), per = kSortThreads / width;
+  const long long units = (row_vecs + 32 * permute_vectors(vb) - 1) / (32 * permute_vectors(vb)), warps = units * ntokens;
+  FLUXB_REQUIRE(warps < (1ll << 31) - 8, "moe_permute: %d rows of %lld bytes are too many", ntokens, row_bytes);
   const long long total = static_cast<long long>(ntokens) * topk;
   const int tail = total < kSortTailCtas ? static_cast<int>(total) : kSortTailCtas;  // (first: they work beside the others)
-  const int grid = tail + (ntokens + per - 1) / per;
+  const int grid = tail + static_cast<int>((warps + kSortThreads / 32 - 1) / (kSortThreads / 32));
   cudaStream_t s = static_cast<cudaStream_t>(stream);
 #define FLUXB_PERMUTE(VB)                                                                                                                       \
   return launch_pdl(moe_permute_kernel<VB>, grid, kSortThreads, s, static_cast<const RawVec<VB>::type*>(tokens), ntokens, topk,                  \
-                    static_cast<int>(row_vecs), width, tail, splits, nexperts, scatter_index, static_cast<RawVec<VB>::type*>(rows_out))
+                    static_cast<int>(row_vecs), static_cast<int>(units), tail, splits, nexperts, scatter_index, static_cast<RawVec<VB>::type*>(rows_out))
   switch (vb) {
     case 16: FLUXB_PERMUTE(16);
     case 8: FLUXB_PERMUTE(8);
