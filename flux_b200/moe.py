@@ -108,8 +108,9 @@ class _RouteFn(torch.autograd.Function):
         dtype, nexperts = ctx.like
         ntokens, topk = chosen.shape
         dlogits = chosen.new_empty((ntokens, nexperts), dtype=dtype)
+        dweights = dweights.contiguous()  # (a copy is held until the launch is queued: other threads allocate during the call)
         _lib.check(_lib.load().fluxb_moe_route_backward(
-            dweights.contiguous().data_ptr(), chosen.data_ptr(), weights.data_ptr(), fluxb_dtype(dtype), ntokens, nexperts, topk,
+            dweights.data_ptr(), chosen.data_ptr(), weights.data_ptr(), fluxb_dtype(dtype), ntokens, nexperts, topk,
             dlogits.data_ptr(), _cur_stream()))
         return dlogits, None
 

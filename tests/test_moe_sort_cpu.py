@@ -1,5 +1,6 @@
 """Refusals of the routing and sort operators: they need no GPU."""
 import ctypes as C
+import weakref
 
 import pytest
 import torch
@@ -59,3 +60,37 @@ def test_no_tokens_is_no_work():
     assert lib.fluxb_moe_route(None, _lib.F32, 0, 8, 2, None, None, None) == _lib.FLUXB_OK
     assert lib.fluxb_moe_permute(None, 0, 2, 64, None, 8, None, None, None) == _lib.FLUXB_OK
     assert lib.fluxb_moe_unpermute(None, _lib.F32, 0, 2, 64, None, None, 0, None, None) == _lib.FLUXB_OK
+
+
+class _Context:
+    """What an autograd function sees of its forward pass."""
+
+    def __init__(self, saved, **kept):
+        self.saved_tensors = saved
+        self.__dict__.update(kept)
+
+
+def test_a_gradient_that_is_copied_lives_until_the_native_call_returns(monkeypatch):
+    """An expanded gradient (as from `w.sum()`) is made contiguous: that copy is the kernel's input, and its memory must not go
+    back to the allocator before the launch is queued."""
+    from flux_b200 import moe
+
+    copies, alive = [], []
+    contiguous = torch.Tensor.contiguous
+
+    def watched(t, *args, **kwargs):
+        c = contiguous(t, *args, **kwargs)
+        copies.append((c.data_ptr(), weakref.ref(c)))
+        return c
+
+    class Library:
+        def fluxb_moe_route_backward(self, dweights, *_):
+            alive.extend(ref() is not None for ptr, ref in copies if ptr == dweights)
+            return _lib.FLUXB_OK
+
+    monkeypatch.setattr(torch.Tensor, "contiguous", watched)
+    monkeypatch.setattr(_lib, "load", Library)
+    monkeypatch.setattr(moe, "_cur_stream", lambda: None)
+    ctx = _Context((torch.zeros(3, 2, dtype=torch.int32), torch.full((3, 2), 0.5)), like=(torch.float32, 8))
+    dlogits, _ = moe._RouteFn.backward(ctx, None, torch.ones(()).expand(3, 2))
+    assert dlogits.shape == (3, 8) and alive == [True]
