@@ -461,16 +461,18 @@ class GemmGroupedV3GatherRS:
         if tuning is None and _tune.TABLE.records:
             tuning = _tune.TABLE.get(_tune.record_key("moe_gather_rs", m, self.n_dim, k, self.input_dtype, w))
         lib = _lib.load()
+        routing_idx = routing_idx.contiguous()  # (copies are held until the launch is queued: other threads allocate during the call)
         if splits_cpu is None:
+            splits = splits_gpu.contiguous()
             _lib.check(lib.fluxb_moe_gather_rs_forward_dev(
-                self._h, input.data_ptr(), m, k, weight.data_ptr(), splits_gpu.contiguous().data_ptr(),
-                routing_idx.contiguous().data_ptr(), _ptr(input_scale), _ptr(weight_scale), _ptr(output_vec_scale),
+                self._h, input.data_ptr(), m, k, weight.data_ptr(), splits.data_ptr(),
+                routing_idx.data_ptr(), _ptr(input_scale), _ptr(weight_scale), _ptr(output_vec_scale),
                 out.data_ptr(), _tuning(tuning), _cur_stream()))
         else:
             splits = splits_cpu.contiguous()
             _lib.check(lib.fluxb_moe_gather_rs_forward_ep(
                 self._h, input.data_ptr(), m, ntokens, k, weight.data_ptr(), splits.data_ptr(),
-                routing_idx.contiguous().data_ptr(), _ptr(input_scale), _ptr(weight_scale), _ptr(output_vec_scale),
+                routing_idx.data_ptr(), _ptr(input_scale), _ptr(weight_scale), _ptr(output_vec_scale),
                 out.data_ptr(), _tuning(tuning), _cur_stream()))
         if with_stream_sync:
             torch.cuda.current_stream().synchronize()

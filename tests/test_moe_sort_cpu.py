@@ -94,3 +94,35 @@ def test_a_gradient_that_is_copied_lives_until_the_native_call_returns(monkeypat
     ctx = _Context((torch.zeros(3, 2, dtype=torch.int32), torch.full((3, 2), 0.5)), like=(torch.float32, 8))
     dlogits, _ = moe._RouteFn.backward(ctx, None, torch.ones(()).expand(3, 2))
     assert dlogits.shape == (3, 8) and alive == [True]
+
+
+@pytest.mark.parametrize("counts_on_device", [False, True])
+def test_indexes_that_are_copied_live_until_the_native_call_returns(monkeypatch, counts_on_device):
+    from flux_b200 import moe
+
+    copies, alive = [], []
+    contiguous = torch.Tensor.contiguous
+
+    def watched(t, *args, **kwargs):
+        c = contiguous(t, *args, **kwargs)
+        copies.append((c.data_ptr(), weakref.ref(c)))
+        return c
+
+    def launched(*args):
+        alive.extend(ref() is not None for ptr, ref in copies if ptr in args)
+        return _lib.FLUXB_OK
+
+    class Library:
+        fluxb_moe_gather_rs_forward_dev = fluxb_moe_gather_rs_forward_ep = staticmethod(launched)
+
+    monkeypatch.setattr(torch.Tensor, "contiguous", watched)
+    monkeypatch.setattr(_lib, "load", Library)
+    monkeypatch.setattr(moe, "_check", lambda ok, what: None)  # (the tensors are not on a GPU)
+    monkeypatch.setattr(moe, "_cur_stream", lambda: None)
+    op = object.__new__(moe.GemmGroupedV3GatherRS)
+    op.__dict__.update(comm=type("", (), {"world": 1}), ep_size=1, nexperts=2, n_dim=4, topk=2, max_m=6, input_dtype=torch.float32,
+                       output_dtype=torch.float32, _h=None)
+    index = torch.zeros(6, 2, dtype=torch.int32)[:, 0]
+    counts = torch.zeros(2, 2, dtype=torch.int32)[:, 0]
+    op._forward(torch.zeros(6, 8), torch.zeros(2, 4, 8), None if counts_on_device else counts, counts if counts_on_device else None, index)
+    assert alive == [True, True]
