@@ -16,6 +16,7 @@ import ctypes as C
 from typing import List, Optional, Sequence
 
 import torch
+from torch.autograd import forward_ad as _forward_ad
 
 from . import _lib
 from . import tune as _tune
@@ -67,6 +68,16 @@ def _on_device(t: torch.Tensor) -> bool:
     return d >= 0 and d == _cur_device()
 
 
+def _refuse_tangent(name: str, *tensors: Optional[torch.Tensor]) -> None:
+    """No operator here has a forward-mode derivative, and the library sees addresses: a tensor's tangent would be lost without a
+    word, with the gradient mode on or off."""
+    if _forward_ad._current_level < 0:  # (outside of `dual_level` there are none)
+        return
+    for t in tensors:
+        if t is not None and _forward_ad.unpack_dual(t).tangent is not None:
+            raise RuntimeError(f"{name} has no forward-mode derivative")
+
+
 def _check_index(name: str, dev: int, splits: torch.Tensor, scatter_index: torch.Tensor) -> torch.Size:
     """Shape [ntokens, topk] of an index whose tensors, like the call's others, are on device `dev`, the current one."""
     if not (splits.get_device() == dev and splits.dtype is torch.int32 and len(splits.shape) == 1 and splits.shape[0] >= 1 and splits.is_contiguous()):
@@ -104,6 +115,7 @@ class _RouteFn(torch.autograd.Function):
     def backward(ctx, _, dweights):
         if dweights is None:
             return None, None
+        _refuse_tangent("moe_route's gradient", dweights)
         chosen, weights = ctx.saved_tensors
         dtype, nexperts = ctx.like
         ntokens, topk = chosen.shape
@@ -122,6 +134,7 @@ def moe_route(logits: torch.Tensor, topk: int):
     weight 0, which `calc_scatter_index` gives no row. Differentiable in the logits."""
     if not (_on_device(logits) and logits.dim() == 2 and logits.dtype in _FLOATS):
         raise RuntimeError("moe_route: logits must be a fp32, bf16 or fp16 [ntokens, nexperts] tensor on the current CUDA device")
+    _refuse_tangent("moe_route", logits)
     topk = int(topk)
     if not 1 <= topk <= logits.shape[1] or logits.shape[0] * topk >= 1 << 30:
         raise RuntimeError(f"moe_route: topk={topk} for {logits.shape[0]} tokens and {logits.shape[1]} experts")
@@ -163,6 +176,7 @@ class _PermuteFn(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, drows):
+        _refuse_tangent("moe_permute's gradient", drows)
         return _unpermute(drows, ctx.saved_tensors[0], None), None, None
 
 
@@ -177,6 +191,7 @@ class _UnpermuteFn(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dout):
+        _refuse_tangent("moe_unpermute's gradient", dout)
         rows, splits, scatter_index, weights = ctx.saved_tensors
         if weights is None:
             return _permute(dout, splits, scatter_index), None, None, None
@@ -208,6 +223,7 @@ def moe_permute(tokens: torch.Tensor, splits: torch.Tensor, scatter_index: torch
     ntokens, _ = _check_index("moe_permute", tokens.get_device(), splits, scatter_index)
     if ntokens != shape[0]:
         raise RuntimeError(f"moe_permute: scatter_index has {ntokens} tokens, not {shape[0]}")
+    _refuse_tangent("moe_permute", tokens)
     if tokens.requires_grad and torch.is_grad_enabled():
         _check(tokens.dtype in _FLOATS, "moe_permute: only fp32, bf16 and fp16 tokens have gradients")
         return _PermuteFn.apply(tokens, splits, scatter_index)
@@ -231,6 +247,7 @@ def moe_unpermute(rows: torch.Tensor, splits: torch.Tensor, scatter_index: torch
             raise RuntimeError("moe_unpermute: weights must be a fp32, bf16 or fp16 [ntokens, topk] tensor on the current CUDA device")
         if not weights.is_contiguous():
             weights = weights.contiguous()
+    _refuse_tangent("moe_unpermute", rows, weights)
     if torch.is_grad_enabled() and (rows.requires_grad or (weights is not None and weights.requires_grad)):
         return _UnpermuteFn.apply(rows, splits, scatter_index, weights)
     return _unpermute(rows, scatter_index, weights)
