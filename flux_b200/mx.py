@@ -11,6 +11,7 @@ are e2m1 (0, 0.5, 1, 1.5, 2, 3, 4, 6 and their negatives), two to a byte, the fi
 from __future__ import annotations
 
 import math
+import threading
 from typing import Dict, Optional
 
 import torch
@@ -22,6 +23,7 @@ from .shm import _LAST, Comm, fluxb_dtype, get_comm
 
 BLOCK = 32
 _COMMS: Dict[int, Comm] = {}
+_LOCK = threading.Lock()
 
 
 def _comm() -> Comm:
@@ -30,11 +32,15 @@ def _comm() -> Comm:
     dev = _cur_device()
     if not _LAST:
         get_comm(None)
-    if _LAST[0].device.index == dev:
-        return _LAST[0]
+    c = _LAST[0]
+    if c.device.index == dev:
+        return c
     c = _COMMS.get(dev)
     if c is None:
-        c = _COMMS[dev] = Comm(None)
+        with _LOCK:
+            c = _COMMS.get(dev)
+            if c is None:
+                c = _COMMS[dev] = Comm(None)
     return c
 
 
@@ -216,7 +222,8 @@ def mx_gemm(x: MXTensor, w: MXTensor, bias: Optional[torch.Tensor] = None, outpu
     out = _output("mx_gemm", output, m, n, output_dtype, _like(x))
     if n == 0:
         return out
-    _lib.check(_lib.load().fluxb_mx_gemm(_comm().handle, x._data_ptr, x._blocks_ptr, w._data_ptr, w._blocks_ptr, out.data_ptr(), m, n, x.k,
+    comm = _comm()
+    _lib.check(_lib.load().fluxb_mx_gemm(comm.handle, x._data_ptr, x._blocks_ptr, w._data_ptr, w._blocks_ptr, out.data_ptr(), m, n, x.k,
                                          fluxb_dtype(output_dtype), _ptr(bias), _tuning(tuning), _cur_stream()))
     return out
 
@@ -235,7 +242,8 @@ def mx_grouped_gemm(x: MXTensor, w: MXTensor, splits: torch.Tensor, output_dtype
         return out
     lib = _lib.load()
     workspace = _like(x).new_empty(lib.fluxb_mx_grouped_workspace_bytes(rows, nexperts, x.k))
-    _lib.check(lib.fluxb_mx_grouped_gemm(_comm().handle, x._data_ptr, x._blocks_ptr, rows, w._data_ptr, w._blocks_ptr, nexperts,
+    comm = _comm()
+    _lib.check(lib.fluxb_mx_grouped_gemm(comm.handle, x._data_ptr, x._blocks_ptr, rows, w._data_ptr, w._blocks_ptr, nexperts,
                                          splits.data_ptr(), out.data_ptr(), n, x.k, fluxb_dtype(output_dtype), workspace.data_ptr(), _tuning(tuning),
                                          _cur_stream()))
     return out

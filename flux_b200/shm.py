@@ -11,6 +11,7 @@ reference (`flux_shm.cc:161-168`). No NVSHMEM and no NCCL call is made here.
 from __future__ import annotations
 
 import ctypes as C
+import threading
 import weakref
 from typing import Dict, List, Optional, Sequence
 
@@ -173,6 +174,7 @@ class Comm:
 
 
 _COMMS: Dict[int, Comm] = {}
+_LOCKS: Dict[int, threading.Lock] = {}  # one per group: setting up is a collective of the group, and must not hold up another's
 _LAST: List[Comm] = []
 
 
@@ -180,8 +182,12 @@ def get_comm(group) -> Comm:
     key = id(group) if group is not None else 0
     c = _COMMS.get(key)
     if c is None:
-        c = Comm(group)
-        _COMMS[key] = c
+        # threads that come here together get one communicator: a second one would replace the first, which would be
+        # released while its handle is in use
+        with _LOCKS.setdefault(key, threading.Lock()):
+            c = _COMMS.get(key)
+            if c is None:
+                c = _COMMS[key] = Comm(group)
     _LAST[:] = [c]
     return c
 

@@ -179,3 +179,39 @@ def test_the_path_from_several_threads():
     torch.cuda.synchronize()
     flux.get_comm(None).check_status()
     assert wrong == []
+
+
+FIRST_PRODUCTS = """
+import threading, torch, flux_b200 as flux
+from flux_b200 import mx
+q = [flux.mx_quantize(torch.randn(40 + i, 256, device="cuda")) for i in range(6)]
+w, splits = flux.mx_quantize(torch.randn(2, 96, 256, device="cuda")), torch.tensor([30, 10], dtype=torch.int32, device="cuda")
+one = flux.MXTensor(w.data[0], w.scales[0])
+torch.cuda.synchronize()
+start, got = threading.Barrier(6), [None] * 6
+def work(i):
+    torch.cuda.set_device(0)
+    start.wait()
+    got[i] = flux.mx_gemm(q[i], one) if i % 2 else flux.mx_grouped_gemm(q[i], w, splits)
+threads = [threading.Thread(target=work, args=(i,)) for i in range(6)]
+for t in threads: t.start()
+for t in threads: t.join()
+torch.cuda.synchronize()
+flux.get_comm(None).check_status()
+for i in range(6):
+    again = flux.mx_gemm(q[i], one) if i % 2 else flux.mx_grouped_gemm(q[i], w, splits)
+    rows = 40 + i if i % 2 else 40
+    assert torch.equal(got[i][:rows], again[:rows])
+print("same")
+"""
+
+
+def test_first_products_of_several_threads():
+    """Of a process without a communicator: the threads make one together."""
+    import os
+    import subprocess
+    import sys
+
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    out = subprocess.run([sys.executable, "-c", FIRST_PRODUCTS], cwd=root, capture_output=True, text=True, timeout=300)
+    assert out.returncode == 0 and out.stdout.strip() == "same", out.stderr[-2000:]
