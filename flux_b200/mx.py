@@ -19,7 +19,7 @@ import torch
 from . import _lib
 from .moe import _FLOATS, _check_index, _on_device, _refuse_tangent
 from .ops import _check, _cur_device, _cur_stream, _ptr, _tuning
-from .shm import _LAST, Comm, fluxb_dtype, get_comm
+from .shm import _LAST, Comm, fluxb_dtype
 
 BLOCK = 32
 _COMMS: Dict[int, Comm] = {}
@@ -27,14 +27,13 @@ _LOCK = threading.Lock()
 
 
 def _comm() -> Comm:
-    """A communicator of the current device, for its status word and time-out: the default one (made if there is none yet),
-    or, beside a default of another device, one that this module keeps."""
+    """A communicator of the current device, for its status word and time-out: the default one, or, where there is none or it is
+    another device's, one of one rank that this module keeps and that does not become the default."""
     dev = _cur_device()
-    if not _LAST:
-        get_comm(None)
-    c = _LAST[0]
-    if c.device.index == dev:
-        return c
+    if _LAST:
+        c = _LAST[0]
+        if c.device.index == dev:
+            return c
     c = _COMMS.get(dev)
     if c is None:
         with _LOCK:

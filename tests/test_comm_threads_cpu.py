@@ -78,3 +78,13 @@ def test_first_products_beside_a_default_of_another_device():
     shm.get_comm(None).device = type("", (), {"index": 1})
     got = _together(lambda i: mx._comm())
     assert len(set(map(id, got))) == 1 and len(_Comm.made) == 2 and got[0] is not shm.default_comm()
+
+
+def test_products_do_not_make_a_default_communicator():
+    """Ops that bind to the communicator of `init_flux_shm` still ask for it."""
+    c = mx._comm()
+    with pytest.raises(RuntimeError, match="call flux.init_flux_shm"):
+        shm.default_comm()
+    assert mx._comm() is c and len(_Comm.made) == 1
+    default = shm.get_comm(None)
+    assert default is not c and mx._comm() is default
