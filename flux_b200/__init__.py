@@ -29,7 +29,7 @@ from .ops import (
 from .layers import ColumnParallelLinear, MoEMLP, MXLinear, MXMoEMLP, RowParallelLinear, TensorParallelMLP
 from .moe import (GemmGroupedV3AGScatter, GemmGroupedV3GatherRS, calc_gather_index, calc_scatter_index, moe_permute,
                   moe_route, moe_unpermute)
-from .mx import MXTensor, mx_dequantize, mx_gemm, mx_grouped_gemm, mx_quantize
+from .mx import MXTensor, mx_check_status, mx_dequantize, mx_gemm, mx_grouped_gemm, mx_quantize
 from .shm import GroupBarrier, default_comm, flux_create_tensor_list, get_comm, init_flux_shm
 from .util import bench_func, get_arch, group_profile, torch_allclose, with_torch_deterministic
 
@@ -41,5 +41,5 @@ __all__ = [
     "GroupBarrier", "flux_create_tensor_list", "create_tensor_list", "get_comm", "init_flux_shm", "bench_func",
     "get_arch", "group_profile", "GemmGroupedV3AGScatter", "GemmGroupedV3GatherRS", "calc_scatter_index",
     "calc_gather_index", "default_comm", "torch_allclose", "with_torch_deterministic", "FluxbError", "Tuning", "util", "TuningRecord", "load_tuning_record",
-    "MXTensor", "mx_quantize", "mx_dequantize", "mx_gemm", "mx_grouped_gemm", "moe_route", "moe_permute", "moe_unpermute", "layers", "tune", "ColumnParallelLinear", "RowParallelLinear", "TensorParallelMLP", "MoEMLP", "MXLinear", "MXMoEMLP",
+    "MXTensor", "mx_quantize", "mx_dequantize", "mx_gemm", "mx_grouped_gemm", "mx_check_status", "moe_route", "moe_permute", "moe_unpermute", "layers", "tune", "ColumnParallelLinear", "RowParallelLinear", "TensorParallelMLP", "MoEMLP", "MXLinear", "MXMoEMLP",
 ]

@@ -12,7 +12,7 @@ from __future__ import annotations
 
 import math
 import threading
-from typing import Dict, Optional
+from typing import Dict, List, Optional
 
 import torch
 
@@ -23,6 +23,7 @@ from .shm import _LAST, Comm, fluxb_dtype
 
 BLOCK = 32
 _COMMS: Dict[int, Comm] = {}
+_USED: Dict[int, List[Comm]] = {}  # per device: the communicators whose status word its products were given
 _LOCK = threading.Lock()
 
 
@@ -30,17 +31,28 @@ def _comm() -> Comm:
     """A communicator of the current device, for its status word and time-out: the default one, or, where there is none or it is
     another device's, one of one rank that this module keeps and that does not become the default."""
     dev = _cur_device()
-    if _LAST:
-        c = _LAST[0]
-        if c.device.index == dev:
-            return c
-    c = _COMMS.get(dev)
-    if c is None:
+    c = _LAST[0] if _LAST else None
+    if c is None or c.device.index != dev:
+        c = _COMMS.get(dev)
+        if c is None:
+            with _LOCK:
+                c = _COMMS.get(dev)
+                if c is None:
+                    c = _COMMS[dev] = Comm(None)
+    used = _USED.setdefault(dev, [])
+    if c not in used:
         with _LOCK:
-            c = _COMMS.get(dev)
-            if c is None:
-                c = _COMMS[dev] = Comm(None)
+            if c not in used:
+                used.append(c)
     return c
+
+
+def mx_check_status() -> None:
+    """Raise if a bounded wait of a product on the current device has run out, whose output is then incomplete (call after a
+    synchronize). It reads the status of every communicator that this device's products have used: the default ones, which
+    `Comm.check_status` reads as well, and the one that they make where there is none."""
+    for c in list(_USED.get(_cur_device(), ())):
+        c.check_status()
 
 
 def _blocks_shape(lead, rows: int, k: int):

@@ -25,6 +25,7 @@ def nothing_made_yet(monkeypatch):
     monkeypatch.setattr(shm, "_COMMS", {})
     monkeypatch.setattr(mx, "Comm", _Comm)
     monkeypatch.setattr(mx, "_COMMS", {})
+    monkeypatch.setattr(mx, "_USED", {}, raising=False)
     monkeypatch.setattr(mx, "_cur_device", lambda: 0)
     last = list(shm._LAST)
     shm._LAST.clear()
@@ -88,3 +89,37 @@ def test_products_do_not_make_a_default_communicator():
     assert mx._comm() is c and len(_Comm.made) == 1
     default = shm.get_comm(None)
     assert default is not c and mx._comm() is default
+
+
+def _with_status(c, status):
+    def check_status():
+        if status:
+            raise RuntimeError(f"status {status}")
+
+    c.check_status = check_status
+    return c
+
+
+def test_the_status_of_products_can_be_read():
+    """Of every communicator that products of the current device have used, whichever is the default by now; of no other device's."""
+    mx.mx_check_status()  # no product yet
+    own = _with_status(mx._comm(), 0)
+    default = _with_status(shm.get_comm(None), 0)
+    mx._comm()
+    later = _with_status(shm.get_comm(object()), 0)
+    mx.mx_check_status()
+    for c, used in ((own, True), (default, True), (later, False)):
+        _with_status(c, 3)
+        if used:
+            with pytest.raises(RuntimeError, match="status 3"):
+                mx.mx_check_status()
+        else:
+            mx.mx_check_status()  # no product has used it
+        _with_status(c, 0)
+    mx._cur_device = lambda: 1  # (put back by the fixture)
+    _with_status(own, 3)
+    mx.mx_check_status()
+    other = _with_status(mx._comm(), 4)
+    assert other not in (own, default, later)
+    with pytest.raises(RuntimeError, match="status 4"):
+        mx.mx_check_status()

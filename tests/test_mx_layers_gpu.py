@@ -197,7 +197,7 @@ threads = [threading.Thread(target=work, args=(i,)) for i in range(6)]
 for t in threads: t.start()
 for t in threads: t.join()
 torch.cuda.synchronize()
-flux.get_comm(None).check_status()
+flux.mx_check_status()
 for i in range(6):
     again = flux.mx_gemm(q[i], one) if i % 2 else flux.mx_grouped_gemm(q[i], w, splits)
     rows = 40 + i if i % 2 else 40
