@@ -55,6 +55,14 @@ def mx_check_status() -> None:
         c.check_status()
 
 
+def _check_size(name: str, rows: int, k: int) -> None:
+    """The library takes sizes of 31 bits; larger ones would arrive there as others."""
+    if k >= 1 << 31:
+        raise RuntimeError(f"{name}: K {k} is too large")
+    if rows >= 1 << 31:
+        raise RuntimeError(f"{name}: {rows} rows are too many")
+
+
 def _blocks_shape(lead, rows: int, k: int):
     return (*lead, (rows + 127) // 128, (k + 127) // 128, 512)
 
@@ -79,6 +87,7 @@ class MXTensor:
         k = data.shape[-1] * 2
         if tuple(scales.shape) != (*lead, n, k // BLOCK):
             raise RuntimeError(f"MXTensor: scales shape {tuple(scales.shape)} != {(*lead, n, k // BLOCK)}")
+        _check_size("MXTensor", math.prod(lead) * n, k)
         data = data.contiguous()
         if data.data_ptr() % 16:
             data = data.clone()
@@ -152,14 +161,14 @@ def mx_quantize(x: torch.Tensor, splits: Optional[torch.Tensor] = None, scatter_
     if len(shape) > 2:
         lead = tuple(shape[:-2])
         batch = math.prod(lead)
+    _check_size("mx_quantize", batch * n, k)
+    if lead:
         x = x.contiguous()
         ldx = k  # (a contiguous tensor's stride along a dimension of one row may be any number)
     else:
         if x.stride(1) != 1:
             x = x.contiguous()
         ldx = x.stride(0) if n > 1 else k
-    if batch * n >= 1 << 31:
-        raise RuntimeError(f"mx_quantize: {batch * n} rows are too many")
     out_rows, topk, nexperts = n, 0, 0
     if scatter_index is not None:
         if splits is None or lead:

@@ -88,3 +88,24 @@ def test_sizes():
         most = max((rows // bn + min(nexperts, rows)) * -(-bn // 128) for bn in (64, 128, 192, 256))
         assert lib.fluxb_mx_grouped_workspace_bytes(rows, nexperts, 160) >= most * 2 * 512
     assert lib.fluxb_mx_scale_bytes(-1, 4, 64) == 0 and lib.fluxb_mx_grouped_workspace_bytes(4, -1, 64) == 0
+
+
+def _far(*shape, dtype=torch.uint8):
+    """A tensor of any size without memory."""
+    return torch.empty(shape, dtype=dtype, device="meta")
+
+
+def test_sizes_that_do_not_fit_the_native_call(monkeypatch):
+    """The library takes 32-bit sizes, and what passes them would arrive as another size: 2^32 + 32 as 32."""
+    from flux_b200 import mx
+
+    monkeypatch.setattr(mx, "_on_device", lambda t: True)
+    monkeypatch.setattr(mx, "_cur_stream", lambda: None)
+    for k in (1 << 31, (1 << 32) + 32):
+        with pytest.raises(RuntimeError, match=f"K {k} is too large"):
+            flux.mx_quantize(_far(1, k, dtype=torch.bfloat16))
+        with pytest.raises(RuntimeError, match=f"K {k} is too large"):
+            flux.MXTensor(_far(1, k // 2), _far(1, k // 32))
+    for shape in ((1 << 31, 16), (1 << 16, 1 << 15, 16), ((1 << 32) + 4, 1, 16)):
+        with pytest.raises(RuntimeError, match="rows are too many"):
+            flux.MXTensor(_far(*shape), _far(*shape[:-1], 1))
