@@ -86,8 +86,11 @@ def _check_index(name: str, dev: int, splits: torch.Tensor, scatter_index: torch
     if not (scatter_index.get_device() == dev and scatter_index.dtype is torch.int32 and len(shape) == 2 and shape[1] >= 1
             and scatter_index.is_contiguous()):
         raise RuntimeError(f"{name}: scatter_index must be a contiguous int32 [ntokens, topk] tensor on the current CUDA device")
-    if shape[0] * shape[1] >= 1 << 30:
+    # (the library takes sizes of 31 bits; larger ones would arrive there as others)
+    if shape[0] * shape[1] >= 1 << 30 or shape[1] >= 1 << 30:
         raise RuntimeError(f"{name}: {shape[0]} x {shape[1]} routed rows are too many")
+    if splits.shape[0] >= 1 << 31:
+        raise RuntimeError(f"{name}: splits of {splits.shape[0]} experts are too many")
     return shape
 
 
@@ -136,8 +139,8 @@ def moe_route(logits: torch.Tensor, topk: int):
         raise RuntimeError("moe_route: logits must be a fp32, bf16 or fp16 [ntokens, nexperts] tensor on the current CUDA device")
     _refuse_tangent("moe_route", logits)
     topk = int(topk)
-    if not 1 <= topk <= logits.shape[1] or logits.shape[0] * topk >= 1 << 30:
-        raise RuntimeError(f"moe_route: topk={topk} for {logits.shape[0]} tokens and {logits.shape[1]} experts")
+    if not 1 <= topk <= min(logits.shape[1], 32) or logits.shape[1] > 1024 or logits.shape[0] * topk >= 1 << 30:
+        raise RuntimeError(f"moe_route: topk={topk} for {logits.shape[0]} tokens and {logits.shape[1]} experts (up to 32 of 1024)")
     if not logits.is_contiguous():
         logits = logits.contiguous()
     if logits.requires_grad and torch.is_grad_enabled():
@@ -240,6 +243,8 @@ def moe_unpermute(rows: torch.Tensor, splits: torch.Tensor, scatter_index: torch
         raise RuntimeError("moe_unpermute: rows must be a fp32, bf16 or fp16 [ntokens * topk, hidden] tensor on the current CUDA device")
     dev = rows.get_device()
     ntokens, topk = _check_index("moe_unpermute", dev, splits, scatter_index)
+    if shape[1] >= 1 << 28:
+        raise RuntimeError(f"moe_unpermute: hidden={shape[1]} is too large")
     if shape[0] != ntokens * topk:
         raise RuntimeError(f"moe_unpermute: {shape[0]} rows for {ntokens} x {topk} entries of scatter_index")
     if weights is not None:

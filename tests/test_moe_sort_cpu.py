@@ -126,3 +126,37 @@ def test_indexes_that_are_copied_live_until_the_native_call_returns(monkeypatch,
     counts = torch.zeros(2, 2, dtype=torch.int32)[:, 0]
     op._forward(torch.zeros(6, 8), torch.zeros(2, 4, 8), None if counts_on_device else counts, counts if counts_on_device else None, index)
     assert alive == [True, True]
+
+
+def test_sizes_that_do_not_fit_the_native_call(monkeypatch):
+    """The library takes 32-bit sizes, and what passes them would arrive as another size: 2^32 + 8 as 8."""
+    from flux_b200 import moe
+
+    monkeypatch.setattr(moe, "_on_device", lambda t: True)
+    monkeypatch.setattr(moe, "_cur_stream", lambda: None)
+
+    class Library:  # takes every call
+        def __getattr__(self, name):
+            return lambda *_: _lib.FLUXB_OK
+
+    monkeypatch.setattr(_lib, "load", Library)
+
+    def far(*shape, dtype=torch.float32):  # of any size, without memory
+        return torch.empty(shape, dtype=dtype, device="meta")
+
+    index, splits = far(4, 2, dtype=torch.int32), far(8, dtype=torch.int32)
+    for experts in (1025, 1 << 31, (1 << 32) + 8):
+        with pytest.raises(RuntimeError, match=f"moe_route: .*{experts} experts"):
+            flux.moe_route(far(4, experts), 2)
+    with pytest.raises(RuntimeError, match="moe_route: topk=33"):
+        flux.moe_route(far(4, 64), 33)
+    for hidden in (1 << 28, (1 << 32) + 64):
+        with pytest.raises(RuntimeError, match=f"moe_unpermute: hidden={hidden}"):
+            flux.moe_unpermute(far(8, hidden), splits, index)
+    for experts in (1 << 31, (1 << 32) + 8):
+        with pytest.raises(RuntimeError, match=f"{experts} experts"):
+            flux.moe_permute(far(4, 8), far(experts, dtype=torch.int32), index)
+    for topk in (1 << 30, (1 << 32) + 2):
+        with pytest.raises(RuntimeError, match="too many"):
+            flux.moe_permute(far(0, 8), splits, far(0, topk, dtype=torch.int32))
+    flux.moe_route(far(4, 1024), 32), flux.moe_unpermute(far(8, (1 << 28) - 1), splits, index), flux.moe_permute(far(4, 8), splits, index)
