@@ -109,6 +109,12 @@ class MXTensor:
         t._set(data, blocks)
         return t
 
+    def __getstate__(self):
+        return self.data, self.blocks  # (addresses are this object's: copies and what is loaded from a file have their own)
+
+    def __setstate__(self, state) -> None:
+        self._set(*state)
+
     @property
     def data(self) -> torch.Tensor:
         if self._data is None:

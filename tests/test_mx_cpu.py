@@ -109,3 +109,43 @@ def test_sizes_that_do_not_fit_the_native_call(monkeypatch):
     for shape in ((1 << 31, 16), (1 << 16, 1 << 15, 16), ((1 << 32) + 4, 1, 16)):
         with pytest.raises(RuntimeError, match="rows are too many"):
             flux.MXTensor(_far(*shape), _far(*shape[:-1], 1))
+
+
+def _stored(lead=(), rows=3, k=64):
+    """An MXTensor as `mx_quantize` makes it, values and scales in one allocation, in host memory."""
+    from flux_b200 import mx
+
+    t = mx.MXTensor.__new__(mx.MXTensor)
+    t.lead, t.rows, t.k, t._dev = lead, rows, k, -1
+    n = rows * k // 2
+    for d in lead:
+        n *= d
+    at = (n + 15) & ~15
+    blocks = mx._blocks_shape(lead, rows, k)
+    t._store = torch.randint(0, 256, (at + torch.Size(blocks).numel(),), dtype=torch.uint8)
+    t._data = t._blocks = None
+    t._data_ptr = t._store.data_ptr()
+    t._blocks_ptr = t._data_ptr + at
+    return t
+
+
+@pytest.mark.parametrize("how", ["deepcopy", "copy", "pickle", "torch.save"])
+@pytest.mark.parametrize("lead", [(), (2, 3)])
+def test_copies_point_to_their_own_memory(how, lead):
+    """A copy's addresses are those of the copy's tensors, not those of tensors that may be gone by the time it is used."""
+    import copy
+    import io
+    import pickle
+
+    q = _stored(lead)
+    if how == "torch.save":
+        f = io.BytesIO()
+        torch.save(q, f)
+        f.seek(0)
+        c = torch.load(f, weights_only=False)
+    else:
+        c = {"deepcopy": copy.deepcopy, "copy": copy.copy, "pickle": lambda t: pickle.loads(pickle.dumps(t))}[how](q)
+    assert c.shape == q.shape and torch.equal(c.data, q.data) and torch.equal(c.blocks, q.blocks) and c._dev == q._dev
+    assert (c._data_ptr, c._blocks_ptr) == (c.data.data_ptr(), c.blocks.data_ptr())
+    assert (c._data_ptr == q._data_ptr) == (how == "copy")
+    assert torch.equal(c.scales, q.scales)

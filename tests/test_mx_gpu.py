@@ -370,3 +370,29 @@ def test_quantise_more_than_32_bits_of_values():
         data, scales = _quantised64(x[r])
         assert torch.equal(q.data[r].cpu(), data)
         assert torch.equal(y[r].cpu().double(), _values(data, scales))
+
+
+@pytest.mark.parametrize("lead", [(), (3,)])
+def test_copies_outlive_what_they_were_copied_from(lead):
+    import copy
+    import io
+
+    import flux_b200 as flux
+
+    x, v = flux.mx_quantize(torch.randn(5, 96, device="cuda")), torch.randn(*lead, 40, 96, device="cuda")
+    w = flux.mx_quantize(v)
+    splits = torch.tensor([2, 1, 2], dtype=torch.int32, device="cuda")
+
+    def product(q):
+        return flux.mx_grouped_gemm(x, q, splits) if lead else flux.mx_gemm(x, q)
+
+    want, values = product(w), w.dequantize()
+    f = io.BytesIO()
+    torch.save(w, f)
+    f.seek(0)
+    copies = [copy.deepcopy(w), copy.copy(w), torch.load(f, weights_only=False)]
+    del w
+    trash = [torch.full((n,), 255, dtype=torch.uint8, device="cuda") for n in (8192, 16384, 65536) for _ in range(4)]  # where it was
+    for c in copies:
+        assert torch.equal(product(c), want) and torch.equal(c.dequantize(), values)
+    del trash
