@@ -78,6 +78,13 @@ def _refuse_tangent(name: str, *tensors: Optional[torch.Tensor]) -> None:
             raise RuntimeError(f"{name} has no forward-mode derivative")
 
 
+def _in_memory(t: torch.Tensor) -> torch.Tensor:
+    """`t` as contiguous memory that holds its values: a conjugation or a sign that torch has put off is carried out."""
+    if t.is_conj() or t.is_neg():
+        t = t.resolve_conj().resolve_neg()
+    return t if t.is_contiguous() else t.contiguous()
+
+
 def _check_index(name: str, dev: int, splits: torch.Tensor, scatter_index: torch.Tensor) -> torch.Size:
     """Shape [ntokens, topk] of an index whose tensors, like the call's others, are on device `dev`, the current one."""
     if not (splits.get_device() == dev and splits.dtype is torch.int32 and len(splits.shape) == 1 and splits.shape[0] >= 1 and splits.is_contiguous()):
@@ -123,7 +130,7 @@ class _RouteFn(torch.autograd.Function):
         dtype, nexperts = ctx.like
         ntokens, topk = chosen.shape
         dlogits = chosen.new_empty((ntokens, nexperts), dtype=dtype)
-        dweights = dweights.contiguous()  # (a copy is held until the launch is queued: other threads allocate during the call)
+        dweights = _in_memory(dweights)  # (a copy is held until the launch is queued: other threads allocate during the call)
         _lib.check(_lib.load().fluxb_moe_route_backward(
             dweights.data_ptr(), chosen.data_ptr(), weights.data_ptr(), fluxb_dtype(dtype), ntokens, nexperts, topk,
             dlogits.data_ptr(), _cur_stream()))
@@ -141,8 +148,7 @@ def moe_route(logits: torch.Tensor, topk: int):
     topk = int(topk)
     if not 1 <= topk <= min(logits.shape[1], 32) or logits.shape[1] > 1024 or logits.shape[0] * topk >= 1 << 30:
         raise RuntimeError(f"moe_route: topk={topk} for {logits.shape[0]} tokens and {logits.shape[1]} experts (up to 32 of 1024)")
-    if not logits.is_contiguous():
-        logits = logits.contiguous()
+    logits = _in_memory(logits)
     if logits.requires_grad and torch.is_grad_enabled():
         return _RouteFn.apply(logits, topk)
     return _route_forward(logits, topk)
@@ -150,8 +156,7 @@ def moe_route(logits: torch.Tensor, topk: int):
 
 def _permute(tokens: torch.Tensor, splits: torch.Tensor, scatter_index: torch.Tensor) -> torch.Tensor:
     ntokens, topk = scatter_index.shape
-    if not tokens.is_contiguous():
-        tokens = tokens.contiguous()
+    tokens = _in_memory(tokens)
     hidden = tokens.shape[1]
     rows = tokens.new_empty((ntokens * topk, hidden))
     _lib.check(_lib.load().fluxb_moe_permute(tokens.data_ptr(), ntokens, topk, hidden * tokens.element_size(), splits.data_ptr(),
@@ -161,8 +166,7 @@ def _permute(tokens: torch.Tensor, splits: torch.Tensor, scatter_index: torch.Te
 
 def _unpermute(rows: torch.Tensor, scatter_index: torch.Tensor, weights: Optional[torch.Tensor]) -> torch.Tensor:
     ntokens, topk = scatter_index.shape
-    if not rows.is_contiguous():
-        rows = rows.contiguous()
+    rows = _in_memory(rows)
     hidden = rows.shape[1]
     out = rows.new_empty((ntokens, hidden))
     _lib.check(_lib.load().fluxb_moe_unpermute(rows.data_ptr(), fluxb_dtype(rows.dtype), ntokens, topk, hidden, scatter_index.data_ptr(),
@@ -200,14 +204,14 @@ class _UnpermuteFn(torch.autograd.Function):
             return _permute(dout, splits, scatter_index), None, None, None
         ntokens, topk = scatter_index.shape
         dtype, hidden = ctx.like
-        dout = dout.contiguous()
+        dout = _in_memory(dout)
         drows = dweights = None
         if ctx.needs_input_grad[0]:
             drows = dout.new_empty((ntokens * topk, hidden))
         if ctx.needs_input_grad[3]:
             # pairs without an expert get a gradient of zero like the others get theirs: the kernel writes every entry
             dweights = torch.empty_like(weights)
-            rows = rows.contiguous()
+            rows = _in_memory(rows)
         else:
             rows = None
         _lib.check(_lib.load().fluxb_moe_unpermute_backward(
@@ -250,8 +254,7 @@ def moe_unpermute(rows: torch.Tensor, splits: torch.Tensor, scatter_index: torch
     if weights is not None:
         if not (weights.get_device() == dev and weights.dtype in _FLOATS and weights.shape == scatter_index.shape):
             raise RuntimeError("moe_unpermute: weights must be a fp32, bf16 or fp16 [ntokens, topk] tensor on the current CUDA device")
-        if not weights.is_contiguous():
-            weights = weights.contiguous()
+        weights = _in_memory(weights)
     _refuse_tangent("moe_unpermute", rows, weights)
     if torch.is_grad_enabled() and (rows.requires_grad or (weights is not None and weights.requires_grad)):
         return _UnpermuteFn.apply(rows, splits, scatter_index, weights)

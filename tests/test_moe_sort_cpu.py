@@ -160,3 +160,47 @@ def test_sizes_that_do_not_fit_the_native_call(monkeypatch):
         with pytest.raises(RuntimeError, match="too many"):
             flux.moe_permute(far(0, 8), splits, far(0, topk, dtype=torch.int32))
     flux.moe_route(far(4, 1024), 32), flux.moe_unpermute(far(8, (1 << 28) - 1), splits, index), flux.moe_permute(far(4, 8), splits, index)
+
+
+def test_conjugations_and_signs_that_torch_has_put_off(monkeypatch):
+    """`conj()` and what follows from it are marks on a tensor, which its memory does not show: the kernels get memory that holds
+    the values."""
+    from flux_b200 import moe
+
+    seen = {}
+
+    class Library:  # keeps what the first argument points to, of the size of the tensor under test
+        def __getattr__(self, name):
+            def call(first, *_):
+                seen[name] = C.string_at(first, nbytes)
+                return _lib.FLUXB_OK
+
+            return call
+
+    monkeypatch.setattr(_lib, "load", Library)
+    for name in ("_on_device", "_cur_stream"):
+        monkeypatch.setattr(moe, name, lambda *_: True)
+    index, splits = torch.zeros(1, 1, dtype=torch.int32), torch.ones(2, dtype=torch.int32)
+
+    def bits(t):
+        return t.resolve_conj().resolve_neg().clone(memory_format=torch.contiguous_format).numpy().tobytes()
+
+    z = torch.randn(1, 5, dtype=torch.complex64)
+    lazy = z.conj()
+    assert lazy.is_conj() and lazy.is_contiguous()
+    nbytes = 40
+    flux.moe_permute(lazy, splits, index)
+    assert seen["fluxb_moe_permute"] == bits(lazy) != bits(z)
+    lazy = torch.randn(1, 1, dtype=torch.complex64).conj().imag
+    assert lazy.is_neg() and lazy.is_contiguous()
+    nbytes = 4
+    flux.moe_permute(lazy, splits, index)
+    flux.moe_unpermute(lazy, splits, index)
+    flux.moe_route(lazy, 1)
+    for name in ("fluxb_moe_permute", "fluxb_moe_unpermute", "fluxb_moe_route"):
+        assert seen[name] == bits(lazy)
+    moe._RouteFn.backward(_Context((index, torch.ones(1, 1)), like=(torch.float32, 8)), None, lazy)
+    rows = torch.ones(1, 1)
+    moe._UnpermuteFn.backward(_Context((rows, splits, index, rows), like=(torch.float32, 1), needs_input_grad=(True, False, False, True)), lazy)
+    for name in ("fluxb_moe_route_backward", "fluxb_moe_unpermute_backward"):
+        assert seen[name] == bits(lazy)
