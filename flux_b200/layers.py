@@ -396,6 +396,8 @@ class MXMoEMLP(torch.nn.Module):
 
     @torch.no_grad()
     def forward(self, x: torch.Tensor) -> torch.Tensor:
+        if x.dim() == 0 or x.shape[-1] != self.hidden:
+            raise RuntimeError(f"MXMoEMLP: tokens of shape {tuple(x.shape)} are not [..., {self.hidden}]")
         tokens = x.reshape(-1, self.hidden)
         if tokens.shape[0] == 0:
             return torch.empty_like(x)

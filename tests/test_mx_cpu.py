@@ -149,3 +149,16 @@ def test_copies_point_to_their_own_memory(how, lead):
     assert (c._data_ptr, c._blocks_ptr) == (c.data.data_ptr(), c.blocks.data_ptr())
     assert (c._data_ptr == q._data_ptr) == (how == "copy")
     assert torch.equal(c.scales, q.scales)
+
+
+def test_tokens_of_another_size_than_the_layer_are_refused():
+    """Twice the layer's size used to be taken as twice as many tokens."""
+    from flux_b200 import mx
+
+    def weight(n, k):
+        return mx.MXTensor._of(torch.zeros(2, n, k // 2, dtype=torch.uint8), torch.zeros(2, 1, 1, 512, dtype=torch.uint8))
+
+    layer = flux.MXMoEMLP(torch.zeros(2, 64), weight(96, 64), weight(64, 96), 1)
+    for shape in ((4, 128), (4, 32), (2, 3, 192), (0, 128), ()):
+        with pytest.raises(RuntimeError, match=r"MXMoEMLP: .*\[\.\.\., 64\]"):
+            layer(torch.zeros(shape))
