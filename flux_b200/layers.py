@@ -369,6 +369,8 @@ class MXMoEMLP(torch.nn.Module):
         super().__init__()
         self.gated = w_gate is not None
         if self.gated:
+            if not (isinstance(w_gate, torch.Tensor) and isinstance(w_up, torch.Tensor) and w_gate.shape == w_up.shape):
+                raise RuntimeError("MXMoEMLP: w_gate and w_up must be tensors of one shape (they are quantised together)")
             w_up = torch.cat((w_gate.detach(), w_up.detach()), dim=1)
         quantised = [w if isinstance(w, _mx.MXTensor) else _mx.mx_quantize(w.detach()) for w in (w_up, w_down)]
         up, down = quantised

@@ -162,3 +162,12 @@ def test_tokens_of_another_size_than_the_layer_are_refused():
     for shape in ((4, 128), (4, 32), (2, 3, 192), (0, 128), ()):
         with pytest.raises(RuntimeError, match=r"MXMoEMLP: .*\[\.\.\., 64\]"):
             layer(torch.zeros(shape))
+
+
+def test_gate_and_up_projection_of_different_sizes_are_refused():
+    """Both together have twice the experts' size, and would be cut in the middle."""
+    with pytest.raises(RuntimeError, match="MXMoEMLP: w_gate"):
+        flux.MXMoEMLP(torch.zeros(2, 64), torch.zeros(2, 128, 64), torch.zeros(2, 64, 96), 1, w_gate=torch.zeros(2, 64, 64))
+    q = _stored((2,), 96, 64)
+    with pytest.raises(RuntimeError, match="MXMoEMLP: w_gate"):
+        flux.MXMoEMLP(torch.zeros(2, 64), q, q, 1, w_gate=q)
