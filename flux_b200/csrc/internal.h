@@ -1,6 +1,7 @@
 // Host-side internals shared by the .cu files of the library: error
 // reporting, the communicator object, tensor-map encoding, launch helpers.
 #pragma once
+#include <initializer_list>
 #include <cuda.h>
 #include <cuda_runtime.h>
 #include <stdarg.h>
@@ -42,6 +43,13 @@ void set_error(const char* fmt, ...);
 // Rows of a buffer that kernels read or write 16 bytes at a time with plain vector accesses (tensor maps check theirs).
 #define FLUXB_REQUIRE_ALIGNED(ptr, what) \
   FLUXB_REQUIRE((reinterpret_cast<uintptr_t>(ptr) & 15) == 0, what " must be 16-byte aligned")
+
+// Whether every address is a multiple of `bytes`, a power of two (NULL is).
+inline bool all_aligned(int bytes, std::initializer_list<const void*> ptrs) {
+  uintptr_t a = 0;
+  for (const void* p : ptrs) a |= reinterpret_cast<uintptr_t>(p);
+  return (a & static_cast<uintptr_t>(bytes - 1)) == 0;
+}
 
 // Launches with the programmatic-dependent-launch attribute: the kernel must call pdl_wait() before it touches global
 // memory, and pdl_trigger() for the next one to be let in early.

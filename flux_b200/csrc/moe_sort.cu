@@ -888,6 +888,7 @@ int fluxb_moe_route(const void* logits, int dtype, int ntokens, int nexperts, in
   if (rc != FLUXB_OK) return rc;
   if (ntokens == 0) return FLUXB_OK;
   FLUXB_REQUIRE(logits != nullptr && chosen_out != nullptr && weights_out != nullptr, "moe_route: NULL argument");
+  FLUXB_REQUIRE(all_aligned(dtype_bytes(dtype), {logits}) && all_aligned(4, {chosen_out, weights_out}), "moe_route: arguments must be aligned to their types");
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (dtype == FLUXB_F32) return launch_route<float>(logits, ntokens, nexperts, topk, chosen_out, weights_out, s);
   if (dtype == FLUXB_BF16) return launch_route<__nv_bfloat16>(logits, ntokens, nexperts, topk, chosen_out, weights_out, s);
@@ -904,6 +905,8 @@ int fluxb_moe_route_backward(const float* dweights, const int* chosen, const flo
   if (rc != FLUXB_OK) return rc;
   if (ntokens == 0) return FLUXB_OK;
   FLUXB_REQUIRE(dweights != nullptr && chosen != nullptr && weights != nullptr && dlogits != nullptr, "moe_route_backward: NULL argument");
+  FLUXB_REQUIRE(all_aligned(dtype_bytes(dtype), {dlogits}) && all_aligned(4, {dweights, chosen, weights}),
+                "moe_route_backward: arguments must be aligned to their types");
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (dtype == FLUXB_F32) return launch_route_backward<float>(dweights, chosen, weights, ntokens, nexperts, topk, dlogits, s);
   if (dtype == FLUXB_BF16) return launch_route_backward<__nv_bfloat16>(dweights, chosen, weights, ntokens, nexperts, topk, dlogits, s);
@@ -918,6 +921,7 @@ int fluxb_moe_permute(const void* tokens, int ntokens, int topk, long long row_b
   if (rc != FLUXB_OK) return rc;
   if (ntokens == 0) return FLUXB_OK;
   FLUXB_REQUIRE(tokens != nullptr && splits != nullptr && scatter_index != nullptr && rows_out != nullptr, "moe_permute: NULL argument");
+  FLUXB_REQUIRE(all_aligned(4, {splits, scatter_index}), "moe_permute: arguments must be aligned to their types");
   const int vb = sort_vec_bytes(row_bytes, 1, {tokens, rows_out});
   const long long row_vecs = row_bytes / vb;
   const long long units = (row_vecs + 32 * permute_vectors(vb) - 1) / (32 * permute_vectors(vb)), warps = units * ntokens;
@@ -967,6 +971,8 @@ int fluxb_moe_unpermute(const void* rows, int dtype, int ntokens, int topk, int 
   if (ntokens == 0) return FLUXB_OK;
   FLUXB_REQUIRE(rows != nullptr && scatter_index != nullptr && out != nullptr, "moe_unpermute: NULL argument");
   const int eb = dtype_bytes(dtype);
+  FLUXB_REQUIRE(all_aligned(eb, {rows, out}) && all_aligned(4, {scatter_index}) && (weights == nullptr || all_aligned(dtype_bytes(weights_dtype), {weights})),
+                "moe_unpermute: arguments must be aligned to their types");
   const long long row_bytes = static_cast<long long>(hidden) * eb;
   const int vb = sort_vec_bytes(row_bytes, eb, {rows, out});
   const int row_vecs = static_cast<int>(row_bytes / vb);
@@ -988,6 +994,8 @@ int fluxb_moe_unpermute_backward(const void* dout, const void* rows, int dtype, 
                 "moe_unpermute_backward: NULL argument");
   FLUXB_REQUIRE((rows != nullptr) == (dweights != nullptr), "moe_unpermute_backward: the weights' gradient needs the rows, and nothing else does");
   const int eb = dtype_bytes(dtype);
+  FLUXB_REQUIRE(all_aligned(eb, {dout, rows, drows}) && all_aligned(4, {splits, scatter_index}) && all_aligned(dtype_bytes(weights_dtype), {weights, dweights}),
+                "moe_unpermute_backward: arguments must be aligned to their types");
   const long long row_bytes = static_cast<long long>(hidden) * eb;
   const int vb = sort_vec_bytes(row_bytes, eb, {dout, rows, drows});
   const int row_vecs = static_cast<int>(row_bytes / vb);

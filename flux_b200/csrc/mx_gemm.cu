@@ -291,6 +291,7 @@ int fluxb_mx_grouped_gemm(fluxb_comm_t comm, const void* xq, const void* xs, int
   if (rows == 0) return FLUXB_OK;
   FLUXB_REQUIRE(splits_dev != nullptr && workspace != nullptr, "mx_grouped_gemm: NULL argument");
   FLUXB_REQUIRE((reinterpret_cast<uintptr_t>(workspace) & 15) == 0, "mx_grouped_gemm: the workspace must be 16-byte aligned");
+  FLUXB_REQUIRE(all_aligned(4, {splits_dev}), "mx_grouped_gemm: splits must be aligned to their type");
   FLUXB_REQUIRE(static_cast<long long>(nexperts) * n < (1ll << 31) - 256, "mx_grouped_gemm: %d experts of %d columns are too many", nexperts, n);
   MxParams p;
   const int rc = mx_fill("mx_grouped_gemm", comm, p, xq, xs, wq, ws, out, n, k, out_dtype);

@@ -294,6 +294,7 @@ int fluxb_mx_quantize(const void* x, int dtype, int batch, int rows, int k, long
   FLUXB_REQUIRE(x != nullptr && data != nullptr && scales != nullptr, "mx_quantize: NULL argument");
   FLUXB_REQUIRE((reinterpret_cast<uintptr_t>(x) & (eb - 1)) == 0 && (reinterpret_cast<uintptr_t>(data) & 7) == 0 && (reinterpret_cast<uintptr_t>(scales) & 3) == 0,
                 "mx_quantize: the input must be aligned to its type, packed values to 8 bytes, scales to 4");
+  FLUXB_REQUIRE(all_aligned(4, {splits_dev, scatter_index_dev}), "mx_quantize: splits and scatter_index must be aligned to their type");
   QuantParams p;
   memset(&p, 0, sizeof(p));
   p.ldx = ldx;

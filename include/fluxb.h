@@ -226,7 +226,7 @@ int fluxb_moe_gather_index(const int* scatter_index, int ntokens, int topk, int*
  * dweights[t, j] = <dout[t], rows[scatter_index[t, j]]>; drows may be NULL, and `rows` with `dweights`.
  * The row matrices have ntokens * topk rows. `splits` and `scatter_index` belong together as fluxb_moe_scatter_index makes
  * them: every row below sum(splits) is named once, entries outside [0, ntokens * topk) are skipped, rows from sum(splits) on
- * are written as zero. */
+ * are written as zero. Every pointer is aligned to its type (rows of fluxb_moe_permute may start anywhere); others are refused. */
 int fluxb_moe_route(const void* logits, int dtype, int ntokens, int nexperts, int topk, int* chosen_out,
                     float* weights_out, fluxb_stream_t stream);
 int fluxb_moe_route_backward(const float* dweights, const int* chosen, const float* weights, int dtype, int ntokens,

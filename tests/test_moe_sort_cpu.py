@@ -204,3 +204,34 @@ def test_conjugations_and_signs_that_torch_has_put_off(monkeypatch):
     moe._UnpermuteFn.backward(_Context((rows, splits, index, rows), like=(torch.float32, 1), needs_input_grad=(True, False, False, True)), lazy)
     for name in ("fluxb_moe_route_backward", "fluxb_moe_unpermute_backward"):
         assert seen[name] == bits(lazy)
+
+
+@pytest.mark.parametrize("dtype,size", [(_lib.F32, 4), (_lib.BF16, 2), (_lib.F16, 2)])
+def test_addresses_off_their_type_are_refused(dtype, size):
+    """A load or store across its type's boundary is a fault of the GPU: such addresses do not reach it."""
+    lib = _lib.load()
+    at = lambda p: C.c_void_p(p)  # noqa: E731
+    good = 256
+
+    def refused(rc, who):
+        assert rc == _lib.FLUXB_ERR_INVALID and who in _lib.last_error() and "aligned" in _lib.last_error()
+
+    def each(call, who, sizes):
+        """Every pointer in turn one byte, and half of its type, off."""
+        for i, n in enumerate(sizes):
+            for off in {1, n // 2}:
+                if off < n:
+                    p = [at(good)] * len(sizes)
+                    p[i] = at(good + off)
+                    if off:
+                        refused(call(*p), who)
+
+    each(lambda z, c, w: lib.fluxb_moe_route(z, dtype, 4, 8, 2, c, w, None), "moe_route", (size, 4, 4))
+    each(lambda dw, c, w, dz: lib.fluxb_moe_route_backward(dw, c, w, dtype, 4, 8, 2, dz, None), "moe_route_backward", (4, 4, 4, size))
+    each(lambda x, s, i, r: lib.fluxb_moe_permute(x, 4, 2, 7, s, 8, i, r, None), "moe_permute", (1, 4, 4, 1))
+    each(lambda r, i, w, o: lib.fluxb_moe_unpermute(r, dtype, 4, 2, 7, i, w, dtype, o, None), "moe_unpermute", (size, 4, size, size))
+    each(lambda do, r, s, i, w, dr, dw: lib.fluxb_moe_unpermute_backward(do, r, dtype, 4, 2, 7, s, 8, i, w, dtype, dr, dw, None), "moe_unpermute_backward",
+         (size, size, 4, 4, size, size, size))
+    each(lambda s, i: lib.fluxb_mx_quantize(at(256), dtype, 1, 4, 32, 32, at(256), at(256), s, 8, i, 2, None), "mx_quantize", (4, 4))
+    each(lambda s: lib.fluxb_mx_grouped_gemm(at(256), at(256), at(256), 4, at(256), at(256), 2, s, at(256), 8, 32, dtype, at(256), None, None),
+         "mx_grouped_gemm", (4,))
