@@ -5,6 +5,8 @@ Quantisation is exact by its definition: bits are compared. Products: with scale
 of 2^-4 below 2^8, so that sums of up to 4096 terms fit into the 24 bits of fp32 and have to come out exactly, whatever
 their order. With scales of any size a sum of K terms in fp32, by adders that round or cut, is off by at most
 K 2^-23 sum|term|; the rounding to the output's type adds eps / 2 of the value."""
+import functools
+
 import pytest
 import torch
 
@@ -396,3 +398,106 @@ def test_copies_outlive_what_they_were_copied_from(lead):
     for c in copies:
         assert torch.equal(product(c), want) and torch.equal(c.dequantize(), values)
     del trash
+
+
+# ------------------------------------------------------------------------------------ several tiles of several stages a CTA
+PERSISTENT = [t for t in TILES if t and "cta_group" in t]
+
+
+@functools.lru_cache(maxsize=64)
+def _shared(shape, seed):
+    """`_random_mx`, the values on the GPU: made once for all variants."""
+    q, v = _random_mx(shape, seed)
+    return q, v.cuda()
+
+
+def _same(got, want):
+    """Exact sums, rounded once to the type of `got`."""
+    assert torch.equal(got, want.to(got.dtype))
+
+
+@pytest.mark.parametrize("dtype,n", [(torch.float32, 600), (torch.bfloat16, 600), (torch.bfloat16, 601)])
+@pytest.mark.parametrize("num_ctas", [2, 3, 6])
+@pytest.mark.parametrize("tuning", PERSISTENT, ids=str)
+def test_product_of_several_tiles_a_cta_is_exact(tuning, num_ctas, dtype, n):
+    """Few CTAs take all tiles: accumulators, scale slots and stages go from tile to tile, with less than, about and more K than
+    the ring and the slots hold."""
+    import flux_b200 as flux
+
+    m = 800
+    for k in (96, 544, 1056, 2336):
+        x, xv = _shared((m, k), m + k)
+        w, wv = _shared((n, k), n + k + 1)
+        y = flux.mx_gemm(x, w, output_dtype=dtype, tuning={**tuning, "num_ctas": num_ctas})
+        _status()
+        _same(y, xv @ wv.t())
+
+
+@pytest.mark.parametrize("dtype,n", [(torch.float32, 520), (torch.bfloat16, 520), (torch.bfloat16, 519)])
+@pytest.mark.parametrize("num_ctas", [2, 3, 6])
+@pytest.mark.parametrize("tuning", PERSISTENT, ids=str)
+def test_grouped_product_of_several_tiles_a_cta_is_exact(tuning, num_ctas, dtype, n):
+    import flux_b200 as flux
+
+    splits = [300, 0, 517, 64, 1, 130, 257, 0, 3]
+    rows = sum(splits) + 5
+    for k in (96, 544, 1312, 2336):
+        x, xv = _shared((rows, k), rows + k)
+        w, wv = _shared((len(splits), n, k), n + k)
+        out = torch.full((rows, n), -77.0, device="cuda", dtype=dtype)
+        flux.mx_grouped_gemm(x, w, torch.tensor(splits, dtype=torch.int32, device="cuda"), dtype, output=out, tuning={**tuning, "num_ctas": num_ctas})
+        _status()
+        _same(out[:-5], _grouped_want(xv, wv, splits))
+        assert bool((out[-5:] == -77.0).all())
+
+
+@pytest.mark.parametrize("tuning", [None, *PERSISTENT], ids=str)
+def test_products_of_several_waves_are_exact(tuning):
+    """Every SM takes several tiles."""
+    import flux_b200 as flux
+
+    k = 1056
+    x, xv = _shared((4100, k), 1)
+    w, wv = _shared((8200, k), 2)
+    y = flux.mx_gemm(x, w, output_dtype=torch.bfloat16, tuning=tuning)
+    _status()
+    _same(y, xv @ wv.t())
+    splits = [900, 17, 0, 2050, 333, 800]
+    w, wv = _shared((6, 4104, k), 3)
+    y = flux.mx_grouped_gemm(x, w, torch.tensor(splits, dtype=torch.int32, device="cuda"), tuning=tuning)
+    _status()
+    _same(y, _grouped_want(xv, wv, splits))
+
+
+@pytest.mark.parametrize("dtype,exponents", [(torch.bfloat16, (0, 1, -1, 100, 125, -100, -119, -120, -124, -125, -126, -127, -129, -132)),
+                                             (torch.float16, (0, 1, -1, 12, 13, -8, -11, -13, -14, -16, -19, -23))])
+def test_quantize_at_every_border_of_16_bits(dtype, exponents):
+    """All ties and their neighbours in the input's own type, at the ends of its range, among its subnormal numbers, and in between."""
+    import flux_b200 as flux
+
+    marks = torch.tensor([0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0, 6.0, 7.0, 7.9], dtype=dtype)
+    bits = marks.view(torch.int16)
+    near = torch.cat((marks, (bits - 1).view(dtype), (bits + 1).view(dtype)))
+    block = torch.cat((near, torch.tensor([4.0, 0.0], dtype=dtype))).float()
+    signs = torch.where(torch.arange(32) % 3 == 0, -1.0, 1.0)
+    rows = [block * signs * 2.0 ** e for e in exponents]
+    # neighbours whose last bits the scaling by 2^e pushed out come back: the smallest numbers of the type, all of them
+    small = torch.arange(32 * 64, dtype=torch.int16).view(dtype).view(-1, 32).float()
+    rows += [*small, *(-small.flip(1))]
+    rows += [torch.zeros(32), -torch.zeros(32), torch.full((32,), torch.finfo(dtype).max), torch.full((32,), torch.finfo(dtype).smallest_normal)]
+    for bad in (float("inf"), -float("inf"), float("nan")):
+        r = block.clone()
+        r[5] = bad
+        rows.append(r)
+    x = torch.stack(rows).to(dtype)
+    data, scales = _quantised64(x)
+    q = flux.mx_quantize(x.cuda())
+    assert torch.equal(q.scales.cpu(), scales)
+    assert torch.equal(q.data.cpu(), data)
+    got, want = q.dequantize(torch.float32).cpu(), _values(data, scales).to(torch.float32)
+    assert torch.equal(got.isnan(), want.isnan()) and torch.equal(got.nan_to_num(0.0), want.nan_to_num(0.0))
+    # unaligned rows go by another way to the same values
+    wide = torch.zeros(x.shape[0], 67, dtype=dtype, device="cuda")
+    wide[:, 3:35] = x.cuda()
+    again = flux.mx_quantize(wide[:, 3:35])
+    assert torch.equal(again.data, q.data) and torch.equal(again.scales, q.scales)
