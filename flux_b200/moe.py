@@ -70,19 +70,16 @@ def _on_device(t: torch.Tensor) -> bool:
 
 def _refuse_tangent(name: str, *tensors: Optional[torch.Tensor]) -> None:
     """No operator here has a forward-mode derivative, and the library sees addresses: a tensor's tangent would be lost without a
-    word, with the gradient mode on or off."""
-    if _forward_ad._current_level < 0:  # (outside of `dual_level` there are none)
-        return
+    word, with the gradient mode on or off. (Outside of `dual_level`, at level -1, there are none: callers look there first.)"""
     for t in tensors:
         if t is not None and _forward_ad.unpack_dual(t).tangent is not None:
             raise RuntimeError(f"{name} has no forward-mode derivative")
 
 
 def _in_memory(t: torch.Tensor) -> torch.Tensor:
-    """`t` as contiguous memory that holds its values: a conjugation or a sign that torch has put off is carried out."""
-    if t.is_conj() or t.is_neg():
-        t = t.resolve_conj().resolve_neg()
-    return t if t.is_contiguous() else t.contiguous()
+    """`t` as contiguous memory that holds its values: a conjugation or a sign that torch has put off is carried out. (Among
+    contiguous tensors only complex ones and single numbers can be marked so: callers look at nothing else.)"""
+    return t.resolve_conj().resolve_neg().contiguous()
 
 
 def _check_index(name: str, dev: int, splits: torch.Tensor, scatter_index: torch.Tensor) -> torch.Size:
@@ -125,7 +122,8 @@ class _RouteFn(torch.autograd.Function):
     def backward(ctx, _, dweights):
         if dweights is None:
             return None, None
-        _refuse_tangent("moe_route's gradient", dweights)
+        if _forward_ad._current_level >= 0:
+            _refuse_tangent("moe_route's gradient", dweights)
         chosen, weights = ctx.saved_tensors
         dtype, nexperts = ctx.like
         ntokens, topk = chosen.shape
@@ -144,11 +142,13 @@ def moe_route(logits: torch.Tensor, topk: int):
     weight 0, which `calc_scatter_index` gives no row. Differentiable in the logits."""
     if not (_on_device(logits) and logits.dim() == 2 and logits.dtype in _FLOATS):
         raise RuntimeError("moe_route: logits must be a fp32, bf16 or fp16 [ntokens, nexperts] tensor on the current CUDA device")
-    _refuse_tangent("moe_route", logits)
+    if _forward_ad._current_level >= 0:
+        _refuse_tangent("moe_route", logits)
     topk = int(topk)
     if not 1 <= topk <= min(logits.shape[1], 32) or logits.shape[1] > 1024 or logits.shape[0] * topk >= 1 << 30:
         raise RuntimeError(f"moe_route: topk={topk} for {logits.shape[0]} tokens and {logits.shape[1]} experts (up to 32 of 1024)")
-    logits = _in_memory(logits)
+    if not logits.is_contiguous() or logits.shape[1] == 1:
+        logits = _in_memory(logits)
     if logits.requires_grad and torch.is_grad_enabled():
         return _RouteFn.apply(logits, topk)
     return _route_forward(logits, topk)
@@ -156,8 +156,9 @@ def moe_route(logits: torch.Tensor, topk: int):
 
 def _permute(tokens: torch.Tensor, splits: torch.Tensor, scatter_index: torch.Tensor) -> torch.Tensor:
     ntokens, topk = scatter_index.shape
-    tokens = _in_memory(tokens)
     hidden = tokens.shape[1]
+    if not tokens.is_contiguous() or hidden == 1 or tokens.is_conj():
+        tokens = _in_memory(tokens)
     rows = tokens.new_empty((ntokens * topk, hidden))
     _lib.check(_lib.load().fluxb_moe_permute(tokens.data_ptr(), ntokens, topk, hidden * tokens.element_size(), splits.data_ptr(),
                                              splits.numel(), scatter_index.data_ptr(), rows.data_ptr(), _cur_stream()))
@@ -166,8 +167,9 @@ def _permute(tokens: torch.Tensor, splits: torch.Tensor, scatter_index: torch.Te
 
 def _unpermute(rows: torch.Tensor, scatter_index: torch.Tensor, weights: Optional[torch.Tensor]) -> torch.Tensor:
     ntokens, topk = scatter_index.shape
-    rows = _in_memory(rows)
     hidden = rows.shape[1]
+    if not rows.is_contiguous() or hidden == 1:
+        rows = _in_memory(rows)
     out = rows.new_empty((ntokens, hidden))
     _lib.check(_lib.load().fluxb_moe_unpermute(rows.data_ptr(), fluxb_dtype(rows.dtype), ntokens, topk, hidden, scatter_index.data_ptr(),
                                                _ptr(weights), 0 if weights is None else fluxb_dtype(weights.dtype), out.data_ptr(), _cur_stream()))
@@ -183,7 +185,8 @@ class _PermuteFn(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, drows):
-        _refuse_tangent("moe_permute's gradient", drows)
+        if _forward_ad._current_level >= 0:
+            _refuse_tangent("moe_permute's gradient", drows)
         return _unpermute(drows, ctx.saved_tensors[0], None), None, None
 
 
@@ -198,7 +201,8 @@ class _UnpermuteFn(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dout):
-        _refuse_tangent("moe_unpermute's gradient", dout)
+        if _forward_ad._current_level >= 0:
+            _refuse_tangent("moe_unpermute's gradient", dout)
         rows, splits, scatter_index, weights = ctx.saved_tensors
         if weights is None:
             return _permute(dout, splits, scatter_index), None, None, None
@@ -230,7 +234,8 @@ def moe_permute(tokens: torch.Tensor, splits: torch.Tensor, scatter_index: torch
     ntokens, _ = _check_index("moe_permute", tokens.get_device(), splits, scatter_index)
     if ntokens != shape[0]:
         raise RuntimeError(f"moe_permute: scatter_index has {ntokens} tokens, not {shape[0]}")
-    _refuse_tangent("moe_permute", tokens)
+    if _forward_ad._current_level >= 0:
+        _refuse_tangent("moe_permute", tokens)
     if tokens.requires_grad and torch.is_grad_enabled():
         _check(tokens.dtype in _FLOATS, "moe_permute: only fp32, bf16 and fp16 tokens have gradients")
         return _PermuteFn.apply(tokens, splits, scatter_index)
@@ -254,8 +259,10 @@ def moe_unpermute(rows: torch.Tensor, splits: torch.Tensor, scatter_index: torch
     if weights is not None:
         if not (weights.get_device() == dev and weights.dtype in _FLOATS and weights.shape == scatter_index.shape):
             raise RuntimeError("moe_unpermute: weights must be a fp32, bf16 or fp16 [ntokens, topk] tensor on the current CUDA device")
-        weights = _in_memory(weights)
-    _refuse_tangent("moe_unpermute", rows, weights)
+        if not weights.is_contiguous() or weights.shape[1] == 1:
+            weights = _in_memory(weights)
+    if _forward_ad._current_level >= 0:
+        _refuse_tangent("moe_unpermute", rows, weights)
     if torch.is_grad_enabled() and (rows.requires_grad or (weights is not None and weights.requires_grad)):
         return _UnpermuteFn.apply(rows, splits, scatter_index, weights)
     return _unpermute(rows, scatter_index, weights)

@@ -15,6 +15,7 @@ import threading
 from typing import Dict, List, Optional
 
 import torch
+from torch.autograd import forward_ad as _forward_ad
 
 from . import _lib
 from .moe import _FLOATS, _check_index, _on_device, _refuse_tangent
@@ -161,7 +162,8 @@ def mx_quantize(x: torch.Tensor, splits: Optional[torch.Tensor] = None, scatter_
         raise RuntimeError("mx_quantize: x must be a fp32, bf16 or fp16 [..., N, K] tensor on the current CUDA device, K a multiple of 32")
     if x.requires_grad and torch.is_grad_enabled():
         raise RuntimeError("mx_quantize has no gradient: detach x, or call it under torch.no_grad()")
-    _refuse_tangent("mx_quantize", x)
+    if _forward_ad._current_level >= 0:
+        _refuse_tangent("mx_quantize", x)
     n, k = shape[-2:]
     lead, batch = (), 1
     if len(shape) > 2:
@@ -244,7 +246,8 @@ def mx_gemm(x: MXTensor, w: MXTensor, bias: Optional[torch.Tensor] = None, outpu
                "mx_gemm: bias must be a contiguous [N] tensor of the output's type")
         if bias.requires_grad and torch.is_grad_enabled():
             raise RuntimeError("mx_gemm has no gradient: detach the bias, or call it under torch.no_grad()")
-        _refuse_tangent("mx_gemm", bias)
+        if _forward_ad._current_level >= 0:
+            _refuse_tangent("mx_gemm", bias)
     out = _output("mx_gemm", output, m, n, output_dtype, _like(x))
     if n == 0:
         return out
