@@ -1,7 +1,6 @@
 // Host-side internals shared by the .cu files of the library: error
 // reporting, the communicator object, tensor-map encoding, launch helpers.
 #pragma once
-#include <initializer_list>
 #include <cuda.h>
 #include <cuda_runtime.h>
 #include <stdarg.h>
@@ -9,6 +8,7 @@
 #include <string.h>
 
 #include <functional>
+#include <initializer_list>
 #include <memory>
 #include <mutex>
 #include <string>

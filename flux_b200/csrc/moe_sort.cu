@@ -15,8 +15,11 @@ namespace fluxb {
 // A group of G lanes per token, VPL logits a lane in registers as order-preserving integers. A choice is a maximum over the
 // lanes, ties to the lower expert, and only the lane that held it looks for its next one. 16-bit logits leave room for the
 // expert in the same word, so that one maximum finds both; for fp32 a vote finds the lowest lane (its experts are lower)
-// that has the largest key. Bound by instructions, so a warp takes as many tokens as it can: 32768 x 8 bf16 top-2 2.8 us (a
-// warp per token 9.0), 16384 x 64 bf16 top-6 4.4, 32768 x 128 fp32 top-8 17.7 (maxima over 64-bit pairs of key and expert 22.5).
+// that has the largest key. So that no lane idles a warp takes as many tokens as it can: 32768 x 8 bf16 top-2 2.8 us (a warp
+// per token 9.0), 16384 x 64 bf16 top-6 4.4, 32768 x 128 fp32 top-8 17.7 (maxima over 64-bit pairs of key and expert 22.5).
+// Bound by instructions where the tokens fill the GPU (32768 x 128: an instruction in 71% of the active cycles with 77% of the
+// warps resident; they wait for their turn, 34%, and for a busy pipe, 27%, more than for shuffles, 8%), by the launch's start and end
+// where its CTAs all fit at once (16384 x 64: a third of the warps, 32% of the SMs' throughput).
 constexpr int kRouteThreads = 128;
 constexpr int kRouteMaxExperts = 1024;
 constexpr int kRouteMaxTopk = 32;
@@ -199,7 +202,7 @@ moe_route_backward_kernel(const float* __restrict__ dweights, const int* __restr
 
 // ---------------------------------------------------------------------------------------------------- permute, unpermute
 constexpr int kSortThreads = 256;
-constexpr int kSortTailCtas = 148;  // the rows that belong to nobody are cleared by CTAs of their own
+constexpr int kSortTailCtas = 148;  // the rows that belong to nobody are cleared by CTAs of their own, as many as a B200 has SMs at most
 
 template <int VB>
 struct RawVec;

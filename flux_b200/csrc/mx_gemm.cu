@@ -90,9 +90,12 @@ static int launch_mx_few(const fluxb_comm* comm, const MxParams& p, long long ti
 // are linear in the launch's numbers, with coefficients (us) fitted to measured times of all variants on 148 problems
 // (dense 1 .. 4096 x 1024 .. 28672 x 1024 .. 8192; 8 to 128 experts, 2 to 65536 rows, of 1024 .. 14336 x 1024 .. 8192;
 // weights from memory, launches back to back in a graph). Over those problems the choice takes 2% longer than the fastest
-// variant on average, 24% at worst (64 x 4096 x 4096 6.7 us against 5.4, grouped 11%); over 297 others, down to 512 x 416, 3%
-// and, among launches of a few us, up to 42% (64 x 1000 x 416 5.4 us against 3.8). One variant for all would be far off on
-// either side: 256 x 4096 x 4096 takes 5.9 us in tiles of 64 and 9.7 in tiles of 256, 4096 x 8192 x 8192 160 and 90.
+// variant on average, 24% at worst (64 x 4096 x 4096 6.7 us against 5.4, grouped 11%). Over 297 others, down to 512 x 416, it is 3%
+// on average and, by how long the launch takes, at worst: up to 10 us 42% (64 x 1000 x 416 5.4 us against 3.8), up to 20 us 10%, up to
+// 40 us 8%, beyond 6% (dense) and 17% (grouped). The last is a K longer than any that was fitted: 8 experts x 4096 x 14336 with 16 and
+// 64 tokens, top-2, 50.4 and 52.6 us, where the few-token kernel's 64 tokens uncut take 43.6 and 45.1; 8192 tokens over 64 experts take
+// 8 to 9% longer in tiles of 192 than of 256. One variant for all would be far off on either side: 256 x 4096 x 4096 takes 5.9 us in
+// tiles of 64 and 9.7 in tiles of 256, 4096 x 8192 x 8192 160 and 90.
 //   tiled:      fixed + waves * (per_stage * K blocks + per_wave) + per_mb * MB of weights (+ grouped)
 //   few tokens: fixed + per_stage * K blocks of a part + per_cta * CTAs per slot + per_block * K blocks per slot
 //               + per_mb * MB of weights (+ grouped)

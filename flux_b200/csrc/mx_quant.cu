@@ -17,7 +17,7 @@ namespace fluxb {
 constexpr int kQuantThreads = 256;
 constexpr int kQuantUnroll = 2;
 constexpr int kQuantUnit = 16;  // values of a thread at a time
-constexpr int kQuantTailCtas = 148;
+constexpr int kQuantTailCtas = 148;  // at most: as many as a B200 has SMs
 constexpr int kDequantUnroll = 4;
 
 struct QuantParams {

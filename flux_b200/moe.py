@@ -84,22 +84,23 @@ def _in_memory(t: torch.Tensor) -> torch.Tensor:
 
 def _check_index(name: str, dev: int, splits: torch.Tensor, scatter_index: torch.Tensor) -> torch.Size:
     """Shape [ntokens, topk] of an index whose tensors, like the call's others, are on device `dev`, the current one."""
-    if not (splits.get_device() == dev and splits.dtype is torch.int32 and len(splits.shape) == 1 and splits.shape[0] >= 1 and splits.is_contiguous()):
+    experts = splits.shape
+    if not (splits.get_device() == dev and splits.dtype is torch.int32 and len(experts) == 1 and experts[0] >= 1 and splits.is_contiguous()):
         raise RuntimeError(f"{name}: splits must be a contiguous int32 [nexperts] tensor on the current CUDA device")
     shape = scatter_index.shape
     if not (scatter_index.get_device() == dev and scatter_index.dtype is torch.int32 and len(shape) == 2 and shape[1] >= 1
             and scatter_index.is_contiguous()):
         raise RuntimeError(f"{name}: scatter_index must be a contiguous int32 [ntokens, topk] tensor on the current CUDA device")
+    ntokens, topk = shape
     # (the library takes sizes of 31 bits; larger ones would arrive there as others)
-    if shape[0] * shape[1] >= 1 << 30 or shape[1] >= 1 << 30:
-        raise RuntimeError(f"{name}: {shape[0]} x {shape[1]} routed rows are too many")
-    if splits.shape[0] >= 1 << 31:
-        raise RuntimeError(f"{name}: splits of {splits.shape[0]} experts are too many")
+    if ntokens * topk >= 1 << 30 or topk >= 1 << 30:
+        raise RuntimeError(f"{name}: {ntokens} x {topk} routed rows are too many")
+    if experts[0] >= 1 << 31:
+        raise RuntimeError(f"{name}: splits of {experts[0]} experts are too many")
     return shape
 
 
-def _route_forward(logits: torch.Tensor, topk: int):
-    ntokens, nexperts = logits.shape
+def _route_forward(logits: torch.Tensor, ntokens: int, nexperts: int, topk: int):
     chosen = logits.new_empty((ntokens, topk), dtype=torch.int32)
     weights = logits.new_empty((ntokens, topk), dtype=torch.float32)
     _lib.check(_lib.load().fluxb_moe_route(logits.data_ptr(), fluxb_dtype(logits.dtype), ntokens, nexperts, topk, chosen.data_ptr(),
@@ -110,7 +111,7 @@ def _route_forward(logits: torch.Tensor, topk: int):
 class _RouteFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, topk):
-        chosen, weights = _route_forward(logits, topk)
+        chosen, weights = _route_forward(logits, *logits.shape, topk)
         ctx.save_for_backward(chosen, weights)
         ctx.mark_non_differentiable(chosen)
         ctx.set_materialize_grads(False)  # no zeros in the place of the gradient that `chosen` does not have
@@ -128,7 +129,8 @@ class _RouteFn(torch.autograd.Function):
         dtype, nexperts = ctx.like
         ntokens, topk = chosen.shape
         dlogits = chosen.new_empty((ntokens, nexperts), dtype=dtype)
-        dweights = _in_memory(dweights)  # (a copy is held until the launch is queued: other threads allocate during the call)
+        if not dweights.is_contiguous() or topk == 1:
+            dweights = _in_memory(dweights)  # (held until the launch is queued: other threads allocate during the call)
         _lib.check(_lib.load().fluxb_moe_route_backward(
             dweights.data_ptr(), chosen.data_ptr(), weights.data_ptr(), fluxb_dtype(dtype), ntokens, nexperts, topk,
             dlogits.data_ptr(), _cur_stream()))
@@ -140,24 +142,24 @@ def moe_route(logits: torch.Tensor, topk: int):
     (fp32, bf16 or fp16): the topk largest of every token in descending order, ties to the lower expert, and the softmax
     over them. A logit of minus infinity is never chosen; where fewer than topk are left the entries are expert -1 with
     weight 0, which `calc_scatter_index` gives no row. Differentiable in the logits."""
-    if not (_on_device(logits) and logits.dim() == 2 and logits.dtype in _FLOATS):
+    shape = logits.shape
+    if not (_on_device(logits) and len(shape) == 2 and logits.dtype in _FLOATS):
         raise RuntimeError("moe_route: logits must be a fp32, bf16 or fp16 [ntokens, nexperts] tensor on the current CUDA device")
     if _forward_ad._current_level >= 0:
         _refuse_tangent("moe_route", logits)
+    ntokens, nexperts = shape
     topk = int(topk)
-    if not 1 <= topk <= min(logits.shape[1], 32) or logits.shape[1] > 1024 or logits.shape[0] * topk >= 1 << 30:
-        raise RuntimeError(f"moe_route: topk={topk} for {logits.shape[0]} tokens and {logits.shape[1]} experts (up to 32 of 1024)")
-    if not logits.is_contiguous() or logits.shape[1] == 1:
+    if not 1 <= topk <= min(nexperts, 32) or nexperts > 1024 or ntokens * topk >= 1 << 30:
+        raise RuntimeError(f"moe_route: topk={topk} for {ntokens} tokens and {nexperts} experts (up to 32 of 1024)")
+    if not logits.is_contiguous() or nexperts == 1:
         logits = _in_memory(logits)
     if logits.requires_grad and torch.is_grad_enabled():
         return _RouteFn.apply(logits, topk)
-    return _route_forward(logits, topk)
+    return _route_forward(logits, ntokens, nexperts, topk)
 
 
-def _permute(tokens: torch.Tensor, splits: torch.Tensor, scatter_index: torch.Tensor) -> torch.Tensor:
-    ntokens, topk = scatter_index.shape
-    hidden = tokens.shape[1]
-    if not tokens.is_contiguous() or hidden == 1 or tokens.is_conj():
+def _permute(tokens: torch.Tensor, splits: torch.Tensor, scatter_index: torch.Tensor, ntokens: int, topk: int, hidden: int) -> torch.Tensor:
+    if not tokens.is_contiguous() or hidden == 1 or tokens.dtype.is_complex:
         tokens = _in_memory(tokens)
     rows = tokens.new_empty((ntokens * topk, hidden))
     _lib.check(_lib.load().fluxb_moe_permute(tokens.data_ptr(), ntokens, topk, hidden * tokens.element_size(), splits.data_ptr(),
@@ -165,9 +167,7 @@ def _permute(tokens: torch.Tensor, splits: torch.Tensor, scatter_index: torch.Te
     return rows
 
 
-def _unpermute(rows: torch.Tensor, scatter_index: torch.Tensor, weights: Optional[torch.Tensor]) -> torch.Tensor:
-    ntokens, topk = scatter_index.shape
-    hidden = rows.shape[1]
+def _unpermute(rows: torch.Tensor, scatter_index: torch.Tensor, weights: Optional[torch.Tensor], ntokens: int, topk: int, hidden: int) -> torch.Tensor:
     if not rows.is_contiguous() or hidden == 1:
         rows = _in_memory(rows)
     out = rows.new_empty((ntokens, hidden))
@@ -180,14 +180,15 @@ class _PermuteFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, tokens, splits, scatter_index):
         ctx.save_for_backward(scatter_index)
-        return _permute(tokens, splits, scatter_index)
+        return _permute(tokens, splits, scatter_index, *scatter_index.shape, tokens.shape[1])
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, drows):
         if _forward_ad._current_level >= 0:
             _refuse_tangent("moe_permute's gradient", drows)
-        return _unpermute(drows, ctx.saved_tensors[0], None), None, None
+        (scatter_index,) = ctx.saved_tensors
+        return _unpermute(drows, scatter_index, None, *scatter_index.shape, drows.shape[1]), None, None
 
 
 class _UnpermuteFn(torch.autograd.Function):
@@ -196,7 +197,7 @@ class _UnpermuteFn(torch.autograd.Function):
         ctx.like = (rows.dtype, rows.shape[1])
         need_rows = weights is not None and weights.requires_grad
         ctx.save_for_backward(rows if need_rows else None, splits, scatter_index, weights)
-        return _unpermute(rows, scatter_index, weights)
+        return _unpermute(rows, scatter_index, weights, *scatter_index.shape, rows.shape[1])
 
     @staticmethod
     @torch.autograd.function.once_differentiable
@@ -205,17 +206,19 @@ class _UnpermuteFn(torch.autograd.Function):
             _refuse_tangent("moe_unpermute's gradient", dout)
         rows, splits, scatter_index, weights = ctx.saved_tensors
         if weights is None:
-            return _permute(dout, splits, scatter_index), None, None, None
+            return _permute(dout, splits, scatter_index, *scatter_index.shape, dout.shape[1]), None, None, None
         ntokens, topk = scatter_index.shape
         dtype, hidden = ctx.like
-        dout = _in_memory(dout)
+        if not dout.is_contiguous() or hidden == 1:
+            dout = _in_memory(dout)
         drows = dweights = None
         if ctx.needs_input_grad[0]:
             drows = dout.new_empty((ntokens * topk, hidden))
         if ctx.needs_input_grad[3]:
             # pairs without an expert get a gradient of zero like the others get theirs: the kernel writes every entry
             dweights = torch.empty_like(weights)
-            rows = _in_memory(rows)
+            if not rows.is_contiguous() or hidden == 1:
+                rows = _in_memory(rows)
         else:
             rows = None
         _lib.check(_lib.load().fluxb_moe_unpermute_backward(
@@ -231,7 +234,7 @@ def moe_permute(tokens: torch.Tensor, splits: torch.Tensor, scatter_index: torch
     shape = tokens.shape
     if not (_on_device(tokens) and len(shape) == 2 and shape[1] >= 1):
         raise RuntimeError("moe_permute: tokens must be a [ntokens, hidden] tensor on the current CUDA device")
-    ntokens, _ = _check_index("moe_permute", tokens.get_device(), splits, scatter_index)
+    ntokens, topk = _check_index("moe_permute", tokens.get_device(), splits, scatter_index)
     if ntokens != shape[0]:
         raise RuntimeError(f"moe_permute: scatter_index has {ntokens} tokens, not {shape[0]}")
     if _forward_ad._current_level >= 0:
@@ -239,7 +242,7 @@ def moe_permute(tokens: torch.Tensor, splits: torch.Tensor, scatter_index: torch
     if tokens.requires_grad and torch.is_grad_enabled():
         _check(tokens.dtype in _FLOATS, "moe_permute: only fp32, bf16 and fp16 tokens have gradients")
         return _PermuteFn.apply(tokens, splits, scatter_index)
-    return _permute(tokens, splits, scatter_index)
+    return _permute(tokens, splits, scatter_index, ntokens, topk, shape[1])
 
 
 def moe_unpermute(rows: torch.Tensor, splits: torch.Tensor, scatter_index: torch.Tensor,
@@ -251,21 +254,22 @@ def moe_unpermute(rows: torch.Tensor, splits: torch.Tensor, scatter_index: torch
     if not (_on_device(rows) and len(shape) == 2 and shape[1] >= 1 and rows.dtype in _FLOATS):
         raise RuntimeError("moe_unpermute: rows must be a fp32, bf16 or fp16 [ntokens * topk, hidden] tensor on the current CUDA device")
     dev = rows.get_device()
-    ntokens, topk = _check_index("moe_unpermute", dev, splits, scatter_index)
+    index_shape = _check_index("moe_unpermute", dev, splits, scatter_index)
+    ntokens, topk = index_shape
     if shape[1] >= 1 << 28:
         raise RuntimeError(f"moe_unpermute: hidden={shape[1]} is too large")
     if shape[0] != ntokens * topk:
         raise RuntimeError(f"moe_unpermute: {shape[0]} rows for {ntokens} x {topk} entries of scatter_index")
     if weights is not None:
-        if not (weights.get_device() == dev and weights.dtype in _FLOATS and weights.shape == scatter_index.shape):
+        if not (weights.get_device() == dev and weights.dtype in _FLOATS and weights.shape == index_shape):
             raise RuntimeError("moe_unpermute: weights must be a fp32, bf16 or fp16 [ntokens, topk] tensor on the current CUDA device")
-        if not weights.is_contiguous() or weights.shape[1] == 1:
+        if not weights.is_contiguous() or topk == 1:
             weights = _in_memory(weights)
     if _forward_ad._current_level >= 0:
         _refuse_tangent("moe_unpermute", rows, weights)
     if torch.is_grad_enabled() and (rows.requires_grad or (weights is not None and weights.requires_grad)):
         return _UnpermuteFn.apply(rows, splits, scatter_index, weights)
-    return _unpermute(rows, scatter_index, weights)
+    return _unpermute(rows, scatter_index, weights, ntokens, topk, shape[1])
 
 
 class GemmGroupedV3AGScatter:

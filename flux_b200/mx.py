@@ -40,11 +40,10 @@ def _comm() -> Comm:
                 c = _COMMS.get(dev)
                 if c is None:
                     c = _COMMS[dev] = Comm(None)
-    used = _USED.setdefault(dev, [])
-    if c not in used:
+    used = _USED.get(dev)
+    if used is None or used[-1] is not c:
         with _LOCK:
-            if c not in used:
-                used.append(c)
+            _USED[dev] = [u for u in _USED.get(dev, ()) if u is not c] + [c]  # (the last one that was used last)
     return c
 
 
@@ -52,7 +51,7 @@ def mx_check_status() -> None:
     """Raise if a bounded wait of a product on the current device has run out, whose output is then incomplete (call after a
     synchronize). It reads the status of every communicator that this device's products have used: the default ones, which
     `Comm.check_status` reads as well, and the one that they make where there is none."""
-    for c in list(_USED.get(_cur_device(), ())):
+    for c in _USED.get(_cur_device(), ()):
         c.check_status()
 
 

@@ -386,3 +386,24 @@ def test_more_than_31_bits_of_values(hidden):
         want = torch.zeros(100, hidden, dtype=torch.float64).index_add_(0, t, term)
         size = torch.zeros(100, hidden, dtype=torch.float64).index_add_(0, t, term.abs())
         _within(dx[at], want, topk * U * size + half * (want.abs() + topk * U * size) + low)
+
+
+def test_gradients_and_tokens_as_torch_hands_them_over():
+    """Expanded and transposed gradients, and tokens whose conjugation is only marked."""
+    import flux_b200 as flux
+
+    si, splits, _ = _routing(37, 8, 2, 0.2, 11)
+    z = torch.randn(37, 8, device="cuda", requires_grad=True)
+    _, w = flux.moe_route(z, 2)
+    dw = torch.randn(2, 37, device="cuda")
+    (dense,) = torch.autograd.grad(w, z, dw.t().contiguous(), retain_graph=True)
+    (strided,) = torch.autograd.grad(w, z, dw.t(), retain_graph=True)
+    (ones,) = torch.autograd.grad(w, z, torch.ones_like(w), retain_graph=True)
+    (expanded,) = torch.autograd.grad(w.sum(), z)
+    assert torch.equal(dense, strided) and torch.equal(ones, expanded)
+    x = torch.randn(37, 5, device="cuda", dtype=torch.complex64)
+    for t in (x.conj(), x.conj().t().contiguous().t(), x.conj().imag, x[:, :1].conj().imag):
+        assert torch.equal(flux.moe_permute(t, splits, si), flux.moe_permute(t.resolve_conj().resolve_neg().contiguous(), splits, si))
+    one = torch.randn(1, 1, device="cuda", dtype=torch.complex64).conj().imag
+    index, counts = torch.zeros(1, 1, dtype=torch.int32, device="cuda"), torch.ones(1, dtype=torch.int32, device="cuda")
+    assert one.is_neg() and torch.equal(flux.moe_permute(one, counts, index), one) and torch.equal(flux.moe_unpermute(one, counts, index), one)
