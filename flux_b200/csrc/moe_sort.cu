@@ -1,6 +1,6 @@
 // The token side of a MoE layer, each step with its gradient: the experts of every token and their weights (route), the
-// tokens copied into the order of their experts (permute) and the weighted sum of a token's rows (unpermute). All of it
-// is bound by memory; every sum is in fp32 and in a fixed order, so results do not change from run to run.
+// tokens copied into the order of their experts (permute) and the weighted sum of a token's rows (unpermute). The last two
+// are bound by memory; every sum is in fp32 and in a fixed order, so results do not change from run to run.
 //
 // `scatter_index` [ntokens, topk] holds the row of every (token, choice) pair, as fluxb_moe_scatter_index makes it: the
 // valid entries are the rows 0 .. sum(splits) - 1, each once; an entry outside [0, ntokens * topk) is a pair without an

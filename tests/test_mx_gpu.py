@@ -501,3 +501,32 @@ def test_quantize_at_every_border_of_16_bits(dtype, exponents):
     wide[:, 3:35] = x.cuda()
     again = flux.mx_quantize(wide[:, 3:35])
     assert torch.equal(again.data, q.data) and torch.equal(again.scales, q.scales)
+
+
+def test_quantise_more_rows_than_a_launch_takes():
+    """Units of 16 (and back, of 8) values are numbered in 31 bits, 8 (4) for a row of 32 here: three launches and two."""
+    import flux_b200 as flux
+
+    torch.cuda.empty_cache()
+    rows, part_rows = 537_000_000, 1_000_000
+    if torch.cuda.mem_get_info()[0] < 100 << 30:
+        pytest.skip("needs 100 GB")
+    x = torch.empty(rows // part_rows, part_rows, 32, dtype=torch.bfloat16, device="cuda")
+    part = torch.randn(part_rows, 32, generator=torch.Generator().manual_seed(5)).to(torch.bfloat16).cuda()
+    for i in range(x.shape[0]):
+        torch.mul(part, 1.0 + i / x.shape[0], out=x[i])
+    x = x.view(rows, 32)
+    q = flux.mx_quantize(x)
+    y = q.dequantize()
+    block_rows = 128
+    for first in (0, 268_435_327, 2 * 268_435_327, 536_870_655, rows - 20):  # launches of the quantisation, and back, begin there
+        r = slice(max(first - 20, 0), min(first + 20, rows))
+        data, scales = _quantised64(x[r])
+        assert torch.equal(q.data[r].cpu(), data)
+        assert torch.equal(y[r].cpu().double(), _values(data, scales))
+        b0 = r.start // block_rows
+        some = q.blocks[b0:(r.stop - 1) // block_rows + 1].view(-1, 1, 32, 4, 4).permute(0, 3, 2, 1, 4).reshape(-1, 4)
+        assert torch.equal(some[r.start - b0 * block_rows:r.stop - b0 * block_rows, :1].cpu(), scales)
+        assert not bool(some[r.start - b0 * block_rows:r.stop - b0 * block_rows, 1:].any())
+    del x, y, q
+    torch.cuda.empty_cache()
